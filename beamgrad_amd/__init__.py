@@ -5,7 +5,11 @@ A drop-in for beamgrad's GPU path: the same Python API (``decode``,
 ``final_scores``, ``backtrack``, ``search``, ``beam_search``,
 ``length_penalty``, ``losses``) and the same ``torch.ops.beamgrad`` operators,
 served by hand-written HIP kernels in ``libdbs_hip`` (whose C ABI is the
-reference's ``dbs_cuda.h``).
+reference's ``dbs_cuda.h``). Beside them, the state of the model that is
+searched: attention over a paged cache (``tree_attention``), the cache's pages
+(``PageTable``, ``fork_pages``, ``extend_pages``, ``write_tokens``,
+``keep_tokens``) and dense states in the order of the beams
+(``reorder_states``).
 
 The public names load on first use. Importing the package itself loads
 nothing, so ``beamgrad_amd._C_hip`` (the operators' HIP kernels) can be
@@ -28,6 +32,13 @@ _PUBLIC = {
     "beam_search": "._search",
     "search": "._search",
     "sequence_scores": "._search",
+    "PageTable": "._cache",
+    "extend_pages": "._cache",
+    "fork_pages": "._cache",
+    "keep_tokens": "._cache",
+    "reorder_states": "._cache",
+    "tree_attention": "._cache",
+    "write_tokens": "._cache",
     "BeamSearchOutput": "._torch",
     "backtrack": "._torch",
     "cuda_available": "._torch",

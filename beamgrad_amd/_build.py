@@ -42,7 +42,9 @@ HIP_FLAGS = [
 LIB_SOURCES = ["csrc/api.hip", "csrc/host_abi.cpp", "csrc/host_results.cpp", "csrc/decode.hip", "csrc/row_pass.hip",
                "csrc/row_logprob.hip", "csrc/row_relay.hip", "csrc/row_stream.hip", "csrc/row_short.hip",
                "csrc/select.hip", "csrc/select_f32.hip",
-               "csrc/select_f16.hip", "csrc/select_bf16.hip", "csrc/backward.hip"]
+               "csrc/select_f16.hip", "csrc/select_bf16.hip", "csrc/backward.hip",
+               "csrc/attend.hip", "csrc/attend_bf16.hip", "csrc/attend_f16.hip", "csrc/attend_f32.hip",
+               "csrc/pages.hip", "csrc/states.hip"]
 
 
 def lib_path() -> str:
@@ -84,8 +86,8 @@ def build_lib() -> str:
     return out
 
 
-def _torch_module(name: str, source: str, hip: bool) -> str:
-    """One torch extension module compiled by g++: ``name`` from ``source``;
+def _torch_module(name: str, sources: list[str], hip: bool) -> str:
+    """One torch extension module compiled by g++: ``name`` from ``sources``;
     with ``hip`` it links libdbs_hip and torch's HIP libraries."""
     import torch
     from torch.utils import cpp_extension as ce
@@ -106,7 +108,7 @@ def _torch_module(name: str, source: str, hip: bool) -> str:
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1",
         f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H",
         *[f"-I{p}" for p in incs], f"-I{py_inc}", f"-I{ROOT}/include", f"-I{ROCM}/include",
-        source, *libs, "-o", out + ".tmp",
+        *sources, *libs, "-o", out + ".tmp",
     ]
     _run(cmd)
     os.replace(out + ".tmp", out)
@@ -115,8 +117,8 @@ def _torch_module(name: str, source: str, hip: bool) -> str:
 
 def build_ext() -> list[str]:
     """The schema owner ``_C`` and the HIP kernels ``_C_hip``."""
-    return [_torch_module("_C", "csrc/torch_schemas.cpp", hip=False),
-            _torch_module("_C_hip", "csrc/torch_ops.cpp", hip=True)]
+    return [_torch_module("_C", ["csrc/torch_schemas.cpp"], hip=False),
+            _torch_module("_C_hip", ["csrc/torch_ops.cpp", "csrc/torch_state.cpp"], hip=True)]
 
 
 def build() -> None:

@@ -1,0 +1,252 @@
+# SPDX-License-Identifier: MIT
+"""A model's state in a search, on the GPU: a paged cache of keys and values,
+the attention that reads it, and dense states in the order of the beams.
+
+A paged cache is one pool of pages per tensor that is cached (keys and values
+of every layer), ``[pages, tokens of a page, ...]``, and one
+:class:`PageTable` for all of them. A step of a search:
+
+1. :func:`fork_pages`: the new beams take over their parents' pages; only a
+   last page that is not full is copied, for all but one of those that continue
+   it;
+2. :func:`extend_pages`: room for the new tokens;
+3. :func:`write_tokens`: their keys and values;
+4. :func:`tree_attention`: their attention over all that is cached, the pages
+   that beams share read once.
+
+:func:`keep_tokens` ends a step of speculative decoding: of a drafted tree,
+whose tokens :func:`tree_attention` verified in one call, the accepted ones
+stay. :func:`reorder_states` is the same for states without pages (recurrent
+states, a short dense cache), with a gradient.
+
+Every call is asynchronous on the current stream and reads nothing back: page
+tables live on the GPU, so the calls can be captured into a graph. The C
+entries are in ``include/beamgrad_state.h``. The reference has no counterpart:
+its step function gathers a model's cache itself (reference
+python/beamgrad/_search.py:100-133, ``BeamState.parents``).
+"""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Sequence
+from typing import NamedTuple
+
+import torch
+
+from ._torch import _ops
+
+
+class PageTable(NamedTuple):
+    """Which pages hold the tokens of ``S`` sequences (of a search: example
+    ``b``'s beam ``k`` is sequence ``b * K + k``)."""
+
+    pages: torch.Tensor  # [S, P] int32, in order; -1 past a sequence's last page
+    lengths: torch.Tensor  # [S] int32: tokens held
+    refs: torch.Tensor  # [pages of the pool] int32: how many sequences hold a page; 0: it is free
+
+    @classmethod
+    def empty(cls, sequences: int, table_pages: int, pool_pages: int, device="cuda") -> PageTable:
+        """The table of sequences that hold nothing yet."""
+        return cls(torch.full((sequences, table_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(sequences, dtype=torch.int32, device=device),
+                   torch.zeros(pool_pages, dtype=torch.int32, device=device))
+
+
+def _tables(table) -> PageTable:
+    if not isinstance(table, PageTable):
+        raise TypeError(f"table must be a beamgrad_amd.PageTable, got {type(table).__name__}")
+    return table
+
+
+def _tensors(name: str, tensors) -> list[torch.Tensor]:
+    tensors = list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a sequence of tensors, got a {type(t).__name__} in it")
+    return tensors
+
+
+def _no_gradient(what: str, tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"beamgrad_amd.{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: PageTable, *,
+                   parents: torch.Tensor | None = None, counts: torch.Tensor | None = None, beams: int = 1,
+                   shared: torch.Tensor | None = None, scale: float | None = None, return_lse: bool = False):
+    """Attention of the last tokens of each sequence over its paged cache.
+
+    ``q`` is ``[S, N, H, D]``, the pools ``k`` and ``v`` ``[pages, tokens of a
+    page, Hkv, D]`` (float32, float16 or bfloat16; ``D`` a multiple of 8 up to
+    256; head ``h`` reads the cache's head ``h // (H // Hkv)``). The last
+    ``counts[s]`` (default: all ``N``) of the ``table.lengths[s]`` cached tokens
+    ask; their keys and values are in the cache already. Each sees the tokens
+    ahead of the asking ones, itself, and
+
+    * the asking tokens before it (a prompt's end, a single token), or
+    * with ``parents`` ``[S, N]``: its ancestors in the drafted tree, node ``i``'s
+      parent being node ``parents[s, i]``, -1 at a root (one that is not
+      an earlier node counts as -1; at most 512 nodes).
+
+    With ``beams`` = K > 1 the sequences come in groups of K beams whose live
+    members (``counts`` > 0) hold the same pages for the whole pages of their
+    first ``shared[b]`` tokens, as :func:`fork_pages` leaves them; these are
+    read once for the group. ``scale`` defaults to ``1 / sqrt(D)``.
+
+    Returns ``[S, N, H, D]`` in ``q``'s type, zeros for rows past ``counts``; with
+    ``return_lse`` also the log of each row's sum of exponentials, float32
+    ``[S, N, H]``, -inf for such rows. Scores, softmax and sums are held in 32
+    bits; 16-bit inputs round each probability to their type. No gradient.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    pages, lengths, _refs = _tables(table)
+    _no_gradient("tree_attention", (q, k, v))
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
+    out, lse = _ops.tree_attention(q, k, v, pages, lengths, parents, counts, beams, shared, scale, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def fork_pages(pools: Sequence[torch.Tensor], table: PageTable, parents: torch.Tensor) -> PageTable:
+    """The table after a step of a search: sequence ``s`` continues sequence
+    ``parents[s]`` (``[S]``, numbers of sequences; negative: it holds nothing).
+
+    Whole pages are shared. A last page that is not full stays with the first
+    sequence that continues its holder; each other one takes a free page and a
+    copy of its tokens, in every pool (written in place). Free pages are taken in order of
+    their number. A sequence that finds none is left with nothing (length 0).
+    """
+    pages, lengths, refs = _tables(table)
+    pools = _tensors("pools", pools)
+    _no_gradient("fork_pages", pools)
+    out = PageTable(*_ops.fork_pages(pools, pages, lengths, refs, parents))
+    torch.autograd.graph.increment_version(pools)
+    return out
+
+
+def extend_pages(table: PageTable, counts: torch.Tensor, page_tokens: int) -> PageTable:
+    """Room for ``counts[s]`` (``[S]``) more tokens in pages of ``page_tokens``.
+
+    Free pages are taken in order of their number, for the sequences in order. A
+    sequence for which the pool or the table has too few keeps its pages and
+    its length: ``new.lengths - table.lengths`` is what each has room for.
+    """
+    pages, lengths, refs = _tables(table)
+    return PageTable(*_ops.extend_pages(pages, lengths, refs, counts, page_tokens))
+
+
+def write_tokens(pools: Sequence[torch.Tensor], news: Sequence[torch.Tensor], table: PageTable,
+                 counts: torch.Tensor | None = None) -> None:
+    """Writes ``news[i]`` (``[S, N, ...]``, a row of pool ``i`` for each token)
+    to the places of the last ``counts[s]`` (default: all ``N``) tokens of each
+    sequence: row ``j`` to the ``j``-th of them."""
+    pages, lengths, _refs = _tables(table)
+    pools, news = _tensors("pools", pools), _tensors("news", news)
+    _no_gradient("write_tokens", pools + news)
+    _ops.write_tokens(pools, news, pages, lengths, counts)
+    torch.autograd.graph.increment_version(pools)
+
+
+def keep_tokens(pools: Sequence[torch.Tensor], table: PageTable, drafted: torch.Tensor, keep: torch.Tensor,
+                kept: torch.Tensor) -> PageTable:
+    """Of the last ``drafted[s]`` tokens of each sequence, those numbered
+    ``keep[s, :kept[s]]`` (``[S, A]``, ascending among the drafted ones; the
+    first number that is not ends the list) stay. They move together, in place in
+    every pool, and the pages that hold no token any more are given back."""
+    pages, lengths, refs = _tables(table)
+    pools = _tensors("pools", pools)
+    _no_gradient("keep_tokens", pools)
+    out = PageTable(*_ops.keep_tokens(pools, pages, lengths, refs, drafted, keep, kept))
+    torch.autograd.graph.increment_version(pools)
+    return out
+
+
+class _Reorder(torch.autograd.Function):
+    """The states in the order of the new beams; the gradient of a state sums
+    over the beams that continue it (:class:`_GatherGrads`)."""
+
+    @staticmethod
+    def forward(parents, *states):
+        return tuple(_ops.reorder_states(states, parents))
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(inputs[0])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        (parents,) = ctx.saved_tensors
+        _refuse_foreign_leaves(ctx)
+        return (None, *_each_type(_GatherGrads, parents, grads))
+
+
+class _GatherGrads(torch.autograd.Function):
+    """The gradient of :class:`_Reorder`, itself differentiable."""
+
+    @staticmethod
+    def forward(parents, *grads):
+        return tuple(_ops.reorder_states_backward(grads, parents))
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(inputs[0])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        (parents,) = ctx.saved_tensors
+        return (None, *_each_type(_Reorder, parents, grads))
+
+
+def _refuse_foreign_leaves(node) -> None:
+    """In a capture: torch hands a leaf's gradient over on the stream that the
+    leaf's accumulator was made on. Where a living graph of another stream holds
+    it, that stream joins the capture and the capture's end ends the process."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    for fn, _ in node.next_functions:
+        leaf = getattr(fn, "variable", None)
+        if leaf is not None and _ops.leaf_of_another_stream(leaf):
+            raise RuntimeError("beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of "
+                               "another stream uses; drop that graph (its outputs and losses) before the capture")
+
+
+def _each_type(fn, parents, grads) -> list[torch.Tensor | None]:
+    """``fn`` over the gradients that there are, one call for each type."""
+    out: list[torch.Tensor | None] = [None] * len(grads)
+    for dtype in {g.dtype for g in grads if g is not None}:
+        at = [i for i, g in enumerate(grads) if g is not None and g.dtype == dtype]
+        for i, g in zip(at, fn.apply(parents, *(grads[i] for i in at)), strict=True):
+            out[i] = g
+    return out
+
+
+def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, *, inplace: bool = False) -> list[torch.Tensor]:
+    """States ``[B, K, ...]`` in the order of the new beams: beam ``k`` of
+    example ``b`` gets the row of beam ``parents[b, k]`` (``[B, K]``, as
+    ``BeamState.parents``), zeros where that is negative. All states move in one
+    launch.
+
+    New tensors are returned, differentiable for float32, float16 and bfloat16:
+    the gradient of a row is the sum over the beams that continue it, in their
+    order and in 32 bits, rounded once. With ``inplace`` the (contiguous)
+    states are overwritten and returned, and rows that stay are not touched.
+    """
+    states = _tensors("states", states)
+    if not isinstance(parents, torch.Tensor):
+        raise TypeError(f"parents must be a torch.Tensor, got {type(parents).__name__}")
+    if inplace:
+        _no_gradient("reorder_states(inplace=True)", states)
+        _ops.reorder_states_(states, parents)
+        torch.autograd.graph.increment_version(states)
+        return states
+    if torch.is_grad_enabled() and any(t.requires_grad for t in states):
+        for t in states:
+            if t.requires_grad and t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise TypeError(f"reorder_states has a gradient for float32, float16 and bfloat16 states, not {t.dtype}")
+        return list(_Reorder.apply(parents, *states))
+    return list(_ops.reorder_states(states, parents))

@@ -112,6 +112,12 @@ int finish(hipStream_t stream, hipError_t e) {
     return status_of(e);
 }
 
+}  // namespace
+
+int dbs_hip::finish_call(hipStream_t stream, hipError_t e) { return finish(stream, e); }
+
+namespace {
+
 // finish() for a decode: when the call synchronises, an overlapped decode
 // whose select pass gave up a wait (fault word set) reports a failed launch;
 // asynchronous callers see it as invalid_input[b] == 2.

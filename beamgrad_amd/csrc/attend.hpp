@@ -1,0 +1,57 @@
+// SPDX-License-Identifier: MIT
+//
+// Attention over a paged cache: internal interface between the C entry
+// (attend.hip) and the kernels (attend_kernels.hpp, one source per data type).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "paged.hpp"
+
+namespace dbs_hip {
+
+constexpr int kAttendThreads = 256;  // four wavefronts
+constexpr int kAttendMaxDim = 256;
+constexpr int kAttendMaxTree = 512;  // drafted tokens with parents
+
+// Tiles of query rows of a workgroup: a wavefront holds kRowBlocks blocks of
+// 16 rows, the four wavefronts lie kRowWaves along the rows and 4 / kRowWaves
+// along the keys.
+enum AttendShape : int { kRows16 = 0, kRows32 = 1, kRows64 = 2, kRows128 = 3, kAttendShapes = 4 };
+constexpr int attend_rows(int shape) { return 16 << shape; }
+
+struct AttendParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t qs, qn, qh;  // strides in bytes
+    int64_t kp, kt, kh;
+    int64_t vp, vt, vh;
+    PageSpan span;
+    const int32_t* pages;
+    const int32_t* lengths;
+    const int32_t* counts;
+    const int32_t* parents;
+    const int32_t* shared;  // null unless beams > 1
+    int32_t S, N, H, Hkv, G, D, K, groups;
+    int32_t shared_tiles;  // row tiles of a group's shared pages, 0 without
+    int32_t own_tiles;     // row tiles of a sequence, at most
+    int32_t items;         // per group: Hkv * (shared_tiles + K * own_tiles)
+    float scale;           // of the scores, times log2(e)
+    void* out;
+    float* lse;
+    // workspace
+    int4* info;      // per item
+    float* partial;  // per slot: [rows][width] sums, [rows] maxima, [rows] totals
+    int32_t grid;    // workgroups
+};
+
+// Workgroups of a CU, and floats of a partial result, of a kernel.
+template <int DTYPE>
+void attend_sizes(int dim, int shape, int& resident, int& slot);
+template <int DTYPE>
+hipError_t launch_attend(const AttendParams& p, int dim, int shape, hipStream_t stream);
+
+}  // namespace dbs_hip

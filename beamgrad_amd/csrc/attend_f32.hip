@@ -1,0 +1,11 @@
+// SPDX-License-Identifier: MIT
+//
+// Attention over a paged cache of float32 keys and values.
+#include "attend_kernels.hpp"
+
+namespace dbs_hip {
+
+template void attend_sizes<0>(int, int, int&, int&);
+template hipError_t launch_attend<0>(const AttendParams&, int, int, hipStream_t);
+
+}  // namespace dbs_hip

@@ -34,6 +34,10 @@ private:
     hipEvent_t stop_ = nullptr;
 };
 
+// The end of an entry point's call on `stream`: the status of its launches,
+// after a synchronisation where one is asked for.
+int finish_call(hipStream_t stream, hipError_t e);
+
 constexpr int kMaxEos = 17;          // eos_token + 16 extra EOS tokens
 constexpr int kRowThreads = 64;      // one wavefront per row in the row pass
 constexpr int kLanes = 256;          // lanes of the fixed logsumexp fold order
