@@ -4,6 +4,7 @@
 // checks, the choice of a kernel, its workspace.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "attend.hpp"
@@ -41,8 +42,10 @@ bool valid_sizes(const BeamgradAttention* a) {
 }
 
 struct Plan {
-    int dim, shape, grid, slot;
-    int64_t items, info_bytes, bytes;
+    int dim, shape;
+    AttendSizes sizes;
+    int batch;  // sequences of a launch
+    int64_t info_bytes, bytes;
 };
 
 int multiprocessors() {
@@ -58,36 +61,41 @@ int multiprocessors() {
 Plan plan_of(const BeamgradAttention& a, AttendParams& p) {
     Plan plan;
     plan.dim = (a.head_dim + 63) / 64 * 64;
-    p.S = a.sequences;
     p.N = a.tokens;
     p.H = a.heads;
     p.Hkv = a.kv_heads;
-    p.G = a.heads / a.kv_heads;
+    p.G = Divider::of(static_cast<uint32_t>(a.heads / a.kv_heads));
     p.D = a.head_dim;
-    p.K = a.shared ? a.beams : 1;
+    // a group whose lengths one workgroup cannot hold reads its shared pages
+    // once for each beam
+    p.K = a.shared && a.beams <= kAttendSequences ? a.beams : 1;
     p.shared = p.K > 1 ? a.shared : nullptr;
-    p.groups = p.S / p.K;
+    plan.batch = std::min(a.sequences, kAttendSequences / p.K * p.K);
     // the smallest tile that takes the rows that read a page together: fewer
     // rows than the tile cost matrix instructions, more read the cache again
-    const int64_t rows = static_cast<int64_t>(p.N) * p.G, together = p.shared ? rows * p.K : rows;
+    const int64_t rows = static_cast<int64_t>(p.N) * p.G.d, together = rows * p.K;
+    p.beam_rows = Divider::of(static_cast<uint32_t>(rows));
     plan.shape = kRows16;
     while (plan.shape < kRows128 && attend_rows(plan.shape) < together) ++plan.shape;
     const int tile = attend_rows(plan.shape);
     p.shared_tiles = p.shared ? static_cast<int>((together + tile - 1) / tile) : 0;
     p.own_tiles = static_cast<int>((rows + tile - 1) / tile);
-    p.items = p.Hkv * (p.shared_tiles + p.K * p.own_tiles);
-    plan.items = static_cast<int64_t>(p.groups) * p.items;
-    int resident = 1;
+    p.head_items = plan.batch / p.K * (p.shared_tiles + p.K * p.own_tiles);
     switch (a.data_type) {
-        case DBS_CUDA_DTYPE_F32: attend_sizes<DBS_CUDA_DTYPE_F32>(plan.dim, plan.shape, resident, plan.slot); break;
-        case DBS_CUDA_DTYPE_F16: attend_sizes<DBS_CUDA_DTYPE_F16>(plan.dim, plan.shape, resident, plan.slot); break;
-        default: attend_sizes<DBS_CUDA_DTYPE_BF16>(plan.dim, plan.shape, resident, plan.slot); break;
+        case DBS_CUDA_DTYPE_F32: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_F32>(plan.dim, plan.shape); break;
+        case DBS_CUDA_DTYPE_F16: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_F16>(plan.dim, plan.shape); break;
+        default: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_BF16>(plan.dim, plan.shape); break;
     }
-    plan.grid = (multiprocessors() * resident + 7) / 8 * 8;
-    p.grid = plan.grid;
-    plan.info_bytes = plan.items * static_cast<int64_t>(sizeof(int4));
-    const int64_t slots = p.shared ? plan.grid + plan.items : 2 * static_cast<int64_t>(plan.grid);
-    plan.bytes = plan.info_bytes + slots * plan.slot * static_cast<int64_t>(sizeof(float));
+    // units in 30 bits, whatever the lengths
+    const double keys = static_cast<double>(a.table_pages) * a.page_tokens;
+    p.unit_shift = 0;
+    while (static_cast<double>(p.head_items) * p.Hkv * (std::ldexp(keys / plan.sizes.keys, -p.unit_shift) + 1.0) > 1.0e9)
+        ++p.unit_shift;
+    p.grid = (multiprocessors() * plan.sizes.resident + 7) / 8 * 8;
+    const int64_t items = static_cast<int64_t>(p.head_items) * p.Hkv;
+    plan.info_bytes = items * static_cast<int64_t>(sizeof(int4));
+    const int64_t slots = p.shared ? p.grid + items : 2 * static_cast<int64_t>(p.grid);
+    plan.bytes = plan.info_bytes + slots * plan.sizes.slot * static_cast<int64_t>(sizeof(float));
     return plan;
 }
 
@@ -129,11 +137,26 @@ DBS_CUDA_EXPORT int beamgrad_tree_attention(const BeamgradAttention* args, void*
     p.info = static_cast<int4*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.info_bytes);
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-    switch (a.data_type) {
-        case DBS_CUDA_DTYPE_F32: return finish_call(stream, launch_attend<DBS_CUDA_DTYPE_F32>(p, plan.dim, plan.shape, stream));
-        case DBS_CUDA_DTYPE_F16: return finish_call(stream, launch_attend<DBS_CUDA_DTYPE_F16>(p, plan.dim, plan.shape, stream));
-        default: return finish_call(stream, launch_attend<DBS_CUDA_DTYPE_BF16>(p, plan.dim, plan.shape, stream));
+    hipError_t e = hipSuccess;
+    for (int s0 = 0; s0 < a.sequences && e == hipSuccess; s0 += plan.batch) {
+        AttendParams b = p;
+        b.S = std::min(plan.batch, a.sequences - s0);
+        const int64_t rows = static_cast<int64_t>(s0) * p.N * p.H;
+        b.q = static_cast<const char*>(p.q) + s0 * p.qs;
+        b.pages += static_cast<int64_t>(s0) * p.span.P;
+        b.lengths += s0;
+        if (b.counts) b.counts += s0;
+        if (b.parents) b.parents += static_cast<int64_t>(s0) * p.N;
+        if (b.shared) b.shared += s0 / p.K;
+        b.out = static_cast<char*>(p.out) + rows * p.D * size;
+        if (b.lse) b.lse += rows;
+        switch (a.data_type) {
+            case DBS_CUDA_DTYPE_F32: e = launch_attend<DBS_CUDA_DTYPE_F32>(b, plan.dim, plan.shape, stream); break;
+            case DBS_CUDA_DTYPE_F16: e = launch_attend<DBS_CUDA_DTYPE_F16>(b, plan.dim, plan.shape, stream); break;
+            default: e = launch_attend<DBS_CUDA_DTYPE_BF16>(b, plan.dim, plan.shape, stream); break;
+        }
     }
+    return finish_call(stream, e);
 }
 
 }  // extern "C"

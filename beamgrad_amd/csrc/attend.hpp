@@ -15,6 +15,7 @@ namespace dbs_hip {
 constexpr int kAttendThreads = 256;  // four wavefronts
 constexpr int kAttendMaxDim = 256;
 constexpr int kAttendMaxTree = 512;  // drafted tokens with parents
+constexpr int kAttendSequences = 256; // of a launch: a thread of each workgroup reads one's length
 
 // Tiles of query rows of a workgroup: a wavefront holds kRowBlocks blocks of
 // 16 rows, the four wavefronts lie kRowWaves along the rows and 4 / kRowWaves
@@ -35,22 +36,27 @@ struct AttendParams {
     const int32_t* counts;
     const int32_t* parents;
     const int32_t* shared;  // null unless beams > 1
-    int32_t S, N, H, Hkv, G, D, K, groups;
+    int32_t S, N, H, Hkv, D, K;
+    Divider G, beam_rows;  // N * G rows of a beam
     int32_t shared_tiles;  // row tiles of a group's shared pages, 0 without
     int32_t own_tiles;     // row tiles of a sequence, at most
-    int32_t items;         // per group: Hkv * (shared_tiles + K * own_tiles)
+    int32_t head_items;    // items of a cache head
+    int32_t unit_shift;    // a unit is the kernel's tile of keys times 2^unit_shift
     float scale;           // of the scores, times log2(e)
     void* out;
     float* lse;
     // workspace
-    int4* info;      // per item
+    int4* info;      // per item of a sequence: its first and last workgroup, whether pages are shared
     float* partial;  // per slot: [rows][width] sums, [rows] maxima, [rows] totals
     int32_t grid;    // workgroups
 };
 
-// Workgroups of a CU, and floats of a partial result, of a kernel.
+// Of a kernel: workgroups of a CU, floats of a partial result, keys of a tile.
+struct AttendSizes {
+    int resident, slot, keys;
+};
 template <int DTYPE>
-void attend_sizes(int dim, int shape, int& resident, int& slot);
+AttendSizes attend_sizes(int dim, int shape);
 template <int DTYPE>
 hipError_t launch_attend(const AttendParams& p, int dim, int shape, hipStream_t stream);
 

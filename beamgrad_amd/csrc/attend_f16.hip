@@ -5,7 +5,7 @@
 
 namespace dbs_hip {
 
-template void attend_sizes<1>(int, int, int&, int&);
+template AttendSizes attend_sizes<1>(int, int);
 template hipError_t launch_attend<1>(const AttendParams&, int, int, hipStream_t);
 
 }  // namespace dbs_hip

@@ -19,8 +19,11 @@
 // from LDS by transposing reads (float32: by plain ones). m is raised only when
 // a tile's maximum passes it by 2^8: sums stay below 2^8 times their number in
 // float32, and most tiles need no rescaling of the sums. P is rounded to the
-// operands' 16 bits for the matrix instruction (float32 inputs: not at all); l
-// sums the unrounded values.
+// operands' 16 bits for the matrix instruction (float32 inputs: not at all). The
+// result is divided by the sum of the rounded values, in 32 bits, by one more
+// matrix instruction with a row of ones: vector instructions are what bounds a
+// tile of many rows, and a weighted mean of rounded weights has no error where the
+// values are equal. The log-sum that a caller asks for is the unrounded values'.
 #pragma once
 
 #include "attend.hpp"
@@ -88,6 +91,16 @@ struct Dims {
     static constexpr int kKeyBlocks = kKeys / 16;
     static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
     static constexpr int kRowBytes = kChunks * 16;
+    // Of values, a lane's operand of a matrix step: eight of the 16-bit types, one
+    // of float32.
+    static constexpr int kFrag = k32 ? 1 : 8;
+    using Frag = typename Elem<DTYPE>::Frag;
+    static __device__ __forceinline__ f32x4 value_mma(const Frag& a, const Frag& b, f32x4 c) {
+        if constexpr (k32)
+            return __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], b[0], c, 0, 0, 0);
+        else
+            return Elem<DTYPE>::mma(a, b, c);
+    }
     static constexpr int kSteps = kChunks / 4;  // matrix steps of a key block's scores
     static constexpr int kDimBlocks = DP / 16;
     static constexpr int kRegion = kKeys * kRowBytes;  // of keys or values of a wavefront's tile
@@ -95,14 +108,19 @@ struct Dims {
     // Chunk c of row r lies at c ^ (r & kSwizzle): reads of one chunk of many
     // rows meet different banks.
     static constexpr int kSwizzle = kChunks % 16 == 0 ? 15 : 7;
-    static constexpr int kTile = 2 * kKeyWaves * kRegion;
+    // Tiles shared by wavefronts have two places: one is filled while the other
+    // is used. A wavefront's own tile has one: the CU's other wavefronts use theirs
+    // meanwhile.
+    static constexpr int kPlaces = kRowWaves > 1 && 4 * kKeyWaves * kRegion <= 136 * 1024 ? 2 : 1;
+    static constexpr int kTile = 2 * kKeyWaves * kRegion;  // keys and values
     static constexpr int kAccs = kDimBlocks * kRowBlocks;
     static constexpr int kMerge = kKeyWaves > 1 ? kAccs * 4 * 64 * 16 : 0;
-    static constexpr int kLds = kTile > kMerge ? kTile : kMerge;
+    static constexpr int kLds = kPlaces * kTile > kMerge ? kPlaces * kTile : kMerge;
     static constexpr int kTokens = kRows;  // of a tile of rows, at most
-    static constexpr int kSlot = kRows * (DP + 2);  // floats of a partial result
-    // workgroups of a CU: what its 160 KB of LDS hold, at most 4
-    static constexpr int kFit = (160 * 1024) / (kLds + kTokens * (kAttendMaxTree / 8) + 2 * kAttendMaxTree + 8 * kKeyWaves * kRows);
+    static constexpr int kSlot = kRows * (DP + 3);  // floats of a partial result
+    // workgroups of a CU: what its 160 KB of LDS hold
+    static constexpr int kOther = kTokens * (kAttendMaxTree / 8) + 2 * kAttendMaxTree + 12 * kKeyWaves * kRows + 20 * kAttendSequences + 64;
+    static constexpr int kFit = 160 * 1024 / (kLds + kOther);
     static constexpr int kResident = kFit >= 2 ? 2 : 1;
 };
 
@@ -110,7 +128,7 @@ struct Dims {
 // leaves at most two: of the item it starts in the middle of, and of the item
 // it does not finish. With them every piece leaves one: workgroup + item grows
 // from piece to piece along the line, so no two have the same.
-__device__ __forceinline__ int64_t slot_of(const AttendParams& p, int64_t workgroup, int item, bool starts) {
+__device__ __forceinline__ int64_t slot_of(const AttendParams& p, int workgroup, int item, bool starts) {
     return p.shared ? workgroup + item : 2 * workgroup + (starts ? 1 : 0);
 }
 
@@ -119,15 +137,64 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
     return static_cast<int64_t>((static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo));
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
-    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+// The kernel's arguments, read again: what a phase of the kernel needs of them
+// is not held in scalar registers over the others, where the loop over the keys
+// has none to spare.
+__device__ __forceinline__ const AttendParams& arguments() {
+    auto at = (const __attribute__((address_space(4))) AttendParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const AttendParams*)at;
 }
+
+// x, of which the compiler knows nothing: what is computed from it stays where it
+// is used, in the branches that are rarely taken, and takes no registers elsewhere.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Waits for loads and LDS operations, which the compiler knows of and moves no
+// access of memory over.
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_all() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The maximum over the four lanes that hold a query: lanes 32 apart, then 16.
+__device__ __forceinline__ float quad_max(float x) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+    const auto half = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t low = half[0], high = half[1];
+    x = fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+    const uint32_t both = __builtin_bit_cast(uint32_t, x);
+    const auto row = __builtin_amdgcn_permlane16_swap(both, both, false, false);
+    const uint32_t even = row[0], odd = row[1];
+    return fmaxf(__builtin_bit_cast(float, even), __builtin_bit_cast(float, odd));
+}
+
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// The sum over the lanes up to each one.
+__device__ __forceinline__ int wave_upto(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return x;
+}
+
 // ---------------------------------------------------------------------------
-// Sequences, groups and their units
+// Sequences and their units
 // ---------------------------------------------------------------------------
 
 struct Sequence {
@@ -142,61 +209,94 @@ __device__ __forceinline__ Sequence sequence(const AttendParams& p, int s) {
     return {length, count};
 }
 
-// Tokens that the beams of a group share, in whole pages.
-__device__ __forceinline__ int shared_tokens(const AttendParams& p, int group, int& leader) {
-    leader = -1;
-    if (!p.shared) return 0;
-    int least = INT32_MAX;
-    for (int k = p.K - 1; k >= 0; --k) {
-        const Sequence s = sequence(p, group * p.K + k);
-        if (s.count > 0) {
-            least = min(least, s.prefix());
-            leader = group * p.K + k;
-        }
-    }
-    if (leader < 0) return 0;
-    const int n = min(max(p.shared[group], 0), least);
-    return static_cast<int>(p.span.page.quotient(n) * p.span.page.d);
-}
-
 // The keys that row tile `tile` of a sequence has to read end here: all of
 // them with a tree; in a chain, those up to its last token's.
 template <int ROWS>
 __device__ __forceinline__ int key_end(const AttendParams& p, const Sequence& s, int tile) {
     if (p.parents) return s.length;
-    return s.prefix() + min(s.count, ((tile + 1) * ROWS - 1) / p.G + 1);
+    return s.prefix() + min(s.count, static_cast<int>(p.G.quotient((tile + 1) * ROWS - 1)) + 1);
 }
 
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int64_t own_units(const AttendParams& p, const Sequence& s, int from) {
-    const int tiles = (s.count * p.G + ROWS - 1) / ROWS;
-    if (p.parents || tiles == 1) return static_cast<int64_t>(tiles) * ((s.length - from + KEYS - 1) / KEYS);
-    int64_t units = 0;
-    for (int t = 0; t < tiles; ++t) units += (key_end<ROWS>(p, s, t) - from + KEYS - 1) / KEYS;
-    return units;
+__device__ __forceinline__ int row_tiles(const AttendParams& p, const Sequence& s, int rows) {
+    return (s.count * static_cast<int>(p.G.d) + rows - 1) / rows;
 }
 
-struct Group {
-    int shared, leader;
-    int64_t head_units; // of one cache head
+// What a workgroup knows of the call's sequences.
+struct Board {
+    int length[kAttendSequences], count[kAttendSequences];
+    int first[kAttendSequences];   // a cache head's units ahead of the sequence's (and its group's shared ones)
+    int shared[kAttendSequences];  // of a group: tokens in pages that its beams share
+    int leader[kAttendSequences];  // of a group: a live sequence
+    int sum[4], items[4], largest[4];
 };
 
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Group group_of(const AttendParams& p, int group) {
-    Group g;
-    g.shared = shared_tokens(p, group, g.leader);
-    g.head_units = static_cast<int64_t>(p.shared_tiles) * ((g.shared + KEYS - 1) / KEYS);
-    for (int k = 0; k < p.K; ++k) {
-        const Sequence s = sequence(p, group * p.K + k);
-        if (s.count > 0) g.head_units += own_units<ROWS, KEYS>(p, s, g.shared);
-    }
-    return g;
-}
+struct Totals {
+    int units, items, largest;  // of a cache head; the largest item's units
+};
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+// Fills the board. Sequence s is thread s's.
+template <int ROWS>
+__device__ __forceinline__ Totals fill_board(const AttendParams& p, Board& b, int unit_log) {
+    const int s = threadIdx.x, unit = 1 << unit_log;
+    Sequence me{0, 0};
+    if (s < p.S) me = sequence(p, s);
+    b.length[s] = me.length;
+    b.count[s] = me.count;
+    int units = 0, from = 0, items = 0, largest = 0;
+    if (p.shared) {
+        const int group = s / p.K, groups = p.S / p.K;
+        const int want = s < groups ? p.shared[s] : 0;
+        b.shared[s] = INT32_MAX;
+        b.leader[s] = INT32_MAX;
+        __syncthreads();
+        if (me.count > 0) {
+            atomicMin(&b.shared[group], me.prefix());
+            atomicMin(&b.leader[group], s);
+        }
+        __syncthreads();
+        if (s < groups) {
+            const int n = b.leader[s] == INT32_MAX ? 0 : min(max(want, 0), b.shared[s]);
+            b.shared[s] = static_cast<int>(p.span.page.quotient(n) * p.span.page.d);
+        }
+        __syncthreads();
+        if (s < p.S) from = b.shared[group];
+        if (s < p.S && s == group * p.K && from > 0) {
+            largest = (from + unit - 1) >> unit_log;
+            items = p.shared_tiles;
+            units = items * largest;
+        }
+    }
+    if (me.count > 0) {
+        const int tiles = row_tiles(p, me, ROWS);
+        items += tiles;
+        largest = max(largest, (me.length - from + unit - 1) >> unit_log);
+        if (p.parents || tiles == 1)
+            units += tiles * ((me.length - from + unit - 1) >> unit_log);
+        else
+            for (int t = 0; t < tiles; ++t) units += (key_end<ROWS>(p, me, t) - from + unit - 1) >> unit_log;
+    }
+    const int upto = wave_upto(units), wave = s >> 6;
+    items = wave_upto(items);
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x += shfl64(x, (threadIdx.x & 63) ^ off);
-    return x;
+    for (int d = 1; d < 64; d <<= 1) largest = max(largest, __shfl_xor(largest, d));
+    if ((s & 63) == 63) {
+        b.sum[wave] = upto;
+        b.items[wave] = items;
+        b.largest[wave] = largest;
+    }
+    __syncthreads();
+    Totals total{0, 0, 0};
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += b.sum[w];
+        total.units += b.sum[w];
+        total.items += b.items[w];
+        total.largest = max(total.largest, b.largest[w]);
+    }
+    b.first[s] = before + upto - units;
+    __syncthreads();
+    return {uniform(total.units), uniform(total.items), uniform(total.largest)};
 }
 
 // ---------------------------------------------------------------------------
@@ -217,7 +317,7 @@ struct Piece {
 };
 
 template <int DTYPE, int DP, int SHAPE>
-__global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)) void attend_kernel(const AttendParams p) {
+__global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)) void attend_kernel(const AttendParams) {
     using E = Elem<DTYPE>;
     using T = typename E::T;
     using Frag = typename E::Frag;
@@ -228,113 +328,133 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     constexpr float kInf = __builtin_inff();
 
     __shared__ __attribute__((aligned(1024))) char lds[X::kLds];
-    __shared__ float stats[2][WK][ROWS];
+    __shared__ float stats[3][WK][ROWS];
     __shared__ uint32_t sees[X::kTokens * (kAttendMaxTree / 32)];
     __shared__ int16_t up[kAttendMaxTree];
+    __shared__ Board board;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int quad = lane >> 4, col = lane & 15;
     const int wr = wave % WR, wk = wave / WR;
 
+    const AttendParams& p0 = arguments();
     // this workgroup's stretch of the units
-    int64_t total = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 64)
-        total += wave_sum64(g0 + lane < p.groups ? group_of<ROWS, KEYS>(p, g0 + lane).head_units * p.Hkv : 0);
-    total = uniform64(total);
-    int64_t each = (total + p.grid - 1) / p.grid;
-    each = (max(each, int64_t{1}) + WK - 1) / WK * WK;
-    // neighbours share keys, so they lie on one XCD: workgroups go round the
-    // eight of them
-    const int64_t busy = (total + each - 1) / each, per_xcd = (busy + 7) / 8;
-    const int64_t mine = static_cast<int64_t>(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per_xcd || mine >= busy) return;
-    int64_t at = mine * each;
-    const int64_t stop = min(at + each, total);
-
-    // the group it starts in
-    int group = 0;
-    int64_t base = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 64) {
-        const int64_t units = g0 + lane < p.groups ? group_of<ROWS, KEYS>(p, g0 + lane).head_units * p.Hkv : 0;
-        int64_t upto = units;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t before = shfl64(upto, max(lane - off, 0));
-            if (lane >= off) upto += before;
-        }
-        const uint64_t past = __ballot(base + upto > at);
-        if (past) {
-            const int first = __builtin_ctzll(past);
-            group = g0 + first;
-            base = uniform64(base + shfl64(upto - units, first));
-            break;
-        }
-        base = uniform64(base + shfl64(upto, 63));
+    constexpr int kKeyLog = KEYS == 64 ? 6 : KEYS == 32 ? 5 : 4;
+    const int unit_log = kKeyLog + p0.unit_shift, unit = 1 << unit_log;
+    const Totals board_totals = fill_board<ROWS>(p0, board, unit_log);
+    const int head_units = board_totals.units, total = head_units * p0.Hkv;
+    int each = (total + p0.grid - 1) / p0.grid;
+    each = (max(each, 1) + WK - 1) / WK * WK;
+    // Many items, none of them larger than a stretch: a workgroup for each whole
+    // one, no pieces to join, and the hardware hands them out as workgroups end.
+    const bool whole_items = WR > 1 && !p0.shared && board_totals.items * p0.Hkv >= 2 * p0.grid && board_totals.largest <= each;
+    int mine, at, stop;
+    Piece chosen;
+    if (whole_items) {
+        // those with the most keys first; the tiles of a sequence and head are a
+        // multiple of eight workgroups apart, so that one XCD reads its keys
+        const int pairs = (p0.S * p0.Hkv + 7) / 8 * 8;
+        const int row = static_cast<int>(blockIdx.x) / pairs, pair = static_cast<int>(blockIdx.x) - row * pairs;
+        chosen.tile = p0.own_tiles - 1 - row;
+        chosen.seq = pair / p0.Hkv;
+        chosen.head = pair - chosen.seq * p0.Hkv;
+        if (chosen.tile < 0 || chosen.seq >= p0.S) return;
+        chosen.own = {uniform(board.length[chosen.seq]), uniform(board.count[chosen.seq])};
+        if (chosen.tile >= row_tiles(p0, chosen.own, ROWS)) return;
+        mine = 0, at = 0, stop = 1;
+    } else {
+        // neighbours share keys, so they lie on one XCD: workgroups go round the
+        // eight of them
+        const int busy = (total + each - 1) / each, per_xcd = (busy + 7) / 8;
+        mine = static_cast<int>(blockIdx.x & 7) * per_xcd + static_cast<int>(blockIdx.x >> 3);
+        if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || mine >= busy) return;
+        at = mine * each;
+        stop = min(at + each, total);
     }
 
     while (at < stop) {
-        Group g = group_of<ROWS, KEYS>(p, group);
-        g.head_units = uniform64(g.head_units);
-        while (at - base >= g.head_units * p.Hkv) {
-            base += g.head_units * p.Hkv;
-            g = group_of<ROWS, KEYS>(p, ++group);
-            g.head_units = uniform64(g.head_units);
-        }
+        const AttendParams& p1 = arguments();
         // the item at `at`, and the piece of it in the stretch
         Piece w;
-        int64_t start = at - base;  // first in the group, then the item's first unit
-        w.head = static_cast<int>(start / g.head_units);
-        int64_t off = start - w.head * g.head_units;  // within the head, then within the item
-        const int head_item = group * p.items + w.head * (p.shared_tiles + p.K * p.own_tiles);
-        int64_t units;
-        const int shared_units = (g.shared + KEYS - 1) / KEYS;
-        int from = 0, end;
-        if (off < static_cast<int64_t>(p.shared_tiles) * shared_units) {
-            w.shared = true;
-            w.tile = static_cast<int>(off / shared_units);
-            off -= static_cast<int64_t>(w.tile) * shared_units;
-            units = shared_units;
-            end = g.shared;
-            w.seq = g.leader;
-            w.own = sequence(p, w.seq);
-            w.item = head_item + w.tile;
-        } else {
+        int group = 0;
+        if (whole_items) {
+            w = chosen;
+            w.key0 = 0;
+            w.end = key_end<ROWS>(p1, w.own, w.tile);
+            w.item = w.head * p1.head_items + w.seq * p1.own_tiles + w.tile;
             w.shared = false;
-            off -= static_cast<int64_t>(p.shared_tiles) * shared_units;
-            from = g.shared;
-            int k = 0;
-            for (;; ++k) {
-                w.own = sequence(p, group * p.K + k);
-                const int64_t u = w.own.count > 0 ? own_units<ROWS, KEYS>(p, w.own, from) : 0;
-                if (off < u) break;
-                off -= u;
-            }
-            w.seq = group * p.K + k;
-            for (w.tile = 0;; ++w.tile) {
-                end = key_end<ROWS>(p, w.own, w.tile);
-                units = (end - from + KEYS - 1) / KEYS;
-                if (off < units) break;
-                off -= units;
-            }
-            w.item = head_item + p.shared_tiles + k * p.own_tiles + w.tile;
+            w.starts = w.whole = true;
+            if (threadIdx.x == 0) p1.info[w.item] = make_int4(0, 0, 0, 0);
+            at = stop;
+        } else {
+        w.head = at / head_units;
+        int off = at - w.head * head_units;  // in the head, then in the sequence, then in the item
+        int seq = -1;
+        for (int s0 = 0; s0 < p1.S; s0 += 64) {
+            const bool ahead = s0 + lane < p1.S && board.first[s0 + lane] <= off;
+            seq += __popcll(__ballot(ahead));
         }
-        off = uniform64(off);
-        units = uniform64(units);
-        w.seq = uniform(w.seq);
+        off -= uniform(board.first[seq]);
+        group = p1.shared ? seq / p1.K : seq;
+        const int from = p1.shared ? uniform(board.shared[group]) : 0;
+        int units = (from + unit - 1) >> unit_log, end = from;
+        int place_in_head = group * (p1.shared_tiles + p1.K * p1.own_tiles);
+        w.shared = p1.shared && seq == group * p1.K && off < p1.shared_tiles * units;
+        if (w.shared) {
+            w.tile = off / units;
+            off -= w.tile * units;
+            w.seq = uniform(board.leader[group]);
+            w.own = {uniform(board.length[w.seq]), uniform(board.count[w.seq])};
+            w.key0 = 0;
+            place_in_head += w.tile;
+        } else {
+            if (p1.shared && seq == group * p1.K) off -= p1.shared_tiles * units;
+            w.seq = seq;
+            w.own = {uniform(board.length[seq]), uniform(board.count[seq])};
+            w.key0 = from;
+            if (p1.parents || row_tiles(p1, w.own, ROWS) == 1) {
+                end = w.own.length;
+                units = (end - from + unit - 1) >> unit_log;
+                w.tile = off / units;
+                off -= w.tile * units;
+            } else {
+                // tiles of rows that read ever more keys: a lane for each
+                for (w.tile = 0;; w.tile += 64) {
+                    const int t = w.tile + lane;
+                    const int mine_end = key_end<ROWS>(p1, w.own, t);
+                    const int n = t < p1.own_tiles ? (mine_end - from + unit - 1) >> unit_log : 0;
+                    const int upto = wave_upto(n);
+                    const uint64_t past = __ballot(upto > off);
+                    if (past) {
+                        const int first = __builtin_ctzll(past);
+                        w.tile += first;
+                        units = __shfl(n, first);
+                        off -= __shfl(upto, first) - units;
+                        end = __shfl(mine_end, first);
+                        break;
+                    }
+                    off -= __shfl(upto, 63);
+                }
+            }
+            place_in_head += p1.shared_tiles + (seq - group * p1.K) * p1.own_tiles + w.tile;
+        }
+        off = uniform(off);
+        units = uniform(units);
+        end = uniform(end);
         w.tile = uniform(w.tile);
-        w.item = uniform(w.item);
-        start = at - off;
-        const int64_t until = min(start + units, stop);
-        w.key0 = uniform(from + static_cast<int>(off) * KEYS);
-        w.end = uniform(min(end, from + static_cast<int>(until - start) * KEYS));
-        w.starts = at == start;
-        w.whole = w.starts && until == start + units && !(p.shared && g.shared > 0);
+        w.item = uniform(w.head * p1.head_items + place_in_head);
+        const int start = at - off, until = min(start + units, stop);
+        w.end = min(end, w.key0 + ((until - start) << unit_log));
+        w.key0 += off << unit_log;
+        w.starts = off == 0;
+        w.whole = w.starts && until == start + units && from == 0;
         if (w.starts && threadIdx.x == 0)
-            p.info[w.item] = make_int4(static_cast<int>(mine), static_cast<int>((start + units - 1) / each),
-                                       g.shared > 0, 0);
+            p1.info[w.item] = make_int4(mine, (start + units - 1) / each, from > 0, 0);
         at = until;
+        }
 
         // ---- the piece's rows ----
+        const AttendParams& p = arguments();
         const int prefix = w.own.prefix();
         int token[RB];     // of the sequence's asking tokens
         int64_t place[RB]; // of the row in out and lse, in rows; -1: no such row
@@ -344,12 +464,12 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
             int r = w.tile * ROWS + (wr * RB + rb) * 16 + col;
             int seq = w.seq, count = w.own.count;
             if (w.shared) {
-                const int beam = r / (p.N * p.G);
-                r -= beam * p.N * p.G;
+                const int beam = static_cast<int>(p.beam_rows.quotient(r));
+                r -= beam * static_cast<int>(p.beam_rows.d);
                 seq = group * p.K + beam;
-                count = beam < p.K ? sequence(p, seq).count : 0;
+                count = beam < p.K ? board.count[seq] : 0;
             }
-            const int n = r / p.G, h = w.head * p.G + (r - n * p.G);
+            const int G = static_cast<int>(p.G.d), n = static_cast<int>(p.G.quotient(r)), h = w.head * G + (r - n * G);
             token[rb] = n;
             const bool row = n < count;
             place[rb] = row ? (static_cast<int64_t>(seq) * p.N + n) * p.H + h : -1;
@@ -362,7 +482,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         }
         // keys before this are seen by every row of the tile
         int masked_from = INT32_MAX;
-        const int first_token = w.tile * ROWS / p.G;
+        const int first_token = static_cast<int>(p.G.quotient(w.tile * ROWS));
         if (!w.shared) masked_from = prefix + (p.parents ? 0 : first_token + 1);
         const int words = (p.N + 31) >> 5;
         if (p.parents && w.end > masked_from) {
@@ -384,58 +504,115 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         }
 
         // ---- over the keys ----
-        char* const k_lds = lds + wk * X::kRegion;
-        char* const v_lds = lds + (WK + wk) * X::kRegion;
         const char* const k_head = static_cast<const char*>(p.k) + w.head * p.kh;
         const char* const v_head = static_cast<const char*>(p.v) + w.head * p.vh;
         const int32_t* const row_pages = p.pages + static_cast<int64_t>(w.seq) * p.span.P;
         const int chunks = p.D * X::kSize / 16;
 
+        const float scale = p.scale;
         f32x4 o[DB][RB];
         float m[RB], l[RB];
+        f32x4 sum_l[RB];  // 16-bit types: the sum of the rounded values, once for every row
+        const bool with_lse = p.lse != nullptr;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             m[rb] = -kInf;
             l[rb] = 0.0f;
+            sum_l[rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        const int rounds = (w.end - w.key0 + WK * KEYS - 1) / (WK * KEYS);
-        for (int round = 0; round < rounds; ++round) {
-            const int first = w.key0 + (round * WK + wk) * KEYS;
-            if (WR == 1 && first >= w.end) break;  // no barriers below
-            // the places of this tile's tokens: lane i has token first + i
-            int64_t k_at = -1, v_at = -1;
-            if (lane < KEYS && first + lane < w.end) {
-                const uint32_t page = p.span.page.quotient(first + lane);
-                const uint32_t in = first + lane - page * p.span.page.d;
-                const int32_t entry = row_pages[page];
-                if (p.span.is_page(entry)) {
-                    k_at = entry * p.kp + in * p.kt;
-                    v_at = entry * p.vp + in * p.vt;
-                }
-            }
-            const uint64_t there = __ballot(k_at >= 0);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (WR > 1) __syncthreads();
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
+        // The page-table entry of token first + lane of a tile, read well before
+        // it is needed; then the place that it gives, -1 without a page.
+        int32_t entry = -1;
+        const auto look_up = [&](int first) {
+            entry = -1;
+            if (lane < KEYS && first + lane < w.end) entry = row_pages[p.span.page.quotient(first + lane)];
+        };
+        int64_t k_at, v_at;
+        const auto locate = [&](int first) {
+            const uint32_t token = first + lane, in = token - p.span.page.quotient(token) * p.span.page.d;
+            const bool there = p.span.is_page(entry);
+            k_at = there ? static_cast<int64_t>(entry) * p.kp + static_cast<int64_t>(in) * p.kt : -1;
+            v_at = there ? static_cast<int64_t>(entry) * p.vp + static_cast<int64_t>(in) * p.vt : -1;
+            return __ballot(there);
+        };
+        // this wavefront's share of a tile, from memory straight into LDS
+        constexpr uint64_t kFull = KEYS == 64 ? ~uint64_t{0} : (uint64_t{1} << KEYS) - 1;
+        const auto fill = [&](char* region, const char* head, int64_t mine_at, uint64_t there) {
+            if (there == kFull) {
 #pragma unroll
                 for (int i = 0; i < X::kLoads; ++i) {
                     const int block = i * WR + wr;  // of 64 chunks
                     const int c = block * 64 + lane, row = c / X::kChunks, chunk = (c % X::kChunks) ^ (row & X::kSwizzle);
-                    const int64_t from_row = shfl64(kv ? v_at : k_at, row);
-                    char* const to = (kv ? v_lds : k_lds) + block * 1024;
-                    if (from_row >= 0 && chunk < chunks)
-                        __builtin_amdgcn_global_load_lds((global_char*)((kv ? v_head : k_head) + from_row + chunk * 16),
-                                                         (lds_char*)to, 16, 0, 0);
-                    else  // what no token fills must not be a NaN or an infinity
-                        *reinterpret_cast<f32x4*>(to + lane * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const char* const from = head + shfl64(mine_at, row) + chunk * 16;
+                    if (chunks == X::kChunks || chunk < chunks)
+                        __builtin_amdgcn_global_load_lds((global_char*)from, (lds_char*)(region + block * 1024), 16, 0, 0);
                 }
+                return;
             }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            if (WR > 1) __syncthreads();
+            const int lane_here = opaque(lane);
+#pragma unroll
+            for (int i = 0; i < X::kLoads; ++i) {
+                const int block = i * WR + wr;
+                const int c = block * 64 + lane_here, row = c / X::kChunks, chunk = (c % X::kChunks) ^ (row & X::kSwizzle);
+                const int64_t row_at = shfl64(mine_at, row);
+                char* const to = region + block * 1024;
+                if (row_at < 0)  // what no token fills must not be a NaN or an infinity
+                    *reinterpret_cast<f32x4*>(to + lane_here * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                else if (chunk < chunks)
+                    __builtin_amdgcn_global_load_lds((global_char*)(head + row_at + chunk * 16), (lds_char*)to, 16, 0, 0);
+            }
+        };
+        const auto region = [&](int round, int value) {
+            return lds + (X::kPlaces == 2 ? (round & 1) * X::kTile : 0) + (value * WK + wk) * X::kRegion;
+        };
+
+        const int rounds = (w.end - w.key0 + WK * KEYS - 1) / (WK * KEYS);
+        uint64_t there_next = 0;
+        look_up(w.key0 + wk * KEYS);
+        __syncthreads();  // the last piece's tiles are done with
+        if (chunks < X::kChunks) {
+            // the columns past the width are zeros in every tile
+            for (int i = threadIdx.x; i < X::kPlaces * X::kTile / 16; i += kAttendThreads)
+                reinterpret_cast<f32x4*>(lds)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            __syncthreads();
+        }
+        if constexpr (X::kPlaces == 2) {
+            there_next = locate(w.key0 + wk * KEYS);
+            look_up(w.key0 + (WK + wk) * KEYS);
+            fill(region(0, 0), k_head, k_at, there_next);
+            fill(region(0, 1), v_head, v_at, there_next);
+        }
+        for (int round = 0; round < rounds; ++round) {
+            const int first = w.key0 + (round * WK + wk) * KEYS;
+            if (WR == 1 && first >= w.end) break;  // no barriers below
+            uint64_t there;
+            char* const k_lds = region(round, 0);
+            char* const v_lds = region(round, 1);
+            if constexpr (X::kPlaces == 2) {
+                there = there_next;
+                // this tile has come, for all wavefronts, and all have done with the
+                // one before it, whose place the next one takes
+                wait_all();
+                barrier();
+                if (round + 1 < rounds) {
+                    there_next = locate(first + WK * KEYS);
+                    look_up(first + 2 * WK * KEYS);
+                    fill(region(round + 1, 0), k_head, k_at, there_next);
+                    fill(region(round + 1, 1), v_head, v_at, there_next);
+                }
+            } else {
+                there = locate(first);
+                look_up(first + WK * KEYS);
+                wait_lds();
+                if (WR > 1) barrier();
+                fill(k_lds, k_head, k_at, there);
+                fill(v_lds, v_head, v_at, there);
+                wait_all();
+                if (WR > 1) barrier();
+            }
 
             // scores: s[kb][rb][i] of key 16 kb + 4 quad + i and row col of block rb
             f32x4 s[KB][RB];
@@ -452,29 +629,35 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     for (int rb = 0; rb < RB; ++rb) s[kb][rb] = E::mma(a, q[rb][i], s[kb][rb]);
                 }
             }
-            const bool masked = there != (KEYS == 64 ? ~uint64_t{0} : (uint64_t{1} << KEYS) - 1) ||
-                                first + KEYS > masked_from;
+            const bool masked = there != kFull || first + KEYS > masked_from;
             if (masked) {
+                const int q4 = opaque(quad * 4);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb) {
+                    // the lane's four keys of the block: without a page, or hidden
+                    const uint32_t page = static_cast<uint32_t>(there >> (kb * 16 + q4));
+                    const int drafted = first + kb * 16 + q4 - prefix;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = kb * 16 + quad * 4 + i;
-                        const bool in = (there >> key) & 1;
-                        const int drafted = first + key - prefix;
-#pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            bool seen = in;
-                            if (in && first + key >= masked_from) {
-                                if (p.parents)
-                                    seen = token[rb] < p.N &&
-                                           ((sees[(token[rb] - first_token) * words + (drafted >> 5)] >> (drafted & 31)) & 1);
-                                else
-                                    seen = drafted <= token[rb];
+                    for (int rb = 0; rb < RB; ++rb) {
+                        uint32_t seen = 15;
+                        if (first + KEYS > masked_from) {
+                            if (p.parents) {
+                                // four bits of the token's row from `drafted` on, those
+                                // before the first drafted token set
+                                const int in = max(drafted, 0), at = min(in >> 5, words - 1), row = min(token[rb] - first_token, X::kTokens - 1) * words;
+                                const uint64_t two = sees[row + at] | static_cast<uint64_t>(at + 1 < words ? sees[row + at + 1] : 0) << 32;
+                                const uint32_t bits = in < p.N ? static_cast<uint32_t>(two >> (in & 31)) : 0;
+                                seen = drafted >= 0 ? bits : drafted <= -4 ? 15 : bits << -drafted | ((1u << -drafted) - 1);
+                            } else {
+                                const int n = token[rb] - drafted + 1;  // of them are seen
+                                seen = n >= 4 ? 15 : n <= 0 ? 0 : (1u << n) - 1;
                             }
-                            if (!seen) s[kb][rb][i] = -kInf;
                         }
+                        seen &= page;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kb][rb][i] = (seen >> i) & 1 ? s[kb][rb][i] : -kInf;
                     }
+                }
             }
             // the maximum, raised where a tile's passes it by 2^8
 #pragma unroll
@@ -484,122 +667,122 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kb][rb][i]);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const bool raise = (m[rb] == -kInf && top > -kInf) || (top - m[rb]) * p.scale > 8.0f;
+                top = quad_max(top);
+                const bool raise = (m[rb] == -kInf && top > -kInf) || (top - m[rb]) * scale > 8.0f;
                 if (__any(raise)) {
                     const float next = raise ? top : m[rb];
                     // nothing seen yet: the sums are zero
-                    const float by = !raise ? 1.0f : m[rb] == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m[rb] - next) * p.scale);
+                    const float by = !raise ? 1.0f : m[rb] == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m[rb] - next) * scale);
                     m[rb] = next;
                     l[rb] *= by;
+                    sum_l[rb] *= by;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db][rb] *= by;
                 }
-                const float shift = m[rb] == -kInf ? 0.0f : -m[rb] * p.scale;
+                const float shift = m[rb] == -kInf ? 0.0f : -m[rb] * scale;
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][rb][i], p.scale, shift));
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][rb][i], scale, shift));
                         s[kb][rb][i] = e;
-                        l[rb] += e;
                     }
-            }
-            // A value that is no number or infinite, of a token that some rows
-            // of the tile do not see, must not reach them as 0 * inf.
-            bool careful = false;
-            if (masked && first + KEYS > masked_from) {
-                bool odd = false;
-                for (int c = lane; c < KEYS * X::kChunks; c += 64) {
-                    const Frag x = *reinterpret_cast<const Frag*>(v_lds + c * 16);
-#pragma unroll
-                    for (int e = 0; e < 16 / X::kSize; ++e) {
-                        const float f = static_cast<float>(x[e]);
-                        odd |= !(__builtin_fabsf(f) < kInf);
-                    }
-                }
-                careful = __any(odd);
-            }
-            if (!careful) {
-                if constexpr (X::k32) {
+                if (X::k32 || with_lse) {
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int row = kb * 16 + quad * 4 + i;
+                        for (int i = 0; i < 4; ++i) l[rb] += s[kb][rb][i];
+                }
+            }
+            // A value that is no number or infinite, of a token that some rows of
+            // the tile do not see, must not reach them as 0 * inf: such values are
+            // taken out, and reach the rows whose probability is above 0 by a
+            // product with where they are.
+            const bool hidden = first + KEYS > masked_from;
+            const auto accumulate = [&](Frag a, const Frag* pr, f32x4* to) {
+                if (hidden) {
+                    bool odd = false;
+                    Frag up, down;
 #pragma unroll
-                            for (int db = 0; db < DB; ++db) {
-                                const float a = *reinterpret_cast<const float*>(
-                                    v_lds + row * X::kRowBytes + ((db * 4 + (col >> 2)) ^ (row & X::kSwizzle)) * 16 + (col & 3) * 4);
-#pragma unroll
-                                for (int rb = 0; rb < RB; ++rb)
-                                    o[db][rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[kb][rb][i], o[db][rb], 0, 0, 0);
-                            }
-                        }
-                } else {
-#pragma unroll
-                    for (int pair = 0; pair < KB / 2; ++pair) {
-                        Frag pr[RB];
+                    for (int e = 0; e < X::kFrag; ++e) {
+                        const float f = static_cast<float>(a[e]);
+                        const bool none = f != f, high = f == kInf || none, low = f == -kInf || none;
+                        up[e] = static_cast<T>(high ? 1.0f : 0.0f);
+                        down[e] = static_cast<T>(low ? 1.0f : 0.0f);
+                        if (high || low) a[e] = static_cast<T>(0.0f);
+                        odd |= high || low;
+                    }
+                    if (__any(odd)) {
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) {
-                            const Quad lo = __builtin_convertvector(s[2 * pair][rb], Quad);
-                            const Quad hi = __builtin_convertvector(s[2 * pair + 1][rb], Quad);
-                            pr[rb] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                        }
-                        // lane 4 j + c of a quad reads half a chunk of row j of
-                        // four, and gets column `col` of the sixteen
-                        const int row = pair * 32 + quad * 4 + (col >> 2), half = (col & 3) >> 1, byte = (col & 1) * 8;
+                            const f32x4 highs = X::value_mma(up, pr[rb], f32x4{}), lows = X::value_mma(down, pr[rb], f32x4{});
 #pragma unroll
-                        for (int db = 0; db < DB; ++db) {
-                            Frag a;
-                            i16x4 part[2];
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                const int r = row + 16 * t;
-                                part[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (__attribute__((address_space(3))) i16x4*)(v_lds + r * X::kRowBytes +
-                                                                              ((db * 2 + half) ^ (r & X::kSwizzle)) * 16 + byte));
+                            for (int i = 0; i < 4; ++i) {
+                                to[rb][i] += highs[i] > 0.0f ? kInf : 0.0f;
+                                to[rb][i] -= lows[i] > 0.0f ? kInf : 0.0f;
                             }
-                            a = __builtin_bit_cast(Frag, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                            for (int rb = 0; rb < RB; ++rb) o[db][rb] = E::mma(a, pr[rb], o[db][rb]);
                         }
                     }
                 }
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) to[rb] = X::value_mma(a, pr[rb], to[rb]);
+            };
+            if constexpr (X::k32) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = kb * 16 + quad * 4 + i;
+                        Frag pr[RB];
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) pr[rb][0] = s[kb][rb][i];
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            Frag a;
+                            a[0] = *reinterpret_cast<const float*>(v_lds + row * X::kRowBytes +
+                                                                   ((db * 4 + (col >> 2)) ^ (row & X::kSwizzle)) * 16 + (col & 3) * 4);
+                            accumulate(a, pr, o[db]);
+                        }
+                    }
             } else {
-                for (int key = 0; key < KEYS; ++key) {
-                    float e[RB];
+                const Frag ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+                for (int pair = 0; pair < KB / 2; ++pair) {
+                    Frag pr[RB];
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
-                        e[rb] = 0.0f;
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (key == kb * 16 + quad * 4 + i) e[rb] = s[kb][rb][i];
-                        e[rb] = __shfl(e[rb], ((key >> 2) & 3) * 16 + col);
+                        const Quad lo = __builtin_convertvector(s[2 * pair][rb], Quad);
+                        const Quad hi = __builtin_convertvector(s[2 * pair + 1][rb], Quad);
+                        pr[rb] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        sum_l[rb] = E::mma(ones, pr[rb], sum_l[rb]);
                     }
+                    // lane 4 j + c of a quad reads half a chunk of row j of four,
+                    // and gets column `col` of the sixteen
+                    const int row = pair * 32 + quad * 4 + (col >> 2), half = (col & 3) >> 1, byte = (col & 1) * 8;
 #pragma unroll
-                    for (int db = 0; db < DB; ++db)
+                    for (int db = 0; db < DB; ++db) {
+                        i16x4 part[2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int byte = (db * 16 + quad * 4 + i) * X::kSize;
-                            const float x = static_cast<float>(*reinterpret_cast<const T*>(
-                                v_lds + key * X::kRowBytes + ((byte >> 4) ^ (key & X::kSwizzle)) * 16 + (byte & 15)));
-#pragma unroll
-                            for (int rb = 0; rb < RB; ++rb)
-                                if (e[rb] != 0.0f) o[db][rb][i] = __builtin_fmaf(e[rb], x, o[db][rb][i]);
+                        for (int t = 0; t < 2; ++t) {
+                            const int r = row + 16 * t;
+                            part[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) i16x4*)(v_lds + r * X::kRowBytes +
+                                                                          ((db * 2 + half) ^ (r & X::kSwizzle)) * 16 + byte));
                         }
+                        accumulate(__builtin_bit_cast(Frag, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)), pr, o[db]);
+                    }
                 }
             }
         }
 
         // ---- the piece's result ----
+        const AttendParams& p2 = arguments();
+        float sum[RB];  // what the result is divided by; l is the log-sum's
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             l[rb] += __shfl_xor(l[rb], 16);
             l[rb] += __shfl_xor(l[rb], 32);
+            sum[rb] = X::k32 ? l[rb] : sum_l[rb][0];
         }
         if constexpr (WK > 1) {
             // the wavefronts along the keys: rescaled to their common maximum
@@ -609,23 +792,29 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 if (quad == 0) {
                     stats[0][wk][(wr * RB + rb) * 16 + col] = m[rb];
                     stats[1][wk][(wr * RB + rb) * 16 + col] = l[rb];
+                    stats[2][wk][(wr * RB + rb) * 16 + col] = sum[rb];
                 }
             __syncthreads();
             f32x4* const sums = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const int r = (wr * RB + rb) * 16 + col;
-                float top = -kInf, sum = 0.0f;
+                float top = -kInf, all_l = 0.0f, all = 0.0f;
 #pragma unroll
                 for (int i = 0; i < WK; ++i) top = fmaxf(top, stats[0][i][r]);
-                const auto weight = [&](float x) { return x == -kInf ? 0.0f : __builtin_amdgcn_exp2f((x - top) * p.scale); };
+                const auto weight = [&](float x) { return x == -kInf ? 0.0f : __builtin_amdgcn_exp2f((x - top) * p2.scale); };
 #pragma unroll
-                for (int i = 0; i < WK; ++i) sum = __builtin_fmaf(weight(stats[0][i][r]), stats[1][i][r], sum);
+                for (int i = 0; i < WK; ++i) {
+                    const float by = weight(stats[0][i][r]);
+                    all_l = __builtin_fmaf(by, stats[1][i][r], all_l);
+                    all = __builtin_fmaf(by, stats[2][i][r], all);
+                }
                 const float by = weight(m[rb]);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) sums[(wave * X::kAccs + db * RB + rb) * 64 + lane] = o[db][rb] * by;
                 m[rb] = top;
-                l[rb] = sum;
+                l[rb] = all_l;
+                sum[rb] = all;
             }
             __syncthreads();
 #pragma unroll
@@ -633,31 +822,30 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 if (db % WK != wk) continue;
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < WK; ++i) sum += sums[((i * WR + wr) * X::kAccs + db * RB + rb) * 64 + lane];
-                    o[db][rb] = sum;
+                    for (int i = 0; i < WK; ++i) x += sums[((i * WR + wr) * X::kAccs + db * RB + rb) * 64 + lane];
+                    o[db][rb] = x;
                 }
             }
-            __syncthreads();  // before the next piece's tiles
-        }
-        float* const part = p.partial + slot_of(p, mine, w.item, w.starts) * X::kSlot;
+            }
+        float* const part = p2.partial + slot_of(p2, mine, w.item, w.starts) * X::kSlot;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             if (place[rb] < 0) continue;
             const int r = (wr * RB + rb) * 16 + col;
             if (w.whole) {
-                const float by = l[rb] > 0.0f || l[rb] != l[rb] ? 1.0f / l[rb] : 0.0f;
-                T* const out = static_cast<T*>(p.out) + place[rb] * p.D;
+                const float by = sum[rb] > 0.0f || sum[rb] != sum[rb] ? 1.0f / sum[rb] : 0.0f;
+                T* const out = static_cast<T*>(p2.out) + place[rb] * p2.D;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     if (db % WK != wk) continue;
                     const int d = db * 16 + quad * 4;
-                    if (d < p.D) *reinterpret_cast<Quad*>(out + d) = __builtin_convertvector(o[db][rb] * by, Quad);
+                    if (d < p2.D) *reinterpret_cast<Quad*>(out + d) = __builtin_convertvector(o[db][rb] * by, Quad);
                 }
-                if (p.lse && wk == 0 && quad == 0)
-                    p.lse[place[rb]] = l[rb] > 0.0f || l[rb] != l[rb]
-                                           ? (m[rb] * p.scale + __builtin_amdgcn_logf(l[rb])) * 0.693147180559945309f
+                if (p2.lse && wk == 0 && quad == 0)
+                    p2.lse[place[rb]] = l[rb] > 0.0f || l[rb] != l[rb]
+                                           ? (m[rb] * p2.scale + __builtin_amdgcn_logf(l[rb])) * 0.693147180559945309f
                                            : -kInf;
             } else {
 #pragma unroll
@@ -667,80 +855,155 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 }
                 if (wk == 0 && quad == 0) {
                     part[ROWS * DP + r] = m[rb];
-                    part[ROWS * DP + ROWS + r] = l[rb];
+                    part[ROWS * DP + ROWS + r] = sum[rb];
+                    part[ROWS * DP + 2 * ROWS + r] = l[rb];
                 }
             }
         }
     }
 }
 
-// The rows' results where they are not whole: a wavefront takes a row, and
-// each lane some of its columns. A row that asks nothing gets 0 and -inf.
+// The rows of an item of a sequence (x) whose results lie in pieces, y of as many
+// as a workgroup takes at once: a thread has four columns of a row, and where rows
+// are few, several threads share the pieces of one. All reads of eight pieces are in
+// flight together: their places follow from the item's first and last workgroup. A
+// row that asks nothing gets 0 and -inf.
 template <int DTYPE, int DP, int SHAPE>
 __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams p) {
-    using T = typename Elem<DTYPE>::T;
+    using E = Elem<DTYPE>;
+    using T = typename E::T;
+    using Quad = typename E::Quad;
     using X = Dims<DTYPE, DP, SHAPE>;
-    constexpr int ROWS = X::kRows, PER = DP / 64;
+    constexpr int ROWS = X::kRows, PER_ROW = DP / 4, SLOTS = kAttendThreads / PER_ROW, AT_ONCE = 8;
     constexpr float kInf = __builtin_inff();
-    const int lane = threadIdx.x & 63;
-    const int64_t rows = static_cast<int64_t>(p.S) * p.N * p.H;
-    const int64_t place = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (place >= rows) return;
-    const int h = static_cast<int>(place % p.H);
-    const int64_t sn = place / p.H;
-    const int n = static_cast<int>(sn % p.N), seq = static_cast<int>(sn / p.N);
-    T* const out = static_cast<T*>(p.out) + place * p.D;
-    const Sequence s = sequence(p, seq);
-    if (n >= s.count) {
-        for (int d = lane; d < p.D; d += 64) out[d] = static_cast<T>(0.0f);
-        if (p.lse && lane == 0) p.lse[place] = -kInf;
-        return;
-    }
-    const int group = seq / p.K, beam = seq % p.K, head = h / p.G, in_head = h % p.G;
-    const int head_item = group * p.items + head * (p.shared_tiles + p.K * p.own_tiles);
-    const int own_row = n * p.G + in_head, shared_row = beam * p.N * p.G + own_row;
-    const int own_item = head_item + p.shared_tiles + beam * p.own_tiles + own_row / ROWS;
-    const int4 own = p.info[own_item];
-    if (own.x == own.y && !own.z) return;
+    __shared__ f32x4 sums[kAttendThreads];
+    __shared__ float tops[kAttendThreads], totals[kAttendThreads], totals_l[kAttendThreads];
 
-    float top = -kInf, total = 0.0f, sum[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sum[i] = 0.0f;
-    const auto take = [&](const int4& info, int item, int r) {
-        for (int w = info.x; w <= info.y; ++w) {
-            const float* const part = p.partial + slot_of(p, w, item, w == info.x) * X::kSlot;
-            const float m = part[ROWS * DP + r], l = part[ROWS * DP + ROWS + r];
-            if (m == -kInf && l == 0.0f) continue;
-            const float next = fmaxf(top, m);
-            const float old = top == -kInf ? 0.0f : __builtin_amdgcn_exp2f((top - next) * p.scale);
-            const float by = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m - next) * p.scale);
-            top = next;
-            total = total * old + l * by;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) sum[i] = sum[i] * old + part[r * DP + i * 64 + lane] * by;
+    const int G = static_cast<int>(p.G.d);
+    int x = blockIdx.x;
+    const int tile = x % p.own_tiles;
+    x /= p.own_tiles;
+    const int head = x % p.Hkv, seq = x / p.Hkv;
+    const int group = seq / p.K, beam = seq - group * p.K;
+    const int group_items = head * p.head_items + group * (p.shared_tiles + p.K * p.own_tiles);
+    const int own_item = group_items + p.shared_tiles + beam * p.own_tiles + tile;
+    const Sequence s = sequence(p, seq);
+    const int tile_rows = min(ROWS, p.N * G - tile * ROWS), live = min(tile_rows, s.count * G - tile * ROWS);
+    int4 own = make_int4(0, 0, 0, 0);
+    if (live > 0) own = p.info[own_item];
+    const bool whole = own.x == own.y && !own.z;
+    if (whole && live == tile_rows) return;
+
+    // threads of a row side by side, then the rows, then the shares of the pieces
+    int shares = 1;
+    while (2 * shares * tile_rows <= SLOTS) shares *= 2;
+    const int rows_at_once = SLOTS / shares;
+    const int slot = threadIdx.x / PER_ROW, share = slot / rows_at_once, column = (threadIdx.x % PER_ROW) * 4;
+    for (int r0 = static_cast<int>(blockIdx.y) * rows_at_once; r0 < tile_rows; r0 += static_cast<int>(gridDim.y) * rows_at_once) {
+        const int in_tile = r0 + slot - share * rows_at_once, row = tile * ROWS + in_tile;
+        const bool mine_row = in_tile < tile_rows && share < shares;
+        const int n = static_cast<int>(p.G.quotient(row)), h = head * G + row - n * G;
+        const int64_t place = (static_cast<int64_t>(seq) * p.N + n) * p.H + h;
+        T* const out = static_cast<T*>(p.out) + place * p.D;
+        if (mine_row && in_tile >= live && share == 0) {
+            if (column < p.D) *reinterpret_cast<Quad*>(out + column) = Quad{};
+            if (p.lse && column == 0) p.lse[place] = -kInf;
         }
-    };
-    if (own.z) {
-        const int item = head_item + shared_row / ROWS;
-        take(p.info[item], item, shared_row % ROWS);
-    }
-    take(own, own_item, own_row % ROWS);
-    const bool any = total > 0.0f || total != total;
-    const float by = any ? 1.0f / total : 0.0f;
+        if (whole || r0 >= live) continue;
+        const bool busy = mine_row && in_tile < live;
+        const int shared_row = beam * static_cast<int>(p.beam_rows.d) + row;
+        const int shared_item = group_items + shared_row / ROWS;
+        int4 common = make_int4(0, -1, 0, 0);
+        if (own.z && busy) common = p.info[shared_item];
+        const int mine = own.y - own.x + 1, pieces = mine + common.y - common.x + 1;
+        float top = -kInf, total = 0.0f, total_l = 0.0f;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = share; busy && i0 < pieces; i0 += AT_ONCE * shares) {
+            float m[AT_ONCE], l[AT_ONCE], ll[AT_ONCE];
+            f32x4 o[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (i * 64 + lane < p.D) out[i * 64 + lane] = static_cast<T>(sum[i] * by);
-    if (p.lse && lane == 0)
-        p.lse[place] = any ? (top * p.scale + __builtin_amdgcn_logf(total)) * 0.693147180559945309f : -kInf;
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int at = min(i0 + i * shares, pieces - 1);
+                const bool is_own = at < mine;
+                const int w = is_own ? own.x + at : common.x + at - mine, r = (is_own ? row : shared_row) % ROWS;
+                const float* const part =
+                    p.partial + slot_of(p, w, is_own ? own_item : shared_item, w == (is_own ? own.x : common.x)) * X::kSlot;
+                m[i] = part[ROWS * DP + r];
+                l[i] = part[ROWS * DP + ROWS + r];
+                ll[i] = part[ROWS * DP + 2 * ROWS + r];
+                o[i] = *reinterpret_cast<const f32x4*>(part + r * DP + column);
+            }
+            float next = top;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) next = fmaxf(next, m[i]);
+            const auto weight = [&](float y) { return y == -kInf ? 0.0f : __builtin_amdgcn_exp2f((y - next) * p.scale); };
+            const float by = weight(top);
+            top = next;
+            total *= by;
+            total_l *= by;
+            sum *= by;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                // a piece that saw nothing holds zeros; its total is no number where
+                // all of its scores were none
+                if (i0 + i * shares >= pieces || (m[i] == -kInf && l[i] == 0.0f)) continue;
+                const float piece_by = m[i] == -kInf ? 1.0f : weight(m[i]);
+                total = __builtin_fmaf(piece_by, l[i], total);
+                total_l = __builtin_fmaf(piece_by, ll[i], total_l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(piece_by, o[i][e], sum[e]);
+            }
+        }
+        if (shares > 1) {
+            __syncthreads();
+            sums[threadIdx.x] = sum;
+            tops[threadIdx.x] = top;
+            totals[threadIdx.x] = total;
+            totals_l[threadIdx.x] = total_l;
+            __syncthreads();
+            if (share == 0) {
+                const int step = rows_at_once * PER_ROW;
+                float next = top;
+                for (int i = 1; i < shares; ++i) next = fmaxf(next, tops[threadIdx.x + i * step]);
+                const auto weight = [&](float y) { return y == -kInf ? 1.0f : __builtin_amdgcn_exp2f((y - next) * p.scale); };
+                const float by = weight(top);
+                total *= by;
+                total_l *= by;
+                sum *= by;
+                for (int i = 1; i < shares; ++i) {
+                    const int at = threadIdx.x + i * step;
+                    const float share_by = weight(tops[at]);
+                    total = __builtin_fmaf(share_by, totals[at], total);
+                    total_l = __builtin_fmaf(share_by, totals_l[at], total_l);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(share_by, sums[at][e], sum[e]);
+                }
+                top = next;
+            }
+        }
+        if (!busy || share != 0) continue;
+        const bool any = total > 0.0f || total != total;
+        const float by = any ? 1.0f / total : 0.0f;
+        if (column < p.D) *reinterpret_cast<Quad*>(out + column) = __builtin_convertvector(sum * by, Quad);
+        if (p.lse && column == 0)
+            p.lse[place] = any ? (top * p.scale + __builtin_amdgcn_logf(total_l)) * 0.693147180559945309f : -kInf;
+    }
 }
 
 template <int DTYPE, int DP, int SHAPE>
 hipError_t launch_shape(const AttendParams& p, hipStream_t stream) {
-    attend_kernel<DTYPE, DP, SHAPE><<<p.grid, kAttendThreads, 0, stream>>>(p);
+    // a workgroup for each item too, where the kernel may want it
+    int workgroups = p.grid;
+    const int64_t tiles = static_cast<int64_t>((p.S * p.Hkv + 7) / 8 * 8) * p.own_tiles;
+    if (Dims<DTYPE, DP, SHAPE>::kRowWaves > 1 && !p.shared && tiles >= 2 * workgroups) workgroups = static_cast<int>(tiles);
+    attend_kernel<DTYPE, DP, SHAPE><<<workgroups, kAttendThreads, 0, stream>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t rows = static_cast<int64_t>(p.S) * p.N * p.H;
-    attend_join<DTYPE, DP, SHAPE><<<static_cast<unsigned>((rows + 3) / 4), kAttendThreads, 0, stream>>>(p);
+    constexpr int kAtOnce = kAttendThreads / (DP / 4);
+    const int rows = min(attend_rows(SHAPE), p.N * static_cast<int>(p.G.d)), items = p.S * p.Hkv * p.own_tiles;
+    const dim3 grid(static_cast<unsigned>(items),
+                    static_cast<unsigned>(min((rows + kAtOnce - 1) / kAtOnce, max(1, 8192 / items))));
+    attend_join<DTYPE, DP, SHAPE><<<grid, kAttendThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -755,24 +1018,25 @@ hipError_t launch_dim(const AttendParams& p, int shape, hipStream_t stream) {
 }
 
 template <int DTYPE, int DP>
-void dim_sizes(int shape, int& resident, int& slot) {
+AttendSizes dim_sizes(int shape) {
+    const auto of = [](auto x) { return AttendSizes{decltype(x)::kResident, decltype(x)::kSlot, decltype(x)::kKeys}; };
     switch (shape) {
-        case kRows16: resident = Dims<DTYPE, DP, kRows16>::kResident, slot = Dims<DTYPE, DP, kRows16>::kSlot; break;
-        case kRows32: resident = Dims<DTYPE, DP, kRows32>::kResident, slot = Dims<DTYPE, DP, kRows32>::kSlot; break;
-        case kRows64: resident = Dims<DTYPE, DP, kRows64>::kResident, slot = Dims<DTYPE, DP, kRows64>::kSlot; break;
-        default: resident = Dims<DTYPE, DP, kRows128>::kResident, slot = Dims<DTYPE, DP, kRows128>::kSlot; break;
+        case kRows16: return of(Dims<DTYPE, DP, kRows16>{});
+        case kRows32: return of(Dims<DTYPE, DP, kRows32>{});
+        case kRows64: return of(Dims<DTYPE, DP, kRows64>{});
+        default: return of(Dims<DTYPE, DP, kRows128>{});
     }
 }
 
 }  // namespace attend
 
 template <int DTYPE>
-void attend_sizes(int dim, int shape, int& resident, int& slot) {
+AttendSizes attend_sizes(int dim, int shape) {
     switch (dim) {
-        case 64: return attend::dim_sizes<DTYPE, 64>(shape, resident, slot);
-        case 128: return attend::dim_sizes<DTYPE, 128>(shape, resident, slot);
-        case 192: return attend::dim_sizes<DTYPE, 192>(shape, resident, slot);
-        default: return attend::dim_sizes<DTYPE, 256>(shape, resident, slot);
+        case 64: return attend::dim_sizes<DTYPE, 64>(shape);
+        case 128: return attend::dim_sizes<DTYPE, 128>(shape);
+        case 192: return attend::dim_sizes<DTYPE, 192>(shape);
+        default: return attend::dim_sizes<DTYPE, 256>(shape);
     }
 }
 
