@@ -26,8 +26,13 @@
 // values are equal. The log-sum that a caller asks for is the unrounded values'.
 #pragma once
 
+#include <type_traits>
+
 #include "attend.hpp"
 #include "dbs_cuda.h"
+
+// of a lambda: its captures and arrays stay in registers
+#define BEAMGRAD_INLINE __attribute__((always_inline))
 
 namespace dbs_hip {
 namespace attend {
@@ -111,7 +116,7 @@ struct Dims {
     // Tiles shared by wavefronts have two places: one is filled while the other
     // is used. A wavefront's own tile has one: the CU's other wavefronts use theirs
     // meanwhile.
-    static constexpr int kPlaces = kRowWaves > 1 && 4 * kKeyWaves * kRegion <= 136 * 1024 ? 2 : 1;
+    static constexpr int kPlaces = kRowWaves > 1 ? 2 : 1;
     static constexpr int kTile = 2 * kKeyWaves * kRegion;  // keys and values
     static constexpr int kAccs = kDimBlocks * kRowBlocks;
     static constexpr int kMerge = kKeyWaves > 1 ? kAccs * 4 * 64 * 16 : 0;
@@ -121,7 +126,9 @@ struct Dims {
     // workgroups of a CU: what its 160 KB of LDS hold
     static constexpr int kOther = kTokens * (kAttendMaxTree / 8) + 2 * kAttendMaxTree + 12 * kKeyWaves * kRows + 20 * kAttendSequences + 64;
     static constexpr int kFit = 160 * 1024 / (kLds + kOther);
-    static constexpr int kResident = kFit >= 2 ? 2 : 1;
+    // and its registers: sums, two tiles' scores and the queries of a wide head take
+    // more than half of a SIMD's
+    static constexpr int kResident = kFit >= 2 && (kRowWaves == 1 || kChunks <= 16) ? 2 : 1;
 };
 
 // The place of a piece's partial result. Without shared pages a workgroup
@@ -332,6 +339,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     __shared__ uint32_t sees[X::kTokens * (kAttendMaxTree / 32)];
     __shared__ int16_t up[kAttendMaxTree];
     __shared__ Board board;
+    __shared__ int odd;  // the piece's rows have to be computed again
 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int quad = lane >> 4, col = lane & 15;
@@ -351,14 +359,41 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     int mine, at, stop;
     Piece chosen;
     if (whole_items) {
-        // those with the most keys first; the tiles of a sequence and head are a
-        // multiple of eight workgroups apart, so that one XCD reads its keys
-        const int pairs = (p0.S * p0.Hkv + 7) / 8 * 8;
-        const int row = static_cast<int>(blockIdx.x) / pairs, pair = static_cast<int>(blockIdx.x) - row * pairs;
-        chosen.tile = p0.own_tiles - 1 - row;
-        chosen.seq = pair / p0.Hkv;
-        chosen.head = pair - chosen.seq * p0.Hkv;
-        if (chosen.tile < 0 || chosen.seq >= p0.S) return;
+        // The items with the most keys first, so that the last to end are short; the
+        // heads of a sequence's tile lie side by side, on as many XCDs as there are
+        // heads up to eight, and a head's tiles find its keys there.
+        const int entries = p0.S * p0.own_tiles;
+        const int rank = static_cast<int>(blockIdx.x) / p0.Hkv;
+        chosen.head = static_cast<int>(blockIdx.x) - rank * p0.Hkv;
+        if (rank >= entries) return;
+        int entry = rank;
+        if (entries <= kAttendThreads) {
+            // sorted: a thread counts the entries ahead of its own
+            const int mine_seq = threadIdx.x / p0.own_tiles, mine_tile = threadIdx.x - mine_seq * p0.own_tiles;
+            int keys = -1;
+            if (static_cast<int>(threadIdx.x) < entries) {
+                const Sequence q{board.length[mine_seq], board.count[mine_seq]};
+                keys = mine_tile < row_tiles(p0, q, ROWS) ? key_end<ROWS>(p0, q, mine_tile) : 0;
+            }
+            int* const sorted = reinterpret_cast<int*>(lds);
+            sorted[threadIdx.x] = keys;
+            __syncthreads();
+            int ahead = 0;
+            for (int i = 0; i < entries; ++i) ahead += sorted[i] > keys || (sorted[i] == keys && i < static_cast<int>(threadIdx.x));
+            __syncthreads();
+            if (keys >= 0) sorted[ahead] = threadIdx.x;
+            __syncthreads();
+            entry = uniform(sorted[rank]);
+        } else {
+            entry = entries - 1 - rank;  // the last tiles have the most
+        }
+        if (entries <= kAttendThreads) {
+            chosen.seq = entry / p0.own_tiles;
+            chosen.tile = entry - chosen.seq * p0.own_tiles;
+        } else {
+            chosen.tile = entry / p0.S;
+            chosen.seq = entry - chosen.tile * p0.S;
+        }
         chosen.own = {uniform(board.length[chosen.seq]), uniform(board.count[chosen.seq])};
         if (chosen.tile >= row_tiles(p0, chosen.own, ROWS)) return;
         mine = 0, at = 0, stop = 1;
@@ -511,36 +546,39 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 
         const float scale = p.scale;
         f32x4 o[DB][RB];
-        float m[RB], l[RB];
+        float m[RB], l[RB], limit[RB], shift[RB];
         f32x4 sum_l[RB];  // 16-bit types: the sum of the rounded values, once for every row
         const bool with_lse = p.lse != nullptr;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            m[rb] = -kInf;
+            m[rb] = limit[rb] = -kInf;
+            shift[rb] = 0.0f;
             l[rb] = 0.0f;
             sum_l[rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        const float slack = 8.0f / scale;
 
         // The page-table entry of token first + lane of a tile, read well before
         // it is needed; then the place that it gives, -1 without a page.
         int32_t entry = -1;
-        const auto look_up = [&](int first) {
+        const auto look_up = [&](int first) BEAMGRAD_INLINE {
             entry = -1;
             if (lane < KEYS && first + lane < w.end) entry = row_pages[p.span.page.quotient(first + lane)];
         };
-        int64_t k_at, v_at;
-        const auto locate = [&](int first) {
+        const bool alike = p.kp == p.vp && p.kt == p.vt;  // the usual: one offset serves both
+        const auto locate = [&](int first, int64_t& k_at, int64_t& v_at) BEAMGRAD_INLINE {
             const uint32_t token = first + lane, in = token - p.span.page.quotient(token) * p.span.page.d;
             const bool there = p.span.is_page(entry);
             k_at = there ? static_cast<int64_t>(entry) * p.kp + static_cast<int64_t>(in) * p.kt : -1;
-            v_at = there ? static_cast<int64_t>(entry) * p.vp + static_cast<int64_t>(in) * p.vt : -1;
+            v_at = k_at;
+            if (!alike) v_at = there ? static_cast<int64_t>(entry) * p.vp + static_cast<int64_t>(in) * p.vt : -1;
             return __ballot(there);
         };
         // this wavefront's share of a tile, from memory straight into LDS
-        constexpr uint64_t kFull = KEYS == 64 ? ~uint64_t{0} : (uint64_t{1} << KEYS) - 1;
-        const auto fill = [&](char* region, const char* head, int64_t mine_at, uint64_t there) {
+        constexpr uint64_t kFull = ~uint64_t{0} >> (64 - KEYS);
+        const auto fill = [&](char* region, const char* head, int64_t mine_at, uint64_t there) BEAMGRAD_INLINE {
             if (there == kFull) {
 #pragma unroll
                 for (int i = 0; i < X::kLoads; ++i) {
@@ -565,57 +603,10 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     __builtin_amdgcn_global_load_lds((global_char*)(head + row_at + chunk * 16), (lds_char*)to, 16, 0, 0);
             }
         };
-        const auto region = [&](int round, int value) {
-            return lds + (X::kPlaces == 2 ? (round & 1) * X::kTile : 0) + (value * WK + wk) * X::kRegion;
-        };
+        const auto region = [&](int place, int value) { return lds + place * X::kTile + (value * WK + wk) * X::kRegion; };
 
-        const int rounds = (w.end - w.key0 + WK * KEYS - 1) / (WK * KEYS);
-        uint64_t there_next = 0;
-        look_up(w.key0 + wk * KEYS);
-        __syncthreads();  // the last piece's tiles are done with
-        if (chunks < X::kChunks) {
-            // the columns past the width are zeros in every tile
-            for (int i = threadIdx.x; i < X::kPlaces * X::kTile / 16; i += kAttendThreads)
-                reinterpret_cast<f32x4*>(lds)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            __syncthreads();
-        }
-        if constexpr (X::kPlaces == 2) {
-            there_next = locate(w.key0 + wk * KEYS);
-            look_up(w.key0 + (WK + wk) * KEYS);
-            fill(region(0, 0), k_head, k_at, there_next);
-            fill(region(0, 1), v_head, v_at, there_next);
-        }
-        for (int round = 0; round < rounds; ++round) {
-            const int first = w.key0 + (round * WK + wk) * KEYS;
-            if (WR == 1 && first >= w.end) break;  // no barriers below
-            uint64_t there;
-            char* const k_lds = region(round, 0);
-            char* const v_lds = region(round, 1);
-            if constexpr (X::kPlaces == 2) {
-                there = there_next;
-                // this tile has come, for all wavefronts, and all have done with the
-                // one before it, whose place the next one takes
-                wait_all();
-                barrier();
-                if (round + 1 < rounds) {
-                    there_next = locate(first + WK * KEYS);
-                    look_up(first + 2 * WK * KEYS);
-                    fill(region(round + 1, 0), k_head, k_at, there_next);
-                    fill(region(round + 1, 1), v_head, v_at, there_next);
-                }
-            } else {
-                there = locate(first);
-                look_up(first + WK * KEYS);
-                wait_lds();
-                if (WR > 1) barrier();
-                fill(k_lds, k_head, k_at, there);
-                fill(v_lds, v_head, v_at, there);
-                wait_all();
-                if (WR > 1) barrier();
-            }
-
-            // scores: s[kb][rb][i] of key 16 kb + 4 quad + i and row col of block rb
-            f32x4 s[KB][RB];
+        // scores: s[kb][rb][i] of key 16 kb + 4 quad + i and row col of block rb
+        const auto score = [&](const char* k_lds, f32x4 (&s)[KB][RB]) BEAMGRAD_INLINE {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -629,8 +620,11 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     for (int rb = 0; rb < RB; ++rb) s[kb][rb] = E::mma(a, q[rb][i], s[kb][rb]);
                 }
             }
-            const bool masked = there != kFull || first + KEYS > masked_from;
-            if (masked) {
+        };
+        // Softmax of a tile's scores and the product with its values.
+        const auto absorb = [&](int first, uint64_t there, const char* v_lds, f32x4 (&s)[KB][RB]) BEAMGRAD_INLINE {
+            const bool hides = first + KEYS > masked_from;
+            if (hides || there != kFull) {
                 const int q4 = opaque(quad * 4);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
@@ -640,7 +634,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         uint32_t seen = 15;
-                        if (first + KEYS > masked_from) {
+                        if (hides) {
                             if (p.parents) {
                                 // four bits of the token's row from `drafted` on, those
                                 // before the first drafted token set
@@ -659,34 +653,41 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     }
                 }
             }
-            // the maximum, raised where a tile's passes it by 2^8
+            // the maximum, raised where the tile's passes it by 2^8
+            float top[RB];
+            bool raise = false;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                float top = s[0][rb][0];
+                top[rb] = s[0][rb][0];
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kb][rb][i]);
-                top = quad_max(top);
-                const bool raise = (m[rb] == -kInf && top > -kInf) || (top - m[rb]) * scale > 8.0f;
-                if (__any(raise)) {
-                    const float next = raise ? top : m[rb];
+                    for (int i = 0; i < 4; ++i) top[rb] = fmaxf(top[rb], s[kb][rb][i]);
+                top[rb] = quad_max(top[rb]);
+                raise |= top[rb] > limit[rb];
+            }
+            if (__any(raise)) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    if (!(top[rb] > limit[rb])) top[rb] = m[rb];
                     // nothing seen yet: the sums are zero
-                    const float by = !raise ? 1.0f : m[rb] == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m[rb] - next) * scale);
-                    m[rb] = next;
+                    const float by = m[rb] == -kInf || m[rb] == top[rb] ? 1.0f : __builtin_amdgcn_exp2f((m[rb] - top[rb]) * scale);
+                    m[rb] = top[rb];
+                    limit[rb] = top[rb] + slack;
+                    shift[rb] = top[rb] == -kInf ? 0.0f : -top[rb] * scale;
                     l[rb] *= by;
                     sum_l[rb] *= by;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db][rb] *= by;
                 }
-                const float shift = m[rb] == -kInf ? 0.0f : -m[rb] * scale;
+            }
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][rb][i], scale, shift));
-                        s[kb][rb][i] = e;
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        s[kb][rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][rb][i], scale, shift[rb]));
                 if (X::k32 || with_lse) {
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb)
@@ -695,38 +696,18 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 }
             }
             // A value that is no number or infinite, of a token that some rows of
-            // the tile do not see, must not reach them as 0 * inf: such values are
-            // taken out, and reach the rows whose probability is above 0 by a
-            // product with where they are.
-            const bool hidden = first + KEYS > masked_from;
-            const auto accumulate = [&](Frag a, const Frag* pr, f32x4* to) {
-                if (hidden) {
-                    bool odd = false;
-                    Frag up, down;
+            // the tile do not see, would reach them as 0 * inf: the join computes
+            // these rows again, one by one.
+            if (hides) {
+                bool none = false;
+                for (int c = opaque(lane); c < KEYS * X::kChunks; c += 64) {
+                    const Frag x = *reinterpret_cast<const Frag*>(v_lds + c * 16);
 #pragma unroll
-                    for (int e = 0; e < X::kFrag; ++e) {
-                        const float f = static_cast<float>(a[e]);
-                        const bool none = f != f, high = f == kInf || none, low = f == -kInf || none;
-                        up[e] = static_cast<T>(high ? 1.0f : 0.0f);
-                        down[e] = static_cast<T>(low ? 1.0f : 0.0f);
-                        if (high || low) a[e] = static_cast<T>(0.0f);
-                        odd |= high || low;
-                    }
-                    if (__any(odd)) {
-#pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            const f32x4 highs = X::value_mma(up, pr[rb], f32x4{}), lows = X::value_mma(down, pr[rb], f32x4{});
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                to[rb][i] += highs[i] > 0.0f ? kInf : 0.0f;
-                                to[rb][i] -= lows[i] > 0.0f ? kInf : 0.0f;
-                            }
-                        }
-                    }
+                    for (int e = 0; e < 16 / X::kSize; ++e)
+                        none |= first + c / X::kChunks >= masked_from && !(__builtin_fabsf(static_cast<float>(x[e])) < kInf);
                 }
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) to[rb] = X::value_mma(a, pr[rb], to[rb]);
-            };
+                if (none) odd = 1;
+            }
             if constexpr (X::k32) {
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
@@ -741,7 +722,9 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                             Frag a;
                             a[0] = *reinterpret_cast<const float*>(v_lds + row * X::kRowBytes +
                                                                    ((db * 4 + (col >> 2)) ^ (row & X::kSwizzle)) * 16 + (col & 3) * 4);
-                            accumulate(a, pr, o[db]);
+                            
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb) o[db][rb] = X::value_mma(a, pr[rb], o[db][rb]);
                         }
                     }
             } else {
@@ -769,14 +752,84 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                                 (__attribute__((address_space(3))) i16x4*)(v_lds + r * X::kRowBytes +
                                                                           ((db * 2 + half) ^ (r & X::kSwizzle)) * 16 + byte));
                         }
-                        accumulate(__builtin_bit_cast(Frag, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)), pr, o[db]);
+                        const Frag a = __builtin_bit_cast(Frag, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) o[db][rb] = E::mma(a, pr[rb], o[db][rb]);
                     }
                 }
+            }
+        };
+        const int rounds = (w.end - w.key0 + WK * KEYS - 1) / (WK * KEYS), mine_first = w.key0 + wk * KEYS;
+        constexpr int kNext = WK * KEYS;
+        look_up(mine_first);
+        __syncthreads();  // the last piece's tiles are done with
+        if (threadIdx.x == 0) odd = 0;
+        if (chunks == X::kChunks) __syncthreads();
+        if (chunks < X::kChunks) {
+            // the columns past the width are zeros in every tile
+            for (int i = threadIdx.x; i < X::kPlaces * X::kTile / 16; i += kAttendThreads)
+                reinterpret_cast<f32x4*>(lds)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            __syncthreads();
+        }
+        if constexpr (X::kPlaces == 2) {
+            // Tile t has place t & 1. While a tile's softmax keeps the vector
+            // instructions busy, the matrix instructions have the next one's scores:
+            // keys come two tiles ahead, values one.
+            f32x4 s[2][KB][RB];
+            int64_t k_at, v_at, v_next;
+            uint64_t there = locate(mine_first, k_at, v_at), there_next = 0;
+            look_up(mine_first + kNext);
+            fill(region(0, 0), k_head, k_at, there);
+            fill(region(0, 1), v_head, v_at, there);
+            if (rounds > 1) {
+                there_next = locate(mine_first + kNext, k_at, v_next);
+                look_up(mine_first + 2 * kNext);
+                fill(region(1, 0), k_head, k_at, there_next);
+            }
+            wait_all();
+            barrier();
+            score(region(0, 0), s[0]);
+            const auto step = [&]<int PLACE>(std::integral_constant<int, PLACE>, int round) BEAMGRAD_INLINE {
+                const int first = mine_first + round * kNext;
+                // keys of the next tile and values of this one have come, for all
+                // wavefronts, and all have done with what the next ones overwrite
+                wait_all();
+                barrier();
+                uint64_t there_after = 0;
+                if (round + 1 < rounds) fill(region(PLACE ^ 1, 1), v_head, v_next, there_next);
+                if (round + 2 < rounds) {
+                    there_after = locate(first + 2 * kNext, k_at, v_next);
+                    look_up(first + 3 * kNext);
+                    fill(region(PLACE, 0), k_head, k_at, there_after);
+                }
+                if (round + 1 < rounds) score(region(PLACE ^ 1, 0), s[PLACE ^ 1]);
+                absorb(first, there, region(PLACE, 1), s[PLACE]);
+                there = there_next;
+                there_next = there_after;
+            };
+            for (int round = 0; round < rounds; round += 2) {
+                step(std::integral_constant<int, 0>{}, round);
+                if (round + 1 < rounds) step(std::integral_constant<int, 1>{}, round + 1);
+            }
+        } else {
+            for (int first = mine_first; first < w.end; first += kNext) {  // no barriers
+                int64_t k_at, v_at;
+                const uint64_t there = locate(first, k_at, v_at);
+                look_up(first + kNext);
+                wait_lds();
+                fill(region(0, 0), k_head, k_at, there);
+                fill(region(0, 1), v_head, v_at, there);
+                wait_all();
+                f32x4 s[KB][RB];
+                score(region(0, 0), s);
+                absorb(first, there, region(0, 1), s);
             }
         }
 
         // ---- the piece's result ----
         const AttendParams& p2 = arguments();
+        __syncthreads();
+        const bool again = odd != 0;
         float sum[RB];  // what the result is divided by; l is the log-sum's
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -829,6 +882,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 }
             }
             }
+        if (w.whole && again && threadIdx.x == 0) p2.info[w.item].w = 1;
         float* const part = p2.partial + slot_of(p2, mine, w.item, w.starts) * X::kSlot;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -854,7 +908,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     *reinterpret_cast<f32x4*>(part + r * DP + db * 16 + quad * 4) = o[db][rb];
                 }
                 if (wk == 0 && quad == 0) {
-                    part[ROWS * DP + r] = m[rb];
+                    part[ROWS * DP + r] = again ? __builtin_nanf("") : m[rb];
                     part[ROWS * DP + ROWS + r] = sum[rb];
                     part[ROWS * DP + 2 * ROWS + r] = l[rb];
                 }
@@ -863,11 +917,76 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     }
 }
 
+// One row by a workgroup, key by key, as the formula has it: for rows that the
+// matrix instructions would spoil.
+template <int DTYPE>
+__device__ __forceinline__ void plain_row(const AttendParams& p, int seq, const Sequence& s, int n, int head, int h, float* weights,
+                                       float* lds) {
+    using T = typename Elem<DTYPE>::T;
+    constexpr float kInf = __builtin_inff();
+    const int64_t place = (static_cast<int64_t>(seq) * p.N + n) * p.H + h;
+    const T* const q = reinterpret_cast<const T*>(static_cast<const char*>(p.q) + seq * p.qs + n * p.qn + h * p.qh);
+    const int32_t* const pages = p.pages + static_cast<int64_t>(seq) * p.span.P;
+    const auto reduce = [&](float x, bool max) {
+        __syncthreads();
+        lds[threadIdx.x] = x;
+        __syncthreads();
+        float all = lds[0];
+        for (int i = 1; i < kAttendThreads; ++i) all = max ? fmaxf(all, lds[i]) : all + lds[i];
+        return all;
+    };
+    float top = -kInf, total = 0.0f, sum = 0.0f;
+    for (int first = 0; first < s.length; first += kAttendThreads) {
+        const int t = first + static_cast<int>(threadIdx.x), drafted = t - s.prefix();
+        const uint32_t page = p.span.page.quotient(t);
+        bool seen = t < s.length && p.span.is_page(pages[min(static_cast<int>(page), p.span.P - 1)]);
+        if (seen && drafted >= 0) {
+            int at = n;
+            if (p.parents)
+                while (at > drafted) {
+                    const int parent = p.parents[static_cast<int64_t>(seq) * p.N + at];
+                    at = parent < at ? parent : -1;
+                }
+            seen = p.parents ? at == drafted : drafted <= n;
+        }
+        float score = -kInf;
+        if (seen) {
+            const int64_t at = pages[page] * p.kp + (t - page * p.span.page.d) * p.kt + head * p.kh;
+            const T* const k = reinterpret_cast<const T*>(static_cast<const char*>(p.k) + at);
+            score = 0.0f;
+            for (int d = 0; d < p.D; ++d) score = __builtin_fmaf(static_cast<float>(q[d]), static_cast<float>(k[d]), score);
+        }
+        const float next = fmaxf(top, reduce(score, true));
+        const float by = top == next || top == -kInf ? 1.0f : __builtin_amdgcn_exp2f((top - next) * p.scale);
+        const float weight = !seen || score == -kInf ? 0.0f : __builtin_amdgcn_exp2f((score - next) * p.scale);
+        top = next;
+        total = total * by + reduce(weight, false);
+        sum *= by;
+        weights[threadIdx.x] = seen ? weight : -1.0f;
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < p.D)
+            for (int i = 0; i < min(s.length - first, kAttendThreads); ++i) {
+                if (weights[i] == -1.0f) continue;
+                const uint32_t column = p.span.page.quotient(first + i);
+                const int64_t at = pages[column] * p.vp + (first + i - column * p.span.page.d) * p.vt + head * p.vh;
+                const T* const v = reinterpret_cast<const T*>(static_cast<const char*>(p.v) + at);
+                sum = __builtin_fmaf(weights[i], static_cast<float>(v[threadIdx.x]), sum);
+            }
+        __syncthreads();
+    }
+    const bool any = total > 0.0f || total != total;
+    if (static_cast<int>(threadIdx.x) < p.D) static_cast<T*>(p.out)[place * p.D + threadIdx.x] = static_cast<T>(any ? sum / total : 0.0f);
+    if (p.lse && threadIdx.x == 0)
+        p.lse[place] = any ? (top * p.scale + __builtin_amdgcn_logf(total)) * 0.693147180559945309f : -kInf;
+}
+
 // The rows of an item of a sequence (x) whose results lie in pieces, y of as many
 // as a workgroup takes at once: a thread has four columns of a row, and where rows
 // are few, several threads share the pieces of one. All reads of eight pieces are in
 // flight together: their places follow from the item's first and last workgroup. A
 // row that asks nothing gets 0 and -inf.
+// Rows of which a piece's maximum is no number are computed again, as are those of
+// an item that says so.
 template <int DTYPE, int DP, int SHAPE>
 __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams p) {
     using E = Elem<DTYPE>;
@@ -878,6 +997,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams
     constexpr float kInf = __builtin_inff();
     __shared__ f32x4 sums[kAttendThreads];
     __shared__ float tops[kAttendThreads], totals[kAttendThreads], totals_l[kAttendThreads];
+    __shared__ int again;
 
     const int G = static_cast<int>(p.G.d);
     int x = blockIdx.x;
@@ -892,7 +1012,9 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams
     int4 own = make_int4(0, 0, 0, 0);
     if (live > 0) own = p.info[own_item];
     const bool whole = own.x == own.y && !own.z;
-    if (whole && live == tile_rows) return;
+    if (whole && !own.w && live == tile_rows) return;
+    if (threadIdx.x == 0) again = own.w;
+    __syncthreads();
 
     // threads of a row side by side, then the rows, then the shares of the pieces
     int shares = 1;
@@ -935,7 +1057,10 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams
             }
             float next = top;
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) next = fmaxf(next, m[i]);
+            for (int i = 0; i < AT_ONCE; ++i) {
+                if (m[i] != m[i]) again = 1;
+                next = fmaxf(next, m[i]);
+            }
             const auto weight = [&](float y) { return y == -kInf ? 0.0f : __builtin_amdgcn_exp2f((y - next) * p.scale); };
             const float by = weight(top);
             top = next;
@@ -988,13 +1113,20 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams
         if (p.lse && column == 0)
             p.lse[place] = any ? (top * p.scale + __builtin_amdgcn_logf(total_l)) * 0.693147180559945309f : -kInf;
     }
+    __syncthreads();
+    if (!again) return;
+    for (int r0 = static_cast<int>(blockIdx.y) * rows_at_once; r0 < live; r0 += static_cast<int>(gridDim.y) * rows_at_once)
+        for (int r = r0; r < min(r0 + rows_at_once, live); ++r) {
+            const int row = tile * ROWS + r, n = static_cast<int>(p.G.quotient(row));
+            plain_row<DTYPE>(p, seq, s, n, head, head * G + row - n * G, reinterpret_cast<float*>(sums), tops);
+        }
 }
 
 template <int DTYPE, int DP, int SHAPE>
 hipError_t launch_shape(const AttendParams& p, hipStream_t stream) {
     // a workgroup for each item too, where the kernel may want it
     int workgroups = p.grid;
-    const int64_t tiles = static_cast<int64_t>((p.S * p.Hkv + 7) / 8 * 8) * p.own_tiles;
+    const int64_t tiles = static_cast<int64_t>(p.S) * p.Hkv * p.own_tiles;
     if (Dims<DTYPE, DP, SHAPE>::kRowWaves > 1 && !p.shared && tiles >= 2 * workgroups) workgroups = static_cast<int>(tiles);
     attend_kernel<DTYPE, DP, SHAPE><<<workgroups, kAttendThreads, 0, stream>>>(p);
     hipError_t e = hipGetLastError();
