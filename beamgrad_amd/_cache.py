@@ -30,11 +30,17 @@ from __future__ import annotations
 
 import math
 from collections.abc import Sequence
+from types import SimpleNamespace
 from typing import NamedTuple
 
 import torch
 
-from ._torch import _ops
+from ._torch import _ops as _torch_ops
+
+
+# the operators' only overloads: torch does not look for the one that fits
+_ops = SimpleNamespace(**{name: getattr(_torch_ops, name).default for name in (
+    "tree_attention", "fork_pages", "extend_pages", "write_tokens", "keep_tokens", "reorder_states", "reorder_states_")})
 
 
 class PageTable(NamedTuple):
@@ -59,17 +65,20 @@ def _tables(table) -> PageTable:
     return table
 
 
-def _tensors(name: str, tensors) -> list[torch.Tensor]:
-    tensors = list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a sequence of tensors, got a {type(t).__name__} in it")
-    return tensors
-
-
-def _no_gradient(what: str, tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"beamgrad_amd.{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+def _call(op, *args, **tensors):
+    """``op(*args)``; where it refuses arguments that should be tensors or lists of
+    them and are not, a TypeError that says which."""
+    try:
+        return op(*args)
+    except RuntimeError:
+        for name, value in tensors.items():
+            many = name in ("pools", "news", "states")
+            for t in value if many else (value,):
+                if not isinstance(t, torch.Tensor):
+                    got = type(t).__name__
+                    raise TypeError(f"{name} must be a sequence of tensors, got a {got} in it" if many
+                                    else f"{name} must be a torch.Tensor, got {got}") from None
+        raise
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: PageTable, *,
@@ -99,14 +108,11 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Pag
     ``[S, N, H]``, -inf for such rows. Scores, softmax and sums are held in 32
     bits; 16-bit inputs round each probability to their type. No gradient.
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     pages, lengths, _refs = _tables(table)
-    _no_gradient("tree_attention", (q, k, v))
     if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
-    out, lse = _ops.tree_attention(q, k, v, pages, lengths, parents, counts, beams, shared, scale, return_lse)
+        scale = 1.0 / math.sqrt(q.shape[-1]) if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
+    out, lse = _call(_ops.tree_attention, q, k, v, pages, lengths, parents, counts, beams, shared, scale, return_lse,
+                     q=q, k=k, v=v)
     return (out, lse) if return_lse else out
 
 
@@ -120,11 +126,8 @@ def fork_pages(pools: Sequence[torch.Tensor], table: PageTable, parents: torch.T
     their number. A sequence that finds none is left with nothing (length 0).
     """
     pages, lengths, refs = _tables(table)
-    pools = _tensors("pools", pools)
-    _no_gradient("fork_pages", pools)
-    out = PageTable(*_ops.fork_pages(pools, pages, lengths, refs, parents))
-    torch.autograd.graph.increment_version(pools)
-    return out
+    pools = list(pools)
+    return PageTable(*_call(_ops.fork_pages, pools, pages, lengths, refs, parents, pools=pools, parents=parents))
 
 
 def extend_pages(table: PageTable, counts: torch.Tensor, page_tokens: int) -> PageTable:
@@ -135,7 +138,7 @@ def extend_pages(table: PageTable, counts: torch.Tensor, page_tokens: int) -> Pa
     its length: ``new.lengths - table.lengths`` is what each has room for.
     """
     pages, lengths, refs = _tables(table)
-    return PageTable(*_ops.extend_pages(pages, lengths, refs, counts, page_tokens))
+    return PageTable(*_call(_ops.extend_pages, pages, lengths, refs, counts, page_tokens, counts=counts))
 
 
 def write_tokens(pools: Sequence[torch.Tensor], news: Sequence[torch.Tensor], table: PageTable,
@@ -144,10 +147,8 @@ def write_tokens(pools: Sequence[torch.Tensor], news: Sequence[torch.Tensor], ta
     to the places of the last ``counts[s]`` (default: all ``N``) tokens of each
     sequence: row ``j`` to the ``j``-th of them."""
     pages, lengths, _refs = _tables(table)
-    pools, news = _tensors("pools", pools), _tensors("news", news)
-    _no_gradient("write_tokens", pools + news)
-    _ops.write_tokens(pools, news, pages, lengths, counts)
-    torch.autograd.graph.increment_version(pools)
+    pools, news = list(pools), list(news)
+    _call(_ops.write_tokens, pools, news, pages, lengths, counts, pools=pools, news=news)
 
 
 def keep_tokens(pools: Sequence[torch.Tensor], table: PageTable, drafted: torch.Tensor, keep: torch.Tensor,
@@ -157,72 +158,9 @@ def keep_tokens(pools: Sequence[torch.Tensor], table: PageTable, drafted: torch.
     first number that is not ends the list) stay. They move together, in place in
     every pool, and the pages that hold no token any more are given back."""
     pages, lengths, refs = _tables(table)
-    pools = _tensors("pools", pools)
-    _no_gradient("keep_tokens", pools)
-    out = PageTable(*_ops.keep_tokens(pools, pages, lengths, refs, drafted, keep, kept))
-    torch.autograd.graph.increment_version(pools)
-    return out
-
-
-class _Reorder(torch.autograd.Function):
-    """The states in the order of the new beams; the gradient of a state sums
-    over the beams that continue it (:class:`_GatherGrads`)."""
-
-    @staticmethod
-    def forward(parents, *states):
-        return tuple(_ops.reorder_states(states, parents))
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        ctx.save_for_backward(inputs[0])
-        ctx.set_materialize_grads(False)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        (parents,) = ctx.saved_tensors
-        _refuse_foreign_leaves(ctx)
-        return (None, *_each_type(_GatherGrads, parents, grads))
-
-
-class _GatherGrads(torch.autograd.Function):
-    """The gradient of :class:`_Reorder`, itself differentiable."""
-
-    @staticmethod
-    def forward(parents, *grads):
-        return tuple(_ops.reorder_states_backward(grads, parents))
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        ctx.save_for_backward(inputs[0])
-        ctx.set_materialize_grads(False)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        (parents,) = ctx.saved_tensors
-        return (None, *_each_type(_Reorder, parents, grads))
-
-
-def _refuse_foreign_leaves(node) -> None:
-    """In a capture: torch hands a leaf's gradient over on the stream that the
-    leaf's accumulator was made on. Where a living graph of another stream holds
-    it, that stream joins the capture and the capture's end ends the process."""
-    if not torch.cuda.is_current_stream_capturing():
-        return
-    for fn, _ in node.next_functions:
-        leaf = getattr(fn, "variable", None)
-        if leaf is not None and _ops.leaf_of_another_stream(leaf):
-            raise RuntimeError("beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of "
-                               "another stream uses; drop that graph (its outputs and losses) before the capture")
-
-
-def _each_type(fn, parents, grads) -> list[torch.Tensor | None]:
-    """``fn`` over the gradients that there are, one call for each type."""
-    out: list[torch.Tensor | None] = [None] * len(grads)
-    for dtype in {g.dtype for g in grads if g is not None}:
-        at = [i for i, g in enumerate(grads) if g is not None and g.dtype == dtype]
-        for i, g in zip(at, fn.apply(parents, *(grads[i] for i in at)), strict=True):
-            out[i] = g
-    return out
+    pools = list(pools)
+    return PageTable(*_call(_ops.keep_tokens, pools, pages, lengths, refs, drafted, keep, kept, pools=pools, drafted=drafted,
+                            keep=keep, kept=kept))
 
 
 def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, *, inplace: bool = False) -> list[torch.Tensor]:
@@ -236,17 +174,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, *, inp
     order and in 32 bits, rounded once. With ``inplace`` the (contiguous)
     states are overwritten and returned, and rows that stay are not touched.
     """
-    states = _tensors("states", states)
-    if not isinstance(parents, torch.Tensor):
-        raise TypeError(f"parents must be a torch.Tensor, got {type(parents).__name__}")
+    states = list(states)
     if inplace:
-        _no_gradient("reorder_states(inplace=True)", states)
-        _ops.reorder_states_(states, parents)
-        torch.autograd.graph.increment_version(states)
+        _call(_ops.reorder_states_, states, parents, states=states, parents=parents)
         return states
-    if torch.is_grad_enabled() and any(t.requires_grad for t in states):
-        for t in states:
-            if t.requires_grad and t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-                raise TypeError(f"reorder_states has a gradient for float32, float16 and bfloat16 states, not {t.dtype}")
-        return list(_Reorder.apply(parents, *states))
-    return list(_ops.reorder_states(states, parents))
+    return _call(_ops.reorder_states, states, parents, states=states, parents=parents)

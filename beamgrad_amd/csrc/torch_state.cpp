@@ -10,10 +10,14 @@
 // page tables stay on the device, and the calls can be captured into a graph.
 #include <torch/all.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -41,6 +45,20 @@ void check_status(int code, const char* what) {
 
 [[noreturn]] void refuse_cpu(const char* what, const Tensor& t) {
     TORCH_CHECK(false, "beamgrad::", what, " runs on the GPU (HIP) only, got a tensor on ", t.device());
+}
+
+// Operators that write or read tensors without recording a gradient.
+void check_no_gradient(at::TensorList tensors, const char* what) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor& t : tensors)
+        TORCH_CHECK(!t.requires_grad(), "beamgrad_amd.", what,
+                    " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+
+// Written in place: an autograd graph that saved such a tensor notices.
+void written(at::TensorList tensors) {
+    for (const Tensor& t : tensors)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 int data_type(const Tensor& t, const char* name) {
@@ -122,9 +140,16 @@ int64_t row_elements(const Tensor& t, int64_t from) {
     return n;
 }
 
+// Whether b lies as a does: most pools of a cache do, and are checked once.
+bool laid_out_alike(const Tensor& a, const Tensor& b) {
+    return a.sizes() == b.sizes() && a.strides() == b.strides() && a.scalar_type() == b.scalar_type() &&
+           a.device() == b.device();
+}
+
 void check_pools(const Tensors& pools, const Tensor& pages, int64_t n_pages) {
     for (size_t i = 0; i < pools.size(); ++i) {
         const Tensor& t = pools[i];
+        if (i > 0 && laid_out_alike(pools[i - 1], t)) continue;
         TORCH_CHECK_VALUE(t.dim() >= 3 && t.numel() > 0, "pools[", i, "] must be a [pages, tokens of a page, ...] tensor, got ",
                           t.sizes());
         TORCH_CHECK_VALUE(t.device() == pages.device(), "pools[", i, "] is on ", t.device(), ", the page table on ",
@@ -135,17 +160,28 @@ void check_pools(const Tensors& pools, const Tensor& pages, int64_t n_pages) {
         TORCH_CHECK_VALUE(row_contiguous(t, 2), "a token's row of pools[", i, "] must be contiguous");
         TORCH_CHECK_VALUE(t.size(0) <= kI32Max, "pools[", i, "] has too many pages");
         // a page or token that lies where another does would be written twice
-        TORCH_CHECK_VALUE((t.size(1) == 1 || t.stride(1) >= row_elements(t, 2)) && (t.size(0) == 1 || t.stride(0) > 0), "the pages and tokens of pools[", i,
-                          "] overlap");
+        TORCH_CHECK_VALUE((t.size(1) == 1 || t.stride(1) >= row_elements(t, 2)) && (t.size(0) == 1 || t.stride(0) > 0),
+                          "the pages and tokens of pools[", i, "] overlap");
     }
     if (!pools.empty()) check_span(pages, pools[0].size(1));
 }
 
 Pools bind_pools(const Tensors& pools, int64_t n_pages, int64_t page_tokens) {
     Pools p;
-    for (const Tensor& t : pools) {
-        const int64_t size = static_cast<int64_t>(t.element_size());
+    p.base.reserve(pools.size());
+    p.row_bytes.reserve(pools.size());
+    p.page_stride.reserve(pools.size());
+    p.token_stride.reserve(pools.size());
+    for (size_t i = 0; i < pools.size(); ++i) {
+        const Tensor& t = pools[i];
         p.base.push_back(t.data_ptr());
+        if (i > 0 && laid_out_alike(pools[i - 1], t)) {
+            p.row_bytes.push_back(p.row_bytes.back());
+            p.page_stride.push_back(p.page_stride.back());
+            p.token_stride.push_back(p.token_stride.back());
+            continue;
+        }
+        const int64_t size = static_cast<int64_t>(t.element_size());
         p.row_bytes.push_back(row_elements(t, 2) * size);
         p.page_stride.push_back(t.stride(0) * size);
         p.token_stride.push_back(t.stride(1) * size);
@@ -181,6 +217,7 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
 // --- fork ---
 
 void check_fork(const Tensors& pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& parents) {
+    check_no_gradient(pools, "fork_pages");
     check_table(pages, lengths, refs);
     TORCH_CHECK_VALUE(!pools.empty(), "pools must hold at least one pool");
     check_pools(pools, pages, refs.numel());
@@ -204,6 +241,7 @@ TableOut fork_pages_hip(Tensors pools, const Tensor& pages, const Tensor& length
     check_status(beamgrad_fork_pages(&p.c, &from, par.const_data_ptr(), par.scalar_type() == torch::kInt64,
                                      narrow(pages.size(0)), narrow(pages.size(1)), &out, ws.data_ptr(), bytes, current_stream()),
                  "fork_pages");
+    written(pools);
     return to.take();
 }
 
@@ -237,12 +275,15 @@ TableOut extend_pages_hip(const Tensor& pages, const Tensor& lengths, const Tens
 // --- write ---
 
 void check_write(const Tensors& pools, const Tensors& news, const Tensor& pages, const Tensor& lengths, const OptTensor& counts) {
+    check_no_gradient(pools, "write_tokens");
+    check_no_gradient(news, "write_tokens");
     check_pages(pages, lengths);
     TORCH_CHECK_VALUE(!pools.empty() && pools.size() == news.size(), "pools and news must be as many, and at least one, got ",
                       pools.size(), " and ", news.size());
     check_pools(pools, pages, -1);
     for (size_t i = 0; i < news.size(); ++i) {
         const Tensor &n = news[i], &p = pools[i];
+        if (i > 0 && laid_out_alike(news[i - 1], n) && laid_out_alike(pools[i - 1], p)) continue;
         bool same = n.dim() == p.dim() && n.dim() >= 3 && n.size(0) == pages.size(0) && n.size(1) > 0 && n.size(1) == news[0].size(1);
         for (int64_t d = 2; same && d < n.dim(); ++d) same = n.size(d) == p.size(d);
         TORCH_CHECK_VALUE(same, "news[", i, "] must be [S, N, ...] with the row of pools[", i, "], got ", n.sizes(), " for ", p.sizes());
@@ -264,8 +305,19 @@ void write_tokens_hip(Tensors pools, Tensors news, const Tensor& pages, const Te
     const Pools p = bind_pools(pools, pools[0].size(0), pools[0].size(1));
     std::vector<const void*> from;
     std::vector<int64_t> strides;
-    for (Tensor& t : news) {
-        if (!row_contiguous(t, 2)) t = t.contiguous();
+    from.reserve(news.size());
+    strides.reserve(2 * news.size());
+    bool plain = true;
+    for (size_t i = 0; i < news.size(); ++i) {
+        Tensor& t = news[i];
+        if (plain && i > 0 && laid_out_alike(news[i - 1], t)) {
+            from.push_back(t.const_data_ptr());
+            strides.push_back(strides[strides.size() - 2]);
+            strides.push_back(strides[strides.size() - 2]);
+            continue;
+        }
+        plain = row_contiguous(t, 2);
+        if (!plain) t = t.contiguous();
         from.push_back(t.const_data_ptr());
         strides.push_back(t.stride(0) * static_cast<int64_t>(t.element_size()));
         strides.push_back(t.stride(1) * static_cast<int64_t>(t.element_size()));
@@ -273,12 +325,14 @@ void write_tokens_hip(Tensors pools, Tensors news, const Tensor& pages, const Te
     check_status(beamgrad_write_tokens(&p.c, from.data(), strides.data(), i32(pages), i32(lengths), i32(n), narrow(pages.size(0)),
                                        narrow(pages.size(1)), narrow(news[0].size(1)), current_stream()),
                  "write_tokens");
+    written(pools);
 }
 
 // --- keep ---
 
 void check_keep(const Tensors& pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& drafted,
                 const Tensor& keep, const Tensor& kept) {
+    check_no_gradient(pools, "keep_tokens");
     check_table(pages, lengths, refs);
     TORCH_CHECK_VALUE(!pools.empty(), "pools must hold at least one pool");
     check_pools(pools, pages, refs.numel());
@@ -305,6 +359,7 @@ TableOut keep_tokens_hip(Tensors pools, const Tensor& pages, const Tensor& lengt
     check_status(beamgrad_keep_tokens(&p.c, &from, i32(d), i32(k), i32(n), narrow(pages.size(0)), narrow(pages.size(1)),
                                       narrow(k.size(1)), &out, current_stream()),
                  "keep_tokens");
+    written(pools);
     return to.take();
 }
 
@@ -314,6 +369,7 @@ TableOut keep_tokens_hip(Tensors pools, const Tensor& pages, const Tensor& lengt
 
 void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths,
                      const OptTensor& parents, const OptTensor& counts, int64_t beams, const OptTensor& shared, double scale) {
+    check_no_gradient({q, k, v}, "tree_attention");
     TORCH_CHECK_VALUE(q.dim() == 4 && q.numel() > 0, "q must be a [S, N, H, D] tensor, got ", q.sizes());
     data_type(q, "q");
     TORCH_CHECK_VALUE(k.dim() == 4 && k.numel() > 0 && v.sizes() == k.sizes(),
@@ -423,6 +479,7 @@ void check_states(const Tensors& states, const Tensor& parents, const char* name
                       parents.sizes());
     for (size_t i = 0; i < states.size(); ++i) {
         const Tensor& t = states[i];
+        if (i > 0 && laid_out_alike(states[i - 1], t)) continue;
         TORCH_CHECK_VALUE(t.dim() >= 2 && t.size(0) == parents.size(0) && t.size(1) == parents.size(1), name, "[", i,
                           "] must be [B, K, ...] = [", parents.size(0), ", ", parents.size(1), ", ...], got ", t.sizes());
         TORCH_CHECK_VALUE(t.device() == parents.device(), name, "[", i, "] is on ", t.device(), ", parents on ", parents.device());
@@ -432,6 +489,7 @@ void check_states(const Tensors& states, const Tensor& parents, const char* name
 }
 
 void check_inplace(const Tensors& states) {
+    check_no_gradient(states, "reorder_states(inplace=True)");
     for (size_t i = 0; i < states.size(); ++i)
         TORCH_CHECK_VALUE(states[i].is_contiguous(), "states[", i, "] must be contiguous to be reordered in place");
 }
@@ -488,6 +546,7 @@ void reorder_states_inplace_hip(Tensors states, const Tensor& parents) {
     for (const Tensor& t : states)
         if (t.numel() > 0) rows.add(t, t, row_elements(t, 2) * static_cast<int64_t>(t.element_size()));
     run_reorder(rows, parents);
+    written(states);
 }
 
 void check_grads(const Tensors& grads, const Tensor& parents) {
@@ -533,6 +592,113 @@ bool leaf_of_another_stream(const Tensor& leaf) {
     return stream && stream->id() != c10::hip::getCurrentHIPStream(leaf.device().index()).id();
 }
 
+// In a capture: torch hands a leaf's gradient over on the stream that the leaf's
+// accumulator was made on. Where a living graph of another stream holds it, that
+// stream joins the capture and the capture's end ends the process.
+void refuse_foreign_leaves(const torch::autograd::Node* node) {
+    if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const auto& edge : node->next_edges()) {
+        const auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
+        TORCH_CHECK(!leaf || !leaf_of_another_stream(leaf->variable),
+                    "beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of another "
+                    "stream uses; drop that graph (its outputs and losses) before the capture");
+    }
+}
+
+Tensors call_reorder(const Tensors& states, const Tensor& parents) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("beamgrad::reorder_states", "")
+                               .typed<Tensors(Tensors, const Tensor&)>();
+    return op.call(states, parents);
+}
+Tensors call_gather(const Tensors& grads, const Tensor& parents) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("beamgrad::reorder_states_backward", "")
+                               .typed<Tensors(Tensors, const Tensor&)>();
+    return op.call(grads, parents);
+}
+
+// The states in the order of the new beams (or, back, their gradients): what
+// comes in for output i goes to input i, by the other of the two operators, which
+// records in its turn where a graph of the backward is made.
+class ReorderNode : public torch::autograd::Node {
+   public:
+    ReorderNode(const Tensors& inputs, const Tensor& parents, bool gathers)
+        : Node(torch::autograd::collect_next_edges(inputs)), parents_(parents, false), gathers_(gathers) {}
+
+    std::string name() const override { return gathers_ ? "ReorderStatesBackwardBackward" : "ReorderStatesBackward"; }
+    void release_variables() override { parents_.reset_data(); }
+
+   protected:
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        refuse_foreign_leaves(this);
+        const Tensor parents = parents_.unpack(shared_from_this());
+        torch::autograd::variable_list out(grads.size());
+        std::vector<bool> done(grads.size());
+        for (size_t i = 0; i < grads.size(); ++i) {  // one call for each type
+            if (done[i] || !grads[i].defined() || !task_should_compute_output(i)) continue;
+            Tensors some;
+            std::vector<size_t> at;
+            for (size_t j = i; j < grads.size(); ++j) {
+                if (done[j] || !grads[j].defined() || grads[j].scalar_type() != grads[i].scalar_type() ||
+                    !task_should_compute_output(j))
+                    continue;
+                done[j] = true;
+                some.push_back(grads[j]);
+                at.push_back(j);
+            }
+            const Tensors got = gathers_ ? call_reorder(some, parents) : call_gather(some, parents);
+            for (size_t j = 0; j < at.size(); ++j) out[at[j]] = got[j];
+        }
+        return out;
+    }
+
+   private:
+    torch::autograd::SavedVariable parents_;
+    bool gathers_;
+};
+
+// The operator's outputs, those of inputs that require a gradient recorded.
+Tensors recorded(const Tensors& inputs, const Tensor& parents, bool gathers) {
+    Tensors taking;
+    for (const Tensor& t : inputs)
+        if (t.requires_grad()) taking.push_back(t);
+    const auto node = std::shared_ptr<ReorderNode>(new ReorderNode(taking, parents, gathers), torch::autograd::deleteNode);
+    Tensors out;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = gathers ? call_gather(inputs, parents) : call_reorder(inputs, parents);
+    }
+    for (size_t i = 0; i < inputs.size(); ++i)
+        if (inputs[i].requires_grad()) torch::autograd::set_history(out[i], node);
+    return out;
+}
+
+bool records(const Tensors& tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor& t : tensors)
+        if (t.requires_grad()) return true;
+    return false;
+}
+
+Tensors reorder_states_autograd(Tensors states, const Tensor& parents) {
+    if (records(states)) {
+        for (const Tensor& t : states)
+            TORCH_CHECK_TYPE(!t.requires_grad() || t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kFloat16 ||
+                                 t.scalar_type() == torch::kBFloat16,
+                             "reorder_states has a gradient for float32, float16 and bfloat16 states, not ", t.scalar_type());
+        return recorded(states, parents, false);
+    }
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call_reorder(states, parents);
+}
+
+Tensors reorder_states_backward_autograd(Tensors grads, const Tensor& parents) {
+    if (records(grads)) return recorded(grads, parents, true);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call_gather(grads, parents);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(beamgrad, m) {
@@ -561,6 +727,11 @@ TORCH_LIBRARY_IMPL(beamgrad, CUDA, m) {
     m.impl("reorder_states", &reorder_states_hip);
     m.impl("reorder_states_", &reorder_states_inplace_hip);
     m.impl("reorder_states_backward", &reorder_states_backward_hip);
+}
+
+TORCH_LIBRARY_IMPL(beamgrad, Autograd, m) {
+    m.impl("reorder_states", &reorder_states_autograd);
+    m.impl("reorder_states_backward", &reorder_states_backward_autograd);
 }
 
 // Checked, then refused.

@@ -370,24 +370,25 @@ def test_reorder_captured_backward():
         assert torch.equal(out, want[0]) and torch.equal(grad, want[1])
 
 
-def test_reorder_backward_of_a_leaf_of_another_stream(monkeypatch):
+def test_reorder_knows_a_leaf_of_another_stream():
     """A backward in a capture whose leaf belongs to a living graph of another
     stream would pull that stream into the capture, which ends the process: it is
-    refused. (The capture is pretended.)"""
+    refused by this test of the leaf."""
+    other = torch.ops.beamgrad.leaf_of_another_stream
     parents = torch.tensor([[0, 0, 2]]).cuda()
     leaf = torch.randn(1, 3, 64, device="cuda").requires_grad_()
+    assert not other(leaf)
     alive = bg.reorder_states([leaf], parents)[0]
+    assert not other(leaf)
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         out = bg.reorder_states([leaf], parents)[0]
-        with monkeypatch.context() as patch:
-            patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-            with pytest.raises(RuntimeError, match="another stream"):
-                torch.autograd.grad(out.sum(), leaf)
+        assert other(leaf)
         del alive, out
-        with monkeypatch.context() as patch:
-            patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-            torch.autograd.grad(bg.reorder_states([leaf], parents)[0].sum(), leaf)
+        assert not other(leaf)
+        out = bg.reorder_states([leaf], parents)[0]
+        assert not other(leaf)
+    assert other(leaf)
     torch.cuda.current_stream().wait_stream(stream)
     torch.cuda.synchronize()
