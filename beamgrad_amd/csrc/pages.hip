@@ -124,13 +124,18 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(const Table t, const v
         return;
     }
     __shared__ int lds[kPlanThreads / 64];
-    // plan.fresh holds the first sequence that continues each one, until the
-    // fresh pages are known
-    int32_t* const first = plan.fresh;
+    // the first sequence that continues each one, and their counts: in LDS where
+    // there is a thread for each, else in memory (plan.fresh until the fresh pages
+    // are known)
+    __shared__ int32_t near[3][kPlanThreads];
+    const bool small = t.S <= kPlanThreads;
+    int32_t* const first = small ? near[0] : plan.fresh;
+    int32_t* const kids = small ? near[1] : plan.kids;
+    int32_t* const copies = small ? near[2] : plan.copies;
     for (int s = threadIdx.x; s < t.S; s += kPlanThreads) {
         first[s] = t.S;
-        plan.kids[s] = 0;
-        plan.copies[s] = 0;
+        kids[s] = 0;
+        copies[s] = 0;
     }
     __syncthreads();
     for (int s = threadIdx.x; s < t.S; s += kPlanThreads) {
@@ -169,14 +174,20 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(const Table t, const v
         if (rank >= 0) {
             if (rank < found) {
                 fresh = list[rank];
-                atomicAdd(&plan.copies[p], 1);
+                atomicAdd(&copies[p], 1);
             } else {
                 live = false;  // no page left for its tokens
                 t.lengths_out[s] = 0;
             }
         }
-        if (live) atomicAdd(&plan.kids[p], 1);
+        if (live) atomicAdd(&kids[p], 1);
         plan.fresh[s] = live ? fresh : -2;
+    }
+    if (!small) return;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < t.S) {
+        plan.kids[threadIdx.x] = kids[threadIdx.x];
+        plan.copies[threadIdx.x] = copies[threadIdx.x];
     }
 }
 
@@ -327,47 +338,54 @@ __device__ Kept kept_of(const Table& t, const int32_t* drafted, const int32_t* k
     return {length - draft, *lds};
 }
 
-// The kept tokens of sequence x in pool y, and with `refs` (the last y) the
-// counts of the pages, copied. Each thread moves 16 bytes of every token: the
-// numbers ascend, so token i's place is read by no later one, and eight are read
+// The kept tokens of sequence x in `each` pools from y * each on, and as the last y
+// the counts of the pages, copied. Where the tokens lie is looked up once, by a
+// thread for each; then a thread moves 16 bytes of every token: the numbers
+// ascend, so a token's new place is read by no later one, and eight are read
 // before they are written.
 __global__ __launch_bounds__(kCopyThreads) void keep_move(const Table t, const int32_t* drafted, const int32_t* keep,
-                                                          const int32_t* kept, const int width, const PoolSet pools) {
-    if (static_cast<int>(blockIdx.y) == pools.n) {
+                                                          const int32_t* kept, const int width, const PoolSet pools,
+                                                          const int each, const Divider chunks) {
+    if (blockIdx.y + 1 == gridDim.y) {
         for (int64_t i = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x; i < t.span.n_pages;
              i += static_cast<int64_t>(gridDim.x) * kCopyThreads)
             t.refs_out[i] = t.refs[i];
         return;
     }
+    constexpr int kAtOnce = 8, kPlaces = 128;
     __shared__ int first_bad;
+    __shared__ int64_t from[kPlaces], to[kPlaces];  // -1: the token stays, or has no page
     const int s = blockIdx.x;
     const Kept k = kept_of(t, drafted, keep, kept, width, s, &first_bad);
-    char* const base = pools.base[blockIdx.y];
-    const auto place = [&](int token) -> char* {
-        const int column = static_cast<int>(t.span.page.quotient(token)), page = page_at(t, s, column);
-        return page < 0 ? nullptr : base + page * pools.page_stride + (token - column * static_cast<int64_t>(t.span.page.d)) * pools.token_stride;
-    };
-    constexpr int kAtOnce = 8;
     const int32_t* const row = keep + static_cast<int64_t>(s) * width;
-    for (int64_t c = threadIdx.x * 16; c < pools.row_bytes; c += kCopyThreads * 16) {
-        const int64_t left = pools.row_bytes - c;
-        for (int i0 = 0; i0 < k.n; i0 += kAtOnce) {
-            u32x4 x[kAtOnce];
-            char* to[kAtOnce];
+    const auto place = [&](int token) -> int64_t {
+        const int column = static_cast<int>(t.span.page.quotient(token)), page = page_at(t, s, column);
+        return page < 0 ? -1 : page * pools.page_stride + (token - column * static_cast<int64_t>(t.span.page.d)) * pools.token_stride;
+    };
+    const int pool0 = static_cast<int>(blockIdx.y) * each, items = min(each, pools.n - pool0) * static_cast<int>(chunks.d);
+    for (int i0 = 0; i0 < k.n; i0 += kPlaces) {
+        const int here = min(k.n - i0, kPlaces);
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < here) {
+            const int i = i0 + threadIdx.x, node = row[i];
+            const int64_t source = node != i ? place(k.start + node) : -1;
+            from[threadIdx.x] = source;
+            to[threadIdx.x] = source >= 0 ? place(k.start + i) : -1;
+        }
+        __syncthreads();
+        for (int item = threadIdx.x; item < items; item += kCopyThreads) {
+            const int pool = static_cast<int>(chunks.quotient(item)), c = (item - pool * static_cast<int>(chunks.d)) * 16;
+            char* const base = pools.base[pool0 + pool] + c;
+            const int64_t left = pools.row_bytes - c;
+            for (int i1 = 0; i1 < here; i1 += kAtOnce) {
+                u32x4 x[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                to[i] = nullptr;
-                if (i0 + i < k.n && row[i0 + i] != i0 + i) {
-                    const char* const from = place(k.start + row[i0 + i]);
-                    if (from) {
-                        to[i] = place(k.start + i0 + i);
-                        x[i] = load16(from + c, left);
-                    }
-                }
+                for (int i = 0; i < kAtOnce; ++i)
+                    if (i1 + i < here && to[i1 + i] >= 0) x[i] = load16(base + from[i1 + i], left);
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+                    if (i1 + i < here && to[i1 + i] >= 0) store16(base + to[i1 + i], x[i], left);
             }
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i)
-                if (to[i]) store16(to[i] + c, x[i], left);
         }
     }
 }
@@ -537,8 +555,15 @@ DBS_CUDA_EXPORT int beamgrad_keep_tokens(const BeamgradPools* pools, const Beamg
     const Table t = table_of(*from, *to, sequences, table_pages, pools->n_pages, pools->page_tokens);
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     hipError_t e = over_pools(*pools, nullptr, nullptr, [&](const PoolSet& set, bool first) {
-        keep_move<<<dim3(static_cast<unsigned>(sequences), static_cast<unsigned>(set.n + (first ? 1 : 0))), kCopyThreads, 0,
-                    stream>>>(t, drafted, keep, kept, width, set);
+        // a workgroup takes several pools while that leaves many workgroups
+        const int64_t chunks = std::max<int64_t>((set.row_bytes + 15) / 16, 1);
+        int each = 1;
+        while (each < set.n && each * chunks < 2 * kCopyThreads && static_cast<int64_t>(sequences) * set.n > 1024 * each) each *= 2;
+        const int rounds = set.n > 0 ? (set.n + each - 1) / each : 0;
+        (void)first;  // every launch copies the counts: to the same values
+        const unsigned y = static_cast<unsigned>(rounds + 1);
+        keep_move<<<dim3(static_cast<unsigned>(sequences), y), kCopyThreads, 0, stream>>>(
+            t, drafted, keep, kept, width, set, each, Divider::of(static_cast<uint32_t>(chunks)));
         return hipGetLastError();
     });
     if (e == hipSuccess) {

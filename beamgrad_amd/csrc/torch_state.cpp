@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -45,6 +46,12 @@ void check_status(int code, const char* what) {
 
 [[noreturn]] void refuse_cpu(const char* what, const Tensor& t) {
     TORCH_CHECK(false, "beamgrad::", what, " runs on the GPU (HIP) only, got a tensor on ", t.device());
+}
+
+// A contiguous tensor from the caching allocator, without a trip through the
+// dispatcher (a call makes several, and small calls take as long as their host work).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+    return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
 }
 
 // Operators that write or read tensors without recording a gradient.
@@ -204,14 +211,14 @@ using TableOut = std::tuple<Tensor, Tensor, Tensor>;
 struct NewTable {
     Tensor pages, lengths, refs;
     NewTable(const Tensor& p, const Tensor& l, const Tensor& r)
-        : pages(torch::empty_like(p)), lengths(torch::empty_like(l)), refs(torch::empty_like(r)) {}
+        : pages(fresh(p.sizes(), torch::kInt32, p)), lengths(fresh(l.sizes(), torch::kInt32, p)), refs(fresh(r.sizes(), torch::kInt32, p)) {}
     BeamgradTable bind() const { return bind_table(pages, lengths, refs); }
     TableOut take() { return {std::move(pages), std::move(lengths), std::move(refs)}; }
 };
 
 Tensor workspace(int64_t bytes, const Tensor& like) {
     TORCH_CHECK_VALUE(bytes >= 0, "beamgrad HIP: unsupported problem size (see the limits in beamgrad_state.h)");
-    return torch::empty({bytes > 0 ? bytes : 1}, like.options().dtype(torch::kUInt8));
+    return fresh({bytes > 0 ? bytes : 1}, torch::kUInt8, like);
 }
 
 // --- fork ---
@@ -434,9 +441,8 @@ std::tuple<Tensor, Tensor> tree_attention_hip(const Tensor& q, const Tensor& k, 
     if (parents) par = as_i32(*parents);
     if (counts) num = as_i32(*counts);
     if (shared) sh = as_i32(*shared);
-    Tensor out = torch::empty(q.sizes(), q.options());
-    Tensor lse = with_lse ? torch::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(torch::kFloat32))
-                          : torch::empty({0}, q.options().dtype(torch::kFloat32));
+    Tensor out = fresh(q.sizes(), q.scalar_type(), q);
+    Tensor lse = with_lse ? fresh({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q) : fresh({0}, torch::kFloat32, q);
     BeamgradAttention a{};
     a.q = query.const_data_ptr();
     a.k = k.const_data_ptr();
@@ -525,7 +531,7 @@ Tensors reorder_states_hip(Tensors states, const Tensor& parents) {
     StateRows rows;
     for (Tensor& t : states) {
         t = t.contiguous();
-        out.push_back(torch::empty(t.sizes(), t.options()));
+        out.push_back(fresh(t.sizes(), t.scalar_type(), t));
         if (t.numel() > 0) rows.add(t, out.back(), row_elements(t, 2) * static_cast<int64_t>(t.element_size()));
     }
     run_reorder(rows, parents);
@@ -569,7 +575,7 @@ Tensors reorder_states_backward_hip(Tensors grads, const Tensor& parents) {
     StateRows rows;
     for (Tensor& t : grads) {
         t = t.contiguous();
-        out.push_back(torch::empty(t.sizes(), t.options()));
+        out.push_back(fresh(t.sizes(), t.scalar_type(), t));
         if (t.numel() > 0) rows.add(t, out.back(), row_elements(t, 2));
     }
     if (rows.from.empty()) return out;
