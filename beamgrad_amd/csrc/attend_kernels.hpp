@@ -122,6 +122,9 @@ struct Dims {
     static constexpr int kMerge = kKeyWaves > 1 ? kAccs * 4 * 64 * 16 : 0;
     static constexpr int kLds = kPlaces * kTile > kMerge ? kPlaces * kTile : kMerge;
     static constexpr int kTokens = kRows;  // of a tile of rows, at most
+    // Beginning and ending a piece takes some 5 us: as long as four rounds of four
+    // small tiles, or one or two large ones.
+    static constexpr int kPieceCost = kRowWaves == 1 ? 4 * kKeyWaves : 2;
     static constexpr int kSlot = kRows * (DP + 3);  // floats of a partial result
     // workgroups of a CU: what its 160 KB of LDS hold
     static constexpr int kOther = kTokens * (kAttendMaxTree / 8) + 2 * kAttendMaxTree + 12 * kKeyWaves * kRows + 20 * kAttendSequences + 64;
@@ -231,15 +234,33 @@ __device__ __forceinline__ int row_tiles(const AttendParams& p, const Sequence& 
 // What a workgroup knows of the call's sequences.
 struct Board {
     int length[kAttendSequences], count[kAttendSequences];
-    int first[kAttendSequences];   // a cache head's units ahead of the sequence's (and its group's shared ones)
+    int first[kAttendSequences];   // a cache head's elements of the line ahead of the sequence's (and its group's shared ones)
     int shared[kAttendSequences];  // of a group: tokens in pages that its beams share
     int leader[kAttendSequences];  // of a group: a live sequence
     int sum[4], items[4], largest[4];
 };
 
 struct Totals {
-    int units, items, largest;  // of a cache head; the largest item's units
+    int line, items, largest;  // of a cache head: units, items; the largest item's units
 };
+
+// The line's elements ahead of each sequence, from those of each (thread s:
+// sequence s); returns a cache head's.
+__device__ __forceinline__ int set_line(Board& b, int elements) {
+    const int upto = wave_upto(elements), wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) b.sum[wave] = upto;
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += b.sum[w];
+        total += b.sum[w];
+    }
+    b.first[threadIdx.x] = before + upto - elements;
+    __syncthreads();
+    return uniform(total);
+}
 
 // Fills the board. Sequence s is thread s's.
 template <int ROWS>
@@ -282,28 +303,40 @@ __device__ __forceinline__ Totals fill_board(const AttendParams& p, Board& b, in
         else
             for (int t = 0; t < tiles; ++t) units += (key_end<ROWS>(p, me, t) - from + unit - 1) >> unit_log;
     }
-    const int upto = wave_upto(units), wave = s >> 6;
     items = wave_upto(items);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) largest = max(largest, __shfl_xor(largest, d));
     if ((s & 63) == 63) {
-        b.sum[wave] = upto;
-        b.items[wave] = items;
-        b.largest[wave] = largest;
+        b.items[s >> 6] = items;
+        b.largest[s >> 6] = largest;
     }
-    __syncthreads();
-    Totals total{0, 0, 0};
-    int before = 0;
+    Totals total{set_line(b, units), 0, 0};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += b.sum[w];
-        total.units += b.sum[w];
         total.items += b.items[w];
         total.largest = max(total.largest, b.largest[w]);
     }
-    b.first[s] = before + upto - units;
-    __syncthreads();
-    return {uniform(total.units), uniform(total.items), uniform(total.largest)};
+    return {total.line, uniform(total.items), uniform(total.largest)};
+}
+
+// The line in pieces of up to `each` units of one item, in place of units.
+template <int ROWS>
+__device__ __forceinline__ int pieces_board(const AttendParams& p, Board& b, int unit_log, int each) {
+    const int s = threadIdx.x, unit = 1 << unit_log;
+    const Sequence me{b.length[s], b.count[s]};
+    int pieces = 0, from = 0;
+    if (p.shared && s < p.S) {
+        from = b.shared[s / p.K];
+        if (s % p.K == 0) pieces = p.shared_tiles * ((((from + unit - 1) >> unit_log) + each - 1) / each);
+    }
+    if (me.count > 0) {
+        const int tiles = row_tiles(p, me, ROWS);
+        if (p.parents || tiles == 1)
+            pieces += tiles * ((((me.length - from + unit - 1) >> unit_log) + each - 1) / each);
+        else
+            for (int t = 0; t < tiles; ++t) pieces += (((key_end<ROWS>(p, me, t) - from + unit - 1) >> unit_log) + each - 1) / each;
+    }
+    return set_line(b, pieces);
 }
 
 // ---------------------------------------------------------------------------
@@ -350,12 +383,31 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     constexpr int kKeyLog = KEYS == 64 ? 6 : KEYS == 32 ? 5 : 4;
     const int unit_log = kKeyLog + p0.unit_shift, unit = 1 << unit_log;
     const Totals board_totals = fill_board<ROWS>(p0, board, unit_log);
-    const int head_units = board_totals.units, total = head_units * p0.Hkv;
+    const int items = board_totals.items * p0.Hkv;
+    int head_line = board_totals.line, total = head_line * p0.Hkv;
     int each = (total + p0.grid - 1) / p0.grid;
     each = (max(each, 1) + WK - 1) / WK * WK;
     // Many items, none of them larger than a stretch: a workgroup for each whole
     // one, no pieces to join, and the hardware hands them out as workgroups end.
-    const bool whole_items = WR > 1 && !p0.shared && board_totals.items * p0.Hkv >= 2 * p0.grid && board_totals.largest <= each;
+    const bool whole_items = WR > 1 && !p0.shared && items >= 2 * p0.grid && board_totals.largest <= each;
+    // Or each item is cut by itself, so that no workgroup has pieces of two: a piece
+    // costs as much as kPieceCost units beside its own, but these cuts are longer.
+    // With `each` of either form there are at most grid pieces: an item has at most
+    // units / each + 1, or at most `cuts`.
+    bool by_pieces = false;
+    if (!whole_items && items <= p0.grid && items > 0) {
+        const int cuts = p0.grid / items;
+        int longer = (board_totals.largest + cuts - 1) / cuts;
+        if (items < p0.grid) longer = min(longer, (total + p0.grid - items - 1) / (p0.grid - items));
+        longer = (max(longer, 1) + WK - 1) / WK * WK;
+        by_pieces = longer - each <= X::kPieceCost || static_cast<int64_t>(longer - each) * total <= static_cast<int64_t>(X::kPieceCost) * each * items;
+        if (by_pieces) {
+            each = longer;
+            head_line = pieces_board<ROWS>(p0, board, unit_log, each);
+            total = head_line * p0.Hkv;
+        }
+    }
+    const int stretch = by_pieces ? 1 : each;
     int mine, at, stop;
     Piece chosen;
     if (whole_items) {
@@ -400,11 +452,11 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
     } else {
         // neighbours share keys, so they lie on one XCD: workgroups go round the
         // eight of them
-        const int busy = (total + each - 1) / each, per_xcd = (busy + 7) / 8;
+        const int busy = (total + stretch - 1) / stretch, per_xcd = (busy + 7) / 8;
         mine = static_cast<int>(blockIdx.x & 7) * per_xcd + static_cast<int>(blockIdx.x >> 3);
         if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || mine >= busy) return;
-        at = mine * each;
-        stop = min(at + each, total);
+        at = mine * stretch;
+        stop = min(at + stretch, total);
     }
 
     while (at < stop) {
@@ -422,8 +474,8 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
             if (threadIdx.x == 0) p1.info[w.item] = make_int4(0, 0, 0, 0);
             at = stop;
         } else {
-        w.head = at / head_units;
-        int off = at - w.head * head_units;  // in the head, then in the sequence, then in the item
+        w.head = at / head_line;
+        int off = at - w.head * head_line;  // in the head, then in the sequence, then in the item
         int seq = -1;
         for (int s0 = 0; s0 < p1.S; s0 += 64) {
             const bool ahead = s0 + lane < p1.S && board.first[s0 + lane] <= off;
@@ -432,39 +484,43 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         off -= uniform(board.first[seq]);
         group = p1.shared ? seq / p1.K : seq;
         const int from = p1.shared ? uniform(board.shared[group]) : 0;
-        int units = (from + unit - 1) >> unit_log, end = from;
+        // elements of the line that so many units are
+        const auto elements = [&](int units) { return by_pieces ? (units + each - 1) / each : units; };
+        int units = (from + unit - 1) >> unit_log, end = from, length = elements(units);
         int place_in_head = group * (p1.shared_tiles + p1.K * p1.own_tiles);
-        w.shared = p1.shared && seq == group * p1.K && off < p1.shared_tiles * units;
+        w.shared = p1.shared && seq == group * p1.K && off < p1.shared_tiles * length;
         if (w.shared) {
-            w.tile = off / units;
-            off -= w.tile * units;
+            w.tile = off / length;
+            off -= w.tile * length;
             w.seq = uniform(board.leader[group]);
             w.own = {uniform(board.length[w.seq]), uniform(board.count[w.seq])};
             w.key0 = 0;
             place_in_head += w.tile;
         } else {
-            if (p1.shared && seq == group * p1.K) off -= p1.shared_tiles * units;
+            if (p1.shared && seq == group * p1.K) off -= p1.shared_tiles * length;
             w.seq = seq;
             w.own = {uniform(board.length[seq]), uniform(board.count[seq])};
             w.key0 = from;
             if (p1.parents || row_tiles(p1, w.own, ROWS) == 1) {
                 end = w.own.length;
                 units = (end - from + unit - 1) >> unit_log;
-                w.tile = off / units;
-                off -= w.tile * units;
+                length = elements(units);
+                w.tile = off / length;
+                off -= w.tile * length;
             } else {
                 // tiles of rows that read ever more keys: a lane for each
                 for (w.tile = 0;; w.tile += 64) {
                     const int t = w.tile + lane;
                     const int mine_end = key_end<ROWS>(p1, w.own, t);
-                    const int n = t < p1.own_tiles ? (mine_end - from + unit - 1) >> unit_log : 0;
-                    const int upto = wave_upto(n);
+                    const int mine_units = t < p1.own_tiles ? (mine_end - from + unit - 1) >> unit_log : 0;
+                    const int n = elements(mine_units), upto = wave_upto(n);
                     const uint64_t past = __ballot(upto > off);
                     if (past) {
                         const int first = __builtin_ctzll(past);
                         w.tile += first;
-                        units = __shfl(n, first);
-                        off -= __shfl(upto, first) - units;
+                        units = __shfl(mine_units, first);
+                        length = __shfl(n, first);
+                        off -= __shfl(upto, first) - length;
                         end = __shfl(mine_end, first);
                         break;
                     }
@@ -475,17 +531,28 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         }
         off = uniform(off);
         units = uniform(units);
+        length = uniform(length);
         end = uniform(end);
         w.tile = uniform(w.tile);
         w.item = uniform(w.head * p1.head_items + place_in_head);
-        const int start = at - off, until = min(start + units, stop);
-        w.end = min(end, w.key0 + ((until - start) << unit_log));
-        w.key0 += off << unit_log;
         w.starts = off == 0;
-        w.whole = w.starts && until == start + units && from == 0;
-        if (w.starts && threadIdx.x == 0)
-            p1.info[w.item] = make_int4(mine, (start + units - 1) / each, from > 0, 0);
-        at = until;
+        int first_unit = off, n_units, last;
+        if (by_pieces) {
+            first_unit = off * each;
+            n_units = min(each, units - first_unit);
+            last = mine - off + length - 1;
+            w.whole = length == 1 && from == 0;
+            at = stop;
+        } else {
+            const int start = at - off, until = min(start + units, stop);
+            n_units = until - at;
+            last = (start + units - 1) / each;
+            w.whole = w.starts && until == start + units && from == 0;
+            at = until;
+        }
+        w.key0 += first_unit << unit_log;
+        w.end = min(end, w.key0 + (n_units << unit_log));
+        if (w.starts && threadIdx.x == 0) p1.info[w.item] = make_int4(mine, last, from > 0, 0);
         }
 
         // ---- the piece's rows ----
@@ -519,8 +586,9 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         int masked_from = INT32_MAX;
         const int first_token = static_cast<int>(p.G.quotient(w.tile * ROWS));
         if (!w.shared) masked_from = prefix + (p.parents ? 0 : first_token + 1);
+        if (masked_from >= w.end) masked_from = INT32_MAX;  // as of a single token
         const int words = (p.N + 31) >> 5;
-        if (p.parents && w.end > masked_from) {
+        if (p.parents && masked_from != INT32_MAX) {
             // which drafted tokens each token of the tile sees, as bits
             __syncthreads();
             for (int i = threadIdx.x; i < p.N; i += kAttendThreads)
@@ -578,7 +646,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         };
         // this wavefront's share of a tile, from memory straight into LDS
         constexpr uint64_t kFull = ~uint64_t{0} >> (64 - KEYS);
-        const auto fill = [&](char* region, const char* head, int64_t mine_at, uint64_t there) BEAMGRAD_INLINE {
+        const auto fill = [&](bool values, char* region, const char* head, int64_t mine_at, uint64_t there) BEAMGRAD_INLINE {
             if (there == kFull) {
 #pragma unroll
                 for (int i = 0; i < X::kLoads; ++i) {
@@ -590,17 +658,24 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 }
                 return;
             }
+            // What no token fills must not be a NaN or an infinity, as a value (as a
+            // key it is masked). All these stores come before the loads: between
+            // them each would wait for the loads ahead of it.
             const int lane_here = opaque(lane);
+            if (values) {
+#pragma unroll
+                for (int i = 0; i < X::kLoads; ++i) {
+                    const int c = (i * WR + wr) * 64 + lane_here;
+                    if (!((there >> (c / X::kChunks)) & 1)) *reinterpret_cast<f32x4*>(region + c * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
 #pragma unroll
             for (int i = 0; i < X::kLoads; ++i) {
                 const int block = i * WR + wr;
                 const int c = block * 64 + lane_here, row = c / X::kChunks, chunk = (c % X::kChunks) ^ (row & X::kSwizzle);
                 const int64_t row_at = shfl64(mine_at, row);
-                char* const to = region + block * 1024;
-                if (row_at < 0)  // what no token fills must not be a NaN or an infinity
-                    *reinterpret_cast<f32x4*>(to + lane_here * 16) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                else if (chunk < chunks)
-                    __builtin_amdgcn_global_load_lds((global_char*)(head + row_at + chunk * 16), (lds_char*)to, 16, 0, 0);
+                if (row_at >= 0 && chunk < chunks)
+                    __builtin_amdgcn_global_load_lds((global_char*)(head + row_at + chunk * 16), (lds_char*)(region + block * 1024), 16, 0, 0);
             }
         };
         const auto region = [&](int place, int value) { return lds + place * X::kTile + (value * WK + wk) * X::kRegion; };
@@ -779,12 +854,12 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
             int64_t k_at, v_at, v_next;
             uint64_t there = locate(mine_first, k_at, v_at), there_next = 0;
             look_up(mine_first + kNext);
-            fill(region(0, 0), k_head, k_at, there);
-            fill(region(0, 1), v_head, v_at, there);
+            fill(true, region(0, 1), v_head, v_at, there);
+            fill(false, region(0, 0), k_head, k_at, there);
             if (rounds > 1) {
                 there_next = locate(mine_first + kNext, k_at, v_next);
                 look_up(mine_first + 2 * kNext);
-                fill(region(1, 0), k_head, k_at, there_next);
+                fill(false, region(1, 0), k_head, k_at, there_next);
             }
             wait_all();
             barrier();
@@ -796,11 +871,11 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 wait_all();
                 barrier();
                 uint64_t there_after = 0;
-                if (round + 1 < rounds) fill(region(PLACE ^ 1, 1), v_head, v_next, there_next);
+                if (round + 1 < rounds) fill(true, region(PLACE ^ 1, 1), v_head, v_next, there_next);
                 if (round + 2 < rounds) {
                     there_after = locate(first + 2 * kNext, k_at, v_next);
                     look_up(first + 3 * kNext);
-                    fill(region(PLACE, 0), k_head, k_at, there_after);
+                    fill(false, region(PLACE, 0), k_head, k_at, there_after);
                 }
                 if (round + 1 < rounds) score(region(PLACE ^ 1, 0), s[PLACE ^ 1]);
                 absorb(first, there, region(PLACE, 1), s[PLACE]);
@@ -817,8 +892,8 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 const uint64_t there = locate(first, k_at, v_at);
                 look_up(first + kNext);
                 wait_lds();
-                fill(region(0, 0), k_head, k_at, there);
-                fill(region(0, 1), v_head, v_at, there);
+                fill(true, region(0, 1), v_head, v_at, there);
+                fill(false, region(0, 0), k_head, k_at, there);
                 wait_all();
                 f32x4 s[KB][RB];
                 score(region(0, 0), s);
