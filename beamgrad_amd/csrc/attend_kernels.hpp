@@ -91,8 +91,9 @@ struct Dims {
     static_assert(kRows == attend_rows(SHAPE));
     // Keys of a wavefront's tile: 32 fill the 16-bit matrix instruction's depth
     // for P V, 16 the float32 one's. A tile shared by four wavefronts is twice
-    // as long where LDS holds two workgroups of it, for half the barriers.
-    static constexpr int kKeys = SHAPE == kRows128 ? (k32 ? 32 : DP <= 128 ? 64 : 32) : (k32 ? 16 : 32);
+    // as long, for half the barriers, where two tiles' scores fit the registers
+    // beside the sums: trees at width 128 take 98 us with 64 keys and 88 with 32.
+    static constexpr int kKeys = SHAPE == kRows128 ? (k32 ? 32 : DP <= 64 ? 64 : 32) : (k32 ? 16 : 32);
     static constexpr int kKeyBlocks = kKeys / 16;
     static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
     static constexpr int kRowBytes = kChunks * 16;
