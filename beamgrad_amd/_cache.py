@@ -43,6 +43,39 @@ _ops = SimpleNamespace(**{name: getattr(_torch_ops, name).default for name in (
     "tree_attention", "fork_pages", "extend_pages", "write_tokens", "keep_tokens", "reorder_states", "reorder_states_")})
 
 
+def _register_fakes() -> None:
+    """Shape-only forms (torch.compile, export, meta tensors)."""
+
+    def tree_attention(q, _k, _v, _pages, _lengths, _parents, _counts, _beams, _shared, _scale, with_lse):
+        return q.new_empty(q.shape), q.new_empty(q.shape[:3] if with_lse else (0,), dtype=torch.float32)
+
+    def table(pages, lengths, refs):
+        return torch.empty_like(pages), torch.empty_like(lengths), torch.empty_like(refs)
+
+    def fork_pages(_pools, pages, lengths, refs, _parents):
+        return table(pages, lengths, refs)
+
+    def extend_pages(pages, lengths, refs, _counts, _page_tokens):
+        return table(pages, lengths, refs)
+
+    def keep_tokens(_pools, pages, lengths, refs, *_rest):
+        return table(pages, lengths, refs)
+
+    def nothing(*_args):
+        return None
+
+    def states(tensors, _parents):
+        return [t.new_empty(t.shape) for t in tensors]
+
+    for name, fn in (("tree_attention", tree_attention), ("fork_pages", fork_pages), ("extend_pages", extend_pages),
+                     ("write_tokens", nothing), ("keep_tokens", keep_tokens), ("reorder_states", states),
+                     ("reorder_states_", nothing), ("reorder_states_backward", states)):
+        torch.library.register_fake(f"beamgrad::{name}", fn)
+
+
+_register_fakes()
+
+
 class PageTable(NamedTuple):
     """Which pages hold the tokens of ``S`` sequences (of a search: example
     ``b``'s beam ``k`` is sequence ``b * K + k``)."""

@@ -20,7 +20,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kStatesOfLaunch = 64;   // whose addresses one launch's arguments hold
 constexpr int kMaxBeams = 4096;
-constexpr int kTileBytes = 64 * 1024; // of LDS, for a tile of an example's rows
+constexpr int kTileBytes = 16 * 1024; // of LDS, for a tile of an example's rows: eight workgroups a CU
+constexpr int kMostTileBytes = 64 * 1024;
 constexpr int kAtOnce = 4;            // 16-byte reads of a thread in flight
 
 // States of one row length.
@@ -59,13 +60,14 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(const StateSet set, c
 // In place: a workgroup takes `width` bytes of every row of example y of state
 // z, reads those that move into LDS, and writes them where they go. Rows that
 // stay are neither read nor written, unless another continues them too.
+// With tiles of 16 KB all of a thread's reads are in flight together.
 __global__ __launch_bounds__(kThreads) void reorder_inplace(const StateSet set, const void* parents, const bool i64,
-                                                            const int K, const int width) {
-    __shared__ u32x4 tile[kTileBytes / 16];
-    __shared__ int16_t parent[kMaxBeams];
-    __shared__ uint8_t moves[kMaxBeams];  // a row that another one continues
+                                                            const int K, const Divider chunks) {
+    extern __shared__ u32x4 tile[];  // K rows of the tile, then the two arrays below
+    int16_t* const parent = reinterpret_cast<int16_t*>(tile + K * chunks.d);
+    uint8_t* const moves = reinterpret_cast<uint8_t*>(parent + K);  // a row that another one continues
     char* const rows = set.to[blockIdx.z] + static_cast<int64_t>(blockIdx.y) * K * set.row_bytes;
-    const int64_t byte0 = static_cast<int64_t>(blockIdx.x) * width;
+    const int64_t byte0 = static_cast<int64_t>(blockIdx.x) * chunks.d * 16;
     for (int k = threadIdx.x; k < K; k += kThreads) moves[k] = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < K; k += kThreads) {
@@ -74,18 +76,27 @@ __global__ __launch_bounds__(kThreads) void reorder_inplace(const StateSet set, 
         if (p >= 0 && p != k) moves[p] = 1;
     }
     __syncthreads();
-    const int chunks = width / 16;
-    for (int i = threadIdx.x; i < K * chunks; i += kThreads) {
-        const int k = i / chunks;
-        const int64_t byte = byte0 + (i - k * chunks) * 16;
-        if (moves[k] && byte < set.row_bytes) tile[i] = load16(rows + k * set.row_bytes + byte, set.row_bytes - byte);
+    const int items = K * static_cast<int>(chunks.d);
+    for (int i0 = threadIdx.x; i0 < items; i0 += kThreads * kAtOnce) {
+        u32x4 x[kAtOnce];
+        bool there[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int i = i0 + j * kThreads, k = static_cast<int>(chunks.quotient(i));
+            const int64_t byte = byte0 + (i - k * static_cast<int>(chunks.d)) * 16;
+            there[j] = i < items && moves[k] && byte < set.row_bytes;
+            if (there[j]) x[j] = load16(rows + k * set.row_bytes + byte, set.row_bytes - byte);
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (there[j]) tile[i0 + j * kThreads] = x[j];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < K * chunks; i += kThreads) {
-        const int k = i / chunks, c = i - k * chunks, p = parent[k];
+    for (int i = threadIdx.x; i < items; i += kThreads) {
+        const int k = static_cast<int>(chunks.quotient(i)), c = i - k * static_cast<int>(chunks.d), p = parent[k];
         const int64_t byte = byte0 + c * 16;
         if (p != k && byte < set.row_bytes)
-            store16(rows + k * set.row_bytes + byte, p < 0 ? u32x4{0, 0, 0, 0} : tile[p * chunks + c], set.row_bytes - byte);
+            store16(rows + k * set.row_bytes + byte, p < 0 ? u32x4{0, 0, 0, 0} : tile[p * static_cast<int>(chunks.d) + c], set.row_bytes - byte);
     }
 }
 
@@ -174,9 +185,12 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states(const void* const* from, void* const
         const int64_t chunks = (set.row_bytes + 15) / 16;
         const unsigned y = static_cast<unsigned>(examples), z = static_cast<unsigned>(set.n);
         if (inplace) {
-            const int64_t width = std::min<int64_t>({chunks * 16, kThreads * 16, kTileBytes / beams / 16 * 16});
-            reorder_inplace<<<dim3(static_cast<unsigned>((set.row_bytes + width - 1) / width), y, z), kThreads, 0, stream>>>(
-                set, parents, parents_i64 != 0, beams, static_cast<int>(width));
+            // many beams: narrower pieces of their rows, of 256 bytes while LDS has room
+            const int64_t room = std::max<int64_t>(kTileBytes / beams, std::min<int64_t>(kMostTileBytes / beams, 256)) / 16;
+            const int64_t of_tile = std::max<int64_t>(1, std::min<int64_t>(chunks, room));
+            const size_t lds = static_cast<size_t>(beams) * (static_cast<size_t>(of_tile) * 16 + 3);
+            reorder_inplace<<<dim3(static_cast<unsigned>((chunks + of_tile - 1) / of_tile), y, z), kThreads, lds, stream>>>(
+                set, parents, parents_i64 != 0, beams, Divider::of(static_cast<uint32_t>(of_tile)));
         } else {
             const int64_t each = kThreads * kAtOnce;
             reorder_kernel<<<dim3(static_cast<unsigned>((beams * chunks + each - 1) / each), y, z), kThreads, 0, stream>>>(

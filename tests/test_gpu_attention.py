@@ -294,3 +294,67 @@ def test_captured():
         torch.cuda.synchronize()
         want = call()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_more_sequences_than_a_launch_takes():
+    """Groups of beams over several launches."""
+    K = 3
+    shared = [(5 * b) % 40 for b in range(110)]
+    lengths = [shared[s // K] + 1 + s % 7 for s in range(110 * K)]
+    check(build(BF16, lengths, 1, 2, 1, 32, 8, K=K, shared=shared))
+
+
+def test_a_table_of_many_pages():
+    """A table that could hold two thousand million tokens a sequence, few of them
+    there: the cuts of the work stay in 31 bits."""
+    c = build(F16, [2500], 1, 32, 32, 8, 1000)
+    wide = torch.full((1, 2_000_000), -1, dtype=torch.int32)
+    wide[:, :c["pages"].shape[1]] = c["pages"]
+    want = expected(c)
+    check(c, run(c, pages=wide.cuda()), want=want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_unseen_values_of_a_long_cache(dtype):
+    """An infinite value in a drafted token of a sequence that several workgroups
+    share."""
+    N, at = 40, 1500 + 11
+    c = build(dtype, [1500 + N, 30], N, 2, 1, 64, 16, tree=True, counts=[N, 0], seed=2)
+    want = expected(c)
+    c["v"][int(c["pages"][0, at // 16]), at % 16, 0, 7] = math.inf
+    out, lse = (t.cpu().double() for t in run(c))
+    bound, lse_bound = ref.attention_bounds(dtype, *want, 1500 + N, 8.0)
+    for i in range(N):
+        if 11 in ref.seen_by(i, N, c["parents"][0]):
+            assert bool(torch.isinf(out[0, i, :, 7]).all()) and bool(out[0, i, :, :7].isfinite().all())
+        else:
+            assert bool(((out[0, i] - want[0][0, i]).abs() <= bound[0, i]).all())
+    assert bool(((lse - want[1]).abs() <= lse_bound)[0].all())
+
+
+def test_many_rows():
+    """So many tiles of rows that each is one workgroup's: the ends of long prompts,
+    of unlike lengths; against 64 bits on the GPU."""
+    N, H, D, page = 2048, 32, 32, 32
+    lengths, counts = [N + 70, N - 100], [N, 1500]
+    rows = ref.sequence_rows(lengths, page)
+    pages, refs = ref.make_table(rows, 1, 0)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(2, N, H, D, device="cuda", generator=g).to(BF16)
+    k, v = (torch.randn(refs.numel(), page, H, D, device="cuda", generator=g).to(BF16) for _ in range(2))
+    table = bg.PageTable(pages.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), refs.cuda())
+    out, lse = bg.tree_attention(q, k, v, table, counts=torch.tensor(counts).cuda(), return_lse=True)
+    for s, (n, c) in enumerate(zip(lengths, counts, strict=True)):
+        held = pages[s, :-(-n // page)].long().cuda()
+        seen = torch.arange(n, device="cuda") <= torch.arange(c, device="cuda")[:, None] + n - c
+        for h in range(0, H, 5):
+            key, value = (t[held, :, h].flatten(0, 1)[:n].double() for t in (k, v))
+            row = q[s, :c, h].double()
+            score = (row @ key.T / math.sqrt(D)).masked_fill(~seen, -math.inf)
+            p = torch.softmax(score, -1)
+            error = (row.abs() @ key.abs().T).amax(-1) / math.sqrt(D) * (D + 2) * 2.0**-24
+            want = (p @ value, torch.logsumexp(score, -1), p @ value.abs(), error)
+            bound, lse_bound = ref.attention_bounds(BF16, *want, n, 8.0)
+            assert bool(((out[s, :c, h].double() - want[0]).abs() <= bound).all())
+            assert bool(((lse[s, :c, h].double() - want[1]).abs() <= lse_bound).all())
+        assert bool((out[s, c:] == 0).all()) and bool(torch.isneginf(lse[s, c:]).all())

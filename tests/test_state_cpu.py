@@ -228,3 +228,20 @@ int main(void) {
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", f"-I{ROOT}/include", str(src), f"-L{lib}", "-ldbs_hip",
                     f"-Wl,-rpath,{lib}", f"-L{_build.ROCM}/lib", f"-Wl,-rpath,{_build.ROCM}/lib", "-lamdhip64", "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], timeout=60).returncode == 0
+
+
+def test_shapes_without_a_gpu():
+    """Meta tensors pass through every operator."""
+    meta = torch.device("meta")
+    t = bg.PageTable.empty(4, 5, 20, device=meta)
+    pool = torch.zeros(20, 8, 2, 16, device=meta)
+    ones = torch.ones(4, dtype=torch.int32, device=meta)
+    out, lse = bg.tree_attention(torch.zeros(4, 3, 4, 16, device=meta), pool, pool, t, return_lse=True)
+    assert out.shape == (4, 3, 4, 16) and lse.shape == (4, 3, 4) and lse.dtype == torch.float32
+    for new in (bg.fork_pages([pool], t, ones), bg.extend_pages(t, ones, 8),
+                bg.keep_tokens([pool], t, ones, torch.zeros(4, 2, dtype=torch.int32, device=meta), ones)):
+        assert [x.shape for x in new] == [x.shape for x in t] and all(x.dtype == torch.int32 for x in new)
+    assert bg.write_tokens([pool], [torch.zeros(4, 3, 2, 16, device=meta)], t) is None
+    parents = torch.zeros(2, 3, dtype=torch.int64, device=meta)
+    states = [torch.zeros(2, 3, 7, device=meta, requires_grad=True)]
+    assert bg.reorder_states(states, parents)[0].shape == (2, 3, 7)
