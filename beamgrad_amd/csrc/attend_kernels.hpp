@@ -24,6 +24,14 @@
 // matrix instruction with a row of ones: vector instructions are what bounds a
 // tile of many rows, and a weighted mean of rounded weights has no error where the
 // values are equal. The log-sum that a caller asks for is the unrounded values'.
+//
+// What bounds it, on one MI355X: few rows, the reads (two sequences of 90000 to
+// 131000 tokens, 8 cache heads of 128, bfloat16: 946 MB in 168 us, 5.6 TB/s); many
+// rows, the latency of a tile's steps with two workgroups a CU, whose registers are
+// full (4 prompts' ends of 1000 tokens over 1500 to 4500, 32 heads of 64: 113 GFLOP
+// in 229 us, vector instructions issued in 55 % of the time, matrix ones busy in 27);
+// short caches, the chain of dependent reads (700 tokens: 10 us, of which the lengths
+// and totals 3).
 #pragma once
 
 #include <type_traits>
@@ -1060,7 +1068,8 @@ __device__ __forceinline__ void plain_row(const AttendParams& p, int seq, const 
 // as a workgroup takes at once: a thread has four columns of a row, and where rows
 // are few, several threads share the pieces of one. All reads of eight pieces are in
 // flight together: their places follow from the item's first and last workgroup. A
-// row that asks nothing gets 0 and -inf.
+// row that asks nothing gets 0 and -inf. Takes 4 us for a few pieces of 32 rows, 9
+// for 33 pieces of each of 64 rows.
 // Rows of which a piece's maximum is no number are computed again, as are those of
 // an item that says so.
 template <int DTYPE, int DP, int SHAPE>
