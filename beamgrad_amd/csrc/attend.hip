@@ -36,7 +36,8 @@ bool valid_sizes(const BeamgradAttention* a) {
     if (static_cast<double>(a->tokens) * a->heads * a->sequences > 2.0e9) return false;
     const int64_t size = a->data_type == DBS_CUDA_DTYPE_F32 ? 4 : 2;
     for (int i = 0; i < 3; ++i)
-        if (!multiple16(a->q_strides[i], size) || !multiple16(a->k_strides[i], size) || !multiple16(a->v_strides[i], size))
+        // (a page's stride in 16 bytes has 32 bits)
+        if (a->k_strides[i] > (int64_t{1} << 33) || a->v_strides[i] > (int64_t{1} << 33) || !multiple16(a->q_strides[i], size) || !multiple16(a->k_strides[i], size) || !multiple16(a->v_strides[i], size))
             return false;
     return true;
 }
@@ -126,6 +127,8 @@ DBS_CUDA_EXPORT int beamgrad_tree_attention(const BeamgradAttention* args, void*
     p.qs = a.q_strides[0] * size, p.qn = a.q_strides[1] * size, p.qh = a.q_strides[2] * size;
     p.kp = a.k_strides[0] * size, p.kt = a.k_strides[1] * size, p.kh = a.k_strides[2] * size;
     p.vp = a.v_strides[0] * size, p.vt = a.v_strides[1] * size, p.vh = a.v_strides[2] * size;
+    p.kp16 = static_cast<uint32_t>(p.kp / 16), p.kt16 = static_cast<uint32_t>(p.kt / 16);
+    p.vp16 = static_cast<uint32_t>(p.vp / 16), p.vt16 = static_cast<uint32_t>(p.vt / 16);
     p.span = {Divider::of(static_cast<uint32_t>(a.page_tokens)), a.n_pages, a.table_pages};
     p.pages = a.pages;
     p.lengths = a.lengths;

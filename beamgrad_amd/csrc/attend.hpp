@@ -30,6 +30,7 @@ struct AttendParams {
     int64_t qs, qn, qh;  // strides in bytes
     int64_t kp, kt, kh;
     int64_t vp, vt, vh;
+    uint32_t kp16, kt16, vp16, vt16;  // of a page and a token, in 16 bytes
     PageSpan span;
     const int32_t* pages;
     const int32_t* lengths;

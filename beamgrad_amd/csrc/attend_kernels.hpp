@@ -640,17 +640,23 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         // The page-table entry of token first + lane of a tile, read well before
         // it is needed; then the place that it gives, -1 without a page.
         int32_t entry = -1;
+        uint32_t in_page = 0;
         const auto look_up = [&](int first) BEAMGRAD_INLINE {
+            const uint32_t token = first + lane, page = p.span.page.quotient(token);
+            in_page = token - page * p.span.page.d;
             entry = -1;
-            if (lane < KEYS && first + lane < w.end) entry = row_pages[p.span.page.quotient(first + lane)];
+            if (lane < KEYS && first + lane < w.end) entry = row_pages[page];
         };
         const bool alike = p.kp == p.vp && p.kt == p.vt;  // the usual: one offset serves both
-        const auto locate = [&](int first, int64_t& k_at, int64_t& v_at) BEAMGRAD_INLINE {
-            const uint32_t token = first + lane, in = token - p.span.page.quotient(token) * p.span.page.d;
+        const auto locate = [&](int64_t& k_at, int64_t& v_at) BEAMGRAD_INLINE {
             const bool there = p.span.is_page(entry);
-            k_at = there ? static_cast<int64_t>(entry) * p.kp + static_cast<int64_t>(in) * p.kt : -1;
+            const auto offset = [&](uint32_t page16, uint32_t token16) BEAMGRAD_INLINE {
+                const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(entry)) * page16 + static_cast<uint64_t>(in_page) * token16;
+                return there ? static_cast<int64_t>(at << 4) : -1;
+            };
+            k_at = offset(p.kp16, p.kt16);
             v_at = k_at;
-            if (!alike) v_at = there ? static_cast<int64_t>(entry) * p.vp + static_cast<int64_t>(in) * p.vt : -1;
+            if (!alike) v_at = offset(p.vp16, p.vt16);
             return __ballot(there);
         };
         // this wavefront's share of a tile, from memory straight into LDS
@@ -709,6 +715,19 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         const auto absorb = [&](int first, uint64_t there, const char* v_lds, f32x4 (&s)[KB][RB]) BEAMGRAD_INLINE {
             const bool hides = first + KEYS > masked_from;
             if (hides || there != kFull) {
+                // A value that is no number or infinite, of a token that some rows of
+                // the tile do not see, would reach them as 0 * inf: the join computes
+                // these rows again, one by one.
+                if (hides) {
+                    bool none = false;
+                    for (int c = opaque(lane); c < KEYS * X::kChunks; c += 64) {
+                        const Frag x = *reinterpret_cast<const Frag*>(v_lds + c * 16);
+    #pragma unroll
+                        for (int e = 0; e < 16 / X::kSize; ++e)
+                            none |= first + c / X::kChunks >= masked_from && !(__builtin_fabsf(static_cast<float>(x[e])) < kInf);
+                    }
+                    if (none) odd = 1;
+                }
                 const int q4 = opaque(quad * 4);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
@@ -772,25 +791,6 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         s[kb][rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][rb][i], scale, shift[rb]));
-                if (X::k32 || with_lse) {
-#pragma unroll
-                    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) l[rb] += s[kb][rb][i];
-                }
-            }
-            // A value that is no number or infinite, of a token that some rows of
-            // the tile do not see, would reach them as 0 * inf: the join computes
-            // these rows again, one by one.
-            if (hides) {
-                bool none = false;
-                for (int c = opaque(lane); c < KEYS * X::kChunks; c += 64) {
-                    const Frag x = *reinterpret_cast<const Frag*>(v_lds + c * 16);
-#pragma unroll
-                    for (int e = 0; e < 16 / X::kSize; ++e)
-                        none |= first + c / X::kChunks >= masked_from && !(__builtin_fabsf(static_cast<float>(x[e])) < kInf);
-                }
-                if (none) odd = 1;
             }
             if constexpr (X::k32) {
 #pragma unroll
@@ -842,6 +842,13 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     }
                 }
             }
+            if (X::k32 || with_lse) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+                        l[rb] += (s[kb][rb][0] + s[kb][rb][1]) + (s[kb][rb][2] + s[kb][rb][3]);
+            }
         };
         const int rounds = (w.end - w.key0 + WK * KEYS - 1) / (WK * KEYS), mine_first = w.key0 + wk * KEYS;
         constexpr int kNext = WK * KEYS;
@@ -861,12 +868,12 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
             // keys come two tiles ahead, values one.
             f32x4 s[2][KB][RB];
             int64_t k_at, v_at, v_next;
-            uint64_t there = locate(mine_first, k_at, v_at), there_next = 0;
+            uint64_t there = locate(k_at, v_at), there_next = 0;
             look_up(mine_first + kNext);
             fill(true, region(0, 1), v_head, v_at, there);
             fill(false, region(0, 0), k_head, k_at, there);
             if (rounds > 1) {
-                there_next = locate(mine_first + kNext, k_at, v_next);
+                there_next = locate(k_at, v_next);
                 look_up(mine_first + 2 * kNext);
                 fill(false, region(1, 0), k_head, k_at, there_next);
             }
@@ -882,7 +889,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 uint64_t there_after = 0;
                 if (round + 1 < rounds) fill(true, region(PLACE ^ 1, 1), v_head, v_next, there_next);
                 if (round + 2 < rounds) {
-                    there_after = locate(first + 2 * kNext, k_at, v_next);
+                    there_after = locate(k_at, v_next);
                     look_up(first + 3 * kNext);
                     fill(false, region(PLACE, 0), k_head, k_at, there_after);
                 }
@@ -898,7 +905,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
         } else {
             for (int first = mine_first; first < w.end; first += kNext) {  // no barriers
                 int64_t k_at, v_at;
-                const uint64_t there = locate(first, k_at, v_at);
+                const uint64_t there = locate(k_at, v_at);
                 look_up(first + kNext);
                 wait_lds();
                 fill(true, region(0, 1), v_head, v_at, there);

@@ -14,19 +14,21 @@ namespace dbs_hip {
 // division: q = (n * m) >> (31 + l), l = ceil(log2 d), m = floor(2^(31+l) / d)
 // + 1. m * d exceeds 2^(31+l) by at most d <= 2^l, so n * m / 2^(31+l) exceeds
 // n / d by at most n * 2^l / (d * 2^(31+l)) < 1 / d: the floor is n / d's.
-// m <= 2^32, so n * m stays below 2^63.
+// d > 2^(l-1), so m < 2^32: but for d = 1 the high word of n * m, shifted by l - 1,
+// is all that is needed.
 struct Divider {
     uint32_t d;
-    uint32_t shift;
-    uint64_t m;
+    uint32_t m;
+    uint32_t shift;  // l - 1; of d = 1: 0, unused
 
     static Divider of(uint32_t d) {
         uint32_t l = 0;
         while ((uint64_t{1} << l) < d) ++l;
-        return {d, 31 + l, (uint64_t{1} << (31 + l)) / d + 1};
+        return {d, static_cast<uint32_t>((uint64_t{1} << (31 + l)) / d + 1), l > 0 ? l - 1 : 0};
     }
     __host__ __device__ uint32_t quotient(uint32_t n) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift);
+        const uint32_t high = static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> 32);
+        return d == 1 ? n : high >> shift;
     }
 };
 
