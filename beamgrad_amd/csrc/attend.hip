@@ -29,7 +29,7 @@ bool valid_sizes(const BeamgradAttention* a) {
     if (a->head_dim <= 0 || a->head_dim > kAttendMaxDim || a->head_dim % 8 != 0) return false;
     if (a->heads % a->kv_heads != 0 || a->sequences % a->beams != 0) return false;
     if (a->parents && a->tokens > kAttendMaxTree) return false;
-    if (!std::isfinite(a->scale) || !(a->scale > 0.0f)) return false;
+    if (!std::isfinite(a->scale * 1.44269504088896341f) || !(a->scale > 0.0f)) return false;
     // places of a sequence's tokens, rows of a group and of the call in 31 bits
     if ((static_cast<int64_t>(a->table_pages) + 1) * a->page_tokens > INT32_MAX - 65536) return false;
     if (static_cast<double>(a->tokens) * a->heads * a->beams > 1.0e9) return false;

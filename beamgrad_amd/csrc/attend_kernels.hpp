@@ -29,7 +29,7 @@
 // 131000 tokens, 8 cache heads of 128, bfloat16: 946 MB in 168 us, 5.6 TB/s); many
 // rows, the latency of a tile's steps with two workgroups a CU, whose registers are
 // full (4 prompts' ends of 1000 tokens over 1500 to 4500, 32 heads of 64: 113 GFLOP
-// in 229 us, vector instructions issued in 55 % of the time, matrix ones busy in 27);
+// in 226 us, vector instructions issued in 55 % of the time, matrix ones busy in 27);
 // short caches, the chain of dependent reads (700 tokens: 10 us, of which the lengths
 // and totals 3).
 #pragma once
@@ -105,16 +105,6 @@ struct Dims {
     static constexpr int kKeyBlocks = kKeys / 16;
     static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
     static constexpr int kRowBytes = kChunks * 16;
-    // Of values, a lane's operand of a matrix step: eight of the 16-bit types, one
-    // of float32.
-    static constexpr int kFrag = k32 ? 1 : 8;
-    using Frag = typename Elem<DTYPE>::Frag;
-    static __device__ __forceinline__ f32x4 value_mma(const Frag& a, const Frag& b, f32x4 c) {
-        if constexpr (k32)
-            return __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], b[0], c, 0, 0, 0);
-        else
-            return Elem<DTYPE>::mma(a, b, c);
-    }
     static constexpr int kSteps = kChunks / 4;  // matrix steps of a key block's scores
     static constexpr int kDimBlocks = DP / 16;
     static constexpr int kRegion = kKeys * kRowBytes;  // of keys or values of a wavefront's tile
@@ -722,7 +712,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     bool none = false;
                     for (int c = opaque(lane); c < KEYS * X::kChunks; c += 64) {
                         const Frag x = *reinterpret_cast<const Frag*>(v_lds + c * 16);
-    #pragma unroll
+#pragma unroll
                         for (int e = 0; e < 16 / X::kSize; ++e)
                             none |= first + c / X::kChunks >= masked_from && !(__builtin_fabsf(static_cast<float>(x[e])) < kInf);
                     }
@@ -798,17 +788,13 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int row = kb * 16 + quad * 4 + i;
-                        Frag pr[RB];
-#pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) pr[rb][0] = s[kb][rb][i];
 #pragma unroll
                         for (int db = 0; db < DB; ++db) {
-                            Frag a;
-                            a[0] = *reinterpret_cast<const float*>(v_lds + row * X::kRowBytes +
-                                                                   ((db * 4 + (col >> 2)) ^ (row & X::kSwizzle)) * 16 + (col & 3) * 4);
-                            
+                            const float a = *reinterpret_cast<const float*>(
+                                v_lds + row * X::kRowBytes + ((db * 4 + (col >> 2)) ^ (row & X::kSwizzle)) * 16 + (col & 3) * 4);
 #pragma unroll
-                            for (int rb = 0; rb < RB; ++rb) o[db][rb] = X::value_mma(a, pr[rb], o[db][rb]);
+                            for (int rb = 0; rb < RB; ++rb)
+                                o[db][rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[kb][rb][i], o[db][rb], 0, 0, 0);
                         }
                     }
             } else {

@@ -71,7 +71,7 @@ typedef struct BeamgradAttention {
     const int32_t* counts;  /* or NULL */
     const int32_t* parents; /* or NULL */
     const int32_t* shared;  /* or NULL */
-    float scale;            /* positive and finite */
+    float scale;            /* positive, finite times log2(e) */
     int32_t reserved;       /* 0 */
     void* out;
     float* lse; /* or NULL */
