@@ -77,7 +77,7 @@ Plan plan_of(const BeamgradAttention& a, AttendParams& p) {
     const int64_t rows = static_cast<int64_t>(p.N) * p.G.d, together = rows * p.K;
     p.beam_rows = Divider::of(static_cast<uint32_t>(rows));
     plan.shape = kRows16;
-    while (plan.shape < kRows128 && attend_rows(plan.shape) < together) ++plan.shape;
+    while (plan.shape < attend_most(a.data_type, plan.dim) && attend_rows(plan.shape) < together) ++plan.shape;
     const int tile = attend_rows(plan.shape);
     p.shared_tiles = p.shared ? static_cast<int>((together + tile - 1) / tile) : 0;
     p.own_tiles = static_cast<int>((rows + tile - 1) / tile);

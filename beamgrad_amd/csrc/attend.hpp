@@ -8,6 +8,7 @@
 
 #include <stdint.h>
 
+#include "dbs_cuda.h"
 #include "paged.hpp"
 
 namespace dbs_hip {
@@ -17,11 +18,13 @@ constexpr int kAttendMaxDim = 256;
 constexpr int kAttendMaxTree = 512;  // drafted tokens with parents
 constexpr int kAttendSequences = 256; // of a launch: a thread of each workgroup reads one's length
 
-// Tiles of query rows of a workgroup: a wavefront holds kRowBlocks blocks of
-// 16 rows, the four wavefronts lie kRowWaves along the rows and 4 / kRowWaves
-// along the keys.
+// Tiles of query rows of a workgroup: its four wavefronts lie along the rows, the
+// keys, or two and two.
 enum AttendShape : int { kRows16 = 0, kRows32 = 1, kRows64 = 2, kRows128 = 3, kAttendShapes = 4 };
 constexpr int attend_rows(int shape) { return 16 << shape; }
+// Wide float32 heads: 16 rows a wavefront, so tiles of 64 rows at most.
+constexpr bool attend_thin(int data_type, int dim) { return data_type == DBS_CUDA_DTYPE_F32 && dim >= 128; }
+constexpr AttendShape attend_most(int data_type, int dim) { return attend_thin(data_type, dim) ? kRows64 : kRows128; }
 
 struct AttendParams {
     const void* q;

@@ -92,11 +92,15 @@ template <int DTYPE, int DP, int SHAPE>
 struct Dims {
     static constexpr bool k32 = DTYPE == DBS_CUDA_DTYPE_F32;
     static constexpr int kSize = k32 ? 4 : 2;
-    static constexpr int kRowBlocks = SHAPE == kRows16 ? 1 : 2;  // of 16 rows, of a wavefront
-    static constexpr int kRowWaves = SHAPE == kRows128 ? 4 : SHAPE == kRows64 ? 2 : 1;
+    static constexpr int kRows = attend_rows(SHAPE);
+    // Blocks of 16 rows of a wavefront, and how the four lie: queries and sums of
+    // two blocks of wide float32 heads do not fit the registers, and its matrix
+    // instructions are so long that one block keeps them busy (300 asking tokens, 2000
+    // cached, heads of 256: 160 us, 541 with two blocks).
+    static constexpr int kRowBlocks = SHAPE == kRows16 || attend_thin(DTYPE, DP) ? 1 : 2;
+    static constexpr int kRowWaves = kRows / (16 * kRowBlocks);
+    static_assert(kRowWaves == 1 || kRowWaves == 2 || kRowWaves == 4);
     static constexpr int kKeyWaves = 4 / kRowWaves;
-    static constexpr int kRows = 16 * kRowBlocks * kRowWaves;
-    static_assert(kRows == attend_rows(SHAPE));
     // Keys of a wavefront's tile: 32 fill the 16-bit matrix instruction's depth
     // for P V, 16 the float32 one's. A tile shared by four wavefronts is twice
     // as long, for half the barriers, where two tiles' scores fit the registers
@@ -123,7 +127,7 @@ struct Dims {
     static constexpr int kTokens = kRows;  // of a tile of rows, at most
     // Beginning and ending a piece takes some 5 us: as long as four rounds of four
     // small tiles, or one or two large ones.
-    static constexpr int kPieceCost = kRowWaves == 1 ? 4 * kKeyWaves : 2;
+    static constexpr int kPieceCost = kRowWaves == 4 ? 2 : 4 * kKeyWaves;
     static constexpr int kSlot = kRows * (DP + 3);  // floats of a partial result
     // workgroups of a CU: what its 160 KB of LDS hold
     static constexpr int kOther = kTokens * (kAttendMaxTree / 8) + 2 * kAttendMaxTree + 12 * kKeyWaves * kRows + 20 * kAttendSequences + 64;
@@ -1223,7 +1227,7 @@ hipError_t launch_dim(const AttendParams& p, int shape, hipStream_t stream) {
         case kRows16: return launch_shape<DTYPE, DP, kRows16>(p, stream);
         case kRows32: return launch_shape<DTYPE, DP, kRows32>(p, stream);
         case kRows64: return launch_shape<DTYPE, DP, kRows64>(p, stream);
-        default: return launch_shape<DTYPE, DP, kRows128>(p, stream);
+        default: return launch_shape<DTYPE, DP, attend_most(DTYPE, DP)>(p, stream);
     }
 }
 
@@ -1234,7 +1238,7 @@ AttendSizes dim_sizes(int shape) {
         case kRows16: return of(Dims<DTYPE, DP, kRows16>{});
         case kRows32: return of(Dims<DTYPE, DP, kRows32>{});
         case kRows64: return of(Dims<DTYPE, DP, kRows64>{});
-        default: return of(Dims<DTYPE, DP, kRows128>{});
+        default: return of(Dims<DTYPE, DP, attend_most(DTYPE, DP)>{});
     }
 }
 
