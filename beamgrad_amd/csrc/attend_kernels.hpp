@@ -96,8 +96,9 @@ struct Dims {
     // Blocks of 16 rows of a wavefront, and how the four lie: queries and sums of
     // two blocks of wide float32 heads do not fit the registers, and its matrix
     // instructions are so long that one block keeps them busy (300 asking tokens, 2000
-    // cached, heads of 256: 160 us, 541 with two blocks).
-    static constexpr int kRowBlocks = SHAPE == kRows16 || attend_thin(DTYPE, DP) ? 1 : 2;
+    // cached, heads of 256: 160 us, 541 with two blocks). 16-bit heads of 256: tiles up
+    // to 64 rows likewise (16 sequences of 4000 to 8000, 60 rows: 220 us, 547 with two).
+    static constexpr int kRowBlocks = SHAPE == kRows16 || attend_thin(DTYPE, DP) || (DP == 256 && SHAPE <= kRows64) ? 1 : 2;
     static constexpr int kRowWaves = kRows / (16 * kRowBlocks);
     static_assert(kRowWaves == 1 || kRowWaves == 2 || kRowWaves == 4);
     static constexpr int kKeyWaves = 4 / kRowWaves;
