@@ -139,7 +139,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Pag
     Returns ``[S, N, H, D]`` in ``q``'s type, zeros for rows past ``counts``; with
     ``return_lse`` also the log of each row's sum of exponentials, float32
     ``[S, N, H]``, -inf for such rows. Scores, softmax and sums are held in 32
-    bits; 16-bit inputs round each probability to their type. No gradient.
+    bits; 16-bit inputs round each probability to their type. No derivatives:
+    inputs that carry a tangent, or require a gradient while one is recorded, are refused.
     """
     pages, lengths, _refs = _tables(table)
     if scale is None:
@@ -204,7 +205,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, *, inp
 
     New tensors are returned, differentiable for float32, float16 and bfloat16:
     the gradient of a row is the sum over the beams that continue it, in their
-    order and in 32 bits, rounded once. With ``inplace`` the (contiguous)
+    order and in 32 bits, rounded once; forward-mode tangents move as the states
+    do. With ``inplace`` (no derivatives) the (contiguous)
     states are overwritten and returned, and rows that stay are not touched.
     """
     states = list(states)

@@ -23,6 +23,7 @@
 
 #include <cmath>
 #include <limits>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -54,12 +55,28 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
     return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
 }
 
-// Operators that write or read tensors without recording a gradient.
-void check_no_gradient(at::TensorList tensors, const char* what) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor& t : tensors)
-        TORCH_CHECK(!t.requires_grad(), "beamgrad_amd.", what,
-                    " has no gradient: call it under torch.no_grad() or on detached tensors");
+// Operators without a derivative, at the Autograd key: what a torch.func
+// transform wraps is still seen here.
+void refuse_derivatives(const Tensor& t, const c10::OperatorHandle& op) {
+    const auto name = [&] {
+        const std::string what = op.schema().name().substr(sizeof("beamgrad::") - 1);
+        return what == "reorder_states_" ? "reorder_states(inplace=True)" : what;
+    };
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "beamgrad_amd.", name(),
+                " has no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), "beamgrad_amd.", name(),
+                " has no forward-mode derivative, and would drop a tensor's tangent: call it on the tensors' primals");
+}
+
+void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+    for (const c10::IValue& argument : torch::jit::last(*stack, op.schema().arguments().size())) {
+        if (argument.isTensor()) {
+            refuse_derivatives(argument.toTensor(), op);
+        } else if (argument.isTensorList()) {
+            for (const auto& t : argument.toListRef()) refuse_derivatives(t.toTensor(), op);
+        }
+    }
+    op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }
 
 // Written in place: an autograd graph that saved such a tensor notices.
@@ -224,7 +241,6 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
 // --- fork ---
 
 void check_fork(const Tensors& pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& parents) {
-    check_no_gradient(pools, "fork_pages");
     check_table(pages, lengths, refs);
     TORCH_CHECK_VALUE(!pools.empty(), "pools must hold at least one pool");
     check_pools(pools, pages, refs.numel());
@@ -282,8 +298,6 @@ TableOut extend_pages_hip(const Tensor& pages, const Tensor& lengths, const Tens
 // --- write ---
 
 void check_write(const Tensors& pools, const Tensors& news, const Tensor& pages, const Tensor& lengths, const OptTensor& counts) {
-    check_no_gradient(pools, "write_tokens");
-    check_no_gradient(news, "write_tokens");
     check_pages(pages, lengths);
     TORCH_CHECK_VALUE(!pools.empty() && pools.size() == news.size(), "pools and news must be as many, and at least one, got ",
                       pools.size(), " and ", news.size());
@@ -339,7 +353,6 @@ void write_tokens_hip(Tensors pools, Tensors news, const Tensor& pages, const Te
 
 void check_keep(const Tensors& pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& drafted,
                 const Tensor& keep, const Tensor& kept) {
-    check_no_gradient(pools, "keep_tokens");
     check_table(pages, lengths, refs);
     TORCH_CHECK_VALUE(!pools.empty(), "pools must hold at least one pool");
     check_pools(pools, pages, refs.numel());
@@ -376,7 +389,6 @@ TableOut keep_tokens_hip(Tensors pools, const Tensor& pages, const Tensor& lengt
 
 void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths,
                      const OptTensor& parents, const OptTensor& counts, int64_t beams, const OptTensor& shared, double scale) {
-    check_no_gradient({q, k, v}, "tree_attention");
     TORCH_CHECK_VALUE(q.dim() == 4 && q.numel() > 0, "q must be a [S, N, H, D] tensor, got ", q.sizes());
     data_type(q, "q");
     TORCH_CHECK_VALUE(k.dim() == 4 && k.numel() > 0 && v.sizes() == k.sizes(),
@@ -495,7 +507,6 @@ void check_states(const Tensors& states, const Tensor& parents, const char* name
 }
 
 void check_inplace(const Tensors& states) {
-    check_no_gradient(states, "reorder_states(inplace=True)");
     for (size_t i = 0; i < states.size(); ++i)
         TORCH_CHECK_VALUE(states[i].is_contiguous(), "states[", i, "] must be contiguous to be reordered in place");
 }
@@ -687,22 +698,46 @@ bool records(const Tensors& tensors) {
     return false;
 }
 
+// The map is linear: an output's tangent is the input's, moved as it is. The
+// tangents go through the whole operator, which records a gradient of them too.
+Tensors with_tangents(const Tensors& inputs, const Tensor& parents, bool gathers, Tensors out) {
+    Tensors tangents;
+    std::vector<size_t> at;
+    for (size_t i = 0; i < inputs.size(); ++i) {
+        if (!torch::autograd::isFwGradDefined(inputs[i])) continue;
+        tangents.push_back(inputs[i]._fw_grad(/*level=*/0));
+        at.push_back(i);
+    }
+    if (tangents.empty()) return out;
+    const Tensors moved = gathers ? call_gather(tangents, parents) : call_reorder(tangents, parents);
+    for (size_t j = 0; j < at.size(); ++j) out[at[j]]._set_fw_grad(moved[j], /*level=*/0, /*is_inplace_op=*/false);
+    return out;
+}
+
 Tensors reorder_states_autograd(Tensors states, const Tensor& parents) {
     if (records(states)) {
         for (const Tensor& t : states)
             TORCH_CHECK_TYPE(!t.requires_grad() || t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kFloat16 ||
                                  t.scalar_type() == torch::kBFloat16,
                              "reorder_states has a gradient for float32, float16 and bfloat16 states, not ", t.scalar_type());
-        return recorded(states, parents, false);
+        return with_tangents(states, parents, false, recorded(states, parents, false));
     }
-    const at::AutoDispatchBelowADInplaceOrView below;
-    return call_reorder(states, parents);
+    Tensors out;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = call_reorder(states, parents);
+    }
+    return with_tangents(states, parents, false, std::move(out));
 }
 
 Tensors reorder_states_backward_autograd(Tensors grads, const Tensor& parents) {
-    if (records(grads)) return recorded(grads, parents, true);
-    const at::AutoDispatchBelowADInplaceOrView below;
-    return call_gather(grads, parents);
+    if (records(grads)) return with_tangents(grads, parents, true, recorded(grads, parents, true));
+    Tensors out;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = call_gather(grads, parents);
+    }
+    return with_tangents(grads, parents, true, std::move(out));
 }
 
 }  // namespace
@@ -738,6 +773,8 @@ TORCH_LIBRARY_IMPL(beamgrad, CUDA, m) {
 TORCH_LIBRARY_IMPL(beamgrad, Autograd, m) {
     m.impl("reorder_states", &reorder_states_autograd);
     m.impl("reorder_states_backward", &reorder_states_backward_autograd);
+    for (const char* name : {"tree_attention", "fork_pages", "write_tokens", "keep_tokens", "reorder_states_"})
+        m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }
 
 // Checked, then refused.
