@@ -20,7 +20,10 @@ stay. :func:`reorder_states` is the same for states without pages (recurrent
 states, a short dense cache), with a gradient.
 
 Every call is asynchronous on the current stream and reads nothing back: page
-tables live on the GPU, so the calls can be captured into a graph. The C
+tables live on the GPU, so the calls can be captured into a graph. The pools (or
+states in place) of a call are written at once in many places: one given twice, or
+two that share memory otherwise, are refused (parts of one buffer that lie apart, in
+turns too, are fine). The C
 entries are in ``include/beamgrad_state.h``. The reference has no counterpart:
 its step function gathers a model's cache itself (reference
 python/beamgrad/_search.py:100-133, ``BeamState.parents``).

@@ -15,6 +15,7 @@
 #include "beamgrad_state.h"
 #include "engine.hpp"
 #include "paged.hpp"
+#include "regions.hpp"
 #include "rows.hpp"
 
 using namespace dbs_hip;
@@ -432,6 +433,18 @@ bool valid_pools(const BeamgradPools* p) {
     return true;
 }
 
+// A pool, or a token of one, that lies where another does would be moved twice, and
+// in no order; what is read meanwhile must not change.
+bool lie_apart(const BeamgradPools& p, const void* const* news, const int64_t* news_strides, int sequences, int tokens) {
+    const auto pool = [&](int i) {
+        return Region{reinterpret_cast<uintptr_t>(p.base[i]), {p.n_pages, p.page_tokens}, {p.page_stride[i], p.token_stride[i]}, p.row_bytes[i]};
+    };
+    const auto rows = [&](int i) {
+        return Region{reinterpret_cast<uintptr_t>(news[i]), {sequences, tokens}, {news_strides[2 * i], news_strides[2 * i + 1]}, p.row_bytes[i]};
+    };
+    return all_apart(p.n, pool, news ? p.n : 0, rows);
+}
+
 bool valid_table(const BeamgradTable* t) { return t && t->pages && t->lengths && t->refs; }
 
 Table table_of(const BeamgradTable& from, const BeamgradTable& to, int S, int P, int n_pages, int page_tokens) {
@@ -489,7 +502,7 @@ DBS_CUDA_EXPORT int beamgrad_fork_pages(const BeamgradPools* pools, const Beamgr
                                         void* workspace, int64_t workspace_bytes, void* stream_ptr) {
     if (!valid_pools(pools) || !valid_table(from) || !valid_table(to) || !parents || !workspace ||
         !valid_span(sequences, table_pages, pools->n_pages, pools->page_tokens) ||
-        workspace_bytes < beamgrad_fork_pages_workspace_size(sequences))
+        workspace_bytes < beamgrad_fork_pages_workspace_size(sequences) || !lie_apart(*pools, nullptr, nullptr, 0, 0))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Table t = table_of(*from, *to, sequences, table_pages, pools->n_pages, pools->page_tokens);
     int32_t* const ws = static_cast<int32_t*>(workspace);
@@ -539,6 +552,7 @@ DBS_CUDA_EXPORT int beamgrad_write_tokens(const BeamgradPools* pools, const void
         if (!news[i] || news_strides[2 * i] < 0 || news_strides[2 * i + 1] < 0 ||
             static_cast<double>(rows) * static_cast<double>(pools->row_bytes[i] / 16 + 1) > 2.0e9)
             return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!lie_apart(*pools, news, news_strides, sequences, tokens)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const PageSpan span{Divider::of(static_cast<uint32_t>(pools->page_tokens)), pools->n_pages, table_pages};
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     const hipError_t e = over_pools(*pools, news, news_strides, [&](const PoolSet& set, bool) {
@@ -556,7 +570,8 @@ DBS_CUDA_EXPORT int beamgrad_keep_tokens(const BeamgradPools* pools, const Beamg
                                          const int32_t* keep, const int32_t* kept, int sequences, int table_pages,
                                          int width, const BeamgradTable* to, void* stream_ptr) {
     if (!valid_pools(pools) || !valid_table(from) || !valid_table(to) || !drafted || !kept || width < 0 ||
-        (width > 0 && !keep) || !valid_span(sequences, table_pages, pools->n_pages, pools->page_tokens))
+        (width > 0 && !keep) || !valid_span(sequences, table_pages, pools->n_pages, pools->page_tokens) ||
+        !lie_apart(*pools, nullptr, nullptr, 0, 0))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Table t = table_of(*from, *to, sequences, table_pages, pools->n_pages, pools->page_tokens);
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);

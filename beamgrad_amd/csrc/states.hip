@@ -11,6 +11,7 @@
 #include "beamgrad_state.h"
 #include "engine.hpp"
 #include "paged.hpp"
+#include "regions.hpp"
 #include "rows.hpp"
 
 using namespace dbs_hip;
@@ -172,6 +173,16 @@ bool valid_states(const void* const* from, void* const* to, const int64_t* size,
     return true;
 }
 
+// A state that lies where another is written would be moved twice, and in no
+// order. `bytes(i)`: of a row.
+template <class Bytes>
+bool lie_apart(const void* const* from, void* const* to, int n, Bytes bytes, int examples, int beams, bool inplace) {
+    const auto whole = [&](const void* base, int i) {
+        return Region{reinterpret_cast<uintptr_t>(base), {1, 1}, {0, 0}, bytes(i) * beams * examples};
+    };
+    return all_apart(n, [&](int i) { return whole(to[i], i); }, inplace ? 0 : n, [&](int i) { return whole(from[i], i); });
+}
+
 }  // namespace
 
 extern "C" {
@@ -183,6 +194,7 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states(const void* const* from, void* const
     bool inplace = n > 0 && from[0] == to[0];
     for (int i = 0; i < n; ++i)
         if ((from[i] == to[i]) != inplace) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (!lie_apart(from, to, n, [&](int i) { return row_bytes[i]; }, examples, beams, inplace)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     const hipError_t e = over_states(from, to, n, [&](int i) { return row_bytes[i]; }, [&](const StateSet& set) {
         const int64_t chunks = (set.row_bytes + 15) / 16;
@@ -210,9 +222,8 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states_backward(const void* const* from, vo
     if (!valid_states(from, to, elements, n, parents, examples, beams) ||
         (data_type != DBS_CUDA_DTYPE_F32 && data_type != DBS_CUDA_DTYPE_F16 && data_type != DBS_CUDA_DTYPE_BF16))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
-    for (int i = 0; i < n; ++i)
-        if (from[i] == to[i]) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const int size = data_type == DBS_CUDA_DTYPE_F32 ? 4 : 2;
+    if (!lie_apart(from, to, n, [&](int i) { return elements[i] * size; }, examples, beams, false)) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     const hipError_t e = over_states(from, to, n, [&](int i) { return elements[i] * size; }, [&](const StateSet& set) {
         const int64_t chunks = (set.row_bytes + 15) / 16;

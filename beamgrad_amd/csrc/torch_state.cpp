@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "beamgrad_state.h"
+#include "regions.hpp"
 
 namespace {
 
@@ -190,6 +191,30 @@ void check_pools(const Tensors& pools, const Tensor& pages, int64_t n_pages) {
     if (!pools.empty()) check_span(pages, pools[0].size(1));
 }
 
+// Pools whose memory meets, or news that lie in one, which the C entries refuse:
+// with the numbers of two.
+dbs_hip::Region rows_of(const Tensor& t) {
+    const int64_t size = static_cast<int64_t>(t.element_size());
+    return {reinterpret_cast<uintptr_t>(t.const_data_ptr()), {t.size(0), t.size(1)}, {t.stride(0) * size, t.stride(1) * size},
+            row_elements(t, 2) * size};
+}
+
+void check_pools_apart(const Tensors& pools, const Tensors& news) {
+    std::vector<dbs_hip::Region> written, read;
+    std::vector<size_t> at;  // in news: those that are no copy
+    for (const Tensor& t : pools) written.push_back(rows_of(t));
+    for (size_t i = 0; i < news.size(); ++i)
+        if (row_contiguous(news[i], 2)) {
+            read.push_back(rows_of(news[i]));
+            at.push_back(i);
+        }
+    const dbs_hip::Meeting m = dbs_hip::find_meeting(written, read);
+    if (m.first < 0) return;
+    TORCH_CHECK_VALUE(!m.reads, "news[", at[m.second], "] and pools[", m.first, "] share memory");
+    TORCH_CHECK_VALUE(m.first != m.second, "the pages and tokens of pools[", m.first, "] overlap");
+    TORCH_CHECK_VALUE(false, "pools[", m.first, "] and pools[", m.second, "] share memory");
+}
+
 Pools bind_pools(const Tensors& pools, int64_t n_pages, int64_t page_tokens) {
     Pools p;
     p.base.reserve(pools.size());
@@ -249,6 +274,7 @@ void check_fork(const Tensors& pools, const Tensor& pages, const Tensor& lengths
 
 TableOut fork_pages_cpu(Tensors pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& parents) {
     check_fork(pools, pages, lengths, refs, parents);
+    check_pools_apart(pools, {});
     refuse_cpu("fork_pages", pages);
 }
 
@@ -261,9 +287,10 @@ TableOut fork_pages_hip(Tensors pools, const Tensor& pages, const Tensor& length
     const int64_t bytes = beamgrad_fork_pages_workspace_size(narrow(pages.size(0)));
     const Tensor ws = workspace(bytes, pages);
     const BeamgradTable from = bind_table(pages, lengths, refs), out = to.bind();
-    check_status(beamgrad_fork_pages(&p.c, &from, par.const_data_ptr(), par.scalar_type() == torch::kInt64,
-                                     narrow(pages.size(0)), narrow(pages.size(1)), &out, ws.data_ptr(), bytes, current_stream()),
-                 "fork_pages");
+    const int status = beamgrad_fork_pages(&p.c, &from, par.const_data_ptr(), par.scalar_type() == torch::kInt64,
+                                           narrow(pages.size(0)), narrow(pages.size(1)), &out, ws.data_ptr(), bytes, current_stream());
+    if (status == DBS_CUDA_STATUS_INVALID_ARGUMENT) check_pools_apart(pools, {});
+    check_status(status, "fork_pages");
     written(pools);
     return to.take();
 }
@@ -316,6 +343,7 @@ void check_write(const Tensors& pools, const Tensors& news, const Tensor& pages,
 
 void write_tokens_cpu(Tensors pools, Tensors news, const Tensor& pages, const Tensor& lengths, const OptTensor& counts) {
     check_write(pools, news, pages, lengths, counts);
+    check_pools_apart(pools, news);
     refuse_cpu("write_tokens", pages);
 }
 
@@ -343,9 +371,10 @@ void write_tokens_hip(Tensors pools, Tensors news, const Tensor& pages, const Te
         strides.push_back(t.stride(0) * static_cast<int64_t>(t.element_size()));
         strides.push_back(t.stride(1) * static_cast<int64_t>(t.element_size()));
     }
-    check_status(beamgrad_write_tokens(&p.c, from.data(), strides.data(), i32(pages), i32(lengths), i32(n), narrow(pages.size(0)),
-                                       narrow(pages.size(1)), narrow(news[0].size(1)), current_stream()),
-                 "write_tokens");
+    const int status = beamgrad_write_tokens(&p.c, from.data(), strides.data(), i32(pages), i32(lengths), i32(n), narrow(pages.size(0)),
+                                             narrow(pages.size(1)), narrow(news[0].size(1)), current_stream());
+    if (status == DBS_CUDA_STATUS_INVALID_ARGUMENT) check_pools_apart(pools, news);
+    check_status(status, "write_tokens");
     written(pools);
 }
 
@@ -365,6 +394,7 @@ void check_keep(const Tensors& pools, const Tensor& pages, const Tensor& lengths
 TableOut keep_tokens_cpu(Tensors pools, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const Tensor& drafted,
                          const Tensor& keep, const Tensor& kept) {
     check_keep(pools, pages, lengths, refs, drafted, keep, kept);
+    check_pools_apart(pools, {});
     refuse_cpu("keep_tokens", pages);
 }
 
@@ -376,9 +406,10 @@ TableOut keep_tokens_hip(Tensors pools, const Tensor& pages, const Tensor& lengt
     const Pools p = bind_pools(pools, refs.numel(), pools[0].size(1));
     NewTable to(pages, lengths, refs);
     const BeamgradTable from = bind_table(pages, lengths, refs), out = to.bind();
-    check_status(beamgrad_keep_tokens(&p.c, &from, i32(d), i32(k), i32(n), narrow(pages.size(0)), narrow(pages.size(1)),
-                                      narrow(k.size(1)), &out, current_stream()),
-                 "keep_tokens");
+    const int status = beamgrad_keep_tokens(&p.c, &from, i32(d), i32(k), i32(n), narrow(pages.size(0)), narrow(pages.size(1)),
+                                            narrow(k.size(1)), &out, current_stream());
+    if (status == DBS_CUDA_STATUS_INVALID_ARGUMENT) check_pools_apart(pools, {});
+    check_status(status, "keep_tokens");
     written(pools);
     return to.take();
 }
@@ -511,6 +542,20 @@ void check_inplace(const Tensors& states) {
         TORCH_CHECK_VALUE(states[i].is_contiguous(), "states[", i, "] must be contiguous to be reordered in place");
 }
 
+// States whose memory meets, which the C entry refuses: with the numbers of two.
+void check_states_apart(const Tensors& states) {
+    std::vector<dbs_hip::Region> written;
+    std::vector<size_t> at;  // in states: those that are not empty
+    for (size_t i = 0; i < states.size(); ++i)
+        if (states[i].numel() > 0) {
+            written.push_back({reinterpret_cast<uintptr_t>(states[i].const_data_ptr()), {1, 1}, {0, 0},
+                               states[i].numel() * static_cast<int64_t>(states[i].element_size())});
+            at.push_back(i);
+        }
+    const dbs_hip::Meeting m = dbs_hip::find_meeting(written, {});
+    TORCH_CHECK_VALUE(m.first < 0, "states[", at[m.first], "] and states[", at[m.second], "] share memory");
+}
+
 struct StateRows {
     std::vector<const void*> from;
     std::vector<void*> to;
@@ -527,12 +572,11 @@ Tensors reorder_states_cpu(Tensors states, const Tensor& parents) {
     refuse_cpu("reorder_states", parents);
 }
 
-void run_reorder(const StateRows& rows, const Tensor& parents) {
+int run_reorder(const StateRows& rows, const Tensor& parents) {
     const Tensor par = parents.contiguous();
-    check_status(beamgrad_reorder_states(rows.from.data(), rows.to.data(), rows.size.data(), narrow(static_cast<int64_t>(rows.from.size())),
-                                         par.const_data_ptr(), par.scalar_type() == torch::kInt64, narrow(par.size(0)),
-                                         narrow(par.size(1)), current_stream()),
-                 "reorder_states");
+    return beamgrad_reorder_states(rows.from.data(), rows.to.data(), rows.size.data(), narrow(static_cast<int64_t>(rows.from.size())),
+                                   par.const_data_ptr(), par.scalar_type() == torch::kInt64, narrow(par.size(0)), narrow(par.size(1)),
+                                   current_stream());
 }
 
 Tensors reorder_states_hip(Tensors states, const Tensor& parents) {
@@ -545,13 +589,14 @@ Tensors reorder_states_hip(Tensors states, const Tensor& parents) {
         out.push_back(fresh(t.sizes(), t.scalar_type(), t));
         if (t.numel() > 0) rows.add(t, out.back(), row_elements(t, 2) * static_cast<int64_t>(t.element_size()));
     }
-    run_reorder(rows, parents);
+    check_status(run_reorder(rows, parents), "reorder_states");
     return out;
 }
 
 void reorder_states_inplace_cpu(Tensors states, const Tensor& parents) {
     check_states(states, parents, "states");
     check_inplace(states);
+    check_states_apart(states);
     refuse_cpu("reorder_states_", parents);
 }
 
@@ -562,7 +607,9 @@ void reorder_states_inplace_hip(Tensors states, const Tensor& parents) {
     StateRows rows;
     for (const Tensor& t : states)
         if (t.numel() > 0) rows.add(t, t, row_elements(t, 2) * static_cast<int64_t>(t.element_size()));
-    run_reorder(rows, parents);
+    const int status = run_reorder(rows, parents);
+    if (status == DBS_CUDA_STATUS_INVALID_ARGUMENT) check_states_apart(states);
+    check_status(status, "reorder_states");
     written(states);
 }
 

@@ -87,7 +87,9 @@ DBS_CUDA_EXPORT int beamgrad_tree_attention(const BeamgradAttention* args, void*
 /* Pools of a cache: n pools of n_pages pages of page_tokens tokens each, a
  * token's row of row_bytes[i] contiguous bytes in pool i at base[i] + page *
  * page_stride[i] + token * token_stride[i] (bytes). The arrays are host
- * memory, read before the call returns. All pools are paged by one table. */
+ * memory, read before the call returns. All pools are paged by one table. They
+ * may lie in one buffer, in turns too, but no byte may be two pools' or two tokens':
+ * the calls write them in many places at once, and refuse pools that meet. */
 typedef struct BeamgradPools {
     void* const* base;
     const int64_t* row_bytes;
@@ -128,7 +130,7 @@ DBS_CUDA_EXPORT int beamgrad_extend_pages(const BeamgradTable* from, const int32
 /* news[i] (pool i's rows, at news[i] + s * news_strides[2 i] + j *
  * news_strides[2 i + 1] bytes) for the last counts[s] tokens of each sequence (all
  * `tokens` where counts is NULL; at most `tokens` and lengths[s]): row j to the
- * j-th of them. */
+ * j-th of them. news that lie in a pool are refused. */
 DBS_CUDA_EXPORT int beamgrad_write_tokens(const BeamgradPools* pools, const void* const* news,
                                           const int64_t* news_strides, const int32_t* pages, const int32_t* lengths,
                                           const int32_t* counts, int sequences, int table_pages, int tokens,
@@ -144,7 +146,8 @@ DBS_CUDA_EXPORT int beamgrad_keep_tokens(const BeamgradPools* pools, const Beamg
 
 /* to[i][b, k] = from[i][b, parents[b, k]], zeros where parents is outside
  * [0, beams): n dense states [examples, beams, row_bytes[i]]; from[i] == to[i]
- * for every i moves the rows in place. At most 4096 beams. */
+ * for every i moves the rows in place. Otherwise no state that is written may meet
+ * one that is read; two that are written never may. At most 4096 beams. */
 DBS_CUDA_EXPORT int beamgrad_reorder_states(const void* const* from, void* const* to, const int64_t* row_bytes, int n,
                                             const void* parents, int parents_i64, int examples, int beams,
                                             void* stream);
