@@ -447,6 +447,19 @@ bool lie_apart(const BeamgradPools& p, const void* const* news, const int64_t* n
 
 bool valid_table(const BeamgradTable* t) { return t && t->pages && t->lengths && t->refs; }
 
+// The new table is written while the old one is read: none of its parts may lie in
+// it, or in each other.
+bool tables_apart(const BeamgradTable& from, const BeamgradTable& to, int S, int P, int n_pages) {
+    const int32_t* const parts[6] = {to.pages, to.lengths, to.refs, from.pages, from.lengths, from.refs};
+    const int64_t size[3] = {static_cast<int64_t>(S) * P, S, n_pages};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 6; ++j) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(parts[i]), b = reinterpret_cast<uintptr_t>(parts[j]);
+            if (a < b + size[j % 3] * sizeof(int32_t) && b < a + size[i] * sizeof(int32_t)) return false;
+        }
+    return true;
+}
+
 Table table_of(const BeamgradTable& from, const BeamgradTable& to, int S, int P, int n_pages, int page_tokens) {
     return {from.pages, from.lengths, from.refs, to.pages, to.lengths, to.refs,
             {Divider::of(static_cast<uint32_t>(page_tokens)), n_pages, P}, S};
@@ -502,7 +515,8 @@ DBS_CUDA_EXPORT int beamgrad_fork_pages(const BeamgradPools* pools, const Beamgr
                                         void* workspace, int64_t workspace_bytes, void* stream_ptr) {
     if (!valid_pools(pools) || !valid_table(from) || !valid_table(to) || !parents || !workspace ||
         !valid_span(sequences, table_pages, pools->n_pages, pools->page_tokens) ||
-        workspace_bytes < beamgrad_fork_pages_workspace_size(sequences) || !lie_apart(*pools, nullptr, nullptr, 0, 0))
+        workspace_bytes < beamgrad_fork_pages_workspace_size(sequences) ||
+        !tables_apart(*from, *to, sequences, table_pages, pools->n_pages) || !lie_apart(*pools, nullptr, nullptr, 0, 0))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Table t = table_of(*from, *to, sequences, table_pages, pools->n_pages, pools->page_tokens);
     int32_t* const ws = static_cast<int32_t*>(workspace);
@@ -530,7 +544,7 @@ DBS_CUDA_EXPORT int beamgrad_extend_pages(const BeamgradTable* from, const int32
                                           void* workspace, int64_t workspace_bytes, void* stream_ptr) {
     if (!valid_table(from) || !valid_table(to) || !counts || !workspace ||
         !valid_span(sequences, table_pages, n_pages, page_tokens) ||
-        workspace_bytes < beamgrad_extend_pages_workspace_size(n_pages))
+        workspace_bytes < beamgrad_extend_pages_workspace_size(n_pages) || !tables_apart(*from, *to, sequences, table_pages, n_pages))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Table t = table_of(*from, *to, sequences, table_pages, n_pages, page_tokens);
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
@@ -571,7 +585,7 @@ DBS_CUDA_EXPORT int beamgrad_keep_tokens(const BeamgradPools* pools, const Beamg
                                          int width, const BeamgradTable* to, void* stream_ptr) {
     if (!valid_pools(pools) || !valid_table(from) || !valid_table(to) || !drafted || !kept || width < 0 ||
         (width > 0 && !keep) || !valid_span(sequences, table_pages, pools->n_pages, pools->page_tokens) ||
-        !lie_apart(*pools, nullptr, nullptr, 0, 0))
+        !tables_apart(*from, *to, sequences, table_pages, pools->n_pages) || !lie_apart(*pools, nullptr, nullptr, 0, 0))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Table t = table_of(*from, *to, sequences, table_pages, pools->n_pages, pools->page_tokens);
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);

@@ -101,6 +101,8 @@ typedef struct BeamgradPools {
     int32_t reserved; /* 0 */
 } BeamgradPools;
 
+/* A call reads one table and writes another, no part of which may lie in the first
+ * or in another part (refused). */
 typedef struct BeamgradTable {
     int32_t* pages; /* [sequences, table_pages], contiguous */
     int32_t* lengths;
