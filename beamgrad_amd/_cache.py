@@ -23,7 +23,8 @@ Every call is asynchronous on the current stream and reads nothing back: page
 tables live on the GPU, so the calls can be captured into a graph. The pools (or
 states in place) of a call are written at once in many places: one given twice, or
 two that share memory otherwise, are refused (parts of one buffer that lie apart, in
-turns too, are fine). The C
+turns too, are fine). Index tensors are int32 or int64, whose numbers
+past 32 bits are out of range like any other. The C
 entries are in ``include/beamgrad_state.h``. The reference has no counterpart:
 its step function gathers a model's cache itself (reference
 python/beamgrad/_search.py:100-133, ``BeamState.parents``).

@@ -17,6 +17,7 @@
 #include "paged.hpp"
 #include "regions.hpp"
 #include "rows.hpp"
+#include "torch_engine.hpp"
 
 using namespace dbs_hip;
 
@@ -416,6 +417,12 @@ __global__ __launch_bounds__(kCopyThreads) void keep_table(const Table t, const 
     }
 }
 
+// One launch, as torch's own conversion (which keeps the low words) takes.
+__global__ __launch_bounds__(kCopyThreads) void narrow_kernel(const int64_t* from, int32_t* to, const int64_t n) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kCopyThreads + threadIdx.x;
+    if (i < n) to[i] = static_cast<int32_t>(min(max(from[i], static_cast<int64_t>(INT32_MIN)), static_cast<int64_t>(INT32_MAX)));
+}
+
 // ---------------------------------------------------------------------------
 // Checks and launches
 // ---------------------------------------------------------------------------
@@ -606,6 +613,13 @@ DBS_CUDA_EXPORT int beamgrad_keep_tokens(const BeamgradPools* pools, const Beamg
         e = hipGetLastError();
     }
     return finish_call(stream, e);
+}
+
+DBS_CUDA_EXPORT int beamgrad_narrow_indices(const int64_t* from, int32_t* to, int64_t n, void* stream_ptr) {
+    if (n < 0 || n > INT32_MAX || (n > 0 && (!from || !to))) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    if (n > 0) narrow_kernel<<<static_cast<unsigned>((n + kCopyThreads - 1) / kCopyThreads), kCopyThreads, 0, stream>>>(from, to, n);
+    return finish_call(stream, n > 0 ? hipGetLastError() : hipSuccess);
 }
 
 }  // extern "C"

@@ -27,3 +27,8 @@ extern "C" __attribute__((visibility("default"))) int beamgrad_advance_beams(
     const uint8_t* from_logprob, const uint8_t* finished, const int64_t* sequences, int batch_size, int beam_size,
     int step, int64_t* sequences_out, int32_t* prefixes_out, int64_t* tokens64, int64_t* parents64, int64_t* lengths64,
     uint8_t* finished_bool, uint8_t* active, int32_t* any_active, void* stream);
+
+// Numbers of 64 bits as 32 hold them: those that pass 32 bits become the end of
+// the range that they pass. Returns a dbs_cuda status.
+extern "C" __attribute__((visibility("default"))) int beamgrad_narrow_indices(const int64_t* from, int32_t* to, int64_t n,
+                                                                              void* stream);

@@ -29,6 +29,7 @@
 
 #include "beamgrad_state.h"
 #include "regions.hpp"
+#include "torch_engine.hpp"
 
 namespace {
 
@@ -102,8 +103,15 @@ void check_index(const Tensor& t, at::IntArrayRef shape, const Tensor& with, con
                       " on ", t.device());
 }
 
-// An index tensor as the kernels read it.
-Tensor as_i32(const Tensor& t) { return t.to(torch::kInt32).contiguous(); }
+// An index tensor as the kernels read it; numbers past 32 bits stay out of range.
+Tensor as_i32(const Tensor& t) {
+    const Tensor whole = t.contiguous();
+    if (whole.scalar_type() == torch::kInt32) return whole;
+    Tensor out = fresh(whole.sizes(), torch::kInt32, whole);
+    check_status(beamgrad_narrow_indices(whole.const_data_ptr<int64_t>(), out.data_ptr<int32_t>(), whole.numel(), current_stream()),
+                 "index conversion");
+    return out;
+}
 const int32_t* i32(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
 
 // ---------------------------------------------------------------------------
