@@ -667,8 +667,12 @@ bool leaf_of_another_stream(const Tensor& leaf) {
 // In a capture: torch hands a leaf's gradient over on the stream that the leaf's
 // accumulator was made on. Where a living graph of another stream holds it, that
 // stream joins the capture and the capture's end ends the process.
-void refuse_foreign_leaves(const torch::autograd::Node* node) {
-    if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+// Gradients without memory (meta and fake tensors) are in no capture, and may be of
+// a device that is not there.
+void refuse_foreign_leaves(const torch::autograd::Node* node, const Tensors& grads) {
+    bool there = false;
+    for (const Tensor& g : grads) there |= g.defined() && g.is_cuda() && !g.unsafeGetTensorImpl()->is_python_dispatch();
+    if (!there || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     for (const auto& edge : node->next_edges()) {
         const auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
         TORCH_CHECK(!leaf || !leaf_of_another_stream(leaf->variable),
@@ -703,7 +707,7 @@ class ReorderNode : public torch::autograd::Node {
 
    protected:
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
-        refuse_foreign_leaves(this);
+        refuse_foreign_leaves(this, grads);
         const Tensor parents = parents_.unpack(shared_from_this());
         torch::autograd::variable_list out(grads.size());
         std::vector<bool> done(grads.size());

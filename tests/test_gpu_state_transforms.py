@@ -50,3 +50,16 @@ def test_tangents_with_gradients():
         tangent = forward_ad.unpack_dual(grad).tangent
     want = ref.reorder_gradient(ref.reorder(t.cpu(), PARENTS) * w.cpu(), PARENTS)[0]
     assert torch.allclose(tangent.cpu().double(), want, atol=1e-5)
+
+
+def test_a_compiled_training_step():
+    """Forward and backward traced together give what they give untraced."""
+    def step(x):
+        return bg.reorder_states([x * 2], PARENTS.cuda())[0]
+
+    x, w = draw(0, 2, 4, 5).cuda(), draw(1, 2, 4, 5).cuda()
+    want = x.clone().requires_grad_()
+    (step(want) * w).sum().backward()
+    got = x.clone().requires_grad_()
+    (torch.compile(step, backend="aot_eager", fullgraph=True)(got) * w).sum().backward()
+    assert torch.equal(got.grad, want.grad)

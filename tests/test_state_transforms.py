@@ -86,3 +86,37 @@ def test_tangents_on_the_cpu_are_refused():
         x = forward_ad.make_dual(torch.zeros(2, 3, 5), torch.zeros(2, 3, 5))
         with pytest.raises(RuntimeError, match="runs on the GPU"):
             bg.reorder_states([x], torch.zeros(2, 3, dtype=torch.int64))
+
+
+def training_step(states, parents):
+    outs = bg.reorder_states([states[0] * 2, states[1]], parents)
+    return torch.autograd.grad(sum((t * t).sum() for t in outs), states)
+
+
+def test_the_backward_has_shapes_without_a_gpu():
+    """Meta and fake tensors."""
+    parents = zeros(2, 3, dtype=torch.int64)
+    states = [zeros(2, 3, 5).requires_grad_(), zeros(2, 3).requires_grad_()]
+    assert [g.shape for g in training_step(states, parents)] == [(2, 3, 5), (2, 3)]
+    with torch._subclasses.FakeTensorMode():
+        states = [torch.zeros(2, 3, 5, requires_grad=True), torch.zeros(2, 3, requires_grad=True)]
+        grads = training_step(states, torch.zeros(2, 3, dtype=torch.int64))
+        assert [g.shape for g in grads] == [(2, 3, 5), (2, 3)]
+
+
+def test_a_training_step_is_traced():
+    """Forward and backward as one graph of the two operators."""
+    from functorch.compile import aot_function, nop
+
+    graphs = []
+
+    def keep(graph, _inputs):
+        graphs.append({node.target for node in graph.graph.nodes})
+        return nop(graph, _inputs)
+
+    step = aot_function(lambda s, parents: bg.reorder_states([s * 2], parents)[0], fw_compiler=keep, bw_compiler=keep)
+    leaf = zeros(2, 3, 5).requires_grad_()
+    step(leaf, zeros(2, 3, dtype=torch.int64)).sum().backward()
+    assert leaf.grad.shape == (2, 3, 5)
+    assert torch.ops.beamgrad.reorder_states.default in graphs[0]
+    assert torch.ops.beamgrad.reorder_states_backward.default in graphs[1]
