@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
@@ -25,6 +26,7 @@
 #include <limits>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "beamgrad_state.h"
@@ -664,6 +666,35 @@ bool leaf_of_another_stream(const Tensor& leaf) {
     return stream && stream->id() != c10::hip::getCurrentHIPStream(leaf.device().index()).id();
 }
 
+// Whether the backward from `node` on reaches such a leaf, over whatever operators.
+// During a backward, along the nodes that it runs alone: the others hand nothing over.
+bool reaches_leaf_of_another_stream(const torch::autograd::Node* node) {
+    const auto* const runs = torch::autograd::get_current_graph_task_exec_info();
+    std::vector<const torch::autograd::Node*> open{node};
+    std::unordered_set<const torch::autograd::Node*> seen{node};
+    while (!open.empty()) {
+        const torch::autograd::Node* const at = open.back();
+        open.pop_back();
+        for (const auto& edge : at->next_edges()) {
+            torch::autograd::Node* const next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (runs && !runs->empty()) {
+                const auto info = runs->find(next);
+                if (info == runs->end() || !info->second.should_execute()) continue;
+            }
+            const auto* const leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(next);
+            if (leaf && leaf_of_another_stream(leaf->variable)) return true;
+            open.push_back(next);
+        }
+    }
+    return false;
+}
+
+bool backward_reaches_leaf_of_another_stream(const Tensor& output) {
+    const auto& node = output.grad_fn();
+    return node && reaches_leaf_of_another_stream(node.get());
+}
+
 // In a capture: torch hands a leaf's gradient over on the stream that the leaf's
 // accumulator was made on. Where a living graph of another stream holds it, that
 // stream joins the capture and the capture's end ends the process.
@@ -673,12 +704,9 @@ void refuse_foreign_leaves(const torch::autograd::Node* node, const Tensors& gra
     bool there = false;
     for (const Tensor& g : grads) there |= g.defined() && g.is_cuda() && !g.unsafeGetTensorImpl()->is_python_dispatch();
     if (!there || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    for (const auto& edge : node->next_edges()) {
-        const auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
-        TORCH_CHECK(!leaf || !leaf_of_another_stream(leaf->variable),
-                    "beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of another "
-                    "stream uses; drop that graph (its outputs and losses) before the capture");
-    }
+    TORCH_CHECK(!reaches_leaf_of_another_stream(node),
+                "beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of another "
+                "stream uses; drop that graph (its outputs and losses) before the capture");
 }
 
 Tensors call_reorder(const Tensors& states, const Tensor& parents) {
@@ -816,6 +844,7 @@ TORCH_LIBRARY_FRAGMENT(beamgrad, m) {
     m.def("reorder_states_(Tensor(a!)[] states, Tensor parents) -> ()");
     m.def("reorder_states_backward(Tensor[] grads, Tensor parents) -> Tensor[]");
     m.def("leaf_of_another_stream(Tensor leaf) -> bool", &leaf_of_another_stream);
+    m.def("backward_reaches_leaf_of_another_stream(Tensor output) -> bool", &backward_reaches_leaf_of_another_stream);
 }
 
 TORCH_LIBRARY_IMPL(beamgrad, CUDA, m) {
