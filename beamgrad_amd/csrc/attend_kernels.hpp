@@ -19,7 +19,11 @@
 // from LDS by transposing reads (float32: by plain ones). m is raised only when
 // a tile's maximum passes it by 2^8: sums stay below 2^8 times their number in
 // float32, and most tiles need no rescaling of the sums. P is rounded to the
-// operands' 16 bits for the matrix instruction (float32 inputs: not at all). The
+// operands' 16 bits for the matrix instruction (float32 inputs: not at all). In
+// float16 all of a row's values are held times 2^7 (and m raised at 2^7), so that the
+// largest lies between 2^7 and 2^14, a quarter of the type's range: many that are
+// small beside one large, 2^-21 of it, keep all of their bits, and what is lost is 2^-32
+// of it a key. The
 // result is divided by the sum of the rounded values, in 32 bits, by one more
 // matrix instruction with a row of ones: vector instructions are what bounds a
 // tile of many rows, and a weighted mean of rounded weights has no error where the
@@ -108,6 +112,9 @@ struct Dims {
     // beside the sums: trees at width 128 take 98 us with 64 keys and 88 with 32.
     static constexpr int kKeys = SHAPE == kRows128 ? (k32 ? 32 : DP <= 64 ? 64 : 32) : (k32 ? 16 : 32);
     static constexpr int kKeyBlocks = kKeys / 16;
+    // The softmax's values are held times 2^kLift; their maximum is raised at 2^kSlack.
+    static constexpr float kLift = DTYPE == DBS_CUDA_DTYPE_F16 ? 7.0f : 0.0f;
+    static constexpr float kSlack = DTYPE == DBS_CUDA_DTYPE_F16 ? 7.0f : 8.0f;
     static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
     static constexpr int kRowBytes = kChunks * 16;
     static constexpr int kSteps = kChunks / 4;  // matrix steps of a key block's scores
@@ -630,7 +637,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const float slack = 8.0f / scale;
+        const float slack = X::kSlack / scale;
 
         // The page-table entry of token first + lane of a tile, read well before
         // it is needed; then the place that it gives, -1 without a page.
@@ -772,7 +779,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     const float by = m[rb] == -kInf || m[rb] == top[rb] ? 1.0f : __builtin_amdgcn_exp2f((m[rb] - top[rb]) * scale);
                     m[rb] = top[rb];
                     limit[rb] = top[rb] + slack;
-                    shift[rb] = top[rb] == -kInf ? 0.0f : -top[rb] * scale;
+                    shift[rb] = top[rb] == -kInf ? 0.0f : __builtin_fmaf(-top[rb], scale, X::kLift);
                     l[rb] *= by;
                     sum_l[rb] *= by;
 #pragma unroll
@@ -981,7 +988,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                 }
                 if (p2.lse && wk == 0 && quad == 0)
                     p2.lse[place[rb]] = l[rb] > 0.0f || l[rb] != l[rb]
-                                           ? (m[rb] * p2.scale + __builtin_amdgcn_logf(l[rb])) * 0.693147180559945309f
+                                           ? (m[rb] * p2.scale + (__builtin_amdgcn_logf(l[rb]) - X::kLift)) * 0.693147180559945309f
                                            : -kInf;
             } else {
 #pragma unroll
@@ -1194,7 +1201,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join(const AttendParams
         const float by = any ? 1.0f / total : 0.0f;
         if (column < p.D) *reinterpret_cast<Quad*>(out + column) = __builtin_convertvector(sum * by, Quad);
         if (p.lse && column == 0)
-            p.lse[place] = any ? (top * p.scale + __builtin_amdgcn_logf(total_l)) * 0.693147180559945309f : -kInf;
+            p.lse[place] = any ? (top * p.scale + (__builtin_amdgcn_logf(total_l) - X::kLift)) * 0.693147180559945309f : -kInf;
     }
     __syncthreads();
     if (!again) return;
