@@ -637,7 +637,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const float slack = X::kSlack / scale;
+        const float slack = fminf(X::kSlack / scale, __FLT_MAX__);  // finite: -inf plus it is -inf
 
         // The page-table entry of token first + lane of a tile, read well before
         // it is needed; then the place that it gives, -1 without a page.

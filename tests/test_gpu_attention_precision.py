@@ -68,3 +68,27 @@ def test_large_scores_stay_finite(dtype):
         grow = math.expm1(2 * 2 * 2.0**-4 * math.log(2))
         bound = half * want.abs() + (half + grow + 1e-4) * (p @ v.view(960, D)[:seen].double().abs()) * (1 + half) + 2.0**-20
         assert bool(((out[0, i, 0].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [1e-38, 1e-45])
+def test_the_smallest_scales(dtype, scale):
+    """All scores are 0: each row is the mean of what it sees, also where the first
+    keys are another row's alone. So many heads that none is cut."""
+    N, H, D, page = 100, 1024, 64, 16
+    parents = torch.full((1, N), -1, dtype=torch.int32)
+    parents[0, 96], parents[0, 98] = 5, 70
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(1, N, H, D, device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn(7, page, 1, D, device="cuda", generator=g).to(dtype) for _ in range(2))
+    table = bg.PageTable(torch.arange(7, dtype=torch.int32, device="cuda")[None], torch.tensor([N], dtype=torch.int32, device="cuda"),
+                         torch.ones(7, dtype=torch.int32, device="cuda"))
+    out, lse = bg.tree_attention(q, k.expand(7, page, H, D), v.expand(7, page, H, D), table, parents=parents.cuda(), scale=scale,
+                                 return_lse=True)
+    values = v.view(7 * page, D).double()
+    for i in range(N):
+        seen = [i] + [int(parents[0, i])] * int(parents[0, i] >= 0)
+        want = values[seen].mean(0)
+        # sums of one or two terms, and the rounding of the result
+        assert bool(((out[0, i].double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 2.0**-20) * values[seen].abs().sum(0)).all())
+        assert bool(((lse[0, i] - math.log(len(seen))).abs() <= 2.0**-20).all())
