@@ -46,7 +46,7 @@ struct Plan {
     int dim, shape;
     AttendSizes sizes;
     int batch;  // sequences of a launch
-    int64_t info_bytes, bytes;
+    int64_t info_bytes, bytes;  // bytes < 0: more items than a launch has
 };
 
 int multiprocessors() {
@@ -59,6 +59,15 @@ int multiprocessors() {
     return cus;
 }
 
+int64_t tiles_of(int64_t rows, int tile) { return (rows + tile - 1) / tile; }
+
+// Items of a launch: a workgroup of 256 threads each, of which HIP takes 2^32.
+constexpr int64_t kMostItems = (int64_t{1} << 24) - 1;
+// Partial results of a launch whose sequences share pages, where that is more than
+// one group's. 256 MB are 4000 tiles of 128 rows and 128 columns, several for each
+// workgroup of the card, so that a further launch costs little beside them.
+constexpr int64_t kPartialBytes = int64_t{256} << 20;
+
 Plan plan_of(const BeamgradAttention& a, AttendParams& p) {
     Plan plan;
     plan.dim = (a.head_dim + 63) / 64 * 64;
@@ -67,36 +76,57 @@ Plan plan_of(const BeamgradAttention& a, AttendParams& p) {
     p.Hkv = a.kv_heads;
     p.G = Divider::of(static_cast<uint32_t>(a.heads / a.kv_heads));
     p.D = a.head_dim;
-    // a group whose lengths one workgroup cannot hold reads its shared pages
-    // once for each beam
-    p.K = a.shared && a.beams <= kAttendSequences ? a.beams : 1;
-    p.shared = p.K > 1 ? a.shared : nullptr;
-    plan.batch = std::min(a.sequences, kAttendSequences / p.K * p.K);
+    const int64_t rows = static_cast<int64_t>(p.N) * p.G.d;
+    p.beam_rows = Divider::of(static_cast<uint32_t>(rows));
+    // A group reads its shared pages together where its beams' own tiles would be more
+    // than 8/7 of what that takes: beams that fill tiles by themselves gain nothing by
+    // it, and leave a partial result for every tile. 8 beams over 16 prompts of 4000, 8 cache
+    // heads of 128, bfloat16, us together and apart: 112 rows a beam (7 tiles, 8) 495, 411;
+    // 256 rows 1163, 837; 132 rows (9 tiles, 16) 711, 815. At 6/5 of the tiles it is one or
+    // the other (0.74 to 1.57 of the time), at 8/7 and below apart is 0.95 to 2.1 times as
+    // fast. A group whose lengths one workgroup cannot hold reads them once for each beam.
+    const int most = attend_rows(attend_most(a.data_type, plan.dim));
+    const bool together = a.shared && a.beams > 1 && a.beams <= kAttendSequences &&
+                          7 * a.beams * tiles_of(rows, most) > 8 * tiles_of(rows * a.beams, most);
+    p.K = together ? a.beams : 1;
+    p.shared = together ? a.shared : nullptr;
     // the smallest tile that takes the rows that read a page together: fewer
     // rows than the tile cost matrix instructions, more read the cache again
-    const int64_t rows = static_cast<int64_t>(p.N) * p.G.d, together = rows * p.K;
-    p.beam_rows = Divider::of(static_cast<uint32_t>(rows));
     plan.shape = kRows16;
-    while (plan.shape < attend_most(a.data_type, plan.dim) && attend_rows(plan.shape) < together) ++plan.shape;
+    while (plan.shape < attend_most(a.data_type, plan.dim) && attend_rows(plan.shape) < rows * p.K) ++plan.shape;
     const int tile = attend_rows(plan.shape);
-    p.shared_tiles = p.shared ? static_cast<int>((together + tile - 1) / tile) : 0;
-    p.own_tiles = static_cast<int>((rows + tile - 1) / tile);
-    p.head_items = plan.batch / p.K * (p.shared_tiles + p.K * p.own_tiles);
+    const int64_t shared_tiles = together ? tiles_of(rows * p.K, tile) : 0, own_tiles = tiles_of(rows, tile);
+    p.shared_tiles = static_cast<int>(shared_tiles);
+    p.own_tiles = static_cast<int>(own_tiles);
     switch (a.data_type) {
         case DBS_CUDA_DTYPE_F32: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_F32>(plan.dim, plan.shape); break;
         case DBS_CUDA_DTYPE_F16: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_F16>(plan.dim, plan.shape); break;
         default: plan.sizes = attend_sizes<DBS_CUDA_DTYPE_BF16>(plan.dim, plan.shape); break;
     }
+    // groups of a launch
+    const int64_t slot_bytes = plan.sizes.slot * static_cast<int64_t>(sizeof(float));
+    const int64_t group_items = (shared_tiles + p.K * own_tiles) * p.Hkv;
+    int64_t groups = std::min<int64_t>(a.sequences, kAttendSequences) / p.K;
+    groups = std::min(groups, std::max<int64_t>(1, kMostItems / group_items));
+    if (together) groups = std::min(groups, std::max<int64_t>(1, kPartialBytes / (group_items * slot_bytes)));
+    // launches of like size
+    const int64_t launches = tiles_of(a.sequences / p.K, static_cast<int>(groups));
+    groups = tiles_of(a.sequences / p.K, static_cast<int>(launches));
+    plan.batch = static_cast<int>(groups) * p.K;
+    const int64_t items = groups * group_items;
+    if (items > kMostItems) {
+        plan.bytes = -1;
+        return plan;
+    }
+    p.head_items = static_cast<int>(items / p.Hkv);
     // units in 30 bits, whatever the lengths
     const double keys = static_cast<double>(a.table_pages) * a.page_tokens;
     p.unit_shift = 0;
-    while (static_cast<double>(p.head_items) * p.Hkv * (std::ldexp(keys / plan.sizes.keys, -p.unit_shift) + 1.0) > 1.0e9)
-        ++p.unit_shift;
+    while (static_cast<double>(items) * (std::ldexp(keys / plan.sizes.keys, -p.unit_shift) + 1.0) > 1.0e9) ++p.unit_shift;
     p.grid = (multiprocessors() * plan.sizes.resident + 7) / 8 * 8;
-    const int64_t items = static_cast<int64_t>(p.head_items) * p.Hkv;
     plan.info_bytes = items * static_cast<int64_t>(sizeof(int4));
-    const int64_t slots = p.shared ? p.grid + items : 2 * static_cast<int64_t>(p.grid);
-    plan.bytes = plan.info_bytes + slots * plan.sizes.slot * static_cast<int64_t>(sizeof(float));
+    const int64_t slots = together ? p.grid + items : 2 * static_cast<int64_t>(p.grid);
+    plan.bytes = plan.info_bytes + slots * slot_bytes;
     return plan;
 }
 
@@ -119,7 +149,7 @@ DBS_CUDA_EXPORT int beamgrad_tree_attention(const BeamgradAttention* args, void*
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     AttendParams p{};
     const Plan plan = plan_of(a, p);
-    if (workspace_bytes < plan.bytes) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (plan.bytes < 0 || workspace_bytes < plan.bytes) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const int64_t size = a.data_type == DBS_CUDA_DTYPE_F32 ? 4 : 2;
     p.q = a.q;
     p.k = a.k;

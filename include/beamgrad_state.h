@@ -77,7 +77,10 @@ typedef struct BeamgradAttention {
     float* lse; /* or NULL */
 } BeamgradAttention;
 
-/* Workspace bytes of the call, or -1 where its sizes are refused. */
+/* Workspace bytes of the call, or -1 where its sizes are refused: partial results
+ * in float32, two tiles of up to 128 rows for each of the card's workgroups (up to two
+ * a CU); with `shared` also one for each tile of a launch, which takes as many groups as
+ * 256 MB of them allow, and one at least. */
 DBS_CUDA_EXPORT int64_t beamgrad_tree_attention_workspace_size(const BeamgradAttention* args);
 
 /* `workspace`: 16-byte aligned, of at least the size above. */
