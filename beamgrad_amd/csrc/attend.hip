@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "attend.hpp"
 #include "beamgrad_state.h"
@@ -165,6 +166,8 @@ DBS_CUDA_EXPORT int beamgrad_tree_attention(const BeamgradAttention* args, void*
     p.counts = a.counts;
     p.parents = a.parents;
     p.scale = a.scale * 1.44269504088896341f;
+    // finite at the smallest scales: -inf plus it has to be -inf
+    p.slack = std::min((a.data_type == DBS_CUDA_DTYPE_F16 ? 7.0f : 8.0f) / p.scale, std::numeric_limits<float>::max());
     p.out = a.out;
     p.lse = a.lse;
     p.info = static_cast<int4*>(workspace);

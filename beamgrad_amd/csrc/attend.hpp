@@ -47,6 +47,7 @@ struct AttendParams {
     int32_t head_items;    // items of a cache head
     int32_t unit_shift;    // a unit is the kernel's tile of keys times 2^unit_shift
     float scale;           // of the scores, times log2(e)
+    float slack;           // a maximum is raised where a score passes it by so much: 2^8, of float16 2^7
     void* out;
     float* lse;
     // workspace

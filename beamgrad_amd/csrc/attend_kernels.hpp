@@ -112,9 +112,8 @@ struct Dims {
     // beside the sums: trees at width 128 take 98 us with 64 keys and 88 with 32.
     static constexpr int kKeys = SHAPE == kRows128 ? (k32 ? 32 : DP <= 64 ? 64 : 32) : (k32 ? 16 : 32);
     static constexpr int kKeyBlocks = kKeys / 16;
-    // The softmax's values are held times 2^kLift; their maximum is raised at 2^kSlack.
+    // The softmax's values are held times 2^kLift.
     static constexpr float kLift = DTYPE == DBS_CUDA_DTYPE_F16 ? 7.0f : 0.0f;
-    static constexpr float kSlack = DTYPE == DBS_CUDA_DTYPE_F16 ? 7.0f : 8.0f;
     static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
     static constexpr int kRowBytes = kChunks * 16;
     static constexpr int kSteps = kChunks / 4;  // matrix steps of a key block's scores
@@ -637,7 +636,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db][rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const float slack = fminf(X::kSlack / scale, __FLT_MAX__);  // finite: -inf plus it is -inf
+        const float slack = p.slack;
 
         // The page-table entry of token first + lane of a tile, read well before
         // it is needed; then the place that it gives, -1 without a page.
