@@ -427,8 +427,11 @@ __global__ __launch_bounds__(kCopyThreads) void narrow_kernel(const int64_t* fro
 // Checks and launches
 // ---------------------------------------------------------------------------
 
+// Tables of up to 2^30 entries: what all sequences want together is summed, and
+// becomes places in a list, in 31 bits.
 bool valid_span(int sequences, int table_pages, int n_pages, int page_tokens) {
     return sequences > 0 && table_pages > 0 && n_pages > 0 && page_tokens > 0 &&
+           static_cast<int64_t>(sequences) * table_pages <= int64_t{1} << 30 &&
            (static_cast<int64_t>(table_pages) + 1) * page_tokens <= INT32_MAX - 65536;
 }
 

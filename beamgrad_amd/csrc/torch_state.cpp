@@ -121,6 +121,7 @@ const int32_t* i32(const Tensor& t) { return t.defined() ? t.const_data_ptr<int3
 // ---------------------------------------------------------------------------
 
 void check_pages(const Tensor& pages, const Tensor& lengths) {
+    TORCH_CHECK_VALUE(pages.numel() <= int64_t{1} << 30, "pages is too large: more than 2**30 entries, ", pages.sizes());
     TORCH_CHECK_VALUE(pages.dim() == 2 && pages.scalar_type() == torch::kInt32 && pages.is_contiguous() &&
                           pages.numel() > 0,
                       "pages must be a contiguous int32 [S, P] tensor, got ", pages.scalar_type(), " ", pages.sizes());
@@ -128,7 +129,6 @@ void check_pages(const Tensor& pages, const Tensor& lengths) {
                           lengths.size(0) == pages.size(0) && lengths.is_contiguous() && lengths.device() == pages.device(),
                       "lengths must be a contiguous int32 [S] = [", pages.size(0), "] tensor on the same device, got ",
                       lengths.scalar_type(), " ", lengths.sizes());
-    TORCH_CHECK_VALUE(pages.size(0) <= kI32Max && pages.size(1) <= kI32Max, "pages is too large");
 }
 
 void check_table(const Tensor& pages, const Tensor& lengths, const Tensor& refs) {

@@ -15,10 +15,10 @@
  *
  * A page table holds S sequences: pages [S, P] (the pages of each sequence in
  * order, -1 past its last), lengths [S] (tokens held) and refs [n_pages] (how
- * many sequences hold each page; 0: it is free). Values read from device
- * memory are checked where they are used: an entry that is no page of the pool
- * counts as -1, a length is cut to [0, P * page_tokens], a token without a
- * page is seen by no query and written nowhere.
+ * many sequences hold each page; 0: it is free); S * P is at most 2^30. Values
+ * read from device memory are checked where they are used: an entry that is no
+ * page of the pool counts as -1, a length is cut to [0, P * page_tokens], a token
+ * without a page is seen by no query and written nowhere.
  */
 #pragma once
 
