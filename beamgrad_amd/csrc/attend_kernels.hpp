@@ -30,12 +30,12 @@
 // values are equal. The log-sum that a caller asks for is the unrounded values'.
 //
 // What bounds it, on one MI355X: few rows, the reads (two sequences of 90000 to
-// 131000 tokens, 8 cache heads of 128, bfloat16: 946 MB in 168 us, 5.6 TB/s); many
+// 131000 tokens, 8 cache heads of 128, bfloat16: 946 MB in 170 us, 5.6 TB/s); many
 // rows, the latency of a tile's steps with two workgroups a CU, whose registers are
 // full (4 prompts' ends of 1000 tokens over 1500 to 4500, 32 heads of 64: 113 GFLOP
-// in 226 us, vector instructions issued in 55 % of the time, matrix ones busy in 27);
-// short caches, the chain of dependent reads (700 tokens: 10 us, of which the lengths
-// and totals 3).
+// in 223 us under the profiler, 209 a call with the join without it; vector
+// instructions issued in 55 % of the time, matrix ones busy in 28); short caches, the
+// chain of dependent reads (700 tokens: 10 us, of which launch and lengths 3).
 #pragma once
 
 #include <type_traits>
@@ -484,85 +484,85 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
             if (threadIdx.x == 0) p1.info[w.item] = make_int4(0, 0, 0, 0);
             at = stop;
         } else {
-        w.head = at / head_line;
-        int off = at - w.head * head_line;  // in the head, then in the sequence, then in the item
-        int seq = -1;
-        for (int s0 = 0; s0 < p1.S; s0 += 64) {
-            const bool ahead = s0 + lane < p1.S && board.first[s0 + lane] <= off;
-            seq += __popcll(__ballot(ahead));
-        }
-        off -= uniform(board.first[seq]);
-        group = p1.shared ? seq / p1.K : seq;
-        const int from = p1.shared ? uniform(board.shared[group]) : 0;
-        // elements of the line that so many units are
-        const auto elements = [&](int units) { return by_pieces ? (units + each - 1) / each : units; };
-        int units = (from + unit - 1) >> unit_log, end = from, length = elements(units);
-        int place_in_head = group * (p1.shared_tiles + p1.K * p1.own_tiles);
-        w.shared = p1.shared && seq == group * p1.K && off < p1.shared_tiles * length;
-        if (w.shared) {
-            w.tile = off / length;
-            off -= w.tile * length;
-            w.seq = uniform(board.leader[group]);
-            w.own = {uniform(board.length[w.seq]), uniform(board.count[w.seq])};
-            w.key0 = 0;
-            place_in_head += w.tile;
-        } else {
-            if (p1.shared && seq == group * p1.K) off -= p1.shared_tiles * length;
-            w.seq = seq;
-            w.own = {uniform(board.length[seq]), uniform(board.count[seq])};
-            w.key0 = from;
-            if (p1.parents || row_tiles(p1, w.own, ROWS) == 1) {
-                end = w.own.length;
-                units = (end - from + unit - 1) >> unit_log;
-                length = elements(units);
+            w.head = at / head_line;
+            int off = at - w.head * head_line;  // in the head, then in the sequence, then in the item
+            int seq = -1;
+            for (int s0 = 0; s0 < p1.S; s0 += 64) {
+                const bool ahead = s0 + lane < p1.S && board.first[s0 + lane] <= off;
+                seq += __popcll(__ballot(ahead));
+            }
+            off -= uniform(board.first[seq]);
+            group = p1.shared ? seq / p1.K : seq;
+            const int from = p1.shared ? uniform(board.shared[group]) : 0;
+            // elements of the line that so many units are
+            const auto elements = [&](int units) { return by_pieces ? (units + each - 1) / each : units; };
+            int units = (from + unit - 1) >> unit_log, end = from, length = elements(units);
+            int place_in_head = group * (p1.shared_tiles + p1.K * p1.own_tiles);
+            w.shared = p1.shared && seq == group * p1.K && off < p1.shared_tiles * length;
+            if (w.shared) {
                 w.tile = off / length;
                 off -= w.tile * length;
+                w.seq = uniform(board.leader[group]);
+                w.own = {uniform(board.length[w.seq]), uniform(board.count[w.seq])};
+                w.key0 = 0;
+                place_in_head += w.tile;
             } else {
-                // tiles of rows that read ever more keys: a lane for each
-                for (w.tile = 0;; w.tile += 64) {
-                    const int t = w.tile + lane;
-                    const int mine_end = key_end<ROWS>(p1, w.own, t);
-                    const int mine_units = t < p1.own_tiles ? (mine_end - from + unit - 1) >> unit_log : 0;
-                    const int n = elements(mine_units), upto = wave_upto(n);
-                    const uint64_t past = __ballot(upto > off);
-                    if (past) {
-                        const int first = __builtin_ctzll(past);
-                        w.tile += first;
-                        units = __shfl(mine_units, first);
-                        length = __shfl(n, first);
-                        off -= __shfl(upto, first) - length;
-                        end = __shfl(mine_end, first);
-                        break;
+                if (p1.shared && seq == group * p1.K) off -= p1.shared_tiles * length;
+                w.seq = seq;
+                w.own = {uniform(board.length[seq]), uniform(board.count[seq])};
+                w.key0 = from;
+                if (p1.parents || row_tiles(p1, w.own, ROWS) == 1) {
+                    end = w.own.length;
+                    units = (end - from + unit - 1) >> unit_log;
+                    length = elements(units);
+                    w.tile = off / length;
+                    off -= w.tile * length;
+                } else {
+                    // tiles of rows that read ever more keys: a lane for each
+                    for (w.tile = 0;; w.tile += 64) {
+                        const int t = w.tile + lane;
+                        const int mine_end = key_end<ROWS>(p1, w.own, t);
+                        const int mine_units = t < p1.own_tiles ? (mine_end - from + unit - 1) >> unit_log : 0;
+                        const int n = elements(mine_units), upto = wave_upto(n);
+                        const uint64_t past = __ballot(upto > off);
+                        if (past) {
+                            const int first = __builtin_ctzll(past);
+                            w.tile += first;
+                            units = __shfl(mine_units, first);
+                            length = __shfl(n, first);
+                            off -= __shfl(upto, first) - length;
+                            end = __shfl(mine_end, first);
+                            break;
+                        }
+                        off -= __shfl(upto, 63);
                     }
-                    off -= __shfl(upto, 63);
                 }
+                place_in_head += p1.shared_tiles + (seq - group * p1.K) * p1.own_tiles + w.tile;
             }
-            place_in_head += p1.shared_tiles + (seq - group * p1.K) * p1.own_tiles + w.tile;
-        }
-        off = uniform(off);
-        units = uniform(units);
-        length = uniform(length);
-        end = uniform(end);
-        w.tile = uniform(w.tile);
-        w.item = uniform(w.head * p1.head_items + place_in_head);
-        w.starts = off == 0;
-        int first_unit = off, n_units, last;
-        if (by_pieces) {
-            first_unit = off * each;
-            n_units = min(each, units - first_unit);
-            last = mine - off + length - 1;
-            w.whole = length == 1 && from == 0;
-            at = stop;
-        } else {
-            const int start = at - off, until = min(start + units, stop);
-            n_units = until - at;
-            last = (start + units - 1) / each;
-            w.whole = w.starts && until == start + units && from == 0;
-            at = until;
-        }
-        w.key0 += first_unit << unit_log;
-        w.end = min(end, w.key0 + (n_units << unit_log));
-        if (w.starts && threadIdx.x == 0) p1.info[w.item] = make_int4(mine, last, from > 0, 0);
+            off = uniform(off);
+            units = uniform(units);
+            length = uniform(length);
+            end = uniform(end);
+            w.tile = uniform(w.tile);
+            w.item = uniform(w.head * p1.head_items + place_in_head);
+            w.starts = off == 0;
+            int first_unit = off, n_units, last;
+            if (by_pieces) {
+                first_unit = off * each;
+                n_units = min(each, units - first_unit);
+                last = mine - off + length - 1;
+                w.whole = length == 1 && from == 0;
+                at = stop;
+            } else {
+                const int start = at - off, until = min(start + units, stop);
+                n_units = until - at;
+                last = (start + units - 1) / each;
+                w.whole = w.starts && until == start + units && from == 0;
+                at = until;
+            }
+            w.key0 += first_unit << unit_log;
+            w.end = min(end, w.key0 + (n_units << unit_log));
+            if (w.starts && threadIdx.x == 0) p1.info[w.item] = make_int4(mine, last, from > 0, 0);
         }
 
         // ---- the piece's rows ----
@@ -969,7 +969,7 @@ __global__ __launch_bounds__(kAttendThreads, (Dims<DTYPE, DP, SHAPE>::kResident)
                     o[db][rb] = x;
                 }
             }
-            }
+        }
         if (w.whole && again && threadIdx.x == 0) p2.info[w.item].w = 1;
         float* const part = p2.partial + slot_of(p2, mine, w.item, w.starts) * X::kSlot;
 #pragma unroll
