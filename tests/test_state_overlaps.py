@@ -155,7 +155,7 @@ int main(void) {
     int64_t row[2] = {16, 16}, page[2] = {64, 64}, token[2] = {16, 16}, strides[4] = {32, 16, 32, 16};
     BeamgradPools p = {base, row, page, token, 2, 4, 4, 0};
     BeamgradTable from = {ints, ints + 16, ints + 20}, to = {ints + 32, ints + 48, ints + 52};
-    const void* news[2] = {memory + 2048, memory + 3072};
+    const void* news[2] = {memory + 2048, memory + 3200};
     if (beamgrad_fork_pages(&p, &from, ints, 0, 4, 4, &to, ints, 4096, 0) != 2) return 1;
     if (beamgrad_keep_tokens(&p, &from, ints, ints, ints, 4, 4, 1, &to, 0) != 2) return 2;
     if (beamgrad_write_tokens(&p, news, strides, ints, ints, 0, 4, 4, 2, 0) != 2) return 3;
