@@ -8,8 +8,10 @@ served by hand-written HIP kernels in ``libdbs_hip`` (whose C ABI is the
 reference's ``dbs_cuda.h``). Beside them, the state of the model that is
 searched: attention over a paged cache (``tree_attention``), the cache's pages
 (``PageTable``, ``fork_pages``, ``extend_pages``, ``write_tokens``,
-``keep_tokens``) and dense states in the order of the beams
-(``reorder_states``).
+``keep_tokens``), its eviction by the attention that tokens got
+(``accumulate_weights``, ``evict_tokens``), rotary positions (``rotary``), dense states
+in the order of the beams (``reorder_states``), and the log-probabilities of given
+tokens (``token_logprobs``).
 
 The public names load on first use. Importing the package itself loads
 nothing, so ``beamgrad_amd._C_hip`` (the operators' HIP kernels) can be
@@ -32,11 +34,17 @@ _PUBLIC = {
     "beam_search": "._search",
     "search": "._search",
     "sequence_scores": "._search",
+    "TokenLogprobs": "._scores",
+    "token_logprobs": "._scores",
     "PageTable": "._cache",
+    "accumulate_weights": "._cache",
+    "evict_tokens": "._cache",
     "extend_pages": "._cache",
     "fork_pages": "._cache",
     "keep_tokens": "._cache",
     "reorder_states": "._cache",
+    "rotary": "._cache",
+    "rotary_frequencies": "._cache",
     "tree_attention": "._cache",
     "write_tokens": "._cache",
     "BeamSearchOutput": "._torch",

@@ -44,7 +44,7 @@ LIB_SOURCES = ["csrc/api.hip", "csrc/host_abi.cpp", "csrc/host_results.cpp", "cs
                "csrc/select.hip", "csrc/select_f32.hip",
                "csrc/select_f16.hip", "csrc/select_bf16.hip", "csrc/backward.hip",
                "csrc/attend.hip", "csrc/attend_bf16.hip", "csrc/attend_f16.hip", "csrc/attend_f32.hip",
-               "csrc/pages.hip", "csrc/states.hip"]
+               "csrc/pages.hip", "csrc/evict.hip", "csrc/weigh.hip", "csrc/rotary.hip", "csrc/states.hip", "csrc/scores.hip"]
 
 
 def lib_path() -> str:
@@ -118,7 +118,8 @@ def _torch_module(name: str, sources: list[str], hip: bool) -> str:
 def build_ext() -> list[str]:
     """The schema owner ``_C`` and the HIP kernels ``_C_hip``."""
     return [_torch_module("_C", ["csrc/torch_schemas.cpp"], hip=False),
-            _torch_module("_C_hip", ["csrc/torch_ops.cpp", "csrc/torch_state.cpp"], hip=True)]
+            _torch_module("_C_hip", ["csrc/torch_ops.cpp", "csrc/torch_state.cpp", "csrc/torch_rotary.cpp",
+                                      "csrc/torch_scores.cpp"], hip=True)]
 
 
 def build() -> None:

@@ -42,6 +42,7 @@
 
 #include "attend.hpp"
 #include "dbs_cuda.h"
+#include "matrix.hpp"
 
 // of a lambda: its captures and arrays stay in registers
 #define BEAMGRAD_INLINE __attribute__((always_inline))
@@ -49,47 +50,10 @@
 namespace dbs_hip {
 namespace attend {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 typedef __attribute__((address_space(3))) char lds_char;
 typedef const __attribute__((address_space(1))) char global_char;
-
-template <int DTYPE>
-struct Elem;
-template <>
-struct Elem<DBS_CUDA_DTYPE_BF16> {
-    using T = __bf16;
-    using Frag = bf16x8;
-    using Quad = bf16x4;
-    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Elem<DBS_CUDA_DTYPE_F16> {
-    using T = _Float16;
-    using Frag = f16x8;
-    using Quad = f16x4;
-    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Elem<DBS_CUDA_DTYPE_F32> {
-    using T = float;
-    using Frag = f32x4;
-    using Quad = f32x4;
-    static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-        return c;
-    }
-};
 
 // Sizes of a kernel.
 template <int DTYPE, int DP, int SHAPE>

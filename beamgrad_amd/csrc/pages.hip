@@ -15,6 +15,7 @@
 #include "beamgrad_state.h"
 #include "engine.hpp"
 #include "paged.hpp"
+#include "pools.hpp"
 #include "regions.hpp"
 #include "rows.hpp"
 #include "torch_engine.hpp"
@@ -35,22 +36,6 @@ struct PoolSet {
     int64_t row_bytes, page_stride, token_stride;
     int32_t n;
 };
-
-struct Table {
-    const int32_t* pages;
-    const int32_t* lengths;
-    const int32_t* refs;
-    int32_t* pages_out;
-    int32_t* lengths_out;
-    int32_t* refs_out;
-    PageSpan span;
-    int32_t S;
-};
-
-__device__ __forceinline__ int page_at(const Table& t, int s, int column) {
-    const int32_t entry = t.pages[static_cast<int64_t>(s) * t.span.P + column];
-    return t.span.is_page(entry) ? entry : -1;
-}
 
 // Exclusive sum over a workgroup of kPlanThreads, and the total.
 __device__ int block_rank(int x, int* lds, int& total) {
@@ -430,22 +415,6 @@ __global__ __launch_bounds__(kCopyThreads) void narrow_kernel(const int64_t* fro
 // Checks and launches
 // ---------------------------------------------------------------------------
 
-// Tables of up to 2^30 entries: what all sequences want together is summed, and
-// becomes places in a list, in 31 bits.
-bool valid_span(int sequences, int table_pages, int n_pages, int page_tokens) {
-    return sequences > 0 && table_pages > 0 && n_pages > 0 && page_tokens > 0 &&
-           static_cast<int64_t>(sequences) * table_pages <= int64_t{1} << 30 &&
-           (static_cast<int64_t>(table_pages) + 1) * page_tokens <= INT32_MAX - 65536;
-}
-
-bool valid_pools(const BeamgradPools* p) {
-    if (!p || p->n < 0 || p->reserved != 0) return false;
-    if (p->n > 0 && (!p->base || !p->row_bytes || !p->page_stride || !p->token_stride)) return false;
-    for (int i = 0; i < p->n; ++i)
-        if (!p->base[i] || p->row_bytes[i] <= 0 || p->page_stride[i] < 0 || p->token_stride[i] < 0) return false;
-    return true;
-}
-
 // A pool, or a token of one, that lies where another does would be moved twice, and
 // in no order; what is read meanwhile must not change.
 bool lie_apart(const BeamgradPools& p, const void* const* news, const int64_t* news_strides, int sequences, int tokens) {
@@ -456,26 +425,6 @@ bool lie_apart(const BeamgradPools& p, const void* const* news, const int64_t* n
         return Region{reinterpret_cast<uintptr_t>(news[i]), {sequences, tokens}, {news_strides[2 * i], news_strides[2 * i + 1]}, p.row_bytes[i]};
     };
     return all_apart(p.n, pool, news ? p.n : 0, rows);
-}
-
-bool valid_table(const BeamgradTable* t) { return t && t->pages && t->lengths && t->refs; }
-
-// The new table is written while the old one is read: none of its parts may lie in
-// it, or in each other.
-bool tables_apart(const BeamgradTable& from, const BeamgradTable& to, int S, int P, int n_pages) {
-    const int32_t* const parts[6] = {to.pages, to.lengths, to.refs, from.pages, from.lengths, from.refs};
-    const int64_t size[3] = {static_cast<int64_t>(S) * P, S, n_pages};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 6; ++j) {
-            const uintptr_t a = reinterpret_cast<uintptr_t>(parts[i]), b = reinterpret_cast<uintptr_t>(parts[j]);
-            if (a < b + size[j % 3] * sizeof(int32_t) && b < a + size[i] * sizeof(int32_t)) return false;
-        }
-    return true;
-}
-
-Table table_of(const BeamgradTable& from, const BeamgradTable& to, int S, int P, int n_pages, int page_tokens) {
-    return {from.pages, from.lengths, from.refs, to.pages, to.lengths, to.refs,
-            {Divider::of(static_cast<uint32_t>(page_tokens)), n_pages, P}, S};
 }
 
 // The pools in sets of one geometry, as many as a launch's arguments hold;

@@ -1,0 +1,562 @@
+// SPDX-License-Identifier: MIT
+//
+// Log-probabilities of given tokens, entropies, the most likely tokens, and
+// the logits' gradient (include/beamgrad_score.h).
+//
+// Mathematics. One pass over a row: each thread keeps the maximum m of its
+// values, s = sum e^(x - m) and, for the entropy, t = sum (x - m) e^(x - m), all
+// brought to a new maximum once for every 64 bytes that it reads; the threads' are
+// joined at the end. log p = (x - m) - log s in this order (m and log s stay
+// apart: their sum would lose the low bits of a likely token's log p), H = log s -
+// t / s.
+//
+// The alternatives come out of the same pass: every thread's m is the maximum of
+// its share of the row, so the top-th largest of the threads' maxima is reached
+// by at least `top` values, and what reaches it lies with the threads whose own
+// maximum does: about `top` threads, whose shares (a few hundred values of a large
+// vocabulary) are read again, from the cache. What they hold beside the alternatives
+// is little (20 of 151936 at random: one or two), unless values are equal
+// in great number: where more than kKept reach it, or fewer than `top` do (-inf),
+// the alternatives are found one after the other.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+#include "beamgrad_score.h"
+#include "engine.hpp"
+#include "paged.hpp"
+#include "rows.hpp"
+
+using namespace dbs_hip;
+
+namespace {
+
+constexpr int kThreads = 256;  // of a row's workgroup; short rows: one wavefront
+constexpr int kAtOnce = 4;     // 16-byte reads of a thread in flight
+constexpr int kMaxTop = 64;
+constexpr int kKept = 512;     // values beside the alternatives that a workgroup ranks
+constexpr int kMaxParts = 64;  // of a row
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kFar = -1000.0f;  // e^kFar is 0 in 32 bits
+
+struct Rows {
+    const char* logits;
+    int64_t outer, inner;  // strides in bytes
+    Divider width;         // rows of an outer one
+    int32_t V, top;
+    const void* tokens;
+    bool i64;
+    float* logprobs;
+    float* entropy;
+    float* top_logprobs;
+    int64_t* top_tokens;
+    float4* stats;  // m, log s, H, unused
+
+    __device__ const char* row(uint32_t r) const {
+        const uint32_t o = width.quotient(r);
+        return logits + o * outer + static_cast<int64_t>(r - o * width.d) * inner;
+    }
+    __device__ int token(uint32_t r) const {  // -1: none
+        const int64_t t = i64 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
+        return t >= 0 && t < V ? static_cast<int>(t) : -1;
+    }
+};
+
+// A part's sums, in the workspace where rows are split.
+struct Sums {
+    float m, s, t, none;
+};
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m);
+    const float da = a.m - m, db = b.m - m, wa = exp_of(da), wb = exp_of(db);
+    return {m, __builtin_fmaf(a.s, wa, b.s * wb),
+            __builtin_fmaf(wa, __builtin_fmaf(a.s, fmaxf(da, kFar), a.t), wb * __builtin_fmaf(b.s, fmaxf(db, kFar), b.t)), 0.0f};
+}
+
+// A value and its place as one number: the larger value, of equal ones the
+// lower place, is larger. 0 is below all of them (NaN does not come here).
+__device__ __forceinline__ uint64_t key_of(float x, int place) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x + 0.0f);
+    const uint32_t high = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    return static_cast<uint64_t>(high) << 32 | (0xffffffffu - static_cast<uint32_t>(place));
+}
+__device__ __forceinline__ int place_of(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t high = static_cast<uint32_t>(key >> 32);
+    return __builtin_bit_cast(float, high & 0x80000000u ? high & 0x7fffffffu : ~high);
+}
+
+template <class T>
+constexpr int kEach = 16 / sizeof(T);
+
+// The 16 bytes at place v of a row's end `V`: what lies past it is -inf.
+template <class T>
+__device__ __forceinline__ void values_at(const char* row, int v, int V, float* x) {
+    const u32x4 raw = load16(row + static_cast<int64_t>(v) * sizeof(T), static_cast<int64_t>(V - v) * sizeof(T));
+    T e[kEach<T>];
+    __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < kEach<T>; ++i) x[i] = v + i < V ? static_cast<float>(e[i]) : -__builtin_inff();
+}
+
+template <bool ENTROPY>
+__device__ __forceinline__ void take(Sums& a, const float* x, int n) {
+    float m = a.m;
+#pragma unroll
+    for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
+    const float d0 = a.m - m, w = exp_of(d0);
+    a.t = ENTROPY ? w * __builtin_fmaf(a.s, fmaxf(d0, kFar), a.t) : 0.0f;
+    a.s *= w;
+    a.m = m;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+        const float d = x[i] - m, e = exp_of(d);
+        a.s += e;
+        if (ENTROPY) a.t = __builtin_fmaf(e, fmaxf(d, kFar), a.t);
+    }
+}
+
+// A thread's share of [from, to) of a row: 16 bytes of every THREADS * 16.
+template <class T, bool ENTROPY, int THREADS>
+__device__ __forceinline__ Sums sums_of(const char* row, int from, int to) {
+    constexpr int E = kEach<T>;
+    Sums a{-FLT_MAX, 0.0f, 0.0f, 0.0f};
+    int64_t v = from + static_cast<int>(threadIdx.x) * E;
+    constexpr int64_t step = THREADS * E;
+    float x[kAtOnce * E];
+    for (; v + (kAtOnce - 1) * step + E <= to; v += kAtOnce * step) {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const u32x4 raw = *reinterpret_cast<const u32x4_any*>(row + (v + i * step) * sizeof(T));
+            T e[E];
+            __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[i * E + j] = static_cast<float>(e[j]);
+        }
+        take<ENTROPY>(a, x, kAtOnce * E);
+    }
+    for (; v < to; v += step) {
+        values_at<T>(row, static_cast<int>(v), to, x);
+        take<ENTROPY>(a, x, E);
+    }
+    return a;
+}
+
+template <int THREADS>
+struct Shared {
+    Sums waves[THREADS / 64];
+    float top[THREADS];          // the threads' maxima
+    int flagged[THREADS], flags, kept;
+    float floor;                 // what reaches it may be an alternative
+    uint64_t keys[kKept];
+    uint64_t best[THREADS / 64];
+};
+
+template <int THREADS>
+__device__ __forceinline__ Sums joined_block(Sums a, Shared<THREADS>& lds) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        a = joined(a, {__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.0f});
+    if ((threadIdx.x & 63) == 0) lds.waves[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = lds.waves[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) a = joined(a, lds.waves[w]);
+    return a;
+}
+
+template <int THREADS>
+__device__ __forceinline__ uint64_t largest_in_block(uint64_t key, Shared<THREADS>& lds) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const uint32_t lo = __shfl_xor(static_cast<uint32_t>(key), d), hi = __shfl_xor(static_cast<uint32_t>(key >> 32), d);
+        const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
+        key = other > key ? other : key;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds.best[threadIdx.x >> 6] = key;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) key = lds.best[w] > key ? lds.best[w] : key;
+    return key;
+}
+
+// The `top` largest keys of [from, to), given the thread's maximum, in order to
+// each(rank, key). Fewer than `top` values: key 0 for the rest.
+template <class T, int THREADS, class Each>
+__device__ __forceinline__ void alternatives(const char* row, int from, int to, int top, float mine, Shared<THREADS>& lds, Each each) {
+    constexpr int E = kEach<T>;
+    const int tid = threadIdx.x;
+    if (tid == 0) lds.flags = lds.kept = 0;
+    lds.top[tid] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int j = 0; j < THREADS; ++j) rank += lds.top[j] > mine || (lds.top[j] == mine && j < tid);
+    if (rank == top - 1) lds.floor = mine;
+    __syncthreads();
+    const float floor = lds.floor;
+    if (mine >= floor) lds.flagged[atomicAdd(&lds.flags, 1)] = tid;
+    __syncthreads();
+    const int shares = (to - from + THREADS * E - 1) / (THREADS * E), items = lds.flags * shares;
+    for (int i = tid; i < items; i += THREADS) {
+        const int v = from + ((i % shares) * THREADS + lds.flagged[i / shares]) * E;
+        if (v >= to) continue;
+        float x[E];
+        values_at<T>(row, v, to, x);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (v + j < to && x[j] >= floor) {
+                const int at = atomicAdd(&lds.kept, 1);
+                if (at < kKept) lds.keys[at] = key_of(x[j], v + j);
+            }
+    }
+    __syncthreads();
+    const int n = lds.kept, values = min(top, to - from);
+    if (n >= values && n <= kKept) {
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t key = lds.keys[i];
+            int above = 0;
+            for (int j = 0; j < n; ++j) above += lds.keys[j] > key;
+            if (above < top) each(above, key);
+        }
+    } else {
+        // one after the other: the largest below the last one
+        uint64_t below = ~uint64_t{0};
+        for (int k = 0; k < values; ++k) {
+            uint64_t best = 0;
+            for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
+                float x[E];
+                values_at<T>(row, static_cast<int>(v), to, x);
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const uint64_t key = key_of(x[j], static_cast<int>(v) + j);
+                    if (v + j < to && key < below && key > best) best = key;
+                }
+            }
+            below = largest_in_block(best, lds);
+            if (tid == 0) each(k, below);
+        }
+    }
+    for (int k = values + tid; k < top; k += THREADS) each(k, uint64_t{0});
+}
+
+struct Normal {
+    float m, log_s, entropy;
+    bool empty;  // nothing in the row is possible
+    __device__ float logp(float x) const { return empty ? -__builtin_inff() : (x - m) - log_s; }
+};
+
+__device__ __forceinline__ Normal normal_of(const Sums& a) {
+    const bool empty = a.s == 0.0f;
+    const float log_s = logf(a.s);
+    return {a.m, log_s, empty ? 0.0f : log_s - a.t / a.s, empty};
+}
+
+template <class T>
+__device__ __forceinline__ float value_at(const char* row, int v) {
+    return static_cast<float>(reinterpret_cast<const T*>(row)[v]);
+}
+
+// What one thread writes of a row.
+template <class T>
+__device__ __forceinline__ void write_row(const Rows& p, uint32_t r, const char* row, int token, const Normal& n) {
+    p.logprobs[r] = n.logp(value_at<T>(row, token));
+    if (p.entropy) p.entropy[r] = n.entropy;
+    if (p.stats) p.stats[r] = float4{n.m, n.empty ? __builtin_inff() : n.log_s, n.entropy, 0.0f};
+}
+
+__device__ __forceinline__ void write_alternative(const Rows& p, uint32_t r, int rank, uint64_t key, const Normal& n) {
+    const int64_t at = static_cast<int64_t>(r) * p.top + rank;
+    p.top_logprobs[at] = n.logp(value_of(key));
+    p.top_tokens[at] = place_of(key);
+}
+
+// A row of no token, or (`bad`) one that holds NaN or +inf: by all threads.
+template <int THREADS>
+__device__ __forceinline__ void write_none(const Rows& p, uint32_t r, bool bad) {
+    const float nan = __builtin_nanf("");
+    if (threadIdx.x == 0) {
+        p.logprobs[r] = bad ? nan : 0.0f;
+        if (p.entropy) p.entropy[r] = bad ? nan : 0.0f;
+        if (p.stats) p.stats[r] = float4{nan, nan, nan, 0.0f};
+    }
+    for (int k = threadIdx.x; k < p.top; k += THREADS) {
+        p.top_logprobs[static_cast<int64_t>(r) * p.top + k] = bad ? nan : -__builtin_inff();
+        p.top_tokens[static_cast<int64_t>(r) * p.top + k] = -1;
+    }
+}
+
+// A workgroup for a row.
+template <class T, bool ENTROPY, int THREADS>
+__global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
+    __shared__ Shared<THREADS> lds;
+    const uint32_t r = blockIdx.x;
+    const int token = p.token(r);
+    if (token < 0) return write_none<THREADS>(p, r, false);
+    const char* const row = p.row(r);
+    const Sums mine = sums_of<T, ENTROPY, THREADS>(row, 0, p.V);
+    const Sums all = joined_block(mine, lds);
+    if (!(all.s <= FLT_MAX)) return write_none<THREADS>(p, r, true);
+    const Normal n = normal_of(all);
+    if (threadIdx.x == 0) write_row<T>(p, r, row, token, n);
+    if (p.top > 0)
+        alternatives<T>(row, 0, p.V, p.top, mine.m, lds, [&](int rank, uint64_t key) { write_alternative(p, r, rank, key, n); });
+}
+
+// x: a part of `part` values of row y. Sums and alternatives go to the workspace.
+template <class T, bool ENTROPY>
+__global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int part, Sums* sums, uint64_t* keys) {
+    __shared__ Shared<kThreads> lds;
+    const uint32_t r = blockIdx.y;
+    if (p.token(r) < 0) return;
+    const char* const row = p.row(r);
+    const int from = blockIdx.x * part, to = min(p.V, from + part);
+    const Sums mine = sums_of<T, ENTROPY, kThreads>(row, from, to);
+    const Sums all = joined_block(mine, lds);
+    const int64_t at = static_cast<int64_t>(r) * gridDim.x + blockIdx.x;
+    if (threadIdx.x == 0) sums[at] = all;
+    if (p.top > 0 && all.s <= FLT_MAX)
+        alternatives<T>(row, from, to, p.top, mine.m, lds, [&](int rank, uint64_t key) { keys[at * p.top + rank] = key; });
+}
+
+// A workgroup joins the parts of a row. The parts' alternatives are in order: of the
+// j-th of each part, j * parts >= top, the lowest is reached by `top` of them, so
+// what lies below it is none.
+template <class T>
+__global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
+    __shared__ uint64_t kept[kMaxParts * kMaxTop];
+    __shared__ uint64_t lowest[kThreads / 64];
+    __shared__ int found;
+    const uint32_t r = blockIdx.x;
+    const int token = p.token(r), tid = threadIdx.x;
+    if (token < 0) return write_none<kThreads>(p, r, false);
+    const int64_t first = static_cast<int64_t>(r) * parts;
+    Sums all = (tid & 63) < parts ? sums[first + (tid & 63)] : Sums{-FLT_MAX, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        all = joined(all, {__shfl_xor(all.m, d), __shfl_xor(all.s, d), __shfl_xor(all.t, d), 0.0f});
+    if (!(all.s <= FLT_MAX)) return write_none<kThreads>(p, r, true);
+    const Normal n = normal_of(all);
+    if (tid == 0) write_row<T>(p, r, p.row(r), token, n);
+    if (p.top == 0) return;
+    const uint64_t* const mine = keys + first * p.top;
+    const int j = (p.top + parts - 1) / parts - 1;
+    uint64_t floor = tid < parts ? mine[tid * p.top + j] : ~uint64_t{0};
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const uint32_t lo = __shfl_xor(static_cast<uint32_t>(floor), d), hi = __shfl_xor(static_cast<uint32_t>(floor >> 32), d);
+        const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
+        floor = other < floor ? other : floor;
+    }
+    if (tid == 0) found = 0;
+    if ((tid & 63) == 0) lowest[tid >> 6] = floor;
+    __syncthreads();
+    floor = lowest[0];
+    for (int i = tid; i < parts * p.top; i += kThreads)
+        if (mine[i] >= floor && mine[i] != 0) kept[atomicAdd(&found, 1)] = mine[i];
+    __syncthreads();
+    const int m = found;
+    for (int i = tid; i < m; i += kThreads) {
+        const uint64_t key = kept[i];
+        int above = 0;
+        for (int k = 0; k < m; ++k) above += kept[k] > key;
+        if (above < p.top) write_alternative(p, r, above, key, n);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The gradient
+// ---------------------------------------------------------------------------
+
+struct Grads {
+    const float* logprobs;
+    const float* entropy;
+    const float* top;
+    char* logits;  // the gradient
+};
+
+// x: `part` values of row y (parts first: grid x = rows * parts). p_v comes
+// from the row's m and log s. The token and the alternatives, whose own gradients
+// come in addition, are written over by a thread for each: with g their sum at v,
+// g (1 - p_v) - p_v (A - g + ...) has no cancellation where p_v is near 1.
+template <class T, bool ENTROPY, int THREADS>
+__global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Grads g, const Divider parts, const int part) {
+    constexpr int E = kEach<T>;
+    __shared__ int places[kMaxTop + 1];
+    __shared__ float given[kMaxTop + 1];
+    const uint32_t r = parts.quotient(blockIdx.x);
+    const int from = static_cast<int>(blockIdx.x - r * parts.d) * part, to = min(p.V, from + part), tid = threadIdx.x;
+    const int token = p.token(r);
+    char* const out = g.logits + static_cast<int64_t>(r) * p.V * sizeof(T);
+    const float4 stats = p.stats[r];
+    const float m = stats.x, log_s = stats.y, H = stats.z;
+    if (token < 0 || log_s == __builtin_inff()) {
+        const u32x4 zero = {0, 0, 0, 0};
+        for (int64_t v = from + tid * E; v < to; v += THREADS * E) store16(out + v * sizeof(T), zero, (to - v) * sizeof(T));
+        return;
+    }
+    const char* const row = p.row(r);
+    const int top = g.top ? p.top : 0;
+    const float given_token = g.logprobs ? g.logprobs[r] : 0.0f, gH = ENTROPY ? g.entropy[r] : 0.0f;
+    float sum = given_token;
+    for (int k = 0; k < top; ++k) sum += g.top[static_cast<int64_t>(r) * p.top + k];
+    const auto rest = [&](float d, float by) { return ENTROPY ? __builtin_fmaf(gH, fmaxf(d, kFar) + H, by) : by; };
+    for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
+        float x[E];
+        values_at<T>(row, static_cast<int>(v), to, x);
+        T y[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float d = (x[i] - m) - log_s;
+            y[i] = static_cast<T>(-exp_of(d) * rest(d, sum));
+        }
+        u32x4 raw;
+        __builtin_memcpy(&raw, y, 16);
+        store16(out + v * sizeof(T), raw, (to - v) * sizeof(T));
+    }
+    for (int k = tid; k <= top; k += THREADS) {
+        places[k] = k == 0 ? token : static_cast<int>(p.top_tokens[static_cast<int64_t>(r) * p.top + k - 1]);
+        given[k] = k == 0 ? given_token : g.top[static_cast<int64_t>(r) * p.top + k - 1];
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int k = tid; k <= top; k += THREADS) {
+        const int v = places[k];
+        if (v < from || v >= to || (k > 0 && v == token)) continue;
+        float by = given[k];
+        if (k == 0)
+            for (int i = 1; i <= top; ++i) by += places[i] == v ? given[i] : 0.0f;
+        const float d = (value_at<T>(row, v) - m) - log_s;
+        reinterpret_cast<T*>(out)[v] = static_cast<T>(__builtin_fmaf(by, -expm1f(d), -exp_of(d) * rest(d, sum - by)));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Checks and launches
+// ---------------------------------------------------------------------------
+
+int element_size(int data_type) { return data_type == DBS_CUDA_DTYPE_F32 ? 4 : 2; }
+
+bool valid_sizes(const BeamgradTokenLogprobs* a) {
+    return a && (a->data_type == DBS_CUDA_DTYPE_F32 || a->data_type == DBS_CUDA_DTYPE_F16 || a->data_type == DBS_CUDA_DTYPE_BF16) &&
+           a->outer > 0 && a->inner > 0 && static_cast<int64_t>(a->outer) * a->inner < int64_t{1} << 24 && a->vocab > 0 &&
+           a->vocab <= 1 << 30 && a->top >= 0 && a->top <= kMaxTop && a->top <= a->vocab && a->strides[0] >= 0 && a->strides[1] >= 0;
+}
+
+Rows rows_of(const BeamgradTokenLogprobs& a) {
+    const int size = element_size(a.data_type);
+    return {static_cast<const char*>(a.logits), a.strides[0] * size, a.strides[1] * size, Divider::of(static_cast<uint32_t>(a.inner)),
+            a.vocab, a.top, a.tokens, a.tokens_i64 != 0, a.logprobs, a.entropy, a.top_logprobs, a.top_tokens, reinterpret_cast<float4*>(a.stats)};
+}
+
+// A row of up to two rounds of a wavefront is one's work.
+bool is_short(int vocab, int size) { return static_cast<int64_t>(vocab) * size <= 2 * 64 * 16 * kAtOnce; }
+
+// Few rows are split, so that the card's 256 CUs have work; a part is 16 KB at
+// least (a round of a workgroup's reads).
+int parts_of(const BeamgradTokenLogprobs& a) {
+    constexpr int64_t kWanted = 1024, kLeast = kThreads * 16 * kAtOnce;
+    const int64_t rows = static_cast<int64_t>(a.outer) * a.inner, bytes = static_cast<int64_t>(a.vocab) * element_size(a.data_type);
+    if (rows >= kWanted || is_short(a.vocab, element_size(a.data_type))) return 1;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(kWanted + rows - 1) / rows, (bytes + kLeast - 1) / kLeast, kMaxParts})));
+}
+
+// Values of a part: whole rounds of a workgroup's reads.
+int part_values(int vocab, int parts, int size) {
+    const int64_t round = kThreads * 16 / size, each = (vocab + parts - 1) / parts;
+    return static_cast<int>(std::min<int64_t>((each + round - 1) / round * round, 1 << 30));
+}
+
+template <class Launch>
+void by_type(int data_type, bool entropy, bool one_wave, Launch launch) {
+    const auto sized = [&](auto t, auto e) {
+        if (one_wave)
+            launch(t, e, std::integral_constant<int, 64>{});
+        else
+            launch(t, e, std::integral_constant<int, kThreads>{});
+    };
+    const auto typed = [&](auto t) {
+        if (entropy)
+            sized(t, std::true_type{});
+        else
+            sized(t, std::false_type{});
+    };
+    if (data_type == DBS_CUDA_DTYPE_F32)
+        typed(float{});
+    else if (data_type == DBS_CUDA_DTYPE_F16)
+        typed(_Float16{});
+    else
+        typed(__bf16{});
+}
+
+}  // namespace
+
+extern "C" {
+
+DBS_CUDA_EXPORT int64_t beamgrad_token_logprobs_workspace_size(const BeamgradTokenLogprobs* args) {
+    if (!valid_sizes(args)) return -1;
+    const int64_t rows = static_cast<int64_t>(args->outer) * args->inner;
+    const int parts = parts_of(*args);
+    return parts == 1 ? 0 : rows * parts * static_cast<int64_t>(sizeof(Sums) + args->top * sizeof(uint64_t));
+}
+
+DBS_CUDA_EXPORT int beamgrad_token_logprobs(const BeamgradTokenLogprobs* args, void* workspace, int64_t workspace_bytes,
+                                            void* stream_ptr) {
+    if (!valid_sizes(args) || !args->logits || !args->tokens || !args->logprobs ||
+        (args->top > 0 && (!args->top_logprobs || !args->top_tokens)))
+        return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    const int64_t rows = static_cast<int64_t>(args->outer) * args->inner;
+    const int64_t bytes = beamgrad_token_logprobs_workspace_size(args);
+    if (bytes > 0 && (!workspace || workspace_bytes < bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
+        return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    const Rows p = rows_of(*args);
+    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    const bool entropy = args->entropy != nullptr;  // its gradient needs it too
+    int parts = parts_of(*args);
+    const int size = element_size(args->data_type), part = part_values(p.V, parts, size);
+    by_type(args->data_type, entropy, is_short(p.V, size), [&](auto t, auto with_entropy, auto threads) {
+        using T = decltype(t);
+        constexpr bool kEntropy = decltype(with_entropy)::value;
+        constexpr int kOfRow = decltype(threads)::value;
+        if (parts == 1) {
+            score_rows<T, kEntropy, kOfRow><<<static_cast<unsigned>(rows), kOfRow, 0, stream>>>(p);
+            return;
+        }
+        parts = (p.V + part - 1) / part;
+        Sums* const sums = static_cast<Sums*>(workspace);
+        uint64_t* const keys = reinterpret_cast<uint64_t*>(sums + rows * parts);
+        score_parts<T, kEntropy><<<dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows)), kThreads, 0, stream>>>(p, part, sums, keys);
+        score_join<T><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(p, parts, sums, keys);
+    });
+    return finish_call(stream, hipGetLastError());
+}
+
+DBS_CUDA_EXPORT int beamgrad_token_logprobs_backward(const BeamgradTokenLogprobs* args, const float* grad_logprobs,
+                                                     const float* grad_entropy, const float* grad_top, void* grad_logits,
+                                                     void* stream_ptr) {
+    if (!valid_sizes(args) || !args->logits || !args->tokens || !args->stats || !grad_logits ||
+        (grad_top && (args->top == 0 || !args->top_tokens)))
+        return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    const Rows p = rows_of(*args);
+    const int64_t rows = static_cast<int64_t>(args->outer) * args->inner;
+    const int size = element_size(args->data_type);
+    // 32 KB of a row for a workgroup
+    const int part = part_values(p.V, static_cast<int>(std::max<int64_t>(1, static_cast<int64_t>(p.V) * size / (32 * 1024))), size);
+    const int64_t parts = (p.V + part - 1) / part;
+    if (rows * parts >= int64_t{1} << 24) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    const Grads g{grad_logprobs, grad_entropy, grad_top, static_cast<char*>(grad_logits)};
+    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    by_type(args->data_type, grad_entropy != nullptr, is_short(p.V, size), [&](auto t, auto with_entropy, auto threads) {
+        constexpr int kOfPart = decltype(threads)::value;
+        score_backward<decltype(t), decltype(with_entropy)::value, kOfPart>
+            <<<static_cast<unsigned>(rows * parts), kOfPart, 0, stream>>>(p, g, Divider::of(static_cast<uint32_t>(parts)), part);
+    });
+    return finish_call(stream, hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,277 +1,18 @@
 // SPDX-License-Identifier: MIT
 //
 // The torch.ops.beamgrad operators of a model's state in a search: attention
-// over a paged cache, its pages, reordering of dense states
+// over a paged cache, its pages, eviction from it, reordering of dense states
 // (include/beamgrad_state.h has the C entries). Part of beamgrad_amd._C_hip.
 //
 // Every operator checks its arguments in one function that needs no GPU. The
 // CPU key runs the checks and then refuses the call, so a wrong argument has its
 // message wherever the tensors are. Nothing is read back and nothing waits:
 // page tables stay on the device, and the calls can be captured into a graph.
-#include <torch/all.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/graph_task.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/autograd/variable.h>
-#include <torch/library.h>
-
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
-
-#include <cmath>
-#include <limits>
-#include <string>
-#include <tuple>
-#include <unordered_set>
-#include <vector>
-
-#include "beamgrad_state.h"
-#include "regions.hpp"
-#include "torch_engine.hpp"
+#include "torch_state.hpp"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = c10::optional<Tensor>;
-using Tensors = std::vector<Tensor>;
-
-constexpr int64_t kI32Max = std::numeric_limits<int32_t>::max();
-
-void* current_stream() { return c10::hip::getCurrentHIPStream().stream(); }
-
-void check_status(int code, const char* what) {
-    if (code == DBS_CUDA_STATUS_OK) return;
-    TORCH_CHECK_VALUE(code != DBS_CUDA_STATUS_INVALID_ARGUMENT, "beamgrad HIP ", what, ": invalid argument");
-    TORCH_CHECK(false, "beamgrad HIP ", what, " failed: ", dbs_cuda_status_string(code));
-}
-
-[[noreturn]] void refuse_cpu(const char* what, const Tensor& t) {
-    TORCH_CHECK(false, "beamgrad::", what, " runs on the GPU (HIP) only, got a tensor on ", t.device());
-}
-
-// A contiguous tensor from the caching allocator, without a trip through the
-// dispatcher (a call makes several, and small calls take as long as their host work).
-Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
-    return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
-}
-
-// Operators without a derivative, at the Autograd key: what a torch.func
-// transform wraps is still seen here.
-void refuse_derivatives(const Tensor& t, const c10::OperatorHandle& op) {
-    const auto name = [&] {
-        const std::string what = op.schema().name().substr(sizeof("beamgrad::") - 1);
-        return what == "reorder_states_" ? "reorder_states(inplace=True)" : what;
-    };
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "beamgrad_amd.", name(),
-                " has no gradient: call it under torch.no_grad() or on detached tensors");
-    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), "beamgrad_amd.", name(),
-                " has no forward-mode derivative, and would drop a tensor's tangent: call it on the tensors' primals");
-}
-
-void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
-    for (const c10::IValue& argument : torch::jit::last(*stack, op.schema().arguments().size())) {
-        if (argument.isTensor()) {
-            refuse_derivatives(argument.toTensor(), op);
-        } else if (argument.isTensorList()) {
-            for (const auto& t : argument.toListRef()) refuse_derivatives(t.toTensor(), op);
-        }
-    }
-    op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
-}
-
-// Written in place: an autograd graph that saved such a tensor notices.
-void written(at::TensorList tensors) {
-    for (const Tensor& t : tensors)
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-int data_type(const Tensor& t, const char* name) {
-    if (t.scalar_type() == torch::kFloat32) return DBS_CUDA_DTYPE_F32;
-    if (t.scalar_type() == torch::kFloat16) return DBS_CUDA_DTYPE_F16;
-    TORCH_CHECK_VALUE(t.scalar_type() == torch::kBFloat16, name, " must be float32, float16 or bfloat16, got ",
-                      t.scalar_type());
-    return DBS_CUDA_DTYPE_BF16;
-}
-
-bool index_type(const Tensor& t) { return t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64; }
-
-void check_index(const Tensor& t, at::IntArrayRef shape, const Tensor& with, const char* name) {
-    TORCH_CHECK_VALUE(index_type(t) && t.sizes() == shape && t.device() == with.device(), name,
-                      " must be an int32 or int64 ", shape, " tensor on the same device, got ", t.scalar_type(), " ", t.sizes(),
-                      " on ", t.device());
-}
-
-// An index tensor as the kernels read it; numbers past 32 bits stay out of range.
-Tensor as_i32(const Tensor& t) {
-    const Tensor whole = t.contiguous();
-    if (whole.scalar_type() == torch::kInt32) return whole;
-    Tensor out = fresh(whole.sizes(), torch::kInt32, whole);
-    check_status(beamgrad_narrow_indices(whole.const_data_ptr<int64_t>(), out.data_ptr<int32_t>(), whole.numel(), current_stream()),
-                 "index conversion");
-    return out;
-}
-const int32_t* i32(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
-
-// ---------------------------------------------------------------------------
-// Page tables and pools
-// ---------------------------------------------------------------------------
-
-void check_pages(const Tensor& pages, const Tensor& lengths) {
-    TORCH_CHECK_VALUE(pages.numel() <= int64_t{1} << 30, "pages is too large: more than 2**30 entries, ", pages.sizes());
-    TORCH_CHECK_VALUE(pages.dim() == 2 && pages.scalar_type() == torch::kInt32 && pages.is_contiguous() &&
-                          pages.numel() > 0,
-                      "pages must be a contiguous int32 [S, P] tensor, got ", pages.scalar_type(), " ", pages.sizes());
-    TORCH_CHECK_VALUE(lengths.scalar_type() == torch::kInt32 && lengths.dim() == 1 &&
-                          lengths.size(0) == pages.size(0) && lengths.is_contiguous() && lengths.device() == pages.device(),
-                      "lengths must be a contiguous int32 [S] = [", pages.size(0), "] tensor on the same device, got ",
-                      lengths.scalar_type(), " ", lengths.sizes());
-}
-
-void check_table(const Tensor& pages, const Tensor& lengths, const Tensor& refs) {
-    check_pages(pages, lengths);
-    TORCH_CHECK_VALUE(refs.dim() == 1 && refs.scalar_type() == torch::kInt32 && refs.is_contiguous() &&
-                          refs.numel() > 0 && refs.numel() <= kI32Max && refs.device() == pages.device(),
-                      "refs must be a contiguous int32 [pages of the pool] tensor on the same device, got ",
-                      refs.scalar_type(), " ", refs.sizes());
-}
-
-void check_span(const Tensor& pages, int64_t page_tokens) {
-    TORCH_CHECK_VALUE(page_tokens > 0, "a page must hold at least one token, got ", page_tokens);
-    TORCH_CHECK_VALUE((pages.size(1) + 1) <= (kI32Max - 65536) / page_tokens,
-                      "a sequence's pages must hold fewer than 2**31 tokens, got ", pages.size(1), " of ", page_tokens);
-}
-
-struct Pools {
-    std::vector<void*> base;
-    std::vector<int64_t> row_bytes, page_stride, token_stride;
-    BeamgradPools c{};
-
-    void bind() {
-        c.base = base.data();
-        c.row_bytes = row_bytes.data();
-        c.page_stride = page_stride.data();
-        c.token_stride = token_stride.data();
-        c.n = static_cast<int32_t>(base.size());
-    }
-};
-
-// Whether a token's row of t (the dimensions from `from` on) is one run.
-bool row_contiguous(const Tensor& t, int64_t from) {
-    int64_t run = 1;
-    for (int64_t d = t.dim() - 1; d >= from; --d) {
-        if (t.size(d) != 1 && t.stride(d) != run) return false;
-        run *= t.size(d);
-    }
-    return true;
-}
-
-int64_t row_elements(const Tensor& t, int64_t from) {
-    int64_t n = 1;
-    for (int64_t d = from; d < t.dim(); ++d) n *= t.size(d);
-    return n;
-}
-
-// Whether b lies as a does: most pools of a cache do, and are checked once.
-bool laid_out_alike(const Tensor& a, const Tensor& b) {
-    return a.sizes() == b.sizes() && a.strides() == b.strides() && a.scalar_type() == b.scalar_type() &&
-           a.device() == b.device();
-}
-
-void check_pools(const Tensors& pools, const Tensor& pages, int64_t n_pages) {
-    for (size_t i = 0; i < pools.size(); ++i) {
-        const Tensor& t = pools[i];
-        if (i > 0 && laid_out_alike(pools[i - 1], t)) continue;
-        TORCH_CHECK_VALUE(t.dim() >= 3 && t.numel() > 0, "pools[", i, "] must be a [pages, tokens of a page, ...] tensor, got ",
-                          t.sizes());
-        TORCH_CHECK_VALUE(t.device() == pages.device(), "pools[", i, "] is on ", t.device(), ", the page table on ",
-                          pages.device());
-        TORCH_CHECK_VALUE(t.size(1) == pools[0].size(1) && t.size(0) == (n_pages < 0 ? pools[0].size(0) : n_pages), "pools[", i,
-                          "] must have ", n_pages < 0 ? pools[0].size(0) : n_pages, " pages of ", pools[0].size(1),
-                          " tokens, got ", t.sizes());
-        TORCH_CHECK_VALUE(row_contiguous(t, 2), "a token's row of pools[", i, "] must be contiguous");
-        TORCH_CHECK_VALUE(t.size(0) <= kI32Max, "pools[", i, "] has too many pages");
-        // a page or token that lies where another does would be written twice
-        TORCH_CHECK_VALUE((t.size(1) == 1 || t.stride(1) >= row_elements(t, 2)) && (t.size(0) == 1 || t.stride(0) > 0),
-                          "the pages and tokens of pools[", i, "] overlap");
-    }
-    if (!pools.empty()) check_span(pages, pools[0].size(1));
-}
-
-// Pools whose memory meets, or news that lie in one, which the C entries refuse:
-// with the numbers of two.
-dbs_hip::Region rows_of(const Tensor& t) {
-    const int64_t size = static_cast<int64_t>(t.element_size());
-    return {reinterpret_cast<uintptr_t>(t.const_data_ptr()), {t.size(0), t.size(1)}, {t.stride(0) * size, t.stride(1) * size},
-            row_elements(t, 2) * size};
-}
-
-void check_pools_apart(const Tensors& pools, const Tensors& news) {
-    std::vector<dbs_hip::Region> written, read;
-    std::vector<size_t> at;  // in news: those that are no copy
-    for (const Tensor& t : pools) written.push_back(rows_of(t));
-    for (size_t i = 0; i < news.size(); ++i)
-        if (row_contiguous(news[i], 2)) {
-            read.push_back(rows_of(news[i]));
-            at.push_back(i);
-        }
-    const dbs_hip::Meeting m = dbs_hip::find_meeting(written, read);
-    if (m.first < 0) return;
-    TORCH_CHECK_VALUE(!m.reads, "news[", at[m.second], "] and pools[", m.first, "] share memory");
-    TORCH_CHECK_VALUE(m.first != m.second, "the pages and tokens of pools[", m.first, "] overlap");
-    TORCH_CHECK_VALUE(false, "pools[", m.first, "] and pools[", m.second, "] share memory");
-}
-
-Pools bind_pools(const Tensors& pools, int64_t n_pages, int64_t page_tokens) {
-    Pools p;
-    p.base.reserve(pools.size());
-    p.row_bytes.reserve(pools.size());
-    p.page_stride.reserve(pools.size());
-    p.token_stride.reserve(pools.size());
-    for (size_t i = 0; i < pools.size(); ++i) {
-        const Tensor& t = pools[i];
-        p.base.push_back(t.data_ptr());
-        if (i > 0 && laid_out_alike(pools[i - 1], t)) {
-            p.row_bytes.push_back(p.row_bytes.back());
-            p.page_stride.push_back(p.page_stride.back());
-            p.token_stride.push_back(p.token_stride.back());
-            continue;
-        }
-        const int64_t size = static_cast<int64_t>(t.element_size());
-        p.row_bytes.push_back(row_elements(t, 2) * size);
-        p.page_stride.push_back(t.stride(0) * size);
-        p.token_stride.push_back(t.stride(1) * size);
-    }
-    p.bind();
-    p.c.n_pages = static_cast<int32_t>(n_pages);
-    p.c.page_tokens = static_cast<int32_t>(page_tokens);
-    return p;
-}
-
-BeamgradTable bind_table(const Tensor& pages, const Tensor& lengths, const Tensor& refs) {
-    return {const_cast<int32_t*>(pages.const_data_ptr<int32_t>()), const_cast<int32_t*>(lengths.const_data_ptr<int32_t>()),
-            const_cast<int32_t*>(refs.const_data_ptr<int32_t>())};
-}
-
-int narrow(int64_t n) { return static_cast<int>(n); }
-
-using TableOut = std::tuple<Tensor, Tensor, Tensor>;
-
-struct NewTable {
-    Tensor pages, lengths, refs;
-    NewTable(const Tensor& p, const Tensor& l, const Tensor& r)
-        : pages(fresh(p.sizes(), torch::kInt32, p)), lengths(fresh(l.sizes(), torch::kInt32, p)), refs(fresh(r.sizes(), torch::kInt32, p)) {}
-    BeamgradTable bind() const { return bind_table(pages, lengths, refs); }
-    TableOut take() { return {std::move(pages), std::move(lengths), std::move(refs)}; }
-};
-
-Tensor workspace(int64_t bytes, const Tensor& like) {
-    TORCH_CHECK_VALUE(bytes >= 0, "beamgrad HIP: unsupported problem size (see the limits in beamgrad_state.h)");
-    return fresh({bytes > 0 ? bytes : 1}, torch::kUInt8, like);
-}
+using namespace beamgrad_torch;
 
 // --- fork ---
 
@@ -468,9 +209,12 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     cache(v, "v");
 }
 
-// strides of the first three dimensions; of a dimension of one entry, 0
-void strides_of(const Tensor& t, int64_t* to) {
-    for (int d = 0; d < 3; ++d) to[d] = t.size(d) == 1 ? 0 : t.stride(d);
+// Queries whose heads are contiguous and begin at multiples of 16 bytes: q, or a copy.
+Tensor aligned_rows(const Tensor& q) {
+    const int64_t size = static_cast<int64_t>(q.element_size());
+    bool fits = q.stride(3) == 1 && reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16 == 0;
+    for (int d = 0; d < 3; ++d) fits = fits && (q.size(d) == 1 || q.stride(d) * size % 16 == 0);
+    return fits ? q : q.clone(at::MemoryFormat::Contiguous);
 }
 
 std::tuple<Tensor, Tensor> tree_attention_cpu(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths,
@@ -485,11 +229,7 @@ std::tuple<Tensor, Tensor> tree_attention_hip(const Tensor& q, const Tensor& k, 
                                               double scale, bool with_lse) {
     check_attention(q, k, v, pages, lengths, parents, counts, beams, shared, scale);
     const at::OptionalDeviceGuard guard(q.device());
-    Tensor query = q;
-    const int64_t size = static_cast<int64_t>(q.element_size());
-    bool fits = q.stride(3) == 1 && reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16 == 0;
-    for (int d = 0; d < 3; ++d) fits = fits && (q.size(d) == 1 || q.stride(d) * size % 16 == 0);
-    if (!fits) query = q.clone(at::MemoryFormat::Contiguous);
+    const Tensor query = aligned_rows(q);
     Tensor par, num, sh;
     if (parents) par = as_i32(*parents);
     if (counts) num = as_i32(*counts);
@@ -525,6 +265,148 @@ std::tuple<Tensor, Tensor> tree_attention_hip(const Tensor& q, const Tensor& k, 
     const Tensor ws = workspace(bytes, q);
     check_status(beamgrad_tree_attention(&a, ws.data_ptr(), bytes, current_stream()), "tree_attention");
     return {out, lse};
+}
+
+// ---------------------------------------------------------------------------
+// Eviction by the attention that tokens got
+// ---------------------------------------------------------------------------
+
+void check_weights_shape(const Tensor& w, at::IntArrayRef shape, const Tensor& with, const std::string& name) {
+    TORCH_CHECK_VALUE(w.scalar_type() == torch::kFloat32 && w.sizes() == shape && w.device() == with.device(), name, " must be a float32 ", shape,
+                      " tensor (sequences, heads, places of a sequence's pages) on the same device, got ", w.scalar_type(), " ", w.sizes(), " on ",
+                      w.device());
+}
+
+void check_accumulate(const Tensor& weights, const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& pages, const Tensor& lengths,
+                      const OptTensor& parents, const OptTensor& counts, double scale) {
+    check_attention(q, k, k, pages, lengths, parents, counts, 1, c10::nullopt, scale);
+    check_weights_shape(weights, {q.size(0), k.size(2), pages.size(1) * k.size(1)}, q, "weights");
+    TORCH_CHECK_VALUE(weights.size(2) == 1 || weights.stride(2) == 1, "weights' places must be contiguous, got strides ", weights.strides());
+    const auto nested = [&](int64_t inner, int64_t outer) {  // one dimension's places lie apart, and all of them along the other
+        const int64_t run = (weights.size(inner) - 1) * weights.stride(inner) + weights.size(2);
+        return (weights.size(inner) == 1 || weights.stride(inner) >= weights.size(2)) && (weights.size(outer) == 1 || weights.stride(outer) >= run);
+    };
+    TORCH_CHECK_VALUE(nested(1, 0) || nested(0, 1), "weights' sequences and heads overlap, got strides ", weights.strides());
+    TORCH_CHECK_VALUE(lse.scalar_type() == torch::kFloat32 && lse.sizes() == q.sizes().slice(0, 3) && lse.device() == q.device(),
+                      "lse must be a float32 ", q.sizes().slice(0, 3), " tensor on q's device, got ", lse.scalar_type(), " ", lse.sizes(), " on ",
+                      lse.device());
+    TORCH_CHECK_VALUE(k.size(2) <= 65535, "a cache must have at most 65535 heads, got ", k.size(2));
+}
+
+void accumulate_weights_cpu(const Tensor& weights, const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& pages, const Tensor& lengths,
+                            const OptTensor& parents, const OptTensor& counts, double scale) {
+    check_accumulate(weights, q, k, lse, pages, lengths, parents, counts, scale);
+    refuse_cpu("accumulate_weights", q);
+}
+
+void accumulate_weights_hip(const Tensor& weights, const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& pages, const Tensor& lengths,
+                            const OptTensor& parents, const OptTensor& counts, double scale) {
+    check_accumulate(weights, q, k, lse, pages, lengths, parents, counts, scale);
+    const at::OptionalDeviceGuard guard(q.device());
+    const Tensor query = aligned_rows(q), sums = lse.contiguous();
+    Tensor par, num;
+    if (parents) par = as_i32(*parents);
+    if (counts) num = as_i32(*counts);
+    BeamgradWeights a{};
+    a.q = query.const_data_ptr();
+    a.k = k.const_data_ptr();
+    a.data_type = data_type(q, "q");
+    a.sequences = narrow(q.size(0));
+    a.tokens = narrow(q.size(1));
+    a.heads = narrow(q.size(2));
+    a.kv_heads = narrow(k.size(2));
+    a.head_dim = narrow(q.size(3));
+    a.page_tokens = narrow(k.size(1));
+    a.n_pages = narrow(k.size(0));
+    a.table_pages = narrow(pages.size(1));
+    a.scale = static_cast<float>(scale);
+    strides_of(query, a.q_strides);
+    strides_of(k, a.k_strides);
+    for (int d = 0; d < 2; ++d) a.weight_strides[d] = weights.size(d) == 1 ? 0 : weights.stride(d);
+    a.pages = i32(pages);
+    a.lengths = i32(lengths);
+    a.counts = i32(num);
+    a.parents = i32(par);
+    a.lse = sums.const_data_ptr<float>();
+    a.weights = weights.data_ptr<float>();
+    const int64_t bytes = beamgrad_accumulate_weights_workspace_size(&a);
+    Tensor ws;
+    if (bytes != 0) ws = workspace(bytes, q);
+    check_status(beamgrad_accumulate_weights(&a, bytes != 0 ? ws.data_ptr() : nullptr, bytes, current_stream()), "accumulate_weights");
+    written({weights});
+}
+
+using EvictOut = std::tuple<Tensor, Tensor, Tensor, Tensors>;
+
+void check_evict(const Tensors& pools, const Tensors& weights, const Tensor& pages, const Tensor& lengths, const Tensor& refs,
+                 const OptTensor& budgets, int64_t budget, int64_t recent, int64_t first) {
+    check_table(pages, lengths, refs);
+    TORCH_CHECK_VALUE(!pools.empty(), "pools must hold at least one pool");
+    check_pools(pools, pages, refs.numel());
+    TORCH_CHECK_VALUE(!weights.empty() && pools.size() % weights.size() == 0, "the pools must be a multiple of the weights, and those at least one, got ",
+                      pools.size(), " and ", weights.size());
+    TORCH_CHECK_VALUE(weights[0].dim() == 3 && weights[0].size(1) >= 1 && weights[0].size(1) <= 1024, "weights[0] must be [S, heads, places], got ",
+                      weights[0].sizes());
+    const int64_t S = pages.size(0), G = weights[0].size(1), places = pages.size(1) * pools[0].size(1);
+    TORCH_CHECK_VALUE(S <= 65535, "a table must have at most 65535 sequences for evict_tokens, got ", S);
+    for (size_t i = 0; i < weights.size(); ++i) {
+        check_weights_shape(weights[i], {S, G, places}, pages, "weights[" + std::to_string(i) + "]");
+    }
+    for (size_t i = 0; i < pools.size(); ++i) {
+        TORCH_CHECK_VALUE(G == 1 || pools[i].size(2) == G, "weights of ", G, " heads need pools [pages, tokens of a page, ", G, ", ...], got pools[", i,
+                          "] ", pools[i].sizes());
+        TORCH_CHECK_VALUE(row_elements(pools[i], 2) * static_cast<int64_t>(pools[i].element_size()) <= 2 << 20, "a token's row of pools[", i,
+                          "] must be at most 2 MB, got ", pools[i].sizes());
+    }
+    if (budgets) check_index(*budgets, {S}, pages, "budget");
+    TORCH_CHECK_VALUE(budgets || (budget >= 0 && budget <= kI32Max), "budget must be in [0, 2**31), got ", budget);
+    TORCH_CHECK_VALUE(recent >= 0 && recent <= kI32Max, "recent must be in [0, 2**31), got ", recent);
+    TORCH_CHECK_VALUE(first >= 0 && first <= kI32Max, "first must be in [0, 2**31), got ", first);
+}
+
+EvictOut evict_tokens_cpu(Tensors pools, Tensors weights, const Tensor& pages, const Tensor& lengths, const Tensor& refs,
+                          const OptTensor& budgets, int64_t budget, int64_t recent, int64_t first) {
+    check_evict(pools, weights, pages, lengths, refs, budgets, budget, recent, first);
+    check_pools_apart(pools, {});
+    refuse_cpu("evict_tokens", pages);
+}
+
+EvictOut evict_tokens_hip(Tensors pools, Tensors weights, const Tensor& pages, const Tensor& lengths, const Tensor& refs, const OptTensor& budgets,
+                          int64_t budget, int64_t recent, int64_t first) {
+    check_evict(pools, weights, pages, lengths, refs, budgets, budget, recent, first);
+    const at::OptionalDeviceGuard guard(pages.device());
+    const Tensor most = budgets ? as_i32(*budgets) : Tensor();
+    const Pools p = bind_pools(pools, refs.numel(), pools[0].size(1));
+    Tensors out;
+    std::vector<const float*> source;
+    std::vector<float*> target;
+    std::vector<int64_t> strides;
+    for (Tensor& w : weights) {
+        if (w.size(2) != 1 && w.stride(2) != 1) w = w.contiguous();
+        out.push_back(fresh(w.sizes(), torch::kFloat32, w));
+        source.push_back(w.const_data_ptr<float>());
+        target.push_back(out.back().data_ptr<float>());
+        for (int d = 0; d < 2; ++d) strides.push_back(w.size(d) == 1 ? 0 : w.stride(d));
+    }
+    BeamgradEviction a{};
+    a.weights = source.data();
+    a.weight_strides = strides.data();
+    a.to_weights = target.data();
+    a.n_weights = narrow(static_cast<int64_t>(weights.size()));
+    a.heads = narrow(weights[0].size(1));
+    a.budgets = i32(most);
+    a.budget = narrow(budget);
+    a.recent = narrow(recent);
+    a.first = narrow(first);
+    NewTable to(pages, lengths, refs);
+    const BeamgradTable from = bind_table(pages, lengths, refs), table = to.bind();
+    const int64_t bytes = beamgrad_evict_tokens_workspace_size(&p.c, &a, narrow(pages.size(0)), narrow(pages.size(1)));
+    const Tensor ws = workspace(bytes, pages);
+    const int status = beamgrad_evict_tokens(&p.c, &a, &from, narrow(pages.size(0)), narrow(pages.size(1)), &table, ws.data_ptr(), bytes, current_stream());
+    if (status == DBS_CUDA_STATUS_INVALID_ARGUMENT) check_pools_apart(pools, {});
+    check_status(status, "evict_tokens");
+    written(pools);
+    return {std::move(to.pages), std::move(to.lengths), std::move(to.refs), std::move(out)};
 }
 
 // ---------------------------------------------------------------------------
@@ -656,59 +538,6 @@ Tensors reorder_states_backward_hip(Tensors grads, const Tensor& parents) {
     return out;
 }
 
-// Whether a living graph holds the leaf's gradient accumulator with a stream
-// that is not the current one.
-bool leaf_of_another_stream(const Tensor& leaf) {
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
-    if (!accumulator || !leaf.is_cuda()) return false;
-    const auto stream = accumulator->stream();
-    // by number: the two sides name the device's type differently on ROCm
-    return stream && stream->id() != c10::hip::getCurrentHIPStream(leaf.device().index()).id();
-}
-
-// Whether the backward from `node` on reaches such a leaf, over whatever operators.
-// During a backward, along the nodes that it runs alone: the others hand nothing over.
-bool reaches_leaf_of_another_stream(const torch::autograd::Node* node) {
-    const auto* const runs = torch::autograd::get_current_graph_task_exec_info();
-    std::vector<const torch::autograd::Node*> open{node};
-    std::unordered_set<const torch::autograd::Node*> seen{node};
-    while (!open.empty()) {
-        const torch::autograd::Node* const at = open.back();
-        open.pop_back();
-        for (const auto& edge : at->next_edges()) {
-            torch::autograd::Node* const next = edge.function.get();
-            if (!next || !seen.insert(next).second) continue;
-            if (runs && !runs->empty()) {
-                const auto info = runs->find(next);
-                if (info == runs->end() || !info->second.should_execute()) continue;
-            }
-            const auto* const leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(next);
-            if (leaf && leaf_of_another_stream(leaf->variable)) return true;
-            open.push_back(next);
-        }
-    }
-    return false;
-}
-
-bool backward_reaches_leaf_of_another_stream(const Tensor& output) {
-    const auto& node = output.grad_fn();
-    return node && reaches_leaf_of_another_stream(node.get());
-}
-
-// In a capture: torch hands a leaf's gradient over on the stream that the leaf's
-// accumulator was made on. Where a living graph of another stream holds it, that
-// stream joins the capture and the capture's end ends the process.
-// Gradients without memory (meta and fake tensors) are in no capture, and may be of
-// a device that is not there.
-void refuse_foreign_leaves(const torch::autograd::Node* node, const Tensors& grads) {
-    bool there = false;
-    for (const Tensor& g : grads) there |= g.defined() && g.is_cuda() && !g.unsafeGetTensorImpl()->is_python_dispatch();
-    if (!there || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    TORCH_CHECK(!reaches_leaf_of_another_stream(node),
-                "beamgrad_amd.reorder_states: a captured backward reaches a leaf that a living graph of another "
-                "stream uses; drop that graph (its outputs and losses) before the capture");
-}
-
 Tensors call_reorder(const Tensors& states, const Tensor& parents) {
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("beamgrad::reorder_states", "")
@@ -735,7 +564,7 @@ class ReorderNode : public torch::autograd::Node {
 
    protected:
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
-        refuse_foreign_leaves(this, grads);
+        refuse_foreign_leaves(this, grads, "reorder_states");
         const Tensor parents = parents_.unpack(shared_from_this());
         torch::autograd::variable_list out(grads.size());
         std::vector<bool> done(grads.size());
@@ -840,6 +669,12 @@ TORCH_LIBRARY_FRAGMENT(beamgrad, m) {
     m.def(
         "keep_tokens(Tensor(a!)[] pools, Tensor pages, Tensor lengths, Tensor refs, Tensor drafted, Tensor keep, Tensor kept) -> "
         "(Tensor, Tensor, Tensor)");
+    m.def(
+        "accumulate_weights(Tensor(a!) weights, Tensor q, Tensor k, Tensor lse, Tensor pages, Tensor lengths, Tensor? parents, "
+        "Tensor? counts, float scale) -> ()");
+    m.def(
+        "evict_tokens(Tensor(a!)[] pools, Tensor[] weights, Tensor pages, Tensor lengths, Tensor refs, Tensor? budgets, int budget, "
+        "int recent, int first) -> (Tensor, Tensor, Tensor, Tensor[])");
     m.def("reorder_states(Tensor[] states, Tensor parents) -> Tensor[]");
     m.def("reorder_states_(Tensor(a!)[] states, Tensor parents) -> ()");
     m.def("reorder_states_backward(Tensor[] grads, Tensor parents) -> Tensor[]");
@@ -853,6 +688,8 @@ TORCH_LIBRARY_IMPL(beamgrad, CUDA, m) {
     m.impl("extend_pages", &extend_pages_hip);
     m.impl("write_tokens", &write_tokens_hip);
     m.impl("keep_tokens", &keep_tokens_hip);
+    m.impl("accumulate_weights", &accumulate_weights_hip);
+    m.impl("evict_tokens", &evict_tokens_hip);
     m.impl("reorder_states", &reorder_states_hip);
     m.impl("reorder_states_", &reorder_states_inplace_hip);
     m.impl("reorder_states_backward", &reorder_states_backward_hip);
@@ -861,7 +698,7 @@ TORCH_LIBRARY_IMPL(beamgrad, CUDA, m) {
 TORCH_LIBRARY_IMPL(beamgrad, Autograd, m) {
     m.impl("reorder_states", &reorder_states_autograd);
     m.impl("reorder_states_backward", &reorder_states_backward_autograd);
-    for (const char* name : {"tree_attention", "fork_pages", "write_tokens", "keep_tokens", "reorder_states_"})
+    for (const char* name : {"tree_attention", "fork_pages", "write_tokens", "keep_tokens", "accumulate_weights", "evict_tokens", "reorder_states_"})
         m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }
 
@@ -872,6 +709,8 @@ TORCH_LIBRARY_IMPL(beamgrad, CPU, m) {
     m.impl("extend_pages", &extend_pages_cpu);
     m.impl("write_tokens", &write_tokens_cpu);
     m.impl("keep_tokens", &keep_tokens_cpu);
+    m.impl("accumulate_weights", &accumulate_weights_cpu);
+    m.impl("evict_tokens", &evict_tokens_cpu);
     m.impl("reorder_states", &reorder_states_cpu);
     m.impl("reorder_states_", &reorder_states_inplace_cpu);
     m.impl("reorder_states_backward", &reorder_states_backward_cpu);

@@ -1,8 +1,8 @@
 /* SPDX-License-Identifier: MIT
  *
  * The state of a model in a beam search, on the GPU: attention over a paged
- * cache of keys and values, the pages of that cache, and the reordering of
- * dense states. Additions of libdbs_hip.so beside the search itself
+ * cache of keys and values, the pages of that cache, the eviction of tokens by the
+ * attention that they get, rotary positions, and the reordering of dense states. Additions of libdbs_hip.so beside the search itself
  * (dbs_cuda.h, dbs_hip.h); the reference has no counterpart.
  *
  * Every pointer is device memory unless said otherwise, every call is
@@ -168,6 +168,120 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states(const void* const* from, void* const
 DBS_CUDA_EXPORT int beamgrad_reorder_states_backward(const void* const* from, void* const* to, const int64_t* elements,
                                                      int n, int data_type, const void* parents, int parents_i64,
                                                      int examples, int beams, void* stream);
+
+/* Rotary positions: of every head of n tensors [sequences, tokens, heads[i],
+ * head_dim[i]] the first 2 * pairs values turn in pairs, by the angles position *
+ * frequency[f] of pair f,
+ *   (a, b) -> scale * (a cos - b sin, a sin + b cos),
+ * values 2 f and 2 f + 1 with `interleaved`, f and pairs + f without; with `inverse`
+ * by the angles' negatives, which is the gradient. The rest of a head is copied. Tokens
+ * n >= counts[s] (counts may be NULL) become zeros, or stay as they are in place. Angles
+ * are computed in 64 bits, at positions of any sign.
+ *
+ * from, to, heads, head_dim and the strides are host arrays, read before the call
+ * returns; strides are of sequences, tokens and heads (three for each tensor), in
+ * elements, and a head is contiguous. from[i] == to[i] for every i (with equal strides)
+ * turns in place; otherwise no memory that is written may meet what is read. What
+ * is written lies apart: a token's heads in one run, or the tokens of all sequences
+ * in equal steps. head_dim is at most 1024, sequences * tokens fewer than 2^26, strides at
+ * most 2^40. */
+typedef struct BeamgradRotary {
+    const void* const* from;
+    void* const* to;
+    const int32_t* heads;
+    const int32_t* head_dim;
+    const int64_t* from_strides;
+    const int64_t* to_strides;
+    int32_t n;
+    int32_t data_type;
+    int32_t sequences;
+    int32_t tokens;
+    int32_t pairs;
+    int32_t interleaved;
+    int32_t inverse;
+    float scale;
+    const void* positions; /* int32, or int64 with positions_i64 */
+    int64_t position_strides[2]; /* sequence, token, in elements */
+    int32_t positions_i64;
+    int32_t reserved; /* 0 */
+    const double* frequencies; /* [pairs] */
+    const int32_t* counts;
+} BeamgradRotary;
+
+DBS_CUDA_EXPORT int beamgrad_rotary(const BeamgradRotary* args, void* stream);
+
+/* The attention that cached tokens get, of the last tokens of S sequences as
+ * beamgrad_tree_attention has them (the fields alike): with p_ihj the weight that
+ * asking token i gives token j in head h, exp(scale * q . k_j - lse[s, i, h]) where it
+ * sees it, and the heads h of the cache's head g,
+ *   weights[s, g, j] += sum_i sum_h p_ihj   for the tokens ahead of the asking ones,
+ *   weights[s, g, j]  = sum_i sum_h p_ihj   for the asking ones,
+ * summed in 32 bits and in an order that does not change from run to run. Tokens
+ * without a page, and places past a sequence's length, keep what they have. A row whose
+ * lse is -inf gives nothing. lse [S, N, H] is what beamgrad_tree_attention leaves,
+ * contiguous; weights [S, Hkv, ...] has weight_strides (elements) and room for
+ * table_pages * page_tokens places, contiguous. */
+typedef struct BeamgradWeights {
+    const void* q;
+    const void* k;
+    int32_t data_type;
+    int32_t sequences; /* S */
+    int32_t tokens;    /* N */
+    int32_t heads;     /* H */
+    int32_t kv_heads;  /* Hkv */
+    int32_t head_dim;  /* D */
+    int32_t page_tokens;
+    int32_t n_pages;
+    int32_t table_pages; /* P */
+    float scale;         /* positive, finite times log2(e) */
+    int64_t q_strides[3]; /* sequence, token, head */
+    int64_t k_strides[3]; /* page, token, head */
+    int64_t weight_strides[2]; /* sequence, head */
+    const int32_t* pages; /* [S, P], contiguous */
+    const int32_t* lengths;
+    const int32_t* counts;  /* or NULL */
+    const int32_t* parents; /* or NULL */
+    const float* lse;
+    float* weights;
+} BeamgradWeights;
+
+DBS_CUDA_EXPORT int64_t beamgrad_accumulate_weights_workspace_size(const BeamgradWeights* args);
+DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, void* workspace, int64_t workspace_bytes,
+                                                void* stream);
+
+/* A cache cut to its heaviest tokens. Of a sequence of more than b tokens (b =
+ * budgets[s], or `budget` where that is NULL) the last r = min(recent, b) stay, the
+ * first f = min(first, b - r), and of those between the b - r - f with the largest
+ * weights, of equal ones the earlier; NaN counts as less than every number. They move
+ * together in their order, in place in every pool, and the pages that hold no token
+ * any more are given back. n_weights sets of weights, one for each pools.n / n_weights
+ * pools in turn: weights[i] [sequences, heads, table_pages * page_tokens] float32 with
+ * weight_strides[2 i], [2 i + 1] (elements, host arrays) chooses for every head by itself,
+ * a pool's row being `heads` parts of equal length. to_weights[i], contiguous, gets the
+ * weights of the tokens that stay, zeros behind them.
+ *
+ * A sequence of at most b tokens stays as it is, as does one that has no page for one of
+ * its tokens, or that would write to a page that others hold too (refs != 1): its
+ * places are copied, weights too. b < 0 counts as 0. At most 65535 sequences, 1024 heads,
+ * rows of 2 MB. */
+typedef struct BeamgradEviction {
+    const float* const* weights;
+    const int64_t* weight_strides;
+    float* const* to_weights;
+    int32_t n_weights;
+    int32_t heads;
+    const int32_t* budgets; /* device, [sequences], or NULL */
+    int32_t budget;
+    int32_t recent;
+    int32_t first;
+    int32_t reserved; /* 0 */
+} BeamgradEviction;
+
+DBS_CUDA_EXPORT int64_t beamgrad_evict_tokens_workspace_size(const BeamgradPools* pools, const BeamgradEviction* args,
+                                                             int sequences, int table_pages);
+DBS_CUDA_EXPORT int beamgrad_evict_tokens(const BeamgradPools* pools, const BeamgradEviction* args,
+                                          const BeamgradTable* from, int sequences, int table_pages,
+                                          const BeamgradTable* to, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

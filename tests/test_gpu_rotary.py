@@ -1,0 +1,205 @@
+# SPDX-License-Identifier: MIT
+"""Rotary positions on the GPU against a 64-bit restatement."""
+
+import math
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import beamgrad_amd as bg
+from tests import model_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def draw(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def positions_of(S, N, seed, far=5000):
+    return torch.randint(-3, far, (S, N), generator=torch.Generator().manual_seed(seed))
+
+
+def frequencies(width):
+    return 10000.0 ** (-2.0 * torch.arange(width // 2, dtype=torch.float64) / width)
+
+
+def near(got, want):
+    out, bound = want
+    far = (got.detach().cpu().double() - out).abs() - bound
+    assert got.shape == out.shape and far.max() <= 0, float(far.max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("S, N, H, Hkv, D, width", [(1, 1, 1, 1, 2, 2), (3, 5, 4, 2, 64, 64), (2, 7, 6, 3, 80, 48), (2, 3, 5, 5, 33, 22),
+                                                   (4, 1100, 3, 1, 40, 40), (2, 9, 2, 2, 256, 100), (1, 4, 2, 1, 1024, 1024), (2, 3, 2, 1, 71, 6)])
+def test_layouts(dtype, interleaved, S, N, H, Hkv, D, width):
+    """Both layouts, parts of heads, odd widths; new, in place, and the gradient."""
+    q, k = draw(0, S, N, H, D, dtype=dtype), draw(1, S, N, Hkv, D, dtype=dtype)
+    at, f = positions_of(S, N, 2), frequencies(width)
+    want = [ref.rotary(x, at, f, interleaved, 1.0) for x in (q, k)]
+    leaves = [x.cuda().requires_grad_(True) for x in (q, k)]
+    out = bg.rotary(leaves, at.cuda(), f.cuda(), interleaved=interleaved)
+    for got, w in zip(out, want, strict=True):
+        near(got, w)
+    up = [draw(5, *x.shape, dtype=dtype) for x in (q, k)]
+    for got, g in zip(torch.autograd.grad(out, leaves, [g.cuda() for g in up]), up, strict=True):
+        near(got, ref.rotary(g, at, f, interleaved, 1.0, inverse=True))
+    inplace = [q.cuda(), k.cuda()]
+    same = bg.rotary(inplace, at.cuda(), f.cuda(), interleaved=interleaved, inplace=True)
+    assert same[0] is inplace[0]
+    for a, b in zip(inplace, out, strict=True):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("far", [1, 1000, 131072, 10**6, 2**31 - 1, 2**40])
+@pytest.mark.parametrize("base", [100.0, 500000.0])
+def test_far_positions(far, base):
+    """An angle is a product of 64 bits and its remainder: sines keep 32 bits however far.
+    (The restatement's own product has 53 bits: its angle is off by 2^-54 of itself.)"""
+    f = base ** (-torch.arange(32, dtype=torch.float64) / 32)
+    at = torch.tensor([[far, -far, far - 1, far // 2, far // 3, 0]])
+    x = draw(0, 1, 6, 1, 64)
+    out, bound = ref.rotary(x, at, f, False, 1.0)
+    bound = bound + far * 2.0**-53 * 8
+    for index in (at, at.int()) if far < 2**31 else (at,):
+        got, = bg.rotary([x.cuda()], index.cuda(), f.cuda())
+        assert ((got.cpu().double() - out).abs() <= bound).all()
+
+
+def test_scale_counts_and_index_types():
+    x, at, f = draw(0, 3, 6, 2, 32), positions_of(3, 6, 1), frequencies(24)
+    counts = torch.tensor([0, 4, 9])
+    poisoned = x.clone()
+    poisoned[0] = math.nan
+    poisoned[1, 4:] = math.inf
+    want = ref.rotary(x, at, f, False, 1.25, counts)
+    for index in (at, at.int()):
+        for n in (counts, counts.int()):
+            leaf = poisoned.cuda().requires_grad_(True)
+            got, = bg.rotary([leaf], index.cuda(), f.cuda(), counts=n.cuda(), scale=1.25)
+            near(got, want)
+            g = draw(3, 3, 6, 2, 32)
+            grad, = torch.autograd.grad(got, leaf, g.cuda())
+            near(grad, ref.rotary(g, at, f, False, 1.25, counts, inverse=True))
+    own = poisoned.cuda()
+    bg.rotary([own], at.cuda(), f.cuda(), counts=counts.cuda(), scale=1.25, inplace=True)
+    near(own[1:2, :4], (want[0][1:2, :4], want[1][1:2, :4]))
+    assert own[0].isnan().all() and (own[1, 4:] == math.inf).all()
+    near(own[2:], (want[0][2:], want[1][2:]))
+    # float32 frequencies are widened
+    a, = bg.rotary([x.cuda()], at.cuda(), f.float().cuda())
+    b, = bg.rotary([x.cuda()], at.cuda(), f.float().double().cuda())
+    assert torch.equal(a, b)
+
+
+def test_strides_and_views():
+    """Parts of one projection, in place and new; transposed heads; expanded positions;
+    the end of a head; misaligned rows."""
+    S, N, H, D = 2, 5, 3, 32
+    f = frequencies(D)
+    at = positions_of(S, N, 0)
+    packed = draw(1, S, N, (H + 2) * D + 3).cuda()
+    q, k = packed[..., :H * D].unflatten(-1, (H, D)), packed[..., H * D + 1:(H + 1) * D + 1].unflatten(-1, (1, D))
+    want = [ref.rotary(t.cpu(), at, f, True, 1.0) for t in (q, k)]
+    rest = packed[..., (H + 1) * D + 1:].clone()
+    for got, w in zip(bg.rotary([q, k], at.cuda(), f.cuda(), interleaved=True), want, strict=True):
+        near(got, w)
+    bg.rotary([q, k], at.cuda(), f.cuda(), interleaved=True, inplace=True)
+    for got, w in zip((q, k), want, strict=True):
+        near(got, w)
+    assert torch.equal(packed[..., (H + 1) * D + 1:], rest)
+    heads_first = draw(2, S, H, N, D).cuda().transpose(1, 2)
+    near(bg.rotary([heads_first], at.cuda(), f.cuda())[0], ref.rotary(heads_first.cpu(), at, f, False, 1.0))
+    columns = draw(3, S, N, D, H).cuda().transpose(2, 3)
+    near(bg.rotary([columns], at.cuda(), f.cuda())[0], ref.rotary(columns.cpu(), at, f, False, 1.0))
+    line = torch.arange(N)
+    near(bg.rotary([heads_first], line.cuda().expand(S, N), f.cuda())[0], ref.rotary(heads_first.cpu(), line.expand(S, N), f, False, 1.0))
+    near(bg.rotary([heads_first], at.T.contiguous().cuda().T, f.cuda())[0], ref.rotary(heads_first.cpu(), at, f, False, 1.0))
+    whole = draw(4, S, N, H, 48).cuda()
+    before = whole.clone()
+    bg.rotary([whole[..., 16:]], at.cuda(), f.cuda(), inplace=True)
+    near(whole[..., 16:], ref.rotary(before[..., 16:].cpu(), at, f, False, 1.0))
+    assert torch.equal(whole[..., :16], before[..., :16])
+    one_token = draw(5, S, 1, H, D).cuda()
+    near(bg.rotary([one_token.transpose(1, 2).contiguous().transpose(1, 2)], at[:, :1].cuda(), f.cuda())[0], ref.rotary(one_token.cpu(), at[:, :1], f, False, 1.0))
+
+
+def test_many_tensors_of_one_call():
+    """More than one launch holds."""
+    at, f = positions_of(2, 3, 0), frequencies(8)
+    xs = [draw(i, 2, 3, 1 + i % 3, 8 + i) for i in range(19)]
+    for got, x in zip(bg.rotary([x.cuda() for x in xs], at.cuda(), f.cuda()), xs, strict=True):
+        near(got, ref.rotary(x, at, f, False, 1.0))
+    assert bg.rotary([], at.cuda(), f.cuda()) == []
+
+
+def test_memory_that_meets_is_refused():
+    at, f = positions_of(2, 3, 0).cuda(), frequencies(8).cuda()
+    x = torch.zeros(2, 3, 4, 8, device="cuda")
+    for tensors in ([x, x], [x, x[:, :, 1:]], [x[:, :1].expand(2, 3, 4, 8)]):
+        with pytest.raises(ValueError, match="share no memory"):
+            bg.rotary(tensors, at, f, inplace=True)
+
+
+def test_all_derivatives():
+    """Second derivatives, tangents, vmap and one traced step."""
+    at, f = positions_of(2, 3, 0), frequencies(8)
+    x, t, w = (draw(i, 2, 3, 2, 10) for i in range(3))
+    leaf, up = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    out, = bg.rotary([leaf], at.cuda(), f.cuda(), scale=2.0)
+    grad, = torch.autograd.grad(out, leaf, up, create_graph=True)
+    second, = torch.autograd.grad(grad, up, t.cuda())
+    near(second, ref.rotary(t, at, f, False, 2.0))
+    with forward_ad.dual_level():
+        dual = bg.rotary([forward_ad.make_dual(x.cuda(), t.cuda())], at.cuda(), f.cuda())[0]
+        primal, tangent = forward_ad.unpack_dual(dual)
+        near(primal, ref.rotary(x, at, f, False, 1.0))
+        near(tangent, ref.rotary(t, at, f, False, 1.0))
+    many = draw(7, 4, 2, 3, 2, 10).cuda()
+    got = torch.vmap(lambda a: bg.rotary([a], at.cuda(), f.cuda())[0])(many)
+    assert torch.equal(got, torch.stack([bg.rotary([m], at.cuda(), f.cuda())[0] for m in many]))
+    got = torch.vmap(lambda p: bg.rotary([many[0]], p, f.cuda())[0])(torch.stack([at, at + 5]).cuda())
+    assert torch.equal(got[1], bg.rotary([many[0]], at.cuda() + 5, f.cuda())[0])
+
+
+def test_captured_and_on_another_stream():
+    at, f = positions_of(2, 3, 0).cuda(), frequencies(8).cuda()
+    x = draw(0, 2, 3, 2, 10).cuda().requires_grad_(True)
+    g = draw(1, 2, 3, 2, 10).cuda()
+
+    def step():
+        out, = bg.rotary([x], at, f)
+        return out, *torch.autograd.grad(out, x, g)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(draw(seed, 2, 3, 2, 10))
+        at.copy_(positions_of(2, 3, seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step(), strict=True):
+            assert torch.equal(a, b)
+
+
+def test_rotated_products_depend_on_distance_alone():
+    """The property that positions are for: q at i, k at j meet as q at i + c, k at j + c do."""
+    q, k = draw(0, 1, 4, 1, 64), draw(1, 1, 4, 1, 64)
+    f = bg.rotary_frequencies(64, factor=8.0, context=4096)
+    near_by, far = (torch.arange(4)[None] + c for c in (0, 100000))
+    score = [(torch.cat(bg.rotary([q.cuda()], p.cuda(), f)).double() * torch.cat(bg.rotary([k.cuda()], p.flip(1).cuda(), f)).double()).sum(-1).cpu()
+             for p in (near_by, far)]
+    size = (q.abs() * k.abs()).sum(-1).double() * 2 + (q.norm(dim=-1) * k.norm(dim=-1)).double()
+    assert ((score[0] - score[1]).abs() <= 24 * ref.STEP * size).all()
