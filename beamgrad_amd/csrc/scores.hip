@@ -11,9 +11,9 @@
 // t / s.
 //
 // The alternatives come out of the same pass: every thread's m is the maximum of
-// its share of the row, so the top-th largest of the threads' maxima is reached
-// by at least `top` values, and what reaches it lies with the threads whose own
-// maximum does: about `top` threads, whose shares (a few hundred values of a large
+// its share of the row, so the least of the `top` largest of the threads' maxima (as
+// many from each wavefront) is reached by at least `top` values, and what reaches it
+// lies with the threads whose own maximum does: little more than `top` threads, whose shares (a few hundred values of a large
 // vocabulary) are read again, from the cache. What they hold beside the alternatives
 // is little (20 of 151936 at random: one or two), unless values are equal
 // in great number: where more than kKept reach it, or fewer than `top` do (-inf),
@@ -38,6 +38,7 @@ constexpr int kAtOnce = 4;     // 16-byte reads of a thread in flight
 constexpr int kMaxTop = 64;
 constexpr int kKept = 512;     // values beside the alternatives that a workgroup ranks
 constexpr int kMaxParts = 64;  // of a row
+constexpr int64_t kCacheBytes = int64_t{200} << 20;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kFar = -1000.0f;  // e^kFar is 0 in 32 bits
 
@@ -71,13 +72,6 @@ struct Sums {
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m);
-    const float da = a.m - m, db = b.m - m, wa = exp_of(da), wb = exp_of(db);
-    return {m, __builtin_fmaf(a.s, wa, b.s * wb),
-            __builtin_fmaf(wa, __builtin_fmaf(a.s, fmaxf(da, kFar), a.t), wb * __builtin_fmaf(b.s, fmaxf(db, kFar), b.t)), 0.0f};
-}
-
 // A value and its place as one number: the larger value, of equal ones the
 // lower place, is larger. 0 is below all of them (NaN does not come here).
 __device__ __forceinline__ uint64_t key_of(float x, int place) {
@@ -93,6 +87,22 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 
 template <class T>
 constexpr int kEach = 16 / sizeof(T);
+
+// 16 bytes of a row, or of its gradient. STREAM: past the caches, where the call's rows
+// would not stay in them.
+template <bool STREAM>
+__device__ __forceinline__ u32x4 read16(const char* from) {
+    const u32x4_any* const at = reinterpret_cast<const u32x4_any*>(from);
+    return STREAM ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool STREAM>
+__device__ __forceinline__ void write16(char* to, u32x4 x) {
+    u32x4_any* const at = reinterpret_cast<u32x4_any*>(to);
+    if (STREAM)
+        __builtin_nontemporal_store(x, at);
+    else
+        *at = x;
+}
 
 // The 16 bytes at place v of a row's end `V`: what lies past it is -inf.
 template <class T>
@@ -110,7 +120,7 @@ __device__ __forceinline__ void take(Sums& a, const float* x, int n) {
 #pragma unroll
     for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
     const float d0 = a.m - m, w = exp_of(d0);
-    a.t = ENTROPY ? w * __builtin_fmaf(a.s, fmaxf(d0, kFar), a.t) : 0.0f;
+    if (ENTROPY) a.t = w * __builtin_fmaf(a.s, fmaxf(d0, kFar), a.t);
     a.s *= w;
     a.m = m;
 #pragma unroll
@@ -122,7 +132,7 @@ __device__ __forceinline__ void take(Sums& a, const float* x, int n) {
 }
 
 // A thread's share of [from, to) of a row: 16 bytes of every THREADS * 16.
-template <class T, bool ENTROPY, int THREADS>
+template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __device__ __forceinline__ Sums sums_of(const char* row, int from, int to) {
     constexpr int E = kEach<T>;
     Sums a{-FLT_MAX, 0.0f, 0.0f, 0.0f};
@@ -132,7 +142,7 @@ __device__ __forceinline__ Sums sums_of(const char* row, int from, int to) {
     for (; v + (kAtOnce - 1) * step + E <= to; v += kAtOnce * step) {
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const u32x4 raw = *reinterpret_cast<const u32x4_any*>(row + (v + i * step) * sizeof(T));
+            const u32x4 raw = read16<STREAM>(row + (v + i * step) * sizeof(T));
             T e[E];
             __builtin_memcpy(e, &raw, 16);
 #pragma unroll
@@ -147,31 +157,79 @@ __device__ __forceinline__ Sums sums_of(const char* row, int from, int to) {
     return a;
 }
 
-template <int THREADS>
+// Over a wavefront, of all lanes at once: lane i takes lane i - 1's, - 2's, - 4's and -
+// 8's within its 16, then the last of each 16's; lane 63 has all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float x, float none) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+template <class Op>
+__device__ __forceinline__ float over_wave(float x, float none, Op op) {
+    x = op(x, moved<0x111, 0xf>(x, none));
+    x = op(x, moved<0x112, 0xf>(x, none));
+    x = op(x, moved<0x114, 0xf>(x, none));
+    x = op(x, moved<0x118, 0xf>(x, none));
+    x = op(x, moved<0x142, 0xa>(x, none));
+    x = op(x, moved<0x143, 0xc>(x, none));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ float wave_max(float x) {
+    return over_wave(x, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return over_wave(x, 0.0f, [](float a, float b) { return a + b; });
+}
+
+// To a maximum that is not lower.
+__device__ __forceinline__ void raise(Sums& a, float m) {
+    const float d = a.m - m, w = exp_of(d);
+    a.t = w * __builtin_fmaf(a.s, fmaxf(d, kFar), a.t);
+    a.s *= w;
+    a.m = m;
+}
+__device__ __forceinline__ Sums joined_wave(Sums a) {
+    raise(a, wave_max(a.m));
+    return {a.m, wave_sum(a.s), wave_sum(a.t), 0.0f};
+}
+
+constexpr int kDumped = 64;  // threads whose values fit LDS
+
+template <int THREADS, int VALUES = 1>
 struct Shared {
     Sums waves[THREADS / 64];
-    float top[THREADS];          // the threads' maxima
     int flagged[THREADS], flags, kept;
-    float floor;                 // what reaches it may be an alternative
-    uint64_t keys[kKept];
+    float floor[THREADS / 64];   // what reaches the least of them may be an alternative
+    uint64_t keys[kKept + 8];
     uint64_t best[THREADS / 64];
+    float dump[VALUES > 1 ? kDumped * (VALUES + 1) : 1];
 };
 
-template <int THREADS>
-__device__ __forceinline__ Sums joined_block(Sums a, Shared<THREADS>& lds) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
-        a = joined(a, {__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.0f});
+template <int THREADS, int VALUES>
+__device__ __forceinline__ Sums joined_block(Sums a, Shared<THREADS, VALUES>& lds) {
+    constexpr int WAVES = THREADS / 64;
+    a = joined_wave(a);
+    if (WAVES == 1) return a;
     if ((threadIdx.x & 63) == 0) lds.waves[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = lds.waves[0];
+    Sums of[WAVES];
+    float m = -FLT_MAX;
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) a = joined(a, lds.waves[w]);
+    for (int w = 0; w < WAVES; ++w) {
+        of[w] = lds.waves[w];
+        m = fmaxf(m, of[w].m);
+    }
+    a = {m, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        raise(of[w], m);
+        a.s += of[w].s;
+        a.t += of[w].t;
+    }
     return a;
 }
 
-template <int THREADS>
-__device__ __forceinline__ uint64_t largest_in_block(uint64_t key, Shared<THREADS>& lds) {
+template <int THREADS, int VALUES>
+__device__ __forceinline__ uint64_t largest_in_block(uint64_t key, Shared<THREADS, VALUES>& lds) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
         const uint32_t lo = __shfl_xor(static_cast<uint32_t>(key), d), hi = __shfl_xor(static_cast<uint32_t>(key >> 32), d);
@@ -186,48 +244,96 @@ __device__ __forceinline__ uint64_t largest_in_block(uint64_t key, Shared<THREAD
     return key;
 }
 
-// The `top` largest keys of [from, to), given the thread's maximum, in order to
-// each(rank, key). Fewer than `top` values: key 0 for the rest.
-template <class T, int THREADS, class Each>
-__device__ __forceinline__ void alternatives(const char* row, int from, int to, int top, float mine, Shared<THREADS>& lds, Each each) {
-    constexpr int E = kEach<T>;
-    const int tid = threadIdx.x;
-    if (tid == 0) lds.flags = lds.kept = 0;
-    lds.top[tid] = mine;
-    __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < THREADS; ++j) rank += lds.top[j] > mine || (lds.top[j] == mine && j < tid);
-    if (rank == top - 1) lds.floor = mine;
-    __syncthreads();
-    const float floor = lds.floor;
-    if (mine >= floor) lds.flagged[atomicAdd(&lds.flags, 1)] = tid;
-    __syncthreads();
-    const int shares = (to - from + THREADS * E - 1) / (THREADS * E), items = lds.flags * shares;
-    for (int i = tid; i < items; i += THREADS) {
-        const int v = from + ((i % shares) * THREADS + lds.flagged[i / shares]) * E;
-        if (v >= to) continue;
-        float x[E];
-        values_at<T>(row, v, to, x);
+// How many of n keys are larger; 8 at once, zeros behind them.
+__device__ __forceinline__ int larger_of(const uint64_t* keys, int n, uint64_t key) {
+    int above = 0;
+    for (int j = 0; j < n; j += 8) {
+        uint64_t other[8];
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (v + j < to && x[j] >= floor) {
-                const int at = atomicAdd(&lds.kept, 1);
-                if (at < kKept) lds.keys[at] = key_of(x[j], v + j);
-            }
+        for (int k = 0; k < 8; ++k) other[k] = keys[j + k];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) above += other[k] > key;
+    }
+    return above;
+}
+
+// The `top` largest keys of [from, to), given the thread's maximum, in order to
+// each(rank, key). `values`: what the thread read of it, where that is all of its share:
+// those of few threads go through LDS, for all threads to look through.
+// Fewer than `top` values: key 0 for the rest.
+template <class T, int THREADS, int VALUES, class Each>
+__device__ __forceinline__ void alternatives(const char* row, int from, int to, int top, float mine, const float (&values)[VALUES],
+                                             Shared<THREADS, VALUES>& lds, Each each) {
+    constexpr int E = kEach<T>, WAVES = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (tid == 0) lds.flags = lds.kept = 0;
+    // of each wavefront's maxima as many as make `top` together: the lowest of these
+    const int wanted = (top + WAVES - 1) / WAVES;
+    if (wanted <= 16) {
+        float left = mine, largest = wave_max(mine);
+        for (int n = __popcll(__ballot(left == largest)); n < wanted; n += __popcll(__ballot(left == largest))) {
+            left = left == largest ? -__builtin_inff() : left;
+            largest = wave_max(left);
+        }
+        if (lane == 0) lds.floor[tid >> 6] = largest;
+    } else {
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+            const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), j));
+            rank += other > mine || (other == mine && j < lane);
+        }
+        if (rank == wanted - 1) lds.floor[tid >> 6] = mine;
     }
     __syncthreads();
-    const int n = lds.kept, values = min(top, to - from);
-    if (n >= values && n <= kKept) {
+    float floor = lds.floor[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) floor = fminf(floor, lds.floor[w]);
+    const auto keep = [&](float x, int place) {
+        if (place >= to || !(x >= floor)) return;
+        const int at = atomicAdd(&lds.kept, 1);
+        if (at < kKept) lds.keys[at] = key_of(x, place);
+    };
+    if (mine >= floor) {
+        const int slot = atomicAdd(&lds.flags, 1);
+        lds.flagged[slot] = tid;
+        if constexpr (VALUES > 1)
+            if (slot < kDumped)
+#pragma unroll
+                for (int i = 0; i < VALUES; ++i) lds.dump[slot * (VALUES + 1) + i] = values[i];
+    }
+    __syncthreads();
+    const int flags = lds.flags;
+    if (VALUES > 1 && flags <= kDumped) {
+        for (int i = tid; i < flags * VALUES; i += THREADS) {
+            const int of = i / VALUES, v = i - of * VALUES;
+            keep(lds.dump[of * (VALUES + 1) + v], from + ((v / E) * THREADS + lds.flagged[of]) * E + v % E);
+        }
+    } else {
+        const int shares = (to - from + THREADS * E - 1) / (THREADS * E), items = flags * shares;
+        for (int i = tid; i < items; i += THREADS) {
+            const int v = from + ((i % shares) * THREADS + lds.flagged[i / shares]) * E;
+            if (v >= to) continue;
+            float x[E];
+            values_at<T>(row, v, to, x);
+#pragma unroll
+            for (int j = 0; j < E; ++j) keep(x[j], v + j);
+        }
+    }
+    __syncthreads();
+    const int n = lds.kept, all = min(top, to - from);
+    if (n >= all && n <= kKept) {
+        if (tid < 8) lds.keys[n + tid] = 0;
+        __syncthreads();
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t key = lds.keys[i];
-            int above = 0;
-            for (int j = 0; j < n; ++j) above += lds.keys[j] > key;
+            const int above = larger_of(lds.keys, n, key);
             if (above < top) each(above, key);
         }
     } else {
         // one after the other: the largest below the last one
         uint64_t below = ~uint64_t{0};
-        for (int k = 0; k < values; ++k) {
+        for (int k = 0; k < all; ++k) {
             uint64_t best = 0;
             for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
                 float x[E];
@@ -242,7 +348,7 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
             if (tid == 0) each(k, below);
         }
     }
-    for (int k = values + tid; k < top; k += THREADS) each(k, uint64_t{0});
+    for (int k = all + tid; k < top; k += THREADS) each(k, uint64_t{0});
 }
 
 struct Normal {
@@ -262,10 +368,9 @@ __device__ __forceinline__ float value_at(const char* row, int v) {
     return static_cast<float>(reinterpret_cast<const T*>(row)[v]);
 }
 
-// What one thread writes of a row.
-template <class T>
-__device__ __forceinline__ void write_row(const Rows& p, uint32_t r, const char* row, int token, const Normal& n) {
-    p.logprobs[r] = n.logp(value_at<T>(row, token));
+// What one thread writes of a row, whose token's logit is x.
+__device__ __forceinline__ void write_row(const Rows& p, uint32_t r, float x, const Normal& n) {
+    p.logprobs[r] = n.logp(x);
     if (p.entropy) p.entropy[r] = n.entropy;
     if (p.stats) p.stats[r] = float4{n.m, n.empty ? __builtin_inff() : n.log_s, n.entropy, 0.0f};
 }
@@ -292,36 +397,66 @@ __device__ __forceinline__ void write_none(const Rows& p, uint32_t r, bool bad) 
 }
 
 // A workgroup for a row.
-template <class T, bool ENTROPY, int THREADS>
+template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
     __shared__ Shared<THREADS> lds;
     const uint32_t r = blockIdx.x;
     const int token = p.token(r);
     if (token < 0) return write_none<THREADS>(p, r, false);
     const char* const row = p.row(r);
-    const Sums mine = sums_of<T, ENTROPY, THREADS>(row, 0, p.V);
+    const float x = value_at<T>(row, token);
+    const Sums mine = sums_of<T, ENTROPY, THREADS, STREAM>(row, 0, p.V);
     const Sums all = joined_block(mine, lds);
     if (!(all.s <= FLT_MAX)) return write_none<THREADS>(p, r, true);
     const Normal n = normal_of(all);
-    if (threadIdx.x == 0) write_row<T>(p, r, row, token, n);
+    if (threadIdx.x == 0) write_row(p, r, x, n);
     if (p.top > 0)
-        alternatives<T>(row, 0, p.V, p.top, mine.m, lds, [&](int rank, uint64_t key) { write_alternative(p, r, rank, key, n); });
+        alternatives<T>(row, 0, p.V, p.top, mine.m, {0.0f}, lds, [&](int rank, uint64_t key) { write_alternative(p, r, rank, key, n); });
 }
 
 // x: a part of `part` values of row y. Sums and alternatives go to the workspace.
-template <class T, bool ENTROPY>
+// With ONE a part is one round of the workgroup's reads, which stay in registers: they
+// begin while the token is still read, and are looked through for the alternatives.
+template <class T, bool ENTROPY, bool ONE>
 __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int part, Sums* sums, uint64_t* keys) {
-    __shared__ Shared<kThreads> lds;
+    constexpr int E = kEach<T>, VALUES = ONE ? kAtOnce * E : 1;
+    __shared__ Shared<kThreads, VALUES> lds;
     const uint32_t r = blockIdx.y;
-    if (p.token(r) < 0) return;
     const char* const row = p.row(r);
     const int from = blockIdx.x * part, to = min(p.V, from + part);
-    const Sums mine = sums_of<T, ENTROPY, kThreads>(row, from, to);
+    float x[VALUES];
+    Sums mine{-FLT_MAX, 0.0f, 0.0f, 0.0f};
+    if constexpr (ONE) {
+        u32x4 raw[kAtOnce];
+        const int v0 = from + static_cast<int>(threadIdx.x) * E;
+        const char* const at = row + static_cast<int64_t>(v0) * sizeof(T);
+        constexpr int kStep = kThreads * E;
+        if (to - from == VALUES * kThreads) {
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) raw[i] = *reinterpret_cast<const u32x4_any*>(at + i * kStep * sizeof(T));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                raw[i] = v0 + i * kStep < to ? load16(at + i * kStep * sizeof(T), static_cast<int64_t>(to - v0 - i * kStep) * sizeof(T)) : u32x4{0, 0, 0, 0};
+        }
+        if (p.token(r) < 0) return;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            T e[E];
+            __builtin_memcpy(e, &raw[i], 16);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[i * E + j] = v0 + i * kStep + j < to ? static_cast<float>(e[j]) : -__builtin_inff();
+        }
+        take<ENTROPY>(mine, x, VALUES);
+    } else {
+        if (p.token(r) < 0) return;
+        mine = sums_of<T, ENTROPY, kThreads, false>(row, from, to);
+    }
     const Sums all = joined_block(mine, lds);
     const int64_t at = static_cast<int64_t>(r) * gridDim.x + blockIdx.x;
     if (threadIdx.x == 0) sums[at] = all;
     if (p.top > 0 && all.s <= FLT_MAX)
-        alternatives<T>(row, from, to, p.top, mine.m, lds, [&](int rank, uint64_t key) { keys[at * p.top + rank] = key; });
+        alternatives<T>(row, from, to, p.top, mine.m, x, lds, [&](int rank, uint64_t key) { keys[at * p.top + rank] = key; });
 }
 
 // A workgroup joins the parts of a row. The parts' alternatives are in order: of the
@@ -329,43 +464,52 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
 // what lies below it is none.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
-    __shared__ uint64_t kept[kMaxParts * kMaxTop];
-    __shared__ uint64_t lowest[kThreads / 64];
+    constexpr int kFirst = 4;  // keys of a thread that are read ahead
+    __shared__ uint64_t kept[kMaxParts * kMaxTop + 8];
+    __shared__ uint64_t lowest;
     __shared__ int found;
     const uint32_t r = blockIdx.x;
     const int token = p.token(r), tid = threadIdx.x;
-    if (token < 0) return write_none<kThreads>(p, r, false);
     const int64_t first = static_cast<int64_t>(r) * parts;
     Sums all = (tid & 63) < parts ? sums[first + (tid & 63)] : Sums{-FLT_MAX, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
-        all = joined(all, {__shfl_xor(all.m, d), __shfl_xor(all.s, d), __shfl_xor(all.t, d), 0.0f});
-    if (!(all.s <= FLT_MAX)) return write_none<kThreads>(p, r, true);
-    const Normal n = normal_of(all);
-    if (tid == 0) write_row<T>(p, r, p.row(r), token, n);
-    if (p.top == 0) return;
     const uint64_t* const mine = keys + first * p.top;
-    const int j = (p.top + parts - 1) / parts - 1;
-    uint64_t floor = tid < parts ? mine[tid * p.top + j] : ~uint64_t{0};
+    const int n = parts * p.top, j = (p.top + parts - 1) / parts - 1;
+    uint64_t ahead[kFirst];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint32_t lo = __shfl_xor(static_cast<uint32_t>(floor), d), hi = __shfl_xor(static_cast<uint32_t>(floor >> 32), d);
-        const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
-        floor = other < floor ? other : floor;
-    }
+    for (int i = 0; i < kFirst; ++i) ahead[i] = i * kThreads + tid < n ? mine[i * kThreads + tid] : 0;
+    uint64_t floor = p.top > 0 && tid < parts ? mine[tid * p.top + j] : ~uint64_t{0};
+    if (token < 0) return write_none<kThreads>(p, r, false);
+    const float x = value_at<T>(p.row(r), token);
     if (tid == 0) found = 0;
-    if ((tid & 63) == 0) lowest[tid >> 6] = floor;
+    all = joined_wave(all);
+    if (!(all.s <= FLT_MAX)) return write_none<kThreads>(p, r, true);
+    const Normal normal = normal_of(all);
+    if (tid == 0) write_row(p, r, x, normal);
+    if (p.top == 0) return;
+    if (tid < 64) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint32_t lo = __shfl_xor(static_cast<uint32_t>(floor), d), hi = __shfl_xor(static_cast<uint32_t>(floor >> 32), d);
+            const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
+            floor = other < floor ? other : floor;
+        }
+        if (tid == 0) lowest = floor;
+    }
     __syncthreads();
-    floor = lowest[0];
-    for (int i = tid; i < parts * p.top; i += kThreads)
-        if (mine[i] >= floor && mine[i] != 0) kept[atomicAdd(&found, 1)] = mine[i];
+    floor = lowest;
+    const auto take = [&](uint64_t key) {
+        if (key >= floor && key != 0) kept[atomicAdd(&found, 1)] = key;
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) take(ahead[i]);
+    for (int i = kFirst * kThreads + tid; i < n; i += kThreads) take(mine[i]);
     __syncthreads();
     const int m = found;
+    if (tid < 8) kept[m + tid] = 0;
+    __syncthreads();
     for (int i = tid; i < m; i += kThreads) {
-        const uint64_t key = kept[i];
-        int above = 0;
-        for (int k = 0; k < m; ++k) above += kept[k] > key;
-        if (above < p.top) write_alternative(p, r, above, key, n);
+        const int above = larger_of(kept, m, kept[i]);
+        if (above < p.top) write_alternative(p, r, above, kept[i], normal);
     }
 }
 
@@ -384,7 +528,7 @@ struct Grads {
 // from the row's m and log s. The token and the alternatives, whose own gradients
 // come in addition, are written over by a thread for each: with g their sum at v,
 // g (1 - p_v) - p_v (A - g + ...) has no cancellation where p_v is near 1.
-template <class T, bool ENTROPY, int THREADS>
+template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Grads g, const Divider parts, const int part) {
     constexpr int E = kEach<T>;
     __shared__ int places[kMaxTop + 1];
@@ -397,7 +541,12 @@ __global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Gr
     const float m = stats.x, log_s = stats.y, H = stats.z;
     if (token < 0 || log_s == __builtin_inff()) {
         const u32x4 zero = {0, 0, 0, 0};
-        for (int64_t v = from + tid * E; v < to; v += THREADS * E) store16(out + v * sizeof(T), zero, (to - v) * sizeof(T));
+        for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
+            if (v + E <= to)
+                write16<STREAM>(out + v * sizeof(T), zero);
+            else
+                store16(out + v * sizeof(T), zero, (to - v) * sizeof(T));
+        }
         return;
     }
     const char* const row = p.row(r);
@@ -407,8 +556,17 @@ __global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Gr
     for (int k = 0; k < top; ++k) sum += g.top[static_cast<int64_t>(r) * p.top + k];
     const auto rest = [&](float d, float by) { return ENTROPY ? __builtin_fmaf(gH, fmaxf(d, kFar) + H, by) : by; };
     for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
+        const bool whole = v + E <= to;
         float x[E];
-        values_at<T>(row, static_cast<int>(v), to, x);
+        if (whole) {
+            const u32x4 raw = read16<STREAM>(row + v * sizeof(T));
+            T e[E];
+            __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = static_cast<float>(e[i]);
+        } else {
+            values_at<T>(row, static_cast<int>(v), to, x);
+        }
         T y[E];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -417,7 +575,10 @@ __global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Gr
         }
         u32x4 raw;
         __builtin_memcpy(&raw, y, 16);
-        store16(out + v * sizeof(T), raw, (to - v) * sizeof(T));
+        if (whole)
+            write16<STREAM>(out + v * sizeof(T), raw);
+        else
+            store16(out + v * sizeof(T), raw, (to - v) * sizeof(T));
     }
     for (int k = tid; k <= top; k += THREADS) {
         places[k] = k == 0 ? token : static_cast<int>(p.top_tokens[static_cast<int64_t>(r) * p.top + k - 1]);
@@ -472,19 +633,33 @@ int part_values(int vocab, int parts, int size) {
     return static_cast<int>(std::min<int64_t>((each + round - 1) / round * round, 1 << 30));
 }
 
+// Rows that the card's 256 MB of memory-side cache do not hold are read, and their
+// gradient is written, past it: what a pass would leave there is gone before the next
+// one asks for it. Forward and backward of bfloat16 rows of 32000, through the caches
+// and past them, us: 131 MB of logits 68, 78; 192 MB 103, 109; 262 MB 157, 143; 790 MB
+// of 128256: 504, 447.
+bool is_stream(int64_t rows, int vocab, int size) { return rows * vocab * size > kCacheBytes; }
+
+// launch(type, entropy, stream, threads)
 template <class Launch>
-void by_type(int data_type, bool entropy, bool one_wave, Launch launch) {
-    const auto sized = [&](auto t, auto e) {
+void by_type(int data_type, bool entropy, bool stream, bool one_wave, Launch launch) {
+    const auto sized = [&](auto t, auto e, auto s) {
         if (one_wave)
-            launch(t, e, std::integral_constant<int, 64>{});
+            launch(t, e, s, std::integral_constant<int, 64>{});
         else
-            launch(t, e, std::integral_constant<int, kThreads>{});
+            launch(t, e, s, std::integral_constant<int, kThreads>{});
+    };
+    const auto streamed = [&](auto t, auto e) {
+        if (stream)
+            sized(t, e, std::true_type{});
+        else
+            sized(t, e, std::false_type{});
     };
     const auto typed = [&](auto t) {
         if (entropy)
-            sized(t, std::true_type{});
+            streamed(t, std::true_type{});
         else
-            sized(t, std::false_type{});
+            streamed(t, std::false_type{});
     };
     if (data_type == DBS_CUDA_DTYPE_F32)
         typed(float{});
@@ -519,18 +694,22 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs(const BeamgradTokenLogprobs* args, v
     const bool entropy = args->entropy != nullptr;  // its gradient needs it too
     int parts = parts_of(*args);
     const int size = element_size(args->data_type), part = part_values(p.V, parts, size);
-    by_type(args->data_type, entropy, is_short(p.V, size), [&](auto t, auto with_entropy, auto threads) {
+    by_type(args->data_type, entropy, is_stream(rows, p.V, size), is_short(p.V, size), [&](auto t, auto with_entropy, auto streams, auto threads) {
         using T = decltype(t);
         constexpr bool kEntropy = decltype(with_entropy)::value;
         constexpr int kOfRow = decltype(threads)::value;
         if (parts == 1) {
-            score_rows<T, kEntropy, kOfRow><<<static_cast<unsigned>(rows), kOfRow, 0, stream>>>(p);
+            score_rows<T, kEntropy, kOfRow, decltype(streams)::value><<<static_cast<unsigned>(rows), kOfRow, 0, stream>>>(p);
             return;
         }
         parts = (p.V + part - 1) / part;
         Sums* const sums = static_cast<Sums*>(workspace);
         uint64_t* const keys = reinterpret_cast<uint64_t*>(sums + rows * parts);
-        score_parts<T, kEntropy><<<dim3(static_cast<unsigned>(parts), static_cast<unsigned>(rows)), kThreads, 0, stream>>>(p, part, sums, keys);
+        const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(rows));
+        if (part <= kThreads * kAtOnce * kEach<T>)
+            score_parts<T, kEntropy, true><<<grid, kThreads, 0, stream>>>(p, part, sums, keys);
+        else
+            score_parts<T, kEntropy, false><<<grid, kThreads, 0, stream>>>(p, part, sums, keys);
         score_join<T><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(p, parts, sums, keys);
     });
     return finish_call(stream, hipGetLastError());
@@ -551,9 +730,10 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs_backward(const BeamgradTokenLogprobs
     if (rows * parts >= int64_t{1} << 24) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Grads g{grad_logprobs, grad_entropy, grad_top, static_cast<char*>(grad_logits)};
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-    by_type(args->data_type, grad_entropy != nullptr, is_short(p.V, size), [&](auto t, auto with_entropy, auto threads) {
+    by_type(args->data_type, grad_entropy != nullptr, is_stream(rows, p.V, size), is_short(p.V, size),
+            [&](auto t, auto with_entropy, auto streams, auto threads) {
         constexpr int kOfPart = decltype(threads)::value;
-        score_backward<decltype(t), decltype(with_entropy)::value, kOfPart>
+        score_backward<decltype(t), decltype(with_entropy)::value, kOfPart, decltype(streams)::value>
             <<<static_cast<unsigned>(rows * parts), kOfPart, 0, stream>>>(p, g, Divider::of(static_cast<uint32_t>(parts)), part);
     });
     return finish_call(stream, hipGetLastError());
