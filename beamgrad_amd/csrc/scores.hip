@@ -150,9 +150,24 @@ __device__ __forceinline__ Sums sums_of(const char* row, int from, int to) {
         }
         take<ENTROPY>(a, x, kAtOnce * E);
     }
-    for (; v < to; v += step) {
-        values_at<T>(row, static_cast<int>(v), to, x);
-        take<ENTROPY>(a, x, E);
+    if (v < to) {  // the last round
+        u32x4 raw[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (v + i * step + E <= to) raw[i] = read16<STREAM>(row + (v + i * step) * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t at = v + i * step;
+            T e[E];
+            __builtin_memcpy(e, &raw[i], 16);
+            if (at < to && at + E > to) {
+                values_at<T>(row, static_cast<int>(at), to, x + i * E);
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) x[i * E + j] = at < to ? static_cast<float>(e[j]) : -__builtin_inff();
+            }
+        }
+        take<ENTROPY>(a, x, kAtOnce * E);
     }
     return a;
 }

@@ -5,14 +5,21 @@
 //
 // Mathematics. With the log-sums that the attention left, a weight is
 // e^(scale q . k - lse) at once, without a pass for the softmax, and a key's sum needs
-// no other key. So keys are what stays: a wavefront holds its keys in registers as
-// the second operand of Q K^T and lets all rows of queries pass; a lane gets four
-// rows of one key, whose weights it adds up. The four lanes of a key join once, at the
-// end. Rows and their sums are in a fixed order.
+// no other key. Q K^T is made of 16 x 16 blocks; a lane gets four rows of one key, adds
+// their weights up, and a key's four lanes join at the end. Rows and their sums are in
+// a fixed order.
+//
+// Few rows (single tokens, small trees): the queries stay, in registers or LDS, and the
+// keys pass, several blocks of a wavefront on their way: bound by HBM. Many rows (the ends of
+// prompts): the keys stay, in registers, and the queries pass through LDS: bound by the
+// exponentials and what surrounds them. Either way the call's work lies in one line, and each workgroup
+// takes an equal stretch of it, whatever the lengths (they are on the device, so the host
+// cannot plan with them).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attend.hpp"
 #include "beamgrad_state.h"
@@ -27,19 +34,38 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSequences = kThreads;  // of a launch: a thread of each workgroup reads one's length
-constexpr int kChunk = 16;            // blocks of 16 rows whose places a workgroup holds
-constexpr int kMaxSplits = 32;
+constexpr int kNone = INT32_MIN;      // below every token
 constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.44269504088896341f;
+
+// of a lambda: its captures and arrays stay in registers
+#define BEAMGRAD_INLINE __attribute__((always_inline))
 
 template <int DTYPE, int DP>
 struct Dims {
     static constexpr int kSize = DTYPE == DBS_CUDA_DTYPE_F32 ? 4 : 2;
-    static constexpr int kSteps = DP * kSize / 64;  // matrix steps of a block
-    // blocks of 16 keys that a wavefront holds: 64 registers of a lane
-    static constexpr int kBlocks = kSteps >= 16 ? 1 : kSteps >= 8 ? 2 : kSteps >= 6 ? 2 : kSteps >= 4 ? 4 : 8;
-    static constexpr int kKeys = 16 * kBlocks;  // of a wavefront
-    static constexpr int kTile = 4 * kKeys;     // of a workgroup
+    static constexpr int kChunks = DP * kSize / 16;  // 16-byte chunks of a row
+    static constexpr int kRowBytes = kChunks * 16;
+    static constexpr int kSteps = kChunks / 4;  // matrix steps of a block
+    // Rows of queries that lie in LDS at once, 16 KB of them. Chunk c of row r lies at
+    // c ^ (r & kSwizzle): reads of one chunk of 16 rows meet different banks.
+    static constexpr int kRows = kRowBytes >= 768 ? 16 : kRowBytes >= 384 ? 32 : 16384 / kRowBytes;
+    static constexpr int kSwizzle = kChunks % 16 == 0 ? 15 : 7;
+    static constexpr int kLoads = kRows * kChunks / kThreads;  // of a thread, for them
+    // Keys that stay: blocks of 16 of a wavefront, 64 registers of a lane.
+    static constexpr int kBlocks = kSteps >= 16 ? 1 : kSteps >= 6 ? 2 : kSteps >= 4 ? 4 : 8;
+    static constexpr int kKeys = 16 * kBlocks;
+    static constexpr int kTile = 4 * kKeys;  // of a workgroup
+    // Keys that pass: blocks of a wavefront that are on their way.
+    static constexpr int kAhead = kSteps >= 12 ? 1 : kSteps >= 6 ? 2 : kSteps >= 4 ? 3 : 6;
+    static constexpr int kFewResident = kSteps >= 6 ? 3 : 4;  // workgroups of a CU
+};
+constexpr int kPass = 64;  // keys that pass a workgroup at once
+
+// A stretch that begins within a tile, whose sums others have parts of.
+struct Piece {
+    int s, head, tile_key;
+    int first;  // the stretch that has the tile's first rows; -1: this one does not end the tile
 };
 
 struct Weigh {
@@ -54,12 +80,20 @@ struct Weigh {
     const int32_t* parents;
     const float* lse;
     float* weights;
-    float* partial;  // [splits][S][Hkv][places], where the rows are split
-    int64_t places;
-    int32_t S, N, H, Hkv, D, splits;
-    Divider G;
+    // of many rows, two of each stretch: of the tile it starts in the middle of, and of the
+    // one it does not finish
+    Piece* pieces;   // [stretches]
+    float* partial;  // [stretches][2][kTile]
+    int32_t S, N, H, D, Hkv;
+    Divider G;    // heads of a cache head
     float scale;  // times log2(e)
+    bool even;    // the heads of a cache head divide 16, and a place's rows lie within 32 bits
 };
+
+// Which of a block's weights count: all, those of the keys up to the token that asks, or
+// those that a tree's token sees.
+enum { kPlain, kChain, kTree };
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 struct Asking {
     int length, count;
@@ -71,171 +105,469 @@ __device__ __forceinline__ Asking asking(const Weigh& p, int s) {
     return {length, min(max(count, 0), min(p.N, length))};
 }
 
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// x, of which the compiler knows nothing: what is computed from it stays where it is
+// used and takes no registers elsewhere.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
-// Item: a tile of keys of a sequence and cache head, and of its rows a split.
-template <int DTYPE, int DP>
-__global__ __launch_bounds__(kThreads) void weigh_kernel(const Weigh p) {
+// Waits for loads, those to LDS too, and LDS operations.
+__device__ __forceinline__ void wait_all() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t lo = uniform(static_cast<int>(x)), hi = uniform(static_cast<int>(x >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef const __attribute__((address_space(1))) char global_char;
+
+// What a workgroup knows of the call's sequences, and how the line of their work lies:
+// all of one cache head's after the other's, or of one sequence's heads.
+struct Board {
+    int64_t first[kSequences + 1];  // work ahead of each sequence
+    int length[kSequences], count[kSequences];
+    int64_t sum[4];
+};
+
+// Fills the board; sequence s is thread s's, work(asking) what it has. Returns all of it.
+template <class Work>
+__device__ __forceinline__ int64_t fill_board(const Weigh& p, Board& b, Work work) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    Asking a{0, 0};
+    if (tid < p.S) a = asking(p, tid);
+    b.length[tid] = a.length;
+    b.count[tid] = a.count;
+    int64_t upto = a.count > 0 ? work(a) : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t lo = __shfl_up(static_cast<uint32_t>(upto), d), hi = __shfl_up(static_cast<uint32_t>(upto >> 32), d);
+        if (lane >= d) upto += static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+    }
+    if (lane == 63) b.sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += b.sum[w];
+    b.first[tid + 1] = upto;
+    if (tid == 0) b.first[0] = 0;
+    __syncthreads();
+    return uniform(b.first[kSequences]);
+}
+
+// The sequence whose work place `at` of the line is.
+__device__ __forceinline__ int sequence_at(const Board& b, int64_t at) {
+    int s = 0;
+#pragma unroll
+    for (int d = kSequences / 2; d > 0; d >>= 1)
+        if (b.first[s + d] <= at) s += d;
+    return uniform(s);
+}
+
+// Which asking tokens each one sees, as bits; both arrays in LDS. Ends with no barrier.
+__device__ __forceinline__ void see(const Weigh& p, int s, int count, int16_t* up, uint32_t* sees, int words, int from, int until) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const int32_t parent = p.parents[static_cast<int64_t>(s) * p.N + i];
+        up[i] = static_cast<int16_t>(parent >= 0 && parent < i ? parent : -1);
+        for (int k = 0; k < words; ++k) sees[i * words + k] = 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kThreads)
+        for (int at = i; at >= 0; at = up[at]) {
+            const int bit = at - from;
+            if (at >= from && at < until) sees[i * words + bit / 32] |= 1u << (bit & 31);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the keys pass
+// ---------------------------------------------------------------------------
+
+// Line: 64 keys each, of a sequence's cache heads one after the other, of the sequences.
+// ONE: the rows are one block, and lie in registers.
+template <int DTYPE, int DP, bool ONE>
+__global__ __launch_bounds__(kThreads, (Dims<DTYPE, DP>::kFewResident)) void weigh_few(const Weigh p) {
     using E = Elem<DTYPE>;
     using Frag = typename E::Frag;
     using X = Dims<DTYPE, DP>;
-    constexpr int STEPS = X::kSteps, KB = X::kBlocks;
+    constexpr int STEPS = X::kSteps, ROWS = ONE ? 16 : X::kRows, AHEAD = X::kAhead, WORDS = ROWS / 32 > 0 ? ROWS / 32 : 1;
+    constexpr bool kHeld = ONE && STEPS <= 8;  // the queries fit registers
     constexpr float kInf = __builtin_inff();
-    extern __shared__ char tree[];  // with parents: [N][kTile / 32] words, which keys a token sees, then the parents
-    __shared__ int first[kSequences + 1], sum[4];
-    __shared__ int64_t row_at[kChunk * 16];
-    __shared__ __attribute__((aligned(16))) float row_lse[kChunk * 16];  // -lse * log2(e); of no row: -inf
-    __shared__ int row_token[kChunk * 16];
+    __shared__ __attribute__((aligned(16))) char queries[ROWS * X::kRowBytes];
+    __shared__ __attribute__((aligned(16))) float row_lse[ROWS];  // -lse * log2(e)
+    __shared__ __attribute__((aligned(16))) int row_token[ROWS];  // kNone: no row, or one that gives nothing
+    __shared__ uint32_t sees[ROWS * WORDS];
+    __shared__ int16_t up[ROWS];
+    __shared__ Board board;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), quad = lane >> 4, col = lane & 15;
+    const int bytes = p.D * X::kSize, G = static_cast<int>(p.G.d);
+    const int64_t total = p.Hkv * fill_board(p, board, [](const Asking& a) { return static_cast<int64_t>((a.length + kPass - 1) / kPass); });
+    const int64_t each = (total + gridDim.x - 1) / gridDim.x, stop = min(total, (blockIdx.x + 1) * each);
+    int64_t at = blockIdx.x * each;
+    while (at < stop) {
+        // the stretch's keys of one sequence and head
+        const int s = sequence_at(board, uniform(at / p.Hkv));
+        const Asking a{uniform(board.length[s]), uniform(board.count[s])};
+        const int tiles = (a.length + kPass - 1) / kPass, prefix = a.prefix(), rows = a.count * G;
+        const int64_t off = at - p.Hkv * uniform(board.first[s]);
+        const int head = uniform(static_cast<int>(off / tiles)), begin = uniform(static_cast<int>(off - static_cast<int64_t>(head) * tiles));
+        const int end = uniform(static_cast<int>(min(static_cast<int64_t>(tiles), begin + (stop - at))));
+        at += end - begin;
+
+        Frag keys[AHEAD][STEPS];
+        float old[AHEAD];
+        bool there[AHEAD];
+        const int32_t* const pages = p.pages + static_cast<int64_t>(s) * p.span.P;
+        float* const weights = p.weights + s * p.ws + head * p.wh;
+        const auto key_of = [&](int tile) { return tile * kPass + wave * 16 + col; };
+        const auto page_of = [&](int tile) {
+            const int key = key_of(tile);
+            return tile < end && key < a.length ? pages[p.span.page.quotient(key)] : -1;
+        };
+        const auto fetch = [&](int i, int tile, int page) BEAMGRAD_INLINE {
+            const int key = key_of(tile);
+            there[i] = p.span.is_page(page);
+            const char* const from = p.k + max(page, 0) * p.kp + (key - static_cast<int>(p.span.page.quotient(key) * p.span.page.d)) * p.kt + head * p.kh + quad * 16;
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                u32x4 x = {0, 0, 0, 0};
+                if (there[i] && (j * 4 + quad) * 16 < bytes) x = *reinterpret_cast<const u32x4*>(from + j * 64);
+                keys[i][j] = __builtin_bit_cast(Frag, x);
+            }
+            old[i] = there[i] && quad == 0 && key < prefix ? weights[key] : 0.0f;
+        };
+        int page[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) page[i] = page_of(begin + i);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            fetch(i, begin + i, page[i]);
+            page[i] = page_of(begin + i + AHEAD);
+        }
+
+        __syncthreads();  // the rows before are done with
+        const char* const q0 = p.q + s * p.qs + static_cast<int64_t>(head) * G * p.qh;
+        for (int i = tid; i < ROWS * X::kChunks; i += kThreads) {
+            const int row = i / X::kChunks, c = i - row * X::kChunks, token = static_cast<int>(p.G.quotient(row)), g = row - token * G;
+            u32x4 x = {0, 0, 0, 0};
+            if (row < rows && c * 16 < bytes) x = *reinterpret_cast<const u32x4*>(q0 + token * p.qn + g * p.qh + c * 16);
+            *reinterpret_cast<u32x4*>(queries + row * X::kRowBytes + (c ^ (row & X::kSwizzle)) * 16) = x;
+        }
+        if (tid < ROWS) {
+            const int token = static_cast<int>(p.G.quotient(tid));
+            float l = -kInf;
+            if (tid < rows) l = p.lse[(static_cast<int64_t>(s) * p.N + token) * p.H + head * G + (tid - token * G)];
+            row_lse[tid] = l == -kInf ? l : -l * kLog2e;
+            row_token[tid] = l == -kInf ? kNone : token;
+        }
+        if (p.parents) see(p, s, a.count, up, sees, WORDS, 0, a.count);
+        __syncthreads();
+
+        const auto query_of = [&](int block, Frag* query) {
+            const char* const row = queries + (block * 16 + col) * X::kRowBytes;
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j)
+                query[j] = *reinterpret_cast<const Frag*>(row + ((j * 4 + quad) ^ (col & X::kSwizzle)) * 16);
+        };
+        Frag held[STEPS];
+        if (kHeld) query_of(0, held);
+        const int blocks = ONE ? 1 : (rows + 15) / 16;
+        const auto weigh = [&](int i, int tile) BEAMGRAD_INLINE {
+            const int key = key_of(tile), asks = key - prefix;
+            const bool seen = p.parents && (tile + 1) * kPass > prefix;
+            float sum = 0.0f;
+            for (int b = 0; b < blocks; ++b) {
+                const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[b * 16 + quad * 4]);
+                const i32x4 t = *reinterpret_cast<const i32x4*>(&row_token[b * 16 + quad * 4]);
+                f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (kHeld) {
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j) score = E::mma(held[j], keys[i][j], score);
+                } else {
+                    Frag query[STEPS];
+                    query_of(b, query);
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j) score = E::mma(query[j], keys[i][j], score);
+                }
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[k], p.scale, l[k]));
+                    bool visible = asks <= t[k];
+                    if (seen && asks >= 0 && t[k] >= 0) visible = asks < a.count && (sees[t[k] * WORDS + asks / 32] >> (asks & 31) & 1);
+                    e[k] = visible ? e[k] : 0.0f;
+                }
+                sum += (e[0] + e[1]) + (e[2] + e[3]);
+            }
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (quad == 0 && there[i]) weights[key] = old[i] + sum;
+        };
+        for (int tile = begin; tile < end; tile += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (tile + i >= end) break;
+                weigh(i, tile + i);
+                fetch(i, tile + i + AHEAD, page[i]);
+                page[i] = page_of(tile + i + 2 * AHEAD);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the keys stay
+// ---------------------------------------------------------------------------
+
+// Line: blocks of 16 rows, of a sequence's tiles of keys one after the other, of the
+// sequences, of the cache heads. Rows of tokens ahead of a tile's first key see none of
+// it, and are not in the line.
+template <int DTYPE, int DP>
+__global__ __launch_bounds__(kThreads, 3) void weigh_many(const Weigh p) {
+    using E = Elem<DTYPE>;
+    using Frag = typename E::Frag;
+    using X = Dims<DTYPE, DP>;
+    constexpr int STEPS = X::kSteps, KB = X::kBlocks, ROWS = X::kRows, TILE = X::kTile, WORDS = TILE / 32;
+    constexpr float kInf = __builtin_inff();
+    extern __shared__ char tree[];  // with parents: [N][WORDS], which of the tile's keys a token sees, then the parents
+    // two places, by name: a wait for what is read of one is not a wait for what is on its
+    // way to the other
+    __shared__ __attribute__((aligned(1024))) char queries0[ROWS * X::kRowBytes];
+    __shared__ __attribute__((aligned(1024))) char queries1[ROWS * X::kRowBytes];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][ROWS];  // -lse * log2(e)
+    __shared__ __attribute__((aligned(16))) int row_token[2][ROWS];  // kNone: no row, or one that gives nothing
+    __shared__ int odd[2][ROWS / 16];  // a block of rows that holds such
+    __shared__ Board board;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), quad = lane >> 4, col = lane & 15;
-    // tiles of keys ahead of each sequence
-    {
-        int tiles = 0;
-        if (tid < p.S) {
-            const Asking a = asking(p, tid);
-            tiles = a.count > 0 ? (a.length + X::kTile - 1) / X::kTile : 0;
+    const int bytes = p.D * X::kSize, G = static_cast<int>(p.G.d);
+    if (bytes < X::kRowBytes)  // what no query fills stays zero
+        for (int i = tid; i < ROWS * X::kChunks; i += kThreads) {
+            reinterpret_cast<u32x4*>(queries0)[i] = u32x4{0, 0, 0, 0};
+            reinterpret_cast<u32x4*>(queries1)[i] = u32x4{0, 0, 0, 0};
         }
-        int upto = tiles;
+    // of a sequence: its blocks of rows, tiles that all of them see keys of, and the blocks
+    // that see none of a later tile
+    const auto blocks_of = [&](const Asking& a) { return (a.count * G + 15) / 16; };
+    const auto whole_of = [&](const Asking& a) {
+        const int tiles = (a.length + TILE - 1) / TILE;
+        return p.parents ? tiles : min(tiles, a.prefix() / TILE + 1);
+    };
+    const auto ahead_of = [&](const Asking& a, int tile) { return static_cast<int>((static_cast<int64_t>(tile) * TILE - a.prefix()) * G / 16); };
+    const int64_t line = fill_board(p, board, [&](const Asking& a) {
+        const int tiles = (a.length + TILE - 1) / TILE, blocks = blocks_of(a), whole = whole_of(a);
+        int64_t n = static_cast<int64_t>(whole) * blocks;
+        for (int t = whole; t < tiles; ++t) n += blocks - ahead_of(a, t);
+        return n;
+    });
+    const int64_t total = line * p.Hkv;
+    const int64_t each = (total + gridDim.x - 1) / gridDim.x;
+    // neighbours in the line, which share a head's queries, on one of the card's eight parts
+    const int stretch = static_cast<int>(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    const int64_t stop = min(total, (stretch + 1) * each);
+    int64_t at = stretch * each;
+    if (tid == 0) p.pieces[stretch] = {0, 0, 0, -1};
+
+    // the 16-byte chunks of a place's rows that the lane fetches, where p.even
+    uint32_t lane_at[X::kLoads];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(upto, d);
-            if (lane >= d) upto += y;
-        }
-        if (lane == 63) sum[wave] = upto;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) upto += sum[w];
-        first[tid + 1] = upto;
-        if (tid == 0) first[0] = 0;
-        __syncthreads();
+    for (int i = 0; i < X::kLoads; ++i) {
+        const int slot = (i * 4 + wave) * 64 + lane, row = slot / X::kChunks, c = (slot - row * X::kChunks) ^ (row & X::kSwizzle);
+        const int t = static_cast<int>(p.G.quotient(row)), g = row - t * G;
+        lane_at[i] = static_cast<uint32_t>(t * p.qn + g * p.qh) + c * 16;
     }
-    const int64_t items = static_cast<int64_t>(uniform(first[kSequences])) * p.Hkv * p.splits;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t of_heads = item / p.Hkv;
-        const int head = static_cast<int>(item - of_heads * p.Hkv), tile = static_cast<int>(of_heads / p.splits);
-        const int split = static_cast<int>(of_heads - static_cast<int64_t>(tile) * p.splits);
-        int s = 0;
+    while (at < stop) {
+        // blocks [begin, end) of rows against tile `tile`, which has `units` of them
+        const int head = uniform(static_cast<int>(at / line));
+        int64_t off = at - head * line;
+        const int s = sequence_at(board, off);
+        const Asking a{uniform(board.length[s]), uniform(board.count[s])};
+        off = uniform(off - board.first[s]);
+        const int prefix = a.prefix(), rows = a.count * G, blocks = blocks_of(a), whole = whole_of(a);
+        int tile, units = blocks, begin = 0;
+        if (off < static_cast<int64_t>(whole) * blocks) {
+            tile = uniform(static_cast<int>(off / blocks));
+            off -= static_cast<int64_t>(tile) * blocks;
+        } else {
+            off -= static_cast<int64_t>(whole) * blocks;
+            for (tile = whole;; ++tile) {
+                begin = ahead_of(a, tile);
+                units = blocks - begin;
+                if (off < units) break;
+                off -= units;
+            }
+            tile = uniform(tile);
+            begin = uniform(begin);
+            units = uniform(units);
+        }
+        const int skipped = uniform(static_cast<int>(off)), taken = uniform(static_cast<int>(min(static_cast<int64_t>(units - skipped), stop - at)));
+        const bool all = taken == units;
+        begin += skipped;
+        const int end = begin + taken, tile_key = tile * TILE, key0 = tile_key + wave * X::kKeys;
+        if (skipped > 0 && tid == 0)
+            p.pieces[stretch] = {s, head, tile_key, skipped + taken == units ? static_cast<int>((at - skipped) / each) : -1};
+        at += taken;
+
+        // rows from block `from` on, to a place of LDS: their queries on their way, the rest in registers
+        const char* const q0 = p.q + s * p.qs + static_cast<int64_t>(head) * G * p.qh;
+        float lse = -kInf;
+        int token = kNone;
+        const auto stage = [&](char* queries, int from) BEAMGRAD_INLINE {
+            // where the rows of a token lie in one block, a lane's place in a chunk is the same in all
+            const char* const rows_at = q0 + static_cast<int64_t>(from * 16 / G) * p.qn;
+            if (p.even && from * 16 + ROWS <= rows && bytes == X::kRowBytes) {
 #pragma unroll
-        for (int d = kSequences / 2; d > 0; d >>= 1)
-            if (first[s + d] <= tile) s += d;
-        s = uniform(s);
-        const Asking a = asking(p, s);
-        const int tile_key = (tile - uniform(first[s])) * X::kTile, key0 = tile_key + wave * X::kKeys, prefix = a.prefix();
+                for (int i = 0; i < X::kLoads; ++i)
+                    __builtin_amdgcn_global_load_lds((global_char*)(rows_at + lane_at[i]), (lds_char*)(queries + (i * 4 + wave) * 1024), 16, 0, 0);
+            } else {
+                const int here = opaque(lane);
+#pragma unroll
+                for (int i = 0; i < X::kLoads; ++i) {
+                    const int slot = (i * 4 + wave) * 64 + here, row = slot / X::kChunks, c = (slot - row * X::kChunks) ^ (row & X::kSwizzle);
+                    const int r = from * 16 + row, t = static_cast<int>(p.G.quotient(r)), g = r - t * G;
+                    if (r < rows && c * 16 < bytes)
+                        __builtin_amdgcn_global_load_lds((global_char*)(q0 + t * p.qn + g * p.qh + c * 16),
+                                                         (lds_char*)(queries + (i * 4 + wave) * 1024), 16, 0, 0);
+                }
+            }
+            lse = -kInf;
+            const int r = from * 16 + tid;
+            if (tid < ROWS && r < rows) {
+                token = static_cast<int>(p.G.quotient(r));
+                lse = p.lse[(static_cast<int64_t>(s) * p.N + token) * p.H + head * G + (r - token * G)];
+            }
+        };
+        const auto write_rows = [&](int place) BEAMGRAD_INLINE {
+            const bool none = lse == -kInf;
+            const uint64_t which = __ballot(none);
+            if (tid < ROWS) {
+                row_lse[place][tid] = none ? lse : -lse * kLog2e;
+                row_token[place][tid] = none ? kNone : token;
+                if (col == 0) odd[place][tid >> 4] = (which >> lane & 0xffff) != 0;
+            }
+        };
         // the keys
         Frag keys[KB][STEPS];
         bool there[KB];
+        {
+            int page[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const int key = key0 + b * 16 + col;
-            int page = -1, column = 0;
-            if (key < a.length) {
-                column = static_cast<int>(p.span.page.quotient(key));
-                const int32_t entry = p.pages[static_cast<int64_t>(s) * p.span.P + column];
-                page = p.span.is_page(entry) ? entry : -1;
+            for (int b = 0; b < KB; ++b) {
+                const int key = key0 + b * 16 + col;
+                page[b] = -1;
+                if (key < a.length) page[b] = p.pages[static_cast<int64_t>(s) * p.span.P + p.span.page.quotient(key)];
             }
-            there[b] = page >= 0;
-            const char* const from = p.k + max(page, 0) * p.kp + (key - column * static_cast<int>(p.span.page.d)) * p.kt + head * p.kh + quad * 16;
+            __syncthreads();  // the tile before is done with LDS
+            stage(queries0, begin);
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                u32x4 x = {0, 0, 0, 0};
-                if (there[b] && (i * 4 + quad) * 16 < p.D * X::kSize) x = *reinterpret_cast<const u32x4*>(from + i * 64);
-                keys[b][i] = __builtin_bit_cast(Frag, x);
-            }
-        }
-        float sums[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) sums[b] = 0.0f;
-
-        const int G = static_cast<int>(p.G.d), rows = a.count * G, blocks = (rows + 15) / 16;
-        const int each = (blocks + p.splits - 1) / p.splits, end = min(blocks, (split + 1) * each);
-        int begin = split * each;
-        uint32_t* const sees = reinterpret_cast<uint32_t*>(tree);
-        if (p.parents) {
-            int16_t* const up = reinterpret_cast<int16_t*>(sees + p.N * (X::kTile / 32));
-            __syncthreads();
-            if (tile_key + X::kTile > prefix) {
-                for (int i = tid; i < a.count; i += kThreads) {
-                    const int32_t parent = p.parents[static_cast<int64_t>(s) * p.N + i];
-                    up[i] = static_cast<int16_t>(parent >= 0 && parent < i ? parent : -1);
-                    for (int w = 0; w < X::kTile / 32; ++w) sees[i * (X::kTile / 32) + w] = 0;
-                }
-                __syncthreads();
-                for (int i = tid; i < a.count; i += kThreads)
-                    for (int at = i; at >= 0; at = up[at]) {
-                        const int bit = prefix + at - tile_key;
-                        if (bit >= 0 && bit < X::kTile) sees[i * (X::kTile / 32) + bit / 32] |= 1u << (bit & 31);
-                    }
-            }
-        } else {
-            // rows of tokens ahead of the tile's first key see none of it
-            begin = max(begin, max(0, tile_key - prefix) * G / 16);
-        }
-        const bool masked = key0 + X::kKeys > prefix;  // some of the wavefront's keys ask themselves
-        const char* const q0 = p.q + s * p.qs + static_cast<int64_t>(head) * G * p.qh + quad * 16;
-        for (int chunk = begin; chunk < end; chunk += kChunk) {
-            __syncthreads();
-            {
-                const int r = chunk * 16 + tid, token = static_cast<int>(p.G.quotient(min(r, rows - 1))), g = r - token * G;
-                const bool live = r < rows;
-                float l = -kInf;
-                if (live) l = p.lse[(static_cast<int64_t>(s) * p.N + token) * p.H + head * G + g];
-                row_lse[tid] = l == -kInf ? l : -l * kLog2e;
-                row_at[tid] = live ? token * p.qn + g * p.qh : -1;
-                row_token[tid] = live ? token : -1;
-            }
-            __syncthreads();
-            const int n = min(kChunk, end - chunk);
-            Frag next[STEPS];
-            const auto fetch = [&](int b) {
-                const int64_t at = row_at[b * 16 + col];
+            for (int b = 0; b < KB; ++b) {
+                const int key = key0 + b * 16 + col;
+                there[b] = p.span.is_page(page[b]);
+                const int in_page = key - static_cast<int>(p.span.page.quotient(key) * p.span.page.d);
+                const char* const from = p.k + max(page[b], 0) * p.kp + in_page * p.kt + head * p.kh + quad * 16;
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
                     u32x4 x = {0, 0, 0, 0};
-                    if (at >= 0 && (i * 4 + quad) * 16 < p.D * X::kSize) x = *reinterpret_cast<const u32x4*>(q0 + at + i * 64);
-                    next[i] = __builtin_bit_cast(Frag, x);
+                    if (there[b] && (i * 4 + quad) * 16 < bytes) x = *reinterpret_cast<const u32x4*>(from + i * 64);
+                    keys[b][i] = __builtin_bit_cast(Frag, x);
                 }
-            };
-            fetch(0);
-            for (int b = 0; b < n; ++b) {
-                Frag query[STEPS];
+            }
+        }
+        uint32_t* const sees = reinterpret_cast<uint32_t*>(tree);
+        const bool asked = tile_key + TILE > prefix;  // some of the tile's keys ask themselves
+        if (p.parents && asked) see(p, s, a.count, reinterpret_cast<int16_t*>(sees + p.N * WORDS), sees, WORDS, tile_key - prefix, tile_key - prefix + TILE);
+        const bool asks_itself = key0 + X::kKeys > prefix;
+        float sums[KB];
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) query[i] = next[i];
-                if (b + 1 < n) fetch(b + 1);
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[b * 16 + quad * 4]);
+        for (int b = 0; b < KB; ++b) sums[b] = 0.0f;
+        write_rows(0);
+        // a chunk of rows, which lies in `queries`, while the next one comes to `others`
+        const auto chunk_of = [&](int chunk, auto which, const char* queries, char* others) BEAMGRAD_INLINE {
+            constexpr int place = decltype(which)::value;
+            wait_all();
+            __syncthreads();
+            const bool more = chunk + ROWS / 16 < end;
+            if (more) stage(others, chunk + ROWS / 16);
+            const int n = min(ROWS / 16, end - chunk);
+            const auto block = [&](int b, auto mask) BEAMGRAD_INLINE {
+                constexpr int MASK = decltype(mask)::value;
+                Frag query[STEPS];
+                const char* const row = queries + (b * 16 + col) * X::kRowBytes;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+                    query[i] = *reinterpret_cast<const Frag*>(row + ((i * 4 + quad) ^ (col & X::kSwizzle)) * 16);
+                const f32x4 l = *reinterpret_cast<const f32x4*>(&row_lse[place][b * 16 + quad * 4]);
+                i32x4 t = {0, 0, 0, 0};
+                if constexpr (MASK != kPlain) t = *reinterpret_cast<const i32x4*>(&row_token[place][b * 16 + quad * 4]);
+                f32x4 score[KB];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) score[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) score[kb] = E::mma(query[i], keys[kb][i], score[kb]);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float e[4];
 #pragma unroll
-                    for (int i = 0; i < STEPS; ++i) score = E::mma(query[i], keys[kb][i], score);
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], p.scale, lse[i]));
-                    if (masked) {
+                    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[kb][i], p.scale, l[i]));
+                    if constexpr (MASK != kPlain) {
                         const int asks = key0 + kb * 16 + col - prefix;  // the asking token that the key is
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int token = row_token[b * 16 + quad * 4 + i];
-                            bool visible = asks <= token;
-                            if (p.parents && asks >= 0) {
-                                const int bit = asks + prefix - tile_key;
-                                visible = token >= 0 && (sees[token * (X::kTile / 32) + bit / 32] >> (bit & 31) & 1);
+                            bool visible = asks <= t[i];
+                            if constexpr (MASK == kTree) {
+                                const int bit = wave * X::kKeys + kb * 16 + col;  // the key's place in the tile
+                                const uint32_t of = sees[max(t[i], 0) * WORDS + bit / 32] >> (bit & 31);
+                                visible = asks < 0 ? visible : visible && (of & 1);
                             }
-                            w[i] = visible ? w[i] : 0.0f;
+                            e[i] = visible ? e[i] : 0.0f;
                         }
                     }
-                    sums[kb] += (w[0] + w[1]) + (w[2] + w[3]);
+                    sums[kb] += (e[0] + e[1]) + (e[2] + e[3]);
+                }
+            };
+            int any = asks_itself;
+#pragma unroll
+            for (int b = 0; b < ROWS / 16; ++b) any |= odd[place][b];
+            if (n == ROWS / 16 && !uniform(any)) {
+#pragma unroll 1
+                for (int b = 0; b < ROWS / 16; ++b) block(b, std::integral_constant<int, kPlain>{});
+            } else {
+#pragma unroll 1
+                for (int b = 0; b < n; ++b) {
+                    if (p.parents && asks_itself) {
+                        block(b, std::integral_constant<int, kTree>{});
+                        continue;
+                    }
+                    const int strange = uniform(odd[place][b]);
+                    const int first_token = uniform(row_token[place][b * 16]), last_token = uniform(row_token[place][b * 16 + 15]);
+                    if (asks_itself && !strange && last_token < key0 - prefix) continue;  // none sees any
+                    if (strange || (asks_itself && first_token < key0 + X::kKeys - 1 - prefix))
+                        block(b, std::integral_constant<int, kChain>{});
+                    else
+                        block(b, std::integral_constant<int, kPlain>{});
                 }
             }
+            if (more) write_rows(place ^ 1);
+        };
+        for (int chunk = begin; chunk < end; chunk += 2 * (ROWS / 16)) {
+            chunk_of(chunk, std::integral_constant<int, 0>{}, queries0, queries1);
+            if (chunk + ROWS / 16 < end) chunk_of(chunk + ROWS / 16, std::integral_constant<int, 1>{}, queries1, queries0);
         }
         // the four lanes of a key
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             sums[b] += __shfl_xor(sums[b], 16);
             sums[b] += __shfl_xor(sums[b], 32);
-            const int key = key0 + b * 16 + col;
-            if (quad != b % 4 || !there[b]) continue;
-            if (p.splits > 1) {
-                p.partial[((static_cast<int64_t>(split) * p.S + s) * p.Hkv + head) * p.places + key] = sums[b];
-            } else {
+            if (quad != b % 4) continue;
+            if (!all) {
+                p.partial[(static_cast<int64_t>(stretch) * 2 + (skipped > 0 ? 0 : 1)) * TILE + wave * X::kKeys + b * 16 + col] = sums[b];
+            } else if (there[b]) {
+                const int key = key0 + b * 16 + col;
                 float* const to = p.weights + s * p.ws + head * p.wh + key;
                 *to = key < prefix ? *to + sums[b] : sums[b];
             }
@@ -243,17 +575,19 @@ __global__ __launch_bounds__(kThreads) void weigh_kernel(const Weigh p) {
     }
 }
 
-// x: places of sequence z, head y.
-__global__ __launch_bounds__(kJoinThreads) void weigh_join(const Weigh p) {
-    const int s = blockIdx.z, head = blockIdx.y, key = blockIdx.x * kJoinThreads + threadIdx.x;
-    const Asking a = asking(p, s);
-    if (a.count == 0 || key >= a.length ||
-        !p.span.is_page(p.pages[static_cast<int64_t>(s) * p.span.P + p.span.page.quotient(key)]))
-        return;
-    float* const to = p.weights + s * p.ws + head * p.wh + key;
-    float sum = key < a.prefix() ? *to : 0.0f;
-    for (int i = 0; i < p.splits; ++i) sum += p.partial[((static_cast<int64_t>(i) * p.S + s) * p.Hkv + head) * p.places + key];
-    *to = sum;
+// x: a stretch that ends a tile which others began: what they have of it, in order.
+__global__ __launch_bounds__(kThreads) void weigh_join(const Weigh p, const int tile) {
+    const Piece piece = p.pieces[blockIdx.x];
+    if (piece.first < 0) return;
+    const Asking a = asking(p, piece.s);
+    for (int i = threadIdx.x; i < tile; i += kThreads) {
+        const int key = piece.tile_key + i;
+        if (key >= a.length || !p.span.is_page(p.pages[static_cast<int64_t>(piece.s) * p.span.P + p.span.page.quotient(key)])) continue;
+        float* const to = p.weights + piece.s * p.ws + piece.head * p.wh + key;
+        float sum = key < a.prefix() ? *to : 0.0f;
+        for (int v = piece.first; v <= static_cast<int>(blockIdx.x); ++v) sum += p.partial[(static_cast<int64_t>(v) * 2 + (v == piece.first ? 1 : 0)) * tile + i];
+        *to = sum;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -287,16 +621,21 @@ bool valid_sizes(const BeamgradWeights* a) {
 }
 
 struct Form {
-    int tile;
-    const void* kernel;
+    int rows, tile, resident;  // few rows at most; keys of a tile of many; workgroups of a CU for few
+    const void *one, *few, *many;
 };
+template <int DTYPE, int DP>
+Form form_of_width() {
+    return {Dims<DTYPE, DP>::kRows, Dims<DTYPE, DP>::kTile, Dims<DTYPE, DP>::kFewResident, reinterpret_cast<const void*>(weigh_few<DTYPE, DP, true>),
+            reinterpret_cast<const void*>(weigh_few<DTYPE, DP, false>), reinterpret_cast<const void*>(weigh_many<DTYPE, DP>)};
+}
 template <int DTYPE>
 Form form_of(int dim) {
     switch ((dim + 63) / 64) {
-        case 1: return {Dims<DTYPE, 64>::kTile, reinterpret_cast<const void*>(weigh_kernel<DTYPE, 64>)};
-        case 2: return {Dims<DTYPE, 128>::kTile, reinterpret_cast<const void*>(weigh_kernel<DTYPE, 128>)};
-        case 3: return {Dims<DTYPE, 192>::kTile, reinterpret_cast<const void*>(weigh_kernel<DTYPE, 192>)};
-        default: return {Dims<DTYPE, 256>::kTile, reinterpret_cast<const void*>(weigh_kernel<DTYPE, 256>)};
+        case 1: return form_of_width<DTYPE, 64>();
+        case 2: return form_of_width<DTYPE, 128>();
+        case 3: return form_of_width<DTYPE, 192>();
+        default: return form_of_width<DTYPE, 256>();
     }
 }
 Form form_of(const BeamgradWeights& a) {
@@ -309,14 +648,30 @@ Form form_of(const BeamgradWeights& a) {
 
 int64_t places_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.table_pages) * a.page_tokens; }
 
-// Many rows over few keys: the rows are split, into eight blocks of 16 at least, so
-// that the card's workgroups have an item each.
-int splits_of(const BeamgradWeights& a, int tile) {
-    constexpr int64_t kWanted = 1024, kLeast = 8;
-    const int64_t sequences = std::min<int64_t>(a.sequences, kSequences);
-    const int64_t items = sequences * a.kv_heads * ((places_of(a) + tile - 1) / tile);
-    const int64_t blocks = (static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads) + 15) / 16;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(kWanted + items - 1) / items, blocks / kLeast, kMaxSplits})));
+int64_t rows_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads); }
+
+// Workgroups of a launch, a multiple of eight. The card holds three of many rows on a CU
+// (two with a large tree's table), but of three that share a CU the oldest runs fastest:
+// twice as many, in equal stretches, are done sooner (two prompts' ends of 512 tokens over
+// 7700 and 15100, 32 heads of 128, bfloat16: 143 us, 151 with one round; more rounds
+// cost more beginnings than they gain). Few rows have shorter beginnings: four rounds (32
+// tokens over 2000 to 16000: 125 us, 140 with one). No more than there is work for,
+// by the table's size.
+unsigned grid_of(const BeamgradWeights& a, const Form& form, size_t lds) {
+    int device = 0, cus = 0;
+    if (hipGetDevice(&device) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) {
+        (void)hipGetLastError();
+        cus = 256;
+    }
+    const bool few = rows_of(a) <= form.rows;
+    const int64_t most = static_cast<int64_t>(cus) * (few ? 4 * form.resident : lds > 14 * 1024 ? 2 * 2 : 2 * 3);
+    const int64_t tile = few ? kPass : form.tile, heads = static_cast<int64_t>(std::min(a.sequences, kSequences)) * a.kv_heads;
+    const double work = static_cast<double>(heads) * static_cast<double>((places_of(a) + tile - 1) / tile) * (few ? 1.0 : static_cast<double>((rows_of(a) + 15) / 16) / 3.0);
+    return static_cast<unsigned>((std::max<int64_t>(1, static_cast<int64_t>(std::min(work, static_cast<double>(most)))) + 7) / 8 * 8);
+}
+
+size_t tree_bytes(const BeamgradWeights& a, const Form& form) {
+    return a.parents && rows_of(a) > form.rows ? static_cast<size_t>(a.tokens) * (form.tile / 32 * sizeof(uint32_t) + sizeof(int16_t)) : 0;
 }
 
 }  // namespace
@@ -325,10 +680,10 @@ extern "C" {
 
 DBS_CUDA_EXPORT int64_t beamgrad_accumulate_weights_workspace_size(const BeamgradWeights* args) {
     if (!valid_sizes(args)) return -1;
-    const int splits = splits_of(*args, form_of(*args).tile);
-    return splits == 1 ? 0
-                       : static_cast<int64_t>(splits) * std::min(args->sequences, kSequences) * args->kv_heads * places_of(*args) *
-                             static_cast<int64_t>(sizeof(float));
+    const Form form = form_of(*args);
+    return rows_of(*args) <= form.rows
+               ? 0
+               : grid_of(*args, form, tree_bytes(*args, form)) * static_cast<int64_t>(sizeof(Piece) + 2 * form.tile * sizeof(float));
 }
 
 DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, void* workspace, int64_t workspace_bytes,
@@ -347,22 +702,20 @@ DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, voi
     p.k = static_cast<const char*>(a.k);
     p.ws = a.weight_strides[0], p.wh = a.weight_strides[1];
     p.span = {Divider::of(static_cast<uint32_t>(a.page_tokens)), a.n_pages, a.table_pages};
-    p.partial = static_cast<float*>(workspace);
-    p.places = places_of(a);
-    p.N = a.tokens, p.H = a.heads, p.Hkv = a.kv_heads, p.D = a.head_dim;
-    p.splits = splits_of(a, form.tile);
+    const size_t lds = tree_bytes(a, form);
+    const unsigned grid = grid_of(a, form, lds);
+    p.pieces = static_cast<Piece*>(workspace);
+    p.partial = reinterpret_cast<float*>(p.pieces + grid);
+    p.N = a.tokens, p.H = a.heads, p.D = a.head_dim, p.Hkv = a.kv_heads;
     p.G = Divider::of(static_cast<uint32_t>(a.heads / a.kv_heads));
     p.scale = a.scale * kLog2e;
-    const size_t lds = a.parents ? static_cast<size_t>(a.tokens) * (form.tile / 32 * sizeof(uint32_t) + sizeof(int16_t)) : 0;
-    // tiles of a launch in 31 bits, whatever the lengths
-    const int64_t tiles = (p.places + form.tile - 1) / form.tile;
-    const int batch = static_cast<int>(std::min<int64_t>(kSequences, std::max<int64_t>(1, INT32_MAX / tiles)));
-    int device = 0, cus = 256, resident = 4;
-    if (hipGetDevice(&device) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) (void)hipGetLastError();
+    p.even = 16 % p.G.d == 0 && p.qn <= INT32_MAX / 256 && p.qh <= INT32_MAX / 32;
+    const bool few = rows_of(a) <= form.rows;
+    const void* const kernel = rows_of(a) <= 16 ? form.one : few ? form.few : form.many;
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     hipError_t e = hipSuccess;
-    for (int s0 = 0; s0 < a.sequences && e == hipSuccess; s0 += batch) {
-        p.S = std::min(batch, a.sequences - s0);
+    for (int s0 = 0; s0 < a.sequences && e == hipSuccess; s0 += kSequences) {
+        p.S = std::min(kSequences, a.sequences - s0);
         p.q = static_cast<const char*>(a.q) + s0 * p.qs;
         p.pages = a.pages + static_cast<int64_t>(s0) * a.table_pages;
         p.lengths = a.lengths + s0;
@@ -370,13 +723,10 @@ DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, voi
         p.parents = a.parents ? a.parents + static_cast<int64_t>(s0) * a.tokens : nullptr;
         p.lse = a.lse + static_cast<int64_t>(s0) * a.tokens * a.heads;
         p.weights = a.weights + s0 * p.ws;
-        const double most = static_cast<double>(p.S) * p.Hkv * p.splits * static_cast<double>(tiles);
-        const unsigned grid = static_cast<unsigned>(std::min<double>(most, static_cast<double>(cus) * resident));
         void* arguments[] = {&p};
-        e = hipLaunchKernel(form.kernel, dim3(grid), dim3(kThreads), arguments, lds, stream);
-        if (e == hipSuccess && p.splits > 1) {
-            weigh_join<<<dim3(static_cast<unsigned>((p.places + kJoinThreads - 1) / kJoinThreads), static_cast<unsigned>(p.Hkv), static_cast<unsigned>(p.S)),
-                         kJoinThreads, 0, stream>>>(p);
+        e = hipLaunchKernel(kernel, dim3(grid), dim3(kThreads), arguments, lds, stream);
+        if (e == hipSuccess && !few) {
+            weigh_join<<<grid, kThreads, 0, stream>>>(p, form.tile);
             e = hipGetLastError();
         }
     }
