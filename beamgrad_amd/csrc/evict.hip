@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "beamgrad_state.h"
@@ -25,12 +26,16 @@ using namespace dbs_hip;
 
 namespace {
 
-constexpr int kCutThreads = 1024;
+constexpr int kCutThreads = 512;
 constexpr int kCutWaves = kCutThreads / 64;
 constexpr int kDigits = 2048;
 constexpr int kEach = 4;     // weights of a thread and round, one after the other
+constexpr int kRound = kCutThreads * kEach;
+constexpr int kHeld = 4;     // rounds whose weights stay in registers
 constexpr int kAtOnce = 8;   // reads of a thread in flight
 constexpr int kMoveThreads = 256;
+constexpr int kLeastWidth = 4;  // columns of a workgroup
+constexpr int kTokens = kMoveThreads / kLeastWidth * kAtOnce;  // of a round, at most
 constexpr int kPoolsOfLaunch = 64;
 constexpr int kSetsOfLaunch = 64;
 constexpr int kMaxHeads = 1024;
@@ -94,10 +99,145 @@ __device__ __forceinline__ uint32_t ahead_of(uint32_t x, uint32_t* lds, uint32_t
     return before + sum - x;
 }
 
+// kEach weights from token i on; 0 from `end` on.
+__device__ __forceinline__ void weights_at(const float* from, int i, int end, float* x) {
+    if (i + kEach <= end) {
+        const u32x4 raw = *reinterpret_cast<const u32x4_any*>(from + i);
+        __builtin_memcpy(x, &raw, sizeof(raw));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) x[j] = i + j < end ? from[i + j] : 0.0f;
+}
+
+// A row of weights [c.first, end), of which `want` stay: what stays, in order, to
+// each(place, token, weight). HELD: their keys fit the registers of the workgroup, and are read once.
+struct Choice {
+    uint32_t counts[kDigits], sums[kCutWaves];
+    uint32_t held_sums[kHeld][kCutWaves];
+    uint32_t digit, rest;
+    bool whole;  // all that have the digit stay
+};
+
+template <bool HELD, class Each>
+__device__ __forceinline__ void choose(const float* from, int first, int end, int want, const float (&w)[kHeld * kEach], Choice& lds, Each each) {
+    const int tid = threadIdx.x;
+    // the want-th largest key, and how many that equal it stay
+    uint32_t key = 0, mask = 0, left = want;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t bits = pass == 2 ? 1023 : 2047;
+        for (int i = tid; i < kDigits; i += kCutThreads) lds.counts[i] = 0;
+        __syncthreads();
+        const auto count = [&](uint32_t o) {
+            if ((o & mask) == key) atomicAdd(&lds.counts[o >> shift & bits], 1u);
+        };
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < kHeld * kEach; ++i)
+                if (first + (i / kEach) * kRound + tid * kEach + i % kEach < end) count(order_of(w[i]));
+        } else {
+            for (int i0 = first + tid; i0 < end; i0 += kCutThreads * kAtOnce) {
+                float x[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) x[j] = i0 + j * kCutThreads < end ? from[i0 + j * kCutThreads] : 0.0f;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j)
+                    if (i0 + j * kCutThreads < end) count(order_of(x[j]));
+            }
+        }
+        __syncthreads();
+        // digits from the largest down, some of a thread
+        constexpr int kOwn = kDigits / kCutThreads;
+        const int top = kDigits - 1 - kOwn * tid;
+        uint32_t of[kOwn], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) sum += of[i] = lds.counts[top - i];
+        uint32_t total;
+        uint32_t above = ahead_of(sum, lds.sums, total);
+        if (above < left && above + sum >= left) {
+            int i = 0;
+            for (; above + of[i] < left; ++i) above += of[i];
+            lds.digit = top - i;
+            lds.rest = left - above;
+            lds.whole = of[i] == left - above;
+        }
+        __syncthreads();
+        key |= lds.digit << shift;
+        mask |= bits << shift;
+        left = lds.rest;
+        const bool whole = lds.whole;
+        __syncthreads();
+        if (whole) break;  // the digits behind do not matter
+    }
+    // larger ones and the first `left` equal ones, in order; both counts in one number
+    const auto tally = [&](int i, const float* x) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const uint32_t m = order_of(x[j]) & mask;
+            if (i + j < end) n += m > key ? 1u : m == key ? 1u << 16 : 0u;
+        }
+        return n;
+    };
+    const auto emit = [&](int i, const float* x, uint32_t big, uint32_t same) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (i + j >= end) continue;
+            const uint32_t m = order_of(x[j]) & mask;
+            if (m > key || (m == key && same < left)) each(first + static_cast<int>(big + min(same, left)), i + j, x[j]);
+            big += m > key;
+            same += m == key;
+        }
+    };
+    uint32_t larger = 0, equal = 0;
+    if constexpr (HELD) {
+        // all rounds' sums at once
+        const int lane = tid & 63, wave = tid >> 6;
+        uint32_t mine[kHeld], upto[kHeld];
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) upto[r] = mine[r] = tally(first + r * kRound + tid * kEach, w + r * kEach);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+            for (int r = 0; r < kHeld; ++r) {
+                const uint32_t y = __shfl_up(upto[r], d);
+                if (lane >= d) upto[r] += y;
+            }
+        if (lane == 63)
+#pragma unroll
+            for (int r = 0; r < kHeld; ++r) lds.held_sums[r][wave] = upto[r];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            uint32_t before = upto[r] - mine[r], total = 0;
+#pragma unroll
+            for (int v = 0; v < kCutWaves; ++v) {
+                if (v < wave) before += lds.held_sums[r][v];
+                total += lds.held_sums[r][v];
+            }
+            emit(first + r * kRound + tid * kEach, w + r * kEach, larger + (before & 0xffff), equal + (before >> 16));
+            larger += total & 0xffff;
+            equal += total >> 16;
+        }
+    } else {
+        for (int i0 = first; i0 < end; i0 += kRound) {
+            const int i = i0 + tid * kEach;
+            float x[kEach];
+            uint32_t total;
+            weights_at(from, i, end, x);
+            const uint32_t before = ahead_of(tally(i, x), lds.sums, total);
+            emit(i, x, larger + (before & 0xffff), equal + (before >> 16));
+            larger += total & 0xffff;
+            equal += total >> 16;
+        }
+    }
+}
+
 // x: a sequence; y: a row of weights, the last: counts of pages, copied; z: a set.
 __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const WeightSet set) {
-    __shared__ uint32_t counts[kDigits], lds[kCutWaves];
-    __shared__ uint32_t digit, rest;
+    __shared__ Choice lds;
     const int s = blockIdx.x, tid = threadIdx.x, head = blockIdx.y;
     if (head == p.heads) {
         if (blockIdx.z == 0 && set.first == 0)
@@ -110,12 +250,18 @@ __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const
     const int64_t row = static_cast<int64_t>(s) * p.heads + head;
     float* const to = set.to[blockIdx.z] + row * p.places;
     const Cut c = cut_of(p, s);
+    const int end = c.n - c.recent, want = c.keep - c.recent - c.first;
+    const bool held = end - c.first <= kHeld * kRound;
     bool stays = c.n <= c.keep;
+    float w[kHeld * kEach];
     if (!stays) {
+        // read while the pages are looked through
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) weights_at(from, c.first + r * kRound + tid * kEach, held ? end : 0, w + r * kEach);
         // every token has a page, and those that are written are the sequence's alone
-        const int held = p.t.span.held(c.n), low = static_cast<int>(p.t.span.page.quotient(c.first)), high = p.t.span.held(c.keep);
+        const int pages = p.t.span.held(c.n), low = static_cast<int>(p.t.span.page.quotient(c.first)), high = p.t.span.held(c.keep);
         bool bad = false;
-        for (int column = tid; column < held; column += kCutThreads) {
+        for (int column = tid; column < pages; column += kCutThreads) {
             const int32_t page = p.t.pages[static_cast<int64_t>(s) * p.t.span.P + column];
             bad |= !p.t.span.is_page(page) || (column >= low && column < high && p.t.refs[page] != 1);
         }
@@ -136,73 +282,15 @@ __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const
         to[c.keep - c.recent + i] = from[c.n - c.recent + i];
     }
     for (int64_t i = c.keep + tid; i < p.places; i += kCutThreads) to[i] = 0.0f;
-    const int end = c.n - c.recent, want = c.keep - c.recent - c.first;
     if (want == 0) return;
-    // the want-th largest key, and how many that equal it stay
-    uint32_t key = 0, mask = 0, left = want;
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t bits = pass == 2 ? 1023 : 2047;
-        for (int i = tid; i < kDigits; i += kCutThreads) counts[i] = 0;
-        __syncthreads();
-        for (int i0 = c.first + tid; i0 < end; i0 += kCutThreads * kAtOnce) {
-            float w[kAtOnce];
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) w[j] = i0 + j * kCutThreads < end ? from[i0 + j * kCutThreads] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
-                const uint32_t o = order_of(w[j]);
-                if (i0 + j * kCutThreads < end && (o & mask) == key) atomicAdd(&counts[o >> shift & bits], 1u);
-            }
-        }
-        __syncthreads();
-        // digits from the largest down, two of a thread
-        const int top = kDigits - 1 - 2 * tid;
-        const uint32_t high = counts[top], low = counts[top - 1];
-        uint32_t total;
-        const uint32_t above = ahead_of(high + low, lds, total);
-        if (above < left && above + high + low >= left) {
-            const bool first = above + high >= left;
-            digit = first ? top : top - 1;
-            rest = left - above - (first ? 0 : high);
-        }
-        __syncthreads();
-        key |= digit << shift;
-        mask |= bits << shift;
-        left = rest;
-        __syncthreads();
-    }
-    // larger ones and the first `left` equal ones, in order; both counts in one number
-    uint32_t larger = 0, equal = 0;
-    for (int i0 = c.first; i0 < end; i0 += kCutThreads * kEach) {
-        const int i = i0 + tid * kEach;
-        float w[kEach];
-        uint32_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            w[j] = i + j < end ? from[i + j] : 0.0f;
-            const uint32_t o = order_of(w[j]);
-            if (i + j < end) mine += o > key ? 1u : o == key ? 1u << 16 : 0u;
-        }
-        uint32_t total;
-        const uint32_t before = ahead_of(mine, lds, total);
-        uint32_t big = larger + (before & 0xffff), same = equal + (before >> 16);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            if (i + j >= end) continue;
-            const uint32_t o = order_of(w[j]);
-            if (o > key || (o == key && same < left)) {
-                const int place = c.first + static_cast<int>(big + min(same, left));
-                list[place] = i + j;
-                to[place] = w[j];
-            }
-            big += o > key;
-            same += o == key;
-        }
-        larger += total & 0xffff;
-        equal += total >> 16;
-    }
+    const auto each = [&](int place, int token, float weight) {
+        list[place] = token;
+        to[place] = weight;
+    };
+    if (held)
+        choose<true>(from, c.first, end, want, w, lds, each);
+    else
+        choose<false>(from, c.first, end, want, w, lds, each);
 }
 
 struct MoveSet {
@@ -230,9 +318,11 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(const Evict p, const 
         return;
     }
     if (keep <= 0) return;
+    // where the tokens of three rounds lie, and go: read, written, looked up
+    __shared__ int64_t from[3][kTokens], to[3][kTokens];
     const int head = blockIdx.y / set.pieces, piece = blockIdx.y - head * set.pieces;
     const int token_of = set.columns.quotient(tid), column = tid - token_of * set.width;
-    const int tokens = kMoveThreads / set.width;  // of a round and read
+    const int tokens = min(kMoveThreads / set.width, kMoveThreads / kLeastWidth), round = tokens * kAtOnce;
     const int64_t byte = (static_cast<int64_t>(piece) * set.width + column) * 16, left = set.part - byte;
     const bool mine = token_of < tokens && left > 0;
     const int64_t row = (static_cast<int64_t>(set.weights[blockIdx.z]) * p.t.S + s) * p.heads + head;
@@ -241,26 +331,54 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(const Evict p, const 
     const int32_t* const pages = p.t.pages + static_cast<int64_t>(s) * p.t.span.P;
     const auto place = [&](int token) {
         const int c = static_cast<int>(p.t.span.page.quotient(token));
-        return base + pages[c] * set.page_stride + (token - c * static_cast<int>(p.t.span.page.d)) * set.token_stride;
+        return pages[c] * set.page_stride + (token - c * static_cast<int>(p.t.span.page.d)) * set.token_stride;
     };
-    for (int64_t j0 = 0; j0 < keep; j0 += tokens * kAtOnce) {
-        u32x4 x[kAtOnce];
-        int source[kAtOnce];
+    const auto look_up = [&](int buffer, int64_t j0) {
+        for (int i = tid; i < round; i += kMoveThreads) {
+            const int64_t j = j0 + i;
+            const int source = j < keep ? list[j] : -1;
+            const bool moves = source >= 0 && source != j;
+            from[buffer][i] = moves ? place(source) : -1;
+            to[buffer][i] = moves ? place(static_cast<int>(j)) : -1;
+        }
+    };
+    u32x4 x[2][kAtOnce];
+    const auto read = [&](auto which, int buffer) {
+        constexpr int w = decltype(which)::value;
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const int64_t j = j0 + i * tokens + token_of;
-            source[i] = mine && j < keep ? list[j] : -1;
-            if (source[i] == j) source[i] = -1;  // stays where it is
+            const int64_t at = mine ? from[buffer][i * tokens + token_of] : -1;
+            if (at >= 0) x[w][i] = load16(base + at, left);
         }
+    };
+    const auto write = [&](auto which, int buffer) {
+        constexpr int w = decltype(which)::value;
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (source[i] >= 0) x[i] = load16(place(source[i]), left);
-        // all reads of the round are done before its writes
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t at = mine ? to[buffer][i * tokens + token_of] : -1;
+            if (at >= 0) store16(base + at, x[w][i], left);
+        }
+    };
+    look_up(0, 0);
+    look_up(1, round);
+    __syncthreads();
+    read(std::integral_constant<int, 0>{}, 0);
+    int buffer = 0;
+    const auto step = [&](int64_t j0, auto which) {
+        constexpr int w = decltype(which)::value;
+        const int next = buffer == 2 ? 0 : buffer + 1, last = next == 2 ? 0 : next + 1;
+        // all reads of the round are done before its writes; the next round's, of later tokens,
+        // lie behind what these write
         __builtin_amdgcn_s_waitcnt(0x0070);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (source[i] >= 0) store16(place(static_cast<int>(j0) + i * tokens + token_of), x[i], left);
+        if (j0 + round < keep) read(std::integral_constant<int, 1 - w>{}, next);
+        write(which, buffer);
+        if (j0 + 2 * round < keep) look_up(last, j0 + 2 * round);
+        buffer = next;
+    };
+    for (int64_t j0 = 0; j0 < keep; j0 += 2 * round) {
+        step(j0, std::integral_constant<int, 0>{});
+        if (j0 + round < keep) step(j0 + round, std::integral_constant<int, 1>{});
     }
 }
 
@@ -365,10 +483,11 @@ DBS_CUDA_EXPORT int beamgrad_evict_tokens(const BeamgradPools* pools, const Beam
             set.weights[set.n] = j / (pools->n / a.n_weights);
             ++set.n;
         }
-        // 256 bytes of a token for a workgroup; where those are few, 64
+        // 128 bytes of a token for a workgroup (a line of the cache; with 256 the call of many
+        // layers took 909 us, with 128 889); where those are few, 64
         const int64_t columns = (set.part + 15) / 16;
-        int64_t width = std::min<int64_t>(columns, 16);
-        while (width > 4 && static_cast<int64_t>(sequences) * set.n * a.heads * ((columns + width - 1) / width) < 1024) width /= 2;
+        int64_t width = std::min<int64_t>(columns, 8);
+        while (width > kLeastWidth && static_cast<int64_t>(sequences) * set.n * a.heads * ((columns + width - 1) / width) < 1024) width /= 2;
         set.width = static_cast<int32_t>(width);
         set.columns = Divider::of(static_cast<uint32_t>(width));
         set.pieces = static_cast<int32_t>((columns + width - 1) / width);
