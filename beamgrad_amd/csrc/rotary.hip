@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 1024;        // of a head
-constexpr int64_t kMostTokens = int64_t{1} << 26;  // of a call: a launch has 2^32 threads
+constexpr int64_t kMostTokens = int64_t{1} << 26;      // of a call
+constexpr int64_t kTokensOfLaunch = int64_t{1} << 24;  // a launch has fewer than 2^32 threads
 constexpr int64_t kMostStride = int64_t{1} << 40;
 constexpr int kTensorsOfLaunch = 16;  // whose addresses one launch's arguments hold
 
@@ -45,7 +46,7 @@ struct Turn {
     const int32_t* counts;
     int64_t position_stride[2];  // in elements
     Divider tokens, pairs;       // tokens of a sequence, pairs of a head
-    int64_t all;                 // tokens of the call
+    int64_t first, all;          // the launch's first token, and the end of its tokens
     float scale;
     bool i64, inverse, inplace;
 };
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Turn p) {
     extern __shared__ float2 units[];  // [TOKENS][pairs]
     __shared__ bool live[TOKENS];
     const Heads& h = p.of[blockIdx.y];
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * TOKENS;
+    const int64_t first = p.first + static_cast<int64_t>(blockIdx.x) * TOKENS;
     const int here = static_cast<int>(min(p.all - first, static_cast<int64_t>(TOKENS))), pairs = p.pairs.d;
     const auto place = [&](int t, int64_t& s) {
         const uint32_t token = static_cast<uint32_t>(first + t), of = p.tokens.quotient(token);
@@ -238,20 +239,26 @@ bool lie_apart(const BeamgradRotary& a) {
 }
 
 template <class T, int PAIRS, bool INTERLEAVED>
-void launch(const Turn& p, int tensors, hipStream_t stream) {
+void launch(Turn& p, int tensors, hipStream_t stream) {
     // Two tokens a workgroup give every thread work between the table and the end, one
     // gives few tokens more workgroups. 2103 tokens of 20 heads of 72, float32: 9.5 us with
     // one, 7.9 with two, 9.6 with four; 16384 of 40 heads of 128, bfloat16: 62 with two or four.
     constexpr int64_t many = 512;
     const size_t table = p.pairs.d * sizeof(float2);
-    if (p.all >= many)
-        rotary_kernel<T, PAIRS, INTERLEAVED, 2><<<dim3(static_cast<unsigned>((p.all + 1) / 2), tensors), kThreads, 2 * table, stream>>>(p);
-    else
-        rotary_kernel<T, PAIRS, INTERLEAVED, 1><<<dim3(static_cast<unsigned>(p.all), tensors), kThreads, table, stream>>>(p);
+    const int64_t all = p.all;
+    for (p.first = 0; p.first < all; p.first += kTokensOfLaunch) {
+        p.all = std::min(all, p.first + kTokensOfLaunch);
+        const int64_t here = p.all - p.first;
+        if (all >= many)
+            rotary_kernel<T, PAIRS, INTERLEAVED, 2><<<dim3(static_cast<unsigned>((here + 1) / 2), tensors), kThreads, 2 * table, stream>>>(p);
+        else
+            rotary_kernel<T, PAIRS, INTERLEAVED, 1><<<dim3(static_cast<unsigned>(here), tensors), kThreads, table, stream>>>(p);
+    }
+    p.all = all;
 }
 
 template <class T, int PAIRS>
-void launch_layout(const Turn& p, bool interleaved, int tensors, hipStream_t stream) {
+void launch_layout(Turn& p, bool interleaved, int tensors, hipStream_t stream) {
     if (interleaved)
         launch<T, PAIRS, true>(p, tensors, stream);
     else
@@ -259,7 +266,7 @@ void launch_layout(const Turn& p, bool interleaved, int tensors, hipStream_t str
 }
 
 template <class T>
-void launch_pairs(const Turn& p, int each, bool interleaved, int tensors, hipStream_t stream) {
+void launch_pairs(Turn& p, int each, bool interleaved, int tensors, hipStream_t stream) {
     if (each == 8) {
         if constexpr (sizeof(T) == 2) launch_layout<T, 8>(p, interleaved, tensors, stream);
     } else if (each == 4) {

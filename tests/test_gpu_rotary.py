@@ -138,6 +138,18 @@ def test_many_tensors_of_one_call():
     assert bg.rotary([], at.cuda(), f.cuda()) == []
 
 
+def test_more_tokens_than_a_launch_has():
+    """Every stretch of them alike: tokens at launches' edges, and the last."""
+    n = (1 << 25) + 777
+    at = torch.arange(n, device="cuda", dtype=torch.int32).view(1, n)
+    x = torch.randn(1, n, 1, 2, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0)).to(torch.bfloat16)
+    f = torch.tensor([0.37], dtype=torch.float64)
+    got, = bg.rotary([x], at, f.cuda())
+    for edge in (0, 1 << 24, (1 << 24) + 777, 1 << 25, n):
+        part = slice(max(0, edge - 50), edge + 50)
+        near(got[:, part], ref.rotary(x[:, part].cpu(), at[:, part].cpu(), f, False, 1.0))
+
+
 def test_memory_that_meets_is_refused():
     at, f = positions_of(2, 3, 0).cuda(), frequencies(8).cuda()
     x = torch.zeros(2, 3, 4, 8, device="cuda")
