@@ -332,7 +332,9 @@ void accumulate_weights_hip(const Tensor& weights, const Tensor& q, const Tensor
     const int64_t bytes = beamgrad_accumulate_weights_workspace_size(&a);
     Tensor ws;
     if (bytes != 0) ws = workspace(bytes, q);
-    check_status(beamgrad_accumulate_weights(&a, bytes != 0 ? ws.data_ptr() : nullptr, bytes, current_stream()), "accumulate_weights");
+    const int status = beamgrad_accumulate_weights(&a, bytes != 0 ? ws.data_ptr() : nullptr, bytes, current_stream());
+    TORCH_CHECK_VALUE(status != DBS_CUDA_STATUS_INVALID_ARGUMENT, "weights must share no memory with q, k or lse");
+    check_status(status, "accumulate_weights");
     written({weights});
 }
 

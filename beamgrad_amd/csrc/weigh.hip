@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 #include <type_traits>
 
 #include "attend.hpp"
@@ -26,6 +27,7 @@
 #include "engine.hpp"
 #include "matrix.hpp"
 #include "paged.hpp"
+#include "regions.hpp"
 #include "rows.hpp"
 
 using namespace dbs_hip;
@@ -648,6 +650,17 @@ Form form_of(const BeamgradWeights& a) {
 
 int64_t places_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.table_pages) * a.page_tokens; }
 
+// The weights are written while queries, keys and log-sums are read.
+bool lies_apart(const BeamgradWeights& a) {
+    const int64_t size = element_size(a.data_type), *q = a.q_strides, *k = a.k_strides, *w = a.weight_strides, wide = sizeof(float);
+    const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+    const Region weights{at(a.weights), {a.sequences, a.kv_heads}, {w[0] * wide, w[1] * wide}, places_of(a) * wide};
+    const Region read[] = {{at(a.q), {a.sequences, a.tokens}, {q[0] * size, q[1] * size}, ((a.heads - 1) * q[2] + a.head_dim) * size},
+                           {at(a.k), {a.n_pages, a.page_tokens}, {k[0] * size, k[1] * size}, ((a.kv_heads - 1) * k[2] + a.head_dim) * size},
+                           {at(a.lse), {1, 1}, {0, 0}, static_cast<int64_t>(a.sequences) * a.tokens * a.heads * wide}};
+    return std::all_of(std::begin(read), std::end(read), [&](const Region& r) { return apart(weights, r); });
+}
+
 int64_t rows_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads); }
 
 // Workgroups of a launch, a multiple of eight. The card holds three of many rows on a CU
@@ -692,7 +705,7 @@ DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, voi
     const BeamgradWeights& a = *args;
     const int64_t bytes = beamgrad_accumulate_weights_workspace_size(args);
     if (!a.q || !a.k || !a.pages || !a.lengths || !a.lse || !a.weights || !aligned16(a.q) || !aligned16(a.k) || bytes < 0 ||
-        (bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < bytes)))
+        (bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < bytes)) || !lies_apart(a))
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Form form = form_of(a);
     const int64_t size = element_size(a.data_type);

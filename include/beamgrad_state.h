@@ -220,7 +220,7 @@ DBS_CUDA_EXPORT int beamgrad_rotary(const BeamgradRotary* args, void* stream);
  * without a page, and places past a sequence's length, keep what they have. A row whose
  * lse is -inf gives nothing. lse [S, N, H] is what beamgrad_tree_attention leaves,
  * contiguous; weights [S, Hkv, ...] has weight_strides (elements) and room for
- * table_pages * page_tokens places, contiguous. */
+ * table_pages * page_tokens places, contiguous, and shares no memory with q, k or lse. */
 typedef struct BeamgradWeights {
     const void* q;
     const void* k;

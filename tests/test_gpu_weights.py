@@ -144,6 +144,20 @@ def test_strides_of_weights_queries_and_cache():
             assert torch.equal(w, want)
 
 
+def test_memory_that_meets_is_refused():
+    """Weights in a part of the queries, keys or log-sums; between two of the cache's rows they fit."""
+    table = bg.PageTable(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.full((1,), 4, dtype=torch.int32, device="cuda"),
+                         torch.ones(1, dtype=torch.int32, device="cuda"))
+    buffer = torch.zeros(1 << 10, device="cuda")
+    q, lse, k = buffer[:16].view(1, 1, 2, 8), buffer[64:66].view(1, 1, 2), buffer[128:192].view(1, 4, 1, 16)[..., :8]
+    for at in (8, 62, 130):
+        with pytest.raises(ValueError, match="share no memory"):
+            bg.accumulate_weights(buffer[at:at + 4].view(1, 1, 4), q, k, lse, table)
+    weights = buffer[136:140].view(1, 1, 4)
+    bg.accumulate_weights(weights, q, k, lse, table)
+    assert torch.equal(weights.cpu(), torch.tensor([[[2.0, 2.0, 2.0, 2.0]]]))  # e^(0 - 0), of two heads
+
+
 def test_the_same_every_time_and_captured():
     p = problem(torch.bfloat16, 2, 300, 4, 2, 64, 16, [400, 333])
     pages, lengths, refs = (t.cuda() for t in p["table"])
