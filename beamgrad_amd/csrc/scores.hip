@@ -16,8 +16,9 @@
 // lies with the threads whose own maximum does: little more than `top` threads, whose shares (a few hundred values of a large
 // vocabulary) are read again, from the cache. What they hold beside the alternatives
 // is little (20 of 151936 at random: one or two), unless values are equal
-// in great number: where more than kKept reach it, or fewer than `top` do (-inf),
-// the alternatives are found one after the other.
+// in great number: where more than kKept reach it, the alternatives are found one after the
+// other. Where fewer than `top` do, all that are above -inf have, and the first
+// ones at -inf follow.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,6 +28,7 @@
 #include "beamgrad_score.h"
 #include "engine.hpp"
 #include "paged.hpp"
+#include "regions.hpp"
 #include "rows.hpp"
 
 using namespace dbs_hip;
@@ -112,6 +114,11 @@ __device__ __forceinline__ void values_at(const char* row, int v, int V, float* 
     __builtin_memcpy(e, &raw, 16);
 #pragma unroll
     for (int i = 0; i < kEach<T>; ++i) x[i] = v + i < V ? static_cast<float>(e[i]) : -__builtin_inff();
+}
+
+template <class T>
+__device__ __forceinline__ float value_at(const char* row, int v) {
+    return static_cast<float>(reinterpret_cast<const T*>(row)[v]);
 }
 
 template <bool ENTROPY>
@@ -337,13 +344,19 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
     }
     __syncthreads();
     const int n = lds.kept, all = min(top, to - from);
-    if (n >= all && n <= kKept) {
+    if (n <= kKept) {
         if (tid < 8) lds.keys[n + tid] = 0;
         __syncthreads();
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t key = lds.keys[i];
             const int above = larger_of(lds.keys, n, key);
             if (above < top) each(above, key);
+        }
+        if (n < all && tid < 64) {  // of the first `all` places at most n are not at -inf
+            const float x = tid < all ? value_at<T>(row, from + tid) : 0.0f;
+            const uint64_t none = __ballot(x == -__builtin_inff());
+            const int at = n + __popcll(none & ((uint64_t{1} << tid) - 1));
+            if (x == -__builtin_inff() && at < all) each(at, key_of(x, from + tid));
         }
     } else {
         // one after the other: the largest below the last one
@@ -376,11 +389,6 @@ __device__ __forceinline__ Normal normal_of(const Sums& a) {
     const bool empty = a.s == 0.0f;
     const float log_s = logf(a.s);
     return {a.m, log_s, empty ? 0.0f : log_s - a.t / a.s, empty};
-}
-
-template <class T>
-__device__ __forceinline__ float value_at(const char* row, int v) {
-    return static_cast<float>(reinterpret_cast<const T*>(row)[v]);
 }
 
 // What one thread writes of a row, whose token's logit is x.
@@ -624,6 +632,12 @@ bool valid_sizes(const BeamgradTokenLogprobs* a) {
            a->vocab <= 1 << 30 && a->top >= 0 && a->top <= kMaxTop && a->top <= a->vocab && a->strides[0] >= 0 && a->strides[1] >= 0;
 }
 
+Region region_of(const void* at, int64_t bytes) { return {reinterpret_cast<uintptr_t>(at), {1, 1}, {0, 0}, bytes}; }
+Region logits_of(const BeamgradTokenLogprobs& a) {
+    const int size = element_size(a.data_type);
+    return {reinterpret_cast<uintptr_t>(a.logits), {a.outer, a.inner}, {a.strides[0] * size, a.strides[1] * size}, static_cast<int64_t>(a.vocab) * size};
+}
+
 Rows rows_of(const BeamgradTokenLogprobs& a) {
     const int size = element_size(a.data_type);
     return {static_cast<const char*>(a.logits), a.strides[0] * size, a.strides[1] * size, Divider::of(static_cast<uint32_t>(a.inner)),
@@ -742,7 +756,8 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs_backward(const BeamgradTokenLogprobs
     // 32 KB of a row for a workgroup
     const int part = part_values(p.V, static_cast<int>(std::max<int64_t>(1, static_cast<int64_t>(p.V) * size / (32 * 1024))), size);
     const int64_t parts = (p.V + part - 1) / part;
-    if (rows * parts >= int64_t{1} << 24) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
+    if (rows * parts >= int64_t{1} << 24 || !apart(region_of(grad_logits, rows * p.V * size), logits_of(*args)))
+        return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Grads g{grad_logprobs, grad_entropy, grad_top, static_cast<char*>(grad_logits)};
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     by_type(args->data_type, grad_entropy != nullptr, is_stream(rows, p.V, size), is_short(p.V, size),

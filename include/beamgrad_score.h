@@ -32,7 +32,8 @@ extern "C" {
  * top_logprobs -inf, top_tokens -1. A row of -inf alone (nothing is possible):
  * logprobs -inf, entropy 0, top_logprobs -inf. A row that holds NaN or +inf: NaN,
  * top_tokens -1. Sums are held in 32 bits. vocab is at most 2^30, top at most 64 and
- * at most vocab, rows fewer than 2^24. */
+ * at most vocab, rows fewer than 2^24. What is written shares no memory with what is
+ * read. */
 typedef struct BeamgradTokenLogprobs {
     const void* logits;
     int32_t data_type; /* DBS_CUDA_DTYPE_F32, _F16 or _BF16 */
@@ -63,7 +64,8 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs(const BeamgradTokenLogprobs* args, v
  * A = g + sum_j g_j over the row's alternatives j and H its entropy,
  *   grad_v = -p_v (A + g_H (log p_v + H)) + [v = t] g + sum_j [v = top_j] g_j,
  * computed in 32 bits and rounded once; zeros where the row was not read or nothing
- * in it is possible, NaN where it holds NaN or +inf. */
+ * in it is possible, NaN where it holds NaN or +inf. In the logits' own place it is
+ * refused. */
 DBS_CUDA_EXPORT int beamgrad_token_logprobs_backward(const BeamgradTokenLogprobs* args, const float* grad_logprobs,
                                                      const float* grad_entropy, const float* grad_top, void* grad_logits,
                                                      void* stream);

@@ -112,6 +112,18 @@ def test_alternatives_of_one_thread():
         check(logits, tokens, 40)
 
 
+@pytest.mark.parametrize("top", [1, 6, 64])
+@pytest.mark.parametrize("V, rows", [(100, 9), (20000, 9), (20000, 1030)])
+def test_alternatives_of_few_possible_tokens(V, rows, top):
+    """Fewer of a row (and of most of its parts) are above -inf than are asked for."""
+    logits, tokens = inputs((rows,), V, torch.bfloat16, 5)
+    tokens[9:] = -1
+    for r in range(9):
+        logits[r, torch.randperm(V, generator=torch.Generator().manual_seed(r))[:V - 3 * r]] = -math.inf
+    logits[8, :70], logits[7, 1:90:2] = 1.5, torch.finfo(torch.bfloat16).min
+    check(logits, tokens, top, True, grads_of((rows,), top, 5))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V, rows", [(100, 9), (3000, 9), (30000, 9), (3000, 1030)])
 def test_masked_and_invalid_rows(dtype, V, rows):

@@ -261,6 +261,9 @@ int main(void) {
     a.data_type = 2; a.outer = 1 << 20; a.inner = 16; CHECK(beamgrad_token_logprobs_workspace_size(&a) == -1);
     a.outer = 1; a.strides[0] = -1; CHECK(beamgrad_token_logprobs_workspace_size(&a) == -1);
     a.strides[0] = 0; CHECK(beamgrad_token_logprobs_backward(&a, 0, 0, 0, room, 0) == BAD); /* no stats */
+    a.inner = 1; a.vocab = 1000; a.stats = (float*)(room + 8192); a.tokens = room + 8448;
+    CHECK(beamgrad_token_logprobs_backward(&a, 0, 0, 0, room, 0) == BAD); /* the gradient in the logits' place */
+    CHECK(beamgrad_token_logprobs_backward(&a, 0, 0, 0, room + 1998, 0) == BAD);
     /* rotary */
     const void* from[2] = {room, room + 4096}; void* to[2] = {room + 8192, room + 16384};
     int32_t heads[2] = {2, 1}, dims[2] = {16, 16}; int64_t st[6] = {96, 32, 16, 48, 16, 16}; double f[8];
@@ -276,13 +279,19 @@ int main(void) {
     st[0] = 96; r.tokens = 1 << 26; CHECK(beamgrad_rotary(&r, 0) == BAD);
     /* weights */
     BeamgradWeights w; memset(&w, 0, sizeof w);
-    w.q = w.k = room; w.pages = w.lengths = (int32_t*)room; w.lse = (float*)room; w.weights = (float*)room; w.data_type = 1; w.sequences = 2; w.tokens = 600;
+    static char far[1 << 25] __attribute__((aligned(16))); /* keys, queries, log-sums, weights */
+    w.k = far; w.q = far + (1 << 20); w.lse = (float*)(far + (1 << 22)); w.weights = (float*)(far + (1 << 23)); w.pages = w.lengths = (int32_t*)room; w.data_type = 1; w.sequences = 2; w.tokens = 600;
     w.heads = 4; w.kv_heads = 2; w.head_dim = 64; w.page_tokens = 16; w.n_pages = 100; w.table_pages = 40; w.scale = 0.125f;
     w.q_strides[0] = 153600; w.q_strides[1] = 256; w.q_strides[2] = 64; w.k_strides[0] = 2048; w.k_strides[1] = 128; w.k_strides[2] = 64;
     w.weight_strides[0] = 1280; w.weight_strides[1] = 640;
     CHECK(beamgrad_accumulate_weights_workspace_size(&w) > 0); /* many rows over few keys */
     CHECK(beamgrad_accumulate_weights_workspace_size(&w) <= 16 << 20);
     CHECK(beamgrad_accumulate_weights(&w, 0, 0, 0) == BAD);
+    const int64_t bytes = beamgrad_accumulate_weights_workspace_size(&w);
+    for (int i = 0; i < 3; ++i) { /* weights in keys, queries, log-sums */
+        w.weights = (float*)(far + (i == 0 ? 400000 : i == 1 ? (1 << 20) + 500000 : (1 << 22) - 256));
+        CHECK(beamgrad_accumulate_weights(&w, far + (1 << 24), bytes, 0) == BAD);
+    }
     w.parents = (int32_t*)room; CHECK(beamgrad_accumulate_weights_workspace_size(&w) == -1); /* a tree of 600 */
     w.parents = 0; w.weight_strides[1] = 639; CHECK(beamgrad_accumulate_weights_workspace_size(&w) == -1);
     w.weight_strides[0] = 640; w.weight_strides[1] = 1280; CHECK(beamgrad_accumulate_weights_workspace_size(&w) > 0);
