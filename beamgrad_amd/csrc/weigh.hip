@@ -189,6 +189,9 @@ __device__ __forceinline__ void see(const Weigh& p, int s, int count, int16_t* u
 // ---------------------------------------------------------------------------
 
 // Line: 64 keys each, of a sequence's cache heads one after the other, of the sequences.
+// Each wavefront has its own 16 keys of them and several such blocks' reads on their way, so
+// that nothing waits for the others. 32 single tokens over caches of 2000 to 16000, 8 heads
+// of 128 in bfloat16: 124 us, 621 MB, 5.0 TB/s.
 // ONE: the rows are one block, and lie in registers.
 template <int DTYPE, int DP, bool ONE>
 __global__ __launch_bounds__(kThreads, (Dims<DTYPE, DP>::kFewResident)) void weigh_few(const Weigh p) {
@@ -326,7 +329,14 @@ __global__ __launch_bounds__(kThreads, (Dims<DTYPE, DP>::kFewResident)) void wei
 
 // Line: blocks of 16 rows, of a sequence's tiles of keys one after the other, of the
 // sequences, of the cache heads. Rows of tokens ahead of a tile's first key see none of
-// it, and are not in the line.
+// it, and are not in the line. 64 keys stay with a wavefront, so that a block of queries
+// that is read from LDS serves 16 matrix instructions of width 128; a score costs the vector
+// unit a product, an exponential and a sum. Two prompts' ends of 512 tokens over 7700 and
+// 15100 of 32 heads of 128 in bfloat16: 143 us, 99 GFLOP, 650 to 690 TFLOP/s; with 2048
+// over 16000 in eight 820. The vector unit is busy for 64 % of the time and the matrix unit for
+// 36 %: they take turns, and with constant operands, which take less power, the 820
+// are 990. Queries read a block ahead, blocks without a loop and raised priority around
+// the products changed nothing.
 template <int DTYPE, int DP>
 __global__ __launch_bounds__(kThreads, 3) void weigh_many(const Weigh p) {
     using E = Elem<DTYPE>;
@@ -577,7 +587,8 @@ __global__ __launch_bounds__(kThreads, 3) void weigh_many(const Weigh p) {
     }
 }
 
-// x: a stretch that ends a tile which others began: what they have of it, in order.
+// x: a stretch that ends a tile which others began: what they have of it, in order. 5 us, most
+// of it a launch and three dependent reads.
 __global__ __launch_bounds__(kThreads) void weigh_join(const Weigh p, const int tile) {
     const Piece piece = p.pieces[blockIdx.x];
     if (piece.first < 0) return;

@@ -176,7 +176,7 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states_backward(const void* const* from, vo
  * values 2 f and 2 f + 1 with `interleaved`, f and pairs + f without; with `inverse`
  * by the angles' negatives, which is the gradient. The rest of a head is copied. Tokens
  * n >= counts[s] (counts may be NULL) become zeros, or stay as they are in place. Angles
- * are computed in 64 bits, at positions of any sign.
+ * are computed in 64 bits: their sines and cosines are good to 32 up to 2^50, of either sign.
  *
  * from, to, heads, head_dim and the strides are host arrays, read before the call
  * returns; strides are of sequences, tokens and heads (three for each tensor), in

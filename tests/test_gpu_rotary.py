@@ -2,6 +2,7 @@
 """Rotary positions on the GPU against a 64-bit restatement."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -69,6 +70,38 @@ def test_far_positions(far, base):
     for index in (at, at.int()) if far < 2**31 else (at,):
         got, = bg.rotary([x.cuda()], index.cuda(), f.cuda())
         assert ((got.cpu().double() - out).abs() <= bound).all()
+
+
+def test_the_farthest_angles():
+    """Angles up to 2^50, against a remainder by exact arithmetic: the quarter turns are counted
+    within 0.17 there, so what is left stays below 1.05, where the sums' first omitted terms
+    are below a half step of 1; 2 half steps beside that, and those of the product."""
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798")
+    at = [2**50, -(2**50), 2**50 - 1, 2**49 + 12345, 3 * 2**48 + 7, 10**15]
+    f = [1.0, 1.0 - 2.0**-53, 0.7310585786300049, 2.0**-30 * 1.1]
+    x = torch.zeros(1, len(at), 1, 2 * len(f))
+    x[..., :len(f)] = 1.0
+    got, = bg.rotary([x.cuda()], torch.tensor([at], device="cuda"), torch.tensor(f, dtype=torch.float64, device="cuda"))
+    for i, position in enumerate(at):
+        for j, frequency in enumerate(f):
+            angle = float((position * Fraction(frequency) + pi) % (2 * pi) - pi)
+            for value, want in ((got[0, i, 0, j], math.cos(angle)), (got[0, i, 0, len(f) + j], math.sin(angle))):
+                assert abs(float(value) - want) <= 4 * ref.STEP, (position, frequency)
+
+
+def test_a_capture_that_reaches_a_leaf_of_another_graph_is_refused():
+    """The question that the capture's refusal asks, outside a capture."""
+    at, f = positions_of(1, 2, 0).cuda(), frequencies(8).cuda()
+    leaf = torch.randn(1, 2, 1, 8, device="cuda").requires_grad_(True)
+    alive = bg.rotary([leaf * 2], at, f)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        out, = bg.rotary([leaf * 2], at, f)
+        assert torch.ops.beamgrad.backward_reaches_leaf_of_another_stream(out)
+        del alive, out
+        assert not torch.ops.beamgrad.backward_reaches_leaf_of_another_stream(bg.rotary([leaf], at, f)[0])
+    torch.cuda.synchronize()
 
 
 def test_scale_counts_and_index_types():
