@@ -36,6 +36,7 @@ using namespace dbs_hip;
 namespace {
 
 constexpr int kThreads = 256;  // of a row's workgroup; short rows: one wavefront
+constexpr int kManyThreads = 512;  // where rows are few
 constexpr int kAtOnce = 4;     // 16-byte reads of a thread in flight
 constexpr int kMaxTop = 64;
 constexpr int kKept = 512;     // values beside the alternatives that a workgroup ranks
@@ -289,8 +290,10 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
     constexpr int E = kEach<T>, WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63;
     if (tid == 0) lds.flags = lds.kept = 0;
-    // of each wavefront's maxima as many as make `top` together: the lowest of these
-    const int wanted = (top + WAVES - 1) / WAVES;
+    // of each wavefront's maxima as many as make `top` together: the lowest of these. (Of
+    // wavefronts that have no full round, none: theirs may be no values. Without any that has one,
+    // all values are few enough.)
+    const int full = min(WAVES, (to - from) / (64 * E)), wanted = full > 0 ? (top + full - 1) / full : 1;
     if (wanted <= 16) {
         float left = mine, largest = wave_max(mine);
         for (int n = __popcll(__ballot(left == largest)); n < wanted; n += __popcll(__ballot(left == largest))) {
@@ -308,9 +311,9 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
         if (rank == wanted - 1) lds.floor[tid >> 6] = mine;
     }
     __syncthreads();
-    float floor = lds.floor[0];
+    float floor = full > 0 ? lds.floor[0] : -FLT_MAX;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) floor = fminf(floor, lds.floor[w]);
+    for (int w = 1; w < WAVES; ++w) floor = w < full ? fminf(floor, lds.floor[w]) : floor;
     const auto keep = [&](float x, int place) {
         if (place >= to || !(x >= floor)) return;
         const int at = atomicAdd(&lds.kept, 1);
@@ -419,9 +422,10 @@ __device__ __forceinline__ void write_none(const Rows& p, uint32_t r, bool bad) 
     }
 }
 
-// A workgroup for a row, where there are rows enough to fill the card; a wavefront for a
-// row of two rounds of its reads. Bound by HBM: some 3080 of 4096 rows of 128256 in
-// bfloat16 (the others have no token) in 129 us, 6.1 TB/s.
+// A workgroup for a row; a wavefront for a row of two rounds of its reads. Bound by HBM
+// where the rows fill the card: some 3080 of 4096 of 128256 in bfloat16 (the others have
+// no token) in 129 us, 6.1 TB/s; 490 of 660 of 50257 in float16, with the entropy and 4
+// alternatives, in 21 us. Few rows: latency, 4 of 32000 in float32 with 5 alternatives 7.1 us.
 template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
     __shared__ Shared<THREADS> lds;
@@ -440,10 +444,8 @@ __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
 }
 
 // x: a part of `part` values of row y. Sums and alternatives go to the workspace.
-// Bound by latency where rows are few: the read, the wavefronts' maxima, the ranking.
-// 4 rows of 32000 in float32 with 5 alternatives 5.0 us, 32 of 151936 in bfloat16 with
-// 20 alternatives 9.4 us (the bytes alone 0.1 and 1.9; a launch that does nothing takes 2 to 3); some 490 of
-// 50257 in float16, with the entropy, 19.9 us.
+// Bound by latency: the read, the wavefronts' maxima, the ranking. 32 rows of 151936 in
+// bfloat16 with 20 alternatives 9.4 us (the bytes alone 1.9; a launch that does nothing 2 to 3).
 // With ONE a part is one round of the workgroup's reads, which stay in registers: they
 // begin while the token is still read, and are looked through for the alternatives.
 template <class T, bool ENTROPY, bool ONE>
@@ -490,8 +492,8 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
 
 // A workgroup joins the parts of a row. The parts' alternatives are in order: of the
 // j-th of each part, j * parts >= top, the lowest is reached by `top` of them, so
-// what lies below it is none. 3.6 us for 4 rows, 5.3 for 32 of 19 parts: latency of two
-// dependent reads and the ranking.
+// what lies below it is none. 32 rows of 19 parts: 5.2 us, of two dependent reads and the
+// ranking.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
     constexpr int kFirst = 4;  // keys of a thread that are read ahead
@@ -657,13 +659,24 @@ Rows rows_of(const BeamgradTokenLogprobs& a) {
 // A row of up to two rounds of a wavefront is one's work.
 bool is_short(int vocab, int size) { return static_cast<int64_t>(vocab) * size <= 2 * 64 * 16 * kAtOnce; }
 
-// Few rows are split, so that the card's 256 CUs have work; a part is 16 KB at
-// least (a round of a workgroup's reads).
+// Few long rows are split, so that the card's 256 CUs have work, in parts of 16 KB at
+// least (a round of a workgroup's reads); a second launch joins them. A workgroup to itself
+// is the sooner done the shorter the rows and the more there are of them. bfloat16 without
+// alternatives, us, split and whole: 16 rows of 32000 6.5, 6.3; of 50257 6.6, 7.2; 64 rows
+// of 50257 8.1, 7.9; of 100000 9.3, 9.9; 130 of 100000 11.9, 10.2; 1000 of 100000 49.1, 39.6.
 int parts_of(const BeamgradTokenLogprobs& a) {
     constexpr int64_t kWanted = 1024, kLeast = kThreads * 16 * kAtOnce;
     const int64_t rows = static_cast<int64_t>(a.outer) * a.inner, bytes = static_cast<int64_t>(a.vocab) * element_size(a.data_type);
-    if (rows >= kWanted || is_short(a.vocab, element_size(a.data_type))) return 1;
+    if (a.vocab <= 40000 || rows * 1000 >= a.vocab) return 1;
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(kWanted + rows - 1) / rows, (bytes + kLeast - 1) / kLeast, kMaxParts})));
+}
+
+// Threads of a row's workgroup. Where the rows do not fill the card by themselves, 512 have
+// more of a row on its way: 200 rows of 64000 in bfloat16 8.9 us, 10.0 with 256; 600 rows
+// 20.7, 18.8.
+int threads_of_row(int64_t rows, int vocab, int size) {
+    if (is_short(vocab, size)) return 64;
+    return rows < 400 && static_cast<int64_t>(vocab) * size > 32 * 1024 ? kManyThreads : kThreads;
 }
 
 // Values of a part: whole rounds of a workgroup's reads.
@@ -681,12 +694,14 @@ bool is_stream(int64_t rows, int vocab, int size) { return rows * vocab * size >
 
 // launch(type, entropy, stream, threads)
 template <class Launch>
-void by_type(int data_type, bool entropy, bool stream, bool one_wave, Launch launch) {
+void by_type(int data_type, bool entropy, bool stream, int threads, Launch launch) {
     const auto sized = [&](auto t, auto e, auto s) {
-        if (one_wave)
+        if (threads == 64)
             launch(t, e, s, std::integral_constant<int, 64>{});
-        else
+        else if (threads == kThreads)
             launch(t, e, s, std::integral_constant<int, kThreads>{});
+        else
+            launch(t, e, s, std::integral_constant<int, kManyThreads>{});
     };
     const auto streamed = [&](auto t, auto e) {
         if (stream)
@@ -733,7 +748,7 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs(const BeamgradTokenLogprobs* args, v
     const bool entropy = args->entropy != nullptr;  // its gradient needs it too
     int parts = parts_of(*args);
     const int size = element_size(args->data_type), part = part_values(p.V, parts, size);
-    by_type(args->data_type, entropy, is_stream(rows, p.V, size), is_short(p.V, size), [&](auto t, auto with_entropy, auto streams, auto threads) {
+    by_type(args->data_type, entropy, is_stream(rows, p.V, size), threads_of_row(rows, p.V, size), [&](auto t, auto with_entropy, auto streams, auto threads) {
         using T = decltype(t);
         constexpr bool kEntropy = decltype(with_entropy)::value;
         constexpr int kOfRow = decltype(threads)::value;
@@ -770,9 +785,9 @@ DBS_CUDA_EXPORT int beamgrad_token_logprobs_backward(const BeamgradTokenLogprobs
         return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const Grads g{grad_logprobs, grad_entropy, grad_top, static_cast<char*>(grad_logits)};
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
-    by_type(args->data_type, grad_entropy != nullptr, is_stream(rows, p.V, size), is_short(p.V, size),
+    by_type(args->data_type, grad_entropy != nullptr, is_stream(rows, p.V, size), is_short(p.V, size) ? 64 : kThreads,
             [&](auto t, auto with_entropy, auto streams, auto threads) {
-        constexpr int kOfPart = decltype(threads)::value;
+        constexpr int kOfPart = std::min(decltype(threads)::value, kThreads);
         score_backward<decltype(t), decltype(with_entropy)::value, kOfPart, decltype(streams)::value>
             <<<static_cast<unsigned>(rows * parts), kOfPart, 0, stream>>>(p, g, Divider::of(static_cast<uint32_t>(parts)), part);
     });

@@ -63,7 +63,7 @@ def check(logits, tokens, top=0, entropy=False, grads=None, place=lambda t: t.cu
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [1, 2, 7, 63, 64, 65, 250, 1023, 2048, 4097, 9001, 50257])
+@pytest.mark.parametrize("V", [1, 2, 7, 63, 64, 65, 250, 1023, 2048, 4097, 9001, 20000, 49155, 50257])
 def test_rows_of_every_length(dtype, V):
     """Short rows (a wavefront), long ones, and split ones; odd lengths."""
     top = min(V, 5)
@@ -71,7 +71,7 @@ def test_rows_of_every_length(dtype, V):
     check(logits, tokens, top, True, grads_of((3, 2), top, V))
 
 
-@pytest.mark.parametrize("V, rows", [(40, 1100), (5000, 1030), (9001, 1), (30000, 33)])
+@pytest.mark.parametrize("V, rows", [(40, 1100), (5000, 1030), (9001, 1), (30000, 33), (10001, 420), (50257, 60), (70001, 33)])
 def test_few_and_many_rows(V, rows):
     logits, tokens = inputs((rows,), V, torch.bfloat16, rows)
     check(logits, tokens, 3, True, grads_of((rows,), 3, rows))
@@ -79,7 +79,7 @@ def test_few_and_many_rows(V, rows):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("top", [1, 2, 20, 63, 64])
-@pytest.mark.parametrize("V", [64, 700, 12000])
+@pytest.mark.parametrize("V", [64, 700, 12000, 49155])
 def test_alternatives(dtype, top, V):
     """Ties go to the lowest token: rounded logits hold many."""
     for ties in (False, True):
@@ -87,7 +87,7 @@ def test_alternatives(dtype, top, V):
         check(logits, tokens, top, False, [None, None, grads_of((4,), top, 3)[2]])
 
 
-@pytest.mark.parametrize("V, rows", [(300, 3), (20000, 3), (20000, 1100)])
+@pytest.mark.parametrize("V, rows", [(300, 3), (20000, 3), (50257, 3), (20000, 1100)])
 def test_alternatives_of_equal_logits(V, rows):
     """More equal values than a workgroup ranks, in the whole row and beside larger ones."""
     logits = torch.zeros(rows, V)
@@ -104,8 +104,8 @@ def test_alternatives_of_equal_logits(V, rows):
 
 def test_alternatives_of_one_thread():
     """The largest values all lie where one thread of a workgroup reads."""
-    for V in (2000, 20000):
-        logits, tokens = inputs((1030 if V > 10000 else 2,), V, torch.float32, 1)
+    for V, rows in ((2000, 2), (20000, 1030), (49155, 4)):
+        logits, tokens = inputs((rows,), V, torch.float32, 1)
         tokens[:-2] = -1
         for at in range(0, V, 1024):
             logits[:, at:at + 4] += 50.0
@@ -113,7 +113,7 @@ def test_alternatives_of_one_thread():
 
 
 @pytest.mark.parametrize("top", [1, 6, 64])
-@pytest.mark.parametrize("V, rows", [(100, 9), (20000, 9), (20000, 1030)])
+@pytest.mark.parametrize("V, rows", [(100, 9), (20000, 9), (50257, 9), (20000, 1030)])
 def test_alternatives_of_few_possible_tokens(V, rows, top):
     """Fewer of a row (and of most of its parts) are above -inf than are asked for."""
     logits, tokens = inputs((rows,), V, torch.bfloat16, 5)
@@ -125,7 +125,7 @@ def test_alternatives_of_few_possible_tokens(V, rows, top):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V, rows", [(100, 9), (3000, 9), (30000, 9), (3000, 1030)])
+@pytest.mark.parametrize("V, rows", [(100, 9), (3000, 9), (30000, 9), (49155, 9), (3000, 1030)])
 def test_masked_and_invalid_rows(dtype, V, rows):
     """-inf (some, all but a few, all), the type's lowest value, NaN, +inf, tokens out of range."""
     logits, tokens = inputs((rows,), V, dtype, 4)
@@ -279,7 +279,7 @@ def test_the_same_every_time_and_on_another_stream():
 def test_captured():
     """Forward and backward, replayed on new inputs; two graphs, in turns."""
     steps = []
-    for rows, V in ((3, 20000), (1100, 100)):
+    for rows, V in ((3, 20000), (3, 49155), (1100, 100)):
         x = torch.zeros(rows, V, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
         t = torch.zeros(rows, dtype=torch.int64, device="cuda")
         g = torch.zeros(rows, device="cuda")
