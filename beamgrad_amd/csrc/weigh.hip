@@ -9,9 +9,9 @@
 // their weights up, and a key's four lanes join at the end. Rows and their sums are in
 // a fixed order.
 //
-// Few rows (single tokens, small trees): the queries stay, in registers or LDS, and the
-// keys pass, several blocks of a wavefront on their way: bound by HBM. Many rows (the ends of
-// prompts): the keys stay, in registers, and the queries pass through LDS: bound by the
+// Few rows (single tokens, trees): the queries stay, in registers or LDS, and the keys pass,
+// several blocks of a wavefront on their way: bound by HBM, with more rows by LDS. Many rows (the
+// ends of prompts): the keys stay, in registers, and the queries pass through LDS: bound by the
 // exponentials and what surrounds them. Either way the call's work lies in one line, and each workgroup
 // takes an equal stretch of it, whatever the lengths (they are on the device, so the host
 // cannot plan with them).
@@ -54,6 +54,8 @@ struct Dims {
     static constexpr int kRows = kRowBytes >= 768 ? 16 : kRowBytes >= 384 ? 32 : 16384 / kRowBytes;
     static constexpr int kSwizzle = kChunks % 16 == 0 ? 15 : 7;
     static constexpr int kLoads = kRows * kChunks / kThreads;  // of a thread, for them
+    // And where keys pass more of them: 64 KB, and what the bits of a tree leave room for.
+    static constexpr int kMoreRows = kRowBytes <= 128 ? 384 : 65536 / kRowBytes / 32 * 32;
     // Keys that stay: blocks of 16 of a wavefront, 64 registers of a lane.
     static constexpr int kBlocks = kSteps >= 16 ? 1 : kSteps >= 6 ? 2 : kSteps >= 4 ? 4 : 8;
     static constexpr int kKeys = 16 * kBlocks;
@@ -191,14 +193,17 @@ __device__ __forceinline__ void see(const Weigh& p, int s, int count, int16_t* u
 // Line: 64 keys each, of a sequence's cache heads one after the other, of the sequences.
 // Each wavefront has its own 16 keys of them and several such blocks' reads on their way, so
 // that nothing waits for the others. 32 single tokens over caches of 2000 to 16000, 8 heads
-// of 128 in bfloat16: 124 us, 621 MB, 5.0 TB/s.
-// ONE: the rows are one block, and lie in registers.
-template <int DTYPE, int DP, bool ONE>
-__global__ __launch_bounds__(kThreads, (Dims<DTYPE, DP>::kFewResident)) void weigh_few(const Weigh p) {
+// of 128 in bfloat16: 124 us, 621 MB, 5.0 TB/s. Five trees of 45 tokens, 135 rows of width 72
+// in float16, over 300 to 2700: 12.8 us, most of it dependent reads (lengths, pages, keys) and
+// the rows' way into LDS.
+// ROWS: at most. 16 are one block, and lie in registers.
+template <int DTYPE, int DP, int ROWS>
+__global__ __launch_bounds__(kThreads, (ROWS > Dims<DTYPE, DP>::kRows ? 2 : Dims<DTYPE, DP>::kFewResident)) void weigh_few(const Weigh p) {
     using E = Elem<DTYPE>;
     using Frag = typename E::Frag;
     using X = Dims<DTYPE, DP>;
-    constexpr int STEPS = X::kSteps, ROWS = ONE ? 16 : X::kRows, AHEAD = X::kAhead, WORDS = ROWS / 32 > 0 ? ROWS / 32 : 1;
+    constexpr int STEPS = X::kSteps, AHEAD = X::kAhead, WORDS = ROWS / 32 > 0 ? ROWS / 32 : 1;
+    constexpr bool ONE = ROWS == 16;
     constexpr bool kHeld = ONE && STEPS <= 8;  // the queries fit registers
     constexpr float kInf = __builtin_inff();
     __shared__ __attribute__((aligned(16))) char queries[ROWS * X::kRowBytes];
@@ -261,12 +266,12 @@ __global__ __launch_bounds__(kThreads, (Dims<DTYPE, DP>::kFewResident)) void wei
             if (row < rows && c * 16 < bytes) x = *reinterpret_cast<const u32x4*>(q0 + token * p.qn + g * p.qh + c * 16);
             *reinterpret_cast<u32x4*>(queries + row * X::kRowBytes + (c ^ (row & X::kSwizzle)) * 16) = x;
         }
-        if (tid < ROWS) {
-            const int token = static_cast<int>(p.G.quotient(tid));
+        for (int row = tid; row < ROWS; row += kThreads) {
+            const int token = static_cast<int>(p.G.quotient(row));
             float l = -kInf;
-            if (tid < rows) l = p.lse[(static_cast<int64_t>(s) * p.N + token) * p.H + head * G + (tid - token * G)];
-            row_lse[tid] = l == -kInf ? l : -l * kLog2e;
-            row_token[tid] = l == -kInf ? kNone : token;
+            if (row < rows) l = p.lse[(static_cast<int64_t>(s) * p.N + token) * p.H + head * G + (row - token * G)];
+            row_lse[row] = l == -kInf ? l : -l * kLog2e;
+            row_token[row] = l == -kInf ? kNone : token;
         }
         if (p.parents) see(p, s, a.count, up, sees, WORDS, 0, a.count);
         __syncthreads();
@@ -633,33 +638,45 @@ bool valid_sizes(const BeamgradWeights* a) {
     return true;
 }
 
+int64_t places_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.table_pages) * a.page_tokens; }
+int64_t rows_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads); }
+
 struct Form {
-    int rows, tile, resident;  // few rows at most; keys of a tile of many; workgroups of a CU for few
-    const void *one, *few, *many;
+    const void* kernel;
+    bool many;
+    int tile, resident, rounds;  // keys of a tile of many; workgroups of a CU, and how often
 };
 template <int DTYPE, int DP>
-Form form_of_width() {
-    return {Dims<DTYPE, DP>::kRows, Dims<DTYPE, DP>::kTile, Dims<DTYPE, DP>::kFewResident, reinterpret_cast<const void*>(weigh_few<DTYPE, DP, true>),
-            reinterpret_cast<const void*>(weigh_few<DTYPE, DP, false>), reinterpret_cast<const void*>(weigh_many<DTYPE, DP>)};
+Form form_of_width(int64_t rows, int64_t passes) {
+    using X = Dims<DTYPE, DP>;
+    if (rows <= 16) return {reinterpret_cast<const void*>(weigh_few<DTYPE, DP, 16>), false, 0, X::kFewResident, 4};
+    if (rows <= X::kRows) return {reinterpret_cast<const void*>(weigh_few<DTYPE, DP, X::kRows>), false, 0, X::kFewResident, 4};
+    // More rows pass each key through more of LDS than keys that stay, but begin sooner and need no
+    // join: so up to this many matrix instructions of a wavefront altogether, and for wide heads,
+    // of whose keys few can stay, always. us, with 64 rows at most and with all of them: 135 rows
+    // of width 72 in float16 over 6 x 300 to 2700 21.6, 26; 180 of 128 in bfloat16 over one of 2700
+    // 15.9, 19.4, over 6 x 2700 to 8000 59.6, 55; 128 in float32 (8 steps) over 6 x 8000 108, 125.
+    if (rows <= X::kMoreRows && (X::kSteps >= 8 || passes * ((rows + 15) / 16) * X::kSteps <= 1 << 17))
+        return {reinterpret_cast<const void*>(weigh_few<DTYPE, DP, X::kMoreRows>), false, 0, 2, 1};
+    return {reinterpret_cast<const void*>(weigh_many<DTYPE, DP>), true, X::kTile, 3, 2};
 }
 template <int DTYPE>
-Form form_of(int dim) {
+Form form_of(int dim, int64_t rows, int64_t passes) {
     switch ((dim + 63) / 64) {
-        case 1: return form_of_width<DTYPE, 64>();
-        case 2: return form_of_width<DTYPE, 128>();
-        case 3: return form_of_width<DTYPE, 192>();
-        default: return form_of_width<DTYPE, 256>();
+        case 1: return form_of_width<DTYPE, 64>(rows, passes);
+        case 2: return form_of_width<DTYPE, 128>(rows, passes);
+        case 3: return form_of_width<DTYPE, 192>(rows, passes);
+        default: return form_of_width<DTYPE, 256>(rows, passes);
     }
 }
 Form form_of(const BeamgradWeights& a) {
+    const int64_t rows = rows_of(a), passes = std::min(a.sequences, kSequences) * static_cast<int64_t>(a.kv_heads) * ((places_of(a) + kPass - 1) / kPass);
     switch (a.data_type) {
-        case DBS_CUDA_DTYPE_F32: return form_of<DBS_CUDA_DTYPE_F32>(a.head_dim);
-        case DBS_CUDA_DTYPE_F16: return form_of<DBS_CUDA_DTYPE_F16>(a.head_dim);
-        default: return form_of<DBS_CUDA_DTYPE_BF16>(a.head_dim);
+        case DBS_CUDA_DTYPE_F32: return form_of<DBS_CUDA_DTYPE_F32>(a.head_dim, rows, passes);
+        case DBS_CUDA_DTYPE_F16: return form_of<DBS_CUDA_DTYPE_F16>(a.head_dim, rows, passes);
+        default: return form_of<DBS_CUDA_DTYPE_BF16>(a.head_dim, rows, passes);
     }
 }
-
-int64_t places_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.table_pages) * a.page_tokens; }
 
 // The weights are written while queries, keys and log-sums are read.
 bool lies_apart(const BeamgradWeights& a) {
@@ -672,30 +689,28 @@ bool lies_apart(const BeamgradWeights& a) {
     return std::all_of(std::begin(read), std::end(read), [&](const Region& r) { return apart(weights, r); });
 }
 
-int64_t rows_of(const BeamgradWeights& a) { return static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads); }
-
 // Workgroups of a launch, a multiple of eight. The card holds three of many rows on a CU
 // (two with a large tree's table), but of three that share a CU the oldest runs fastest:
 // twice as many, in equal stretches, are done sooner (two prompts' ends of 512 tokens over
 // 7700 and 15100, 32 heads of 128, bfloat16: 143 us, 151 with one round; more rounds
 // cost more beginnings than they gain). Few rows have shorter beginnings: four rounds (32
-// tokens over 2000 to 16000: 125 us, 140 with one). No more than there is work for,
-// by the table's size.
+// tokens over 2000 to 16000: 125 us, 140 with one). More rows that keys pass fill LDS of
+// a CU twice, and begin longer: one round (68 rows of 128 in bfloat16 over 32 x 2700 to 8000
+// 117 us, 167 with six). No more than there is work for, by the table's size.
 unsigned grid_of(const BeamgradWeights& a, const Form& form, size_t lds) {
     int device = 0, cus = 0;
     if (hipGetDevice(&device) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) {
         (void)hipGetLastError();
         cus = 256;
     }
-    const bool few = rows_of(a) <= form.rows;
-    const int64_t most = static_cast<int64_t>(cus) * (few ? 4 * form.resident : lds > 14 * 1024 ? 2 * 2 : 2 * 3);
-    const int64_t tile = few ? kPass : form.tile, heads = static_cast<int64_t>(std::min(a.sequences, kSequences)) * a.kv_heads;
-    const double work = static_cast<double>(heads) * static_cast<double>((places_of(a) + tile - 1) / tile) * (few ? 1.0 : static_cast<double>((rows_of(a) + 15) / 16) / 3.0);
+    const int64_t most = static_cast<int64_t>(cus) * form.rounds * (lds > 14 * 1024 ? 2 : form.resident);
+    const int64_t tile = form.many ? form.tile : kPass, heads = static_cast<int64_t>(std::min(a.sequences, kSequences)) * a.kv_heads;
+    const double work = static_cast<double>(heads) * static_cast<double>((places_of(a) + tile - 1) / tile) * (form.many ? static_cast<double>((rows_of(a) + 15) / 16) / 3.0 : 1.0);
     return static_cast<unsigned>((std::max<int64_t>(1, static_cast<int64_t>(std::min(work, static_cast<double>(most)))) + 7) / 8 * 8);
 }
 
 size_t tree_bytes(const BeamgradWeights& a, const Form& form) {
-    return a.parents && rows_of(a) > form.rows ? static_cast<size_t>(a.tokens) * (form.tile / 32 * sizeof(uint32_t) + sizeof(int16_t)) : 0;
+    return a.parents && form.many ? static_cast<size_t>(a.tokens) * (form.tile / 32 * sizeof(uint32_t) + sizeof(int16_t)) : 0;
 }
 
 }  // namespace
@@ -705,9 +720,7 @@ extern "C" {
 DBS_CUDA_EXPORT int64_t beamgrad_accumulate_weights_workspace_size(const BeamgradWeights* args) {
     if (!valid_sizes(args)) return -1;
     const Form form = form_of(*args);
-    return rows_of(*args) <= form.rows
-               ? 0
-               : grid_of(*args, form, tree_bytes(*args, form)) * static_cast<int64_t>(sizeof(Piece) + 2 * form.tile * sizeof(float));
+    return form.many ? grid_of(*args, form, tree_bytes(*args, form)) * static_cast<int64_t>(sizeof(Piece) + 2 * form.tile * sizeof(float)) : 0;
 }
 
 DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, void* workspace, int64_t workspace_bytes,
@@ -734,8 +747,6 @@ DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, voi
     p.G = Divider::of(static_cast<uint32_t>(a.heads / a.kv_heads));
     p.scale = a.scale * kLog2e;
     p.even = 16 % p.G.d == 0 && p.qn <= INT32_MAX / 256 && p.qh <= INT32_MAX / 32;
-    const bool few = rows_of(a) <= form.rows;
-    const void* const kernel = rows_of(a) <= 16 ? form.one : few ? form.few : form.many;
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     hipError_t e = hipSuccess;
     for (int s0 = 0; s0 < a.sequences && e == hipSuccess; s0 += kSequences) {
@@ -748,8 +759,8 @@ DBS_CUDA_EXPORT int beamgrad_accumulate_weights(const BeamgradWeights* args, voi
         p.lse = a.lse + static_cast<int64_t>(s0) * a.tokens * a.heads;
         p.weights = a.weights + s0 * p.ws;
         void* arguments[] = {&p};
-        e = hipLaunchKernel(kernel, dim3(grid), dim3(kThreads), arguments, lds, stream);
-        if (e == hipSuccess && !few) {
+        e = hipLaunchKernel(form.kernel, dim3(grid), dim3(kThreads), arguments, lds, stream);
+        if (e == hipSuccess && form.many) {
             weigh_join<<<grid, kThreads, 0, stream>>>(p, form.tile);
             e = hipGetLastError();
         }

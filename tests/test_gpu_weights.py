@@ -56,6 +56,16 @@ def test_widths(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [40, 64, 128, 192, 256])
+@pytest.mark.parametrize("N", [4, 8, 14, 30, 45, 60, 80, 96, 100])
+def test_rows_of_every_number(dtype, D, N):
+    """One block of rows, as many as pass keys' way holds, and more; trees and chains."""
+    lengths, counts = [130 + N, N, 700, 3], [N, N, N - 3, 2]
+    check(problem(dtype, 4, N, 8, 2, D, 24, lengths, counts, tree=True, seed=N))
+    check(problem(dtype, 4, N, 8, 2, D, 24, lengths, counts, seed=N))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lengths, counts, N, H, Hkv, page", [
     ([1], None, 1, 1, 1, 1),
     ([1, 700, 63, 64, 65], None, 1, 8, 2, 16),
@@ -94,10 +104,11 @@ def test_large_trees():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_bad_pages_masks_and_empty_rows(dtype):
+@pytest.mark.parametrize("H", [4, 32, 80, 256])
+def test_bad_pages_masks_and_empty_rows(dtype, H):
     """Pages that are not there, lengths past the table, NaN behind a sequence and in
     unseen places, rows whose log-sum is -inf."""
-    p = problem(dtype, 4, 4, 4, 2, 64, 8, [40, 33, 20, 8], [4, 2, 4, 3])
+    p = problem(dtype, 4, 4, H, 2, 64, 8, [40, 33, 20, 8], [4, 2, 4, 3])
     pages, lengths, refs = p["table"]
     nan_pages = [int(pages[1, 4]), int(pages[3, 0])]
     pages[0, 1], pages[0, 2] = -7, refs.numel()
@@ -108,7 +119,7 @@ def test_bad_pages_masks_and_empty_rows(dtype):
     check(p)
     # no page at all: every row is empty
     pages[3] = -1
-    lse = torch.randn(4, 4, 4).abs() + 5
+    lse = torch.randn(4, 4, H).abs() + 5
     lse[3] = -math.inf
     lse[0, 0] = -math.inf
     lse[0, 1, 2] = math.inf
