@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <new>
 #include <type_traits>
 #include <vector>
 
@@ -435,7 +436,7 @@ DBS_CUDA_EXPORT int64_t beamgrad_evict_tokens_workspace_size(const BeamgradPools
 
 DBS_CUDA_EXPORT int beamgrad_evict_tokens(const BeamgradPools* pools, const BeamgradEviction* args,
                                           const BeamgradTable* from, int sequences, int table_pages,
-                                          const BeamgradTable* to, void* workspace, int64_t workspace_bytes, void* stream_ptr) {
+                                          const BeamgradTable* to, void* workspace, int64_t workspace_bytes, void* stream_ptr) try {
     const int64_t bytes = beamgrad_evict_tokens_workspace_size(pools, args, sequences, table_pages);
     if (bytes < 0 || !workspace || workspace_bytes < bytes || !valid_table(from) || !valid_table(to) || !args->weights ||
         !args->weight_strides || !args->to_weights || !tables_apart(*from, *to, sequences, table_pages, pools->n_pages))
@@ -502,6 +503,8 @@ DBS_CUDA_EXPORT int beamgrad_evict_tokens(const BeamgradPools* pools, const Beam
         table = false;
     }
     return finish_call(stream, e);
+} catch (const std::bad_alloc&) {
+    return DBS_CUDA_STATUS_OUT_OF_MEMORY;
 }
 
 }  // extern "C"

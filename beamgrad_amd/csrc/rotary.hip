@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <new>
 #include <type_traits>
 
 #include "beamgrad_state.h"
@@ -285,7 +286,7 @@ void launch_pairs(Turn& p, int each, bool interleaved, int tensors, hipStream_t 
 
 extern "C" {
 
-DBS_CUDA_EXPORT int beamgrad_rotary(const BeamgradRotary* args, void* stream_ptr) {
+DBS_CUDA_EXPORT int beamgrad_rotary(const BeamgradRotary* args, void* stream_ptr) try {
     if (!valid(args) || (args->n > 0 && !lie_apart(*args))) return DBS_CUDA_STATUS_INVALID_ARGUMENT;
     const BeamgradRotary& a = *args;
     const int size = element_size(a.data_type);
@@ -332,6 +333,8 @@ DBS_CUDA_EXPORT int beamgrad_rotary(const BeamgradRotary* args, void* stream_ptr
         e = hipGetLastError();
     }
     return finish_call(stream, e);
+} catch (const std::bad_alloc&) {
+    return DBS_CUDA_STATUS_OUT_OF_MEMORY;
 }
 
 }  // extern "C"
