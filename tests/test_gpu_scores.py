@@ -77,6 +77,14 @@ def test_few_and_many_rows(V, rows):
     check(logits, tokens, 3, True, grads_of((rows,), 3, rows))
 
 
+@pytest.mark.parametrize("V, rows", [(70001, 66), (600001, 2)])
+def test_parts_of_several_rounds(V, rows):
+    """Rows cut into parts that a workgroup does not read at once."""
+    logits, tokens = inputs((rows,), V, torch.float32, rows)
+    tokens[2::2] = -1
+    check(logits, tokens, 20, True, grads_of((rows,), 20, rows))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("top", [1, 2, 20, 63, 64])
 @pytest.mark.parametrize("V", [64, 700, 12000, 49155])
