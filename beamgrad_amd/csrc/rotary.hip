@@ -228,18 +228,20 @@ bool valid(const BeamgradRotary* a) {
 // What is written lies apart, and in what is read only where it is the same.
 bool lie_apart(const BeamgradRotary& a) {
     const bool inplace = a.from[0] == a.to[0];
-    std::vector<Region> written, read;
-    for (int i = 0; i < a.n; ++i) {
-        Region r;
+    Region r;
+    for (int i = 0; i < a.n; ++i)
         if (!region_of(a, i, r)) return false;
-        written.push_back(r);
-        if (inplace) continue;
+    const auto written = [&](int i) {
+        Region to;
+        region_of(a, i, to);
+        return to;
+    };
+    const auto read = [&](int i) {
         const int64_t size = element_size(a.data_type), *st = a.from_strides + 3 * i;
-        read.push_back({reinterpret_cast<uintptr_t>(a.from[i]), {a.sequences, a.tokens}, {st[0] * size, st[1] * size},
-                        ((a.heads[i] - 1) * st[2] + a.head_dim[i]) * size});
-    }
-    return all_apart(static_cast<int>(written.size()), [&](int i) { return written[i]; }, static_cast<int>(read.size()),
-                     [&](int i) { return read[i]; });
+        return Region{reinterpret_cast<uintptr_t>(a.from[i]), {a.sequences, a.tokens}, {st[0] * size, st[1] * size},
+                      ((a.heads[i] - 1) * st[2] + a.head_dim[i]) * size};
+    };
+    return all_apart(a.n, written, inplace ? 0 : a.n, read);
 }
 
 template <class T, int PAIRS, bool INTERLEAVED>

@@ -49,22 +49,22 @@ void check_inplace(const Tensors& heads) {
 }
 
 int run_rotary(const Tensors& from, const Tensors& to, const Tensor& positions, const Tensor& frequencies, const OptTensor& counts, const Form& form) {
-    std::vector<const void*> source;
-    std::vector<void*> target;
-    std::vector<int32_t> heads, dims;
-    std::vector<int64_t> source_strides, target_strides;
-    for (size_t i = 0; i < from.size(); ++i) {
-        source.push_back(from[i].const_data_ptr());
-        target.push_back(to[i].data_ptr());
-        heads.push_back(narrow(from[i].size(2)));
-        dims.push_back(narrow(from[i].size(3)));
-        int64_t strides[3];
-        strides_of(from[i], strides);
-        source_strides.insert(source_strides.end(), strides, strides + 3);
-        strides_of(to[i], strides);
-        target_strides.insert(target_strides.end(), strides, strides + 3);
+    constexpr unsigned kUsual = 4;  // tensors without memory of their own (small calls take as long as their host work)
+    const size_t count = from.size();
+    c10::SmallVector<const void*, kUsual> source(count);
+    c10::SmallVector<void*, kUsual> target(count);
+    c10::SmallVector<int32_t, kUsual> heads(count), dims(count);
+    c10::SmallVector<int64_t, 3 * kUsual> source_strides(3 * count), target_strides(3 * count);
+    for (size_t i = 0; i < count; ++i) {
+        source[i] = from[i].const_data_ptr();
+        target[i] = to[i].data_ptr();
+        heads[i] = narrow(from[i].size(2));
+        dims[i] = narrow(from[i].size(3));
+        strides_of(from[i], &source_strides[3 * i]);
+        strides_of(to[i], &target_strides[3 * i]);
     }
-    const Tensor f = frequencies.to(torch::kFloat64).contiguous(), n = counts ? as_i32(*counts) : Tensor();
+    const bool ready = frequencies.scalar_type() == torch::kFloat64 && frequencies.is_contiguous();
+    const Tensor f = ready ? frequencies : frequencies.to(torch::kFloat64).contiguous(), n = counts ? as_i32(*counts) : Tensor();
     BeamgradRotary a{};
     a.from = source.data();
     a.to = target.data();
@@ -72,7 +72,7 @@ int run_rotary(const Tensors& from, const Tensors& to, const Tensor& positions, 
     a.head_dim = dims.data();
     a.from_strides = source_strides.data();
     a.to_strides = target_strides.data();
-    a.n = narrow(static_cast<int64_t>(from.size()));
+    a.n = narrow(static_cast<int64_t>(count));
     a.data_type = data_type(from[0], "tensors");
     a.sequences = narrow(positions.size(0));
     a.tokens = narrow(positions.size(1));
