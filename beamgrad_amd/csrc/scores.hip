@@ -491,9 +491,9 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
 }
 
 // A workgroup joins the parts of a row. The parts' alternatives are in order: of the
-// j-th of each part, j * parts >= top, the lowest is reached by `top` of them, so
-// what lies below it is none. 32 rows of 19 parts: 5.2 us, of two dependent reads and the
-// ranking.
+// j-th of each part but the last, j * (parts - 1) >= top, the lowest is reached by `top` of
+// them, so what lies below it is none. (The last part may be short, and its j-th low.) 32 rows
+// of 19 parts: 5.2 us, of two dependent reads and the ranking.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
     constexpr int kFirst = 4;  // keys of a thread that are read ahead
@@ -505,11 +505,11 @@ __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int p
     const int64_t first = static_cast<int64_t>(r) * parts;
     Sums all = (tid & 63) < parts ? sums[first + (tid & 63)] : Sums{-FLT_MAX, 0.0f, 0.0f, 0.0f};
     const uint64_t* const mine = keys + first * p.top;
-    const int n = parts * p.top, j = (p.top + parts - 1) / parts - 1;
+    const int n = parts * p.top, whole = parts - 1, j = (p.top + whole - 1) / whole - 1;
     uint64_t ahead[kFirst];
 #pragma unroll
     for (int i = 0; i < kFirst; ++i) ahead[i] = i * kThreads + tid < n ? mine[i * kThreads + tid] : 0;
-    uint64_t floor = p.top > 0 && tid < parts ? mine[tid * p.top + j] : ~uint64_t{0};
+    uint64_t floor = p.top > 0 && tid < whole ? mine[tid * p.top + j] : ~uint64_t{0};
     if (token < 0) return write_none<kThreads>(p, r, false);
     const float x = value_at<T>(p.row(r), token);
     if (tid == 0) found = 0;
