@@ -16,8 +16,8 @@
 // lies with the threads whose own maximum does: little more than `top` threads, whose shares (a few hundred values of a large
 // vocabulary) are read again, from the cache. What they hold beside the alternatives
 // is little (20 of 151936 at random: one or two), unless values are equal
-// in great number: where more than kKept reach it, the alternatives are found one after the
-// other. Where fewer than `top` do, all that are above -inf have, and the first
+// in great number: where more than kKept reach it, the alternatives are found value after
+// value, equal ones together. Where fewer than `top` do, all that are above -inf have, and the first
 // ones at -inf follow.
 #include <hip/hip_runtime.h>
 
@@ -220,7 +220,7 @@ constexpr int kDumped = 64;  // threads whose values fit LDS
 template <int THREADS, int VALUES = 1>
 struct Shared {
     Sums waves[THREADS / 64];
-    int flagged[THREADS], flags, kept;
+    int flagged[THREADS], flags, kept, found[THREADS / 64];
     float floor[THREADS / 64];   // what reaches the least of them may be an alternative
     uint64_t keys[kKept + 8];
     uint64_t best[THREADS / 64];
@@ -362,21 +362,47 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
             if (x == -__builtin_inff() && at < all) each(at, key_of(x, from + tid));
         }
     } else {
-        // one after the other: the largest below the last one
+        // value after value: the largest below the last one, where it stands first
         uint64_t below = ~uint64_t{0};
-        for (int k = 0; k < all; ++k) {
+        for (int k = 0; k < all;) {
             uint64_t best = 0;
             for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
                 float x[E];
                 values_at<T>(row, static_cast<int>(v), to, x);
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    const uint64_t key = key_of(x[j], static_cast<int>(v) + j);
+                    const uint64_t key = key_of(x[j], 0);
                     if (v + j < to && key < below && key > best) best = key;
                 }
             }
             below = largest_in_block(best, lds);
-            if (tid == 0) each(k, below);
+            for (int64_t v0 = from; v0 < to && k < all; v0 += THREADS * E) {
+                const int v = static_cast<int>(v0) + tid * E;
+                float x[E];
+                values_at<T>(row, min(v, to), to, x);
+                unsigned hits = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j) hits |= static_cast<unsigned>(v + j < to && key_of(x[j], 0) == below) << j;
+                if (!__syncthreads_or(hits)) continue;
+                const int here = __popc(hits);
+                int upto = here;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int y = __shfl_up(upto, d);
+                    if (lane >= d) upto += y;
+                }
+                if (lane == 63) lds.found[tid >> 6] = upto;
+                __syncthreads();
+                int at = k + upto - here;
+                for (int w = 0; w < WAVES; ++w) {
+                    if (w < tid >> 6) at += lds.found[w];
+                    k += lds.found[w];
+                }
+                __syncthreads();
+                for (; hits != 0 && at < all; hits &= hits - 1, ++at) {
+                    const int place = v + __builtin_ctz(hits);
+                    each(at, below - static_cast<uint32_t>(place));
+                }
+            }
         }
     }
     for (int k = all + tid; k < top; k += THREADS) each(k, uint64_t{0});
