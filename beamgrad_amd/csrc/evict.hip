@@ -237,9 +237,9 @@ __device__ __forceinline__ void choose(const float* from, int first, int end, in
 }
 
 // x: a sequence; y: a row of weights, the last: counts of pages, copied; z: a set.
-// 1024 rows of 4500 to 8000 weights, of which 4096 stay, in 38 us (0.7 TB/s: the counts of
-// digits in LDS, which the leading digits of like weights crowd); ten rows of 900 in 9 us, of
-// latency.
+// 1024 rows of 4500 to 8000 weights, of which 4096 stay, in 38 us (26 MB read and 33 written;
+// the vector unit is busy for 42 % of it, the rest waits for the digits' counts); ten rows of
+// 900 in 9 us, most of it dependent reads: lengths, pages, their counts.
 __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const WeightSet set) {
     __shared__ Choice lds;
     const int s = blockIdx.x, tid = threadIdx.x, head = blockIdx.y;
