@@ -15,10 +15,14 @@
 // many from each wavefront) is reached by at least `top` values, and what reaches it
 // lies with the threads whose own maximum does: little more than `top` threads, whose shares (a few hundred values of a large
 // vocabulary) are read again, from the cache. What they hold beside the alternatives
-// is little (20 of 151936 at random: one or two), unless values are equal
-// in great number: where more than kKept reach it, the alternatives are found value after
-// value, equal ones together. Where fewer than `top` do, all that are above -inf have, and the first
-// ones at -inf follow.
+// is little where the large values lie anywhere (20 of 151936 at random: one or two). It is much
+// where they lie together, so that some wavefront has none of them: logits that fall or rise
+// with the token, a mask that leaves one stretch; where one wavefront has a short row and
+// all its threads are wanted; and where values are equal in great number. Where more than kKept reach it,
+// the threshold is raised: a pass over the row counts what reaches it in 1024 equal steps of the values'
+// order, the step of the `top`-th largest is counted in its turn until few enough reach its low
+// end (one pass, seldom two, at most four) or it is one value, whose first ones are taken. Where fewer than `top`
+// reach the first threshold, all that are above -inf have, and the first ones at -inf follow.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -40,6 +44,7 @@ constexpr int kManyThreads = 512;  // where rows are few
 constexpr int kAtOnce = 4;     // 16-byte reads of a thread in flight
 constexpr int kMaxTop = 64;
 constexpr int kKept = 512;     // values beside the alternatives that a workgroup ranks
+constexpr int kCounts = 1024;  // equal steps of values that are counted at once
 constexpr int kMaxParts = 64;  // of a row
 constexpr int64_t kCacheBytes = int64_t{200} << 20;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -75,18 +80,23 @@ struct Sums {
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-// A value and its place as one number: the larger value, of equal ones the
-// lower place, is larger. 0 is below all of them (NaN does not come here).
-__device__ __forceinline__ uint64_t key_of(float x, int place) {
+template <class X>
+__device__ __forceinline__ X uniform(X x) { return static_cast<X>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))); }
+
+// Values in the order of unsigned numbers, the two zeros as one (NaN does not come here).
+__device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, x + 0.0f);
-    const uint32_t high = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-    return static_cast<uint64_t>(high) << 32 | (0xffffffffu - static_cast<uint32_t>(place));
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float of_order(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+// A value and its place as one number: the larger value, of equal ones the
+// lower place, is larger. 0 is below all of them.
+__device__ __forceinline__ uint64_t key_of(float x, int place) {
+    return static_cast<uint64_t>(order_of(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(place));
 }
 __device__ __forceinline__ int place_of(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
-__device__ __forceinline__ float value_of(uint64_t key) {
-    const uint32_t high = static_cast<uint32_t>(key >> 32);
-    return __builtin_bit_cast(float, high & 0x80000000u ? high & 0x7fffffffu : ~high);
-}
+__device__ __forceinline__ float value_of(uint64_t key) { return of_order(static_cast<uint32_t>(key >> 32)); }
 
 template <class T>
 constexpr int kEach = 16 / sizeof(T);
@@ -222,8 +232,12 @@ struct Shared {
     Sums waves[THREADS / 64];
     int flagged[THREADS], flags, kept, found[THREADS / 64];
     float floor[THREADS / 64];   // what reaches the least of them may be an alternative
-    uint64_t keys[kKept + 8];
-    uint64_t best[THREADS / 64];
+    union {
+        uint64_t keys[kKept + 8];
+        uint32_t counts[kCounts];
+    };
+    uint32_t low, high;  // of what is counted
+    int above;           // values over `high`
     float dump[VALUES > 1 ? kDumped * (VALUES + 1) : 1];
 };
 
@@ -251,25 +265,11 @@ __device__ __forceinline__ Sums joined_block(Sums a, Shared<THREADS, VALUES>& ld
     return a;
 }
 
-template <int THREADS, int VALUES>
-__device__ __forceinline__ uint64_t largest_in_block(uint64_t key, Shared<THREADS, VALUES>& lds) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint32_t lo = __shfl_xor(static_cast<uint32_t>(key), d), hi = __shfl_xor(static_cast<uint32_t>(key >> 32), d);
-        const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
-        key = other > key ? other : key;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds.best[threadIdx.x >> 6] = key;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) key = lds.best[w] > key ? lds.best[w] : key;
-    return key;
-}
-
-// How many of n keys are larger; 8 at once, zeros behind them.
+// How many of n keys are larger; 8 at once (and MORE such reads, where registers are free), zeros behind them.
+template <int MORE>
 __device__ __forceinline__ int larger_of(const uint64_t* keys, int n, uint64_t key) {
     int above = 0;
+#pragma unroll MORE
     for (int j = 0; j < n; j += 8) {
         uint64_t other[8];
 #pragma unroll
@@ -280,12 +280,12 @@ __device__ __forceinline__ int larger_of(const uint64_t* keys, int n, uint64_t k
     return above;
 }
 
-// The `top` largest keys of [from, to), given the thread's maximum, in order to
+// The `top` largest keys of [from, to), given the thread's maximum and that of all, in order to
 // each(rank, key). `values`: what the thread read of it, where that is all of its share:
 // those of few threads go through LDS, for all threads to look through.
 // Fewer than `top` values: key 0 for the rest.
 template <class T, int THREADS, int VALUES, class Each>
-__device__ __forceinline__ void alternatives(const char* row, int from, int to, int top, float mine, const float (&values)[VALUES],
+__device__ __forceinline__ void alternatives(const char* row, int from, int to, int top, float mine, float most, const float (&values)[VALUES],
                                              Shared<THREADS, VALUES>& lds, Each each) {
     constexpr int E = kEach<T>, WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -346,63 +346,138 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
         }
     }
     __syncthreads();
-    const int n = lds.kept, all = min(top, to - from);
-    if (n <= kKept) {
-        if (tid < 8) lds.keys[n + tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t key = lds.keys[i];
-            const int above = larger_of(lds.keys, n, key);
-            if (above < top) each(above, key);
-        }
-        if (n < all && tid < 64) {  // of the first `all` places at most n are not at -inf
-            const float x = tid < all ? value_at<T>(row, from + tid) : 0.0f;
-            const uint64_t none = __ballot(x == -__builtin_inff());
-            const int at = n + __popcll(none & ((uint64_t{1} << tid) - 1));
-            if (x == -__builtin_inff() && at < all) each(at, key_of(x, from + tid));
-        }
-    } else {
-        // value after value: the largest below the last one, where it stands first
-        uint64_t below = ~uint64_t{0};
-        for (int k = 0; k < all;) {
-            uint64_t best = 0;
-            for (int64_t v = from + tid * E; v < to; v += THREADS * E) {
-                float x[E];
-                values_at<T>(row, static_cast<int>(v), to, x);
+    const int all = min(top, to - from);
+    int n = uniform(lds.kept);
+    bool tied = false;  // those at the floor are not kept, and are more than are wanted
+    constexpr int kFew = std::min(kKept, 4 * THREADS);  // that are ranked sooner than their number is brought down
+    if (n > kFew) {
+        // All values from the floor to the maximum are counted in equal steps, then those of
+        // the step that the `top`-th largest lies in, until few reach its low end or it is one value.
+        constexpr int kUnused = sizeof(T) == 4 ? 0 : std::is_same<T, _Float16>::value ? 13 : 16;  // low bits that T does not have
+        const auto all_values = [&](auto use) {
+            constexpr int kStep = THREADS * E;
+            int v0 = from;
+#pragma unroll 1
+            for (; to - v0 >= kAtOnce * kStep; v0 += kAtOnce * kStep) {
+                u32x4 raw[kAtOnce];
+                const char* const at = row + static_cast<int64_t>(v0 + tid * E) * sizeof(T);
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const uint64_t key = key_of(x[j], 0);
-                    if (v + j < to && key < below && key > best) best = key;
+                for (int i = 0; i < kAtOnce; ++i) raw[i] = *reinterpret_cast<const u32x4_any*>(at + i * kStep * sizeof(T));
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    T e[E];
+                    __builtin_memcpy(e, &raw[i], 16);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) use(static_cast<float>(e[j]), v0 + i * kStep + tid * E + j);
                 }
             }
-            below = largest_in_block(best, lds);
-            for (int64_t v0 = from; v0 < to && k < all; v0 += THREADS * E) {
-                const int v = static_cast<int>(v0) + tid * E;
+#pragma unroll 1
+            for (; v0 < to; v0 += kStep) {
+                const int v = v0 + tid * E;
                 float x[E];
                 values_at<T>(row, min(v, to), to, x);
-                unsigned hits = 0;
 #pragma unroll
-                for (int j = 0; j < E; ++j) hits |= static_cast<unsigned>(v + j < to && key_of(x[j], 0) == below) << j;
-                if (!__syncthreads_or(hits)) continue;
-                const int here = __popc(hits);
-                int upto = here;
+                for (int j = 0; j < E; ++j) use(x[j], min(v + j, to));
+            }
+        };
+        uint32_t low = uniform(order_of(floor) >> kUnused), high = uniform(order_of(most) >> kUnused);
+        int above = 0;
+        for (;;) {
+            tied = low == high;
+            if (tied) break;
+            const int shift = max(0, 22 - __builtin_clz(high - low));
+            __syncthreads();  // what is read of LDS before is read
+#pragma unroll 1
+            for (int i = tid; i < kCounts; i += THREADS) lds.counts[i] = 0;
+            __syncthreads();
+            all_values([&](float x, int place) {
+                const uint32_t o = order_of(x) >> kUnused, step = (o - low) >> shift;
+                const bool counts = place < to && o >= low && o <= high;
+                // the first lane's step by one addition: many values may be in one
+                const uint64_t which = __ballot(counts);
+                if (which == 0) return;
+                const int lead = __builtin_ctzll(which);
+                const bool same = counts && step == static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(step), lead));
+                const int together = __popcll(__ballot(same));
+                if (counts && (!same || lane == lead)) atomicAdd(&lds.counts[step], same ? static_cast<uint32_t>(together) : 1u);
+            });
+            __syncthreads();
+            if (tid < 64) {  // steps from the highest down, some of a lane
+                constexpr int kOwn = kCounts / 64;
+                uint32_t sum = 0;
+#pragma unroll 4
+                for (int i = 0; i < kOwn; ++i) sum += lds.counts[kCounts - 1 - (tid * kOwn + i)];
+                uint32_t upto = sum;
+#pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
-                    const int y = __shfl_up(upto, d);
+                    const uint32_t y = __shfl_up(upto, d);
                     if (lane >= d) upto += y;
                 }
-                if (lane == 63) lds.found[tid >> 6] = upto;
-                __syncthreads();
-                int at = k + upto - here;
-                for (int w = 0; w < WAVES; ++w) {
-                    if (w < tid >> 6) at += lds.found[w];
-                    k += lds.found[w];
-                }
-                __syncthreads();
-                for (; hits != 0 && at < all; hits &= hits - 1, ++at) {
-                    const int place = v + __builtin_ctz(hits);
-                    each(at, below - static_cast<uint32_t>(place));
+                const uint32_t left = static_cast<uint32_t>(top - above);
+                uint32_t before = upto - sum;
+                if (before < left && upto >= left) {
+                    int step = kCounts - 1 - tid * kOwn;
+#pragma unroll 1
+                    for (; before + lds.counts[step] < left; --step) before += lds.counts[step];
+                    lds.low = low + (static_cast<uint32_t>(step) << shift);
+                    lds.high = min(high, lds.low + ((1u << shift) - 1));
+                    lds.above = above + static_cast<int>(before);
+                    lds.kept = lds.above + static_cast<int>(lds.counts[step]);
                 }
             }
+            __syncthreads();
+            low = uniform(lds.low), high = uniform(lds.high), above = uniform(lds.above);
+            if (uniform(lds.kept) <= kFew) break;
+        }
+        floor = of_order(low << kUnused | (low >> (31 - kUnused) != 0 ? 0u : (1u << kUnused) - 1));  // a value of T
+        __syncthreads();
+        if (tid == 0) lds.kept = 0;
+        __syncthreads();
+        if (!tied || above > 0)
+            all_values([&](float x, int place) {
+                if (!tied || order_of(x) >> kUnused > low) keep(x, place);
+            });
+        __syncthreads();
+        n = uniform(lds.kept);
+    }
+    if (tid < 8) lds.keys[n + tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+        const uint64_t key = lds.keys[i];
+        const int above = larger_of<2>(lds.keys, n, key);
+        if (above < top) each(above, key);
+    }
+    if (n < all && !tied && tid < 64) {  // of the first `all` places at most n are not at -inf
+        const float x = tid < all ? value_at<T>(row, from + tid) : 0.0f;
+        const uint64_t none = __ballot(x == -__builtin_inff());
+        const int at = n + __popcll(none & ((uint64_t{1} << tid) - 1));
+        if (x == -__builtin_inff() && at < all) each(at, key_of(x, from + tid));
+    }
+    if (tied) {
+        // the first ones that equal the floor, round after round
+        for (int64_t v0 = from; v0 < to && n < all; v0 += THREADS * E) {
+            const int v = static_cast<int>(v0) + tid * E;
+            float x[E];
+            values_at<T>(row, min(v, to), to, x);
+            unsigned hits = 0;
+#pragma unroll
+            for (int j = 0; j < E; ++j) hits |= static_cast<unsigned>(v + j < to && x[j] == floor) << j;
+            if (!__syncthreads_or(hits)) continue;
+            const int here = __popc(hits);
+            int upto = here;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int y = __shfl_up(upto, d);
+                if (lane >= d) upto += y;
+            }
+            if (lane == 63) lds.found[tid >> 6] = upto;
+            __syncthreads();
+            int at = n + upto - here;
+            for (int w = 0; w < WAVES; ++w) {
+                if (w < tid >> 6) at += lds.found[w];
+                n += uniform(lds.found[w]);
+            }
+            __syncthreads();
+            for (; hits != 0 && at < all; hits &= hits - 1, ++at) each(at, key_of(floor, v + __builtin_ctz(hits)));
         }
     }
     for (int k = all + tid; k < top; k += THREADS) each(k, uint64_t{0});
@@ -466,7 +541,7 @@ __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
     const Normal n = normal_of(all);
     if (threadIdx.x == 0) write_row(p, r, x, n);
     if (p.top > 0)
-        alternatives<T>(row, 0, p.V, p.top, mine.m, {0.0f}, lds, [&](int rank, uint64_t key) { write_alternative(p, r, rank, key, n); });
+        alternatives<T>(row, 0, p.V, p.top, mine.m, all.m, {0.0f}, lds, [&](int rank, uint64_t key) { write_alternative(p, r, rank, key, n); });
 }
 
 // x: a part of `part` values of row y. Sums and alternatives go to the workspace.
@@ -513,18 +588,20 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
     const int64_t at = static_cast<int64_t>(r) * gridDim.x + blockIdx.x;
     if (threadIdx.x == 0) sums[at] = all;
     if (p.top > 0 && all.s <= FLT_MAX)
-        alternatives<T>(row, from, to, p.top, mine.m, x, lds, [&](int rank, uint64_t key) { keys[at * p.top + rank] = key; });
+        alternatives<T>(row, from, to, p.top, mine.m, all.m, x, lds, [&](int rank, uint64_t key) { keys[at * p.top + rank] = key; });
 }
 
 // A workgroup joins the parts of a row. The parts' alternatives are in order: of the
 // j-th of each part but the last, j * (parts - 1) >= top, the lowest is reached by `top` of
-// them, so what lies below it is none. (The last part may be short, and its j-th low.) 32 rows
-// of 19 parts: 5.2 us, of two dependent reads and the ranking.
+// them, so what lies below it is none. (The last part may be short, and its j-th low.) Where
+// the largest lie in a few parts, much reaches it; then the same is asked of the j-th of the
+// ceil(top / j) parts in which it is largest, for j = 1, 2, 4 .. top, and the highest answer
+// counts: of no j more than 1 / j of the keys pass. 32 rows of 19 parts: 5.2 us, of two dependent reads and the ranking.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
     constexpr int kFirst = 4;  // keys of a thread that are read ahead
     __shared__ uint64_t kept[kMaxParts * kMaxTop + 8];
-    __shared__ uint64_t lowest;
+    __shared__ uint64_t lowest, floors[kThreads / 64];
     __shared__ int found;
     const uint32_t r = blockIdx.x;
     const int token = p.token(r), tid = threadIdx.x;
@@ -558,15 +635,41 @@ __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int p
     const auto take = [&](uint64_t key) {
         if (key >= floor && key != 0) kept[atomicAdd(&found, 1)] = key;
     };
+    const auto take_all = [&] {
 #pragma unroll
-    for (int i = 0; i < kFirst; ++i) take(ahead[i]);
-    for (int i = kFirst * kThreads + tid; i < n; i += kThreads) take(mine[i]);
-    __syncthreads();
-    const int m = found;
+        for (int i = 0; i < kFirst; ++i) take(ahead[i]);
+        for (int i = kFirst * kThreads + tid; i < n; i += kThreads) take(mine[i]);
+        __syncthreads();
+    };
+    take_all();
+    int m = uniform(found);
+    if (m > kKept) {
+        const int lane = tid & 63, wave = tid >> 6;
+        for (int i = wave; 1 << i < 2 * p.top; i += kThreads / 64) {
+            const int each = min(1 << i, p.top), of = (p.top + each - 1) / each;
+            if (of > parts) continue;
+            const uint64_t key = lane < parts ? mine[lane * p.top + each - 1] : 0;
+            const auto at = [&](int q) {
+                const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(key), q), hi = __builtin_amdgcn_readlane(static_cast<int>(key >> 32), q);
+                return static_cast<uint64_t>(hi) << 32 | lo;
+            };
+            int above = 0;
+            for (int q = 0; q < parts; ++q) above += at(q) > key;
+            const uint64_t which = __ballot(key != 0 && above == of - 1);
+            if (which != 0) floor = max(floor, at(__builtin_ctzll(which)));
+        }
+        if (lane == 0) floors[wave] = floor;
+        if (tid == 0) found = 0;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) floor = max(floor, floors[w]);
+        take_all();
+        m = uniform(found);
+    }
     if (tid < 8) kept[m + tid] = 0;
     __syncthreads();
     for (int i = tid; i < m; i += kThreads) {
-        const int above = larger_of(kept, m, kept[i]);
+        const int above = larger_of<4>(kept, m, kept[i]);
         if (above < p.top) write_alternative(p, r, above, kept[i], normal);
     }
 }

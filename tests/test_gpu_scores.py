@@ -120,6 +120,87 @@ def test_alternatives_of_one_thread():
         check(logits, tokens, 40)
 
 
+def gathered(kind, rows, V, dtype, seed=0):
+    """Rows whose large values lie together, or are equal in great number."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, V, generator=g) * 3
+    if kind == "falling":
+        x = x.sort(1, descending=True).values
+    elif kind == "rising":
+        x = x.sort(1).values
+    elif kind == "rank":
+        x = -torch.arange(1, V + 1).float().log() + 0.3 * x
+    elif kind == "neighbours":
+        for r, n in enumerate((600, 1000, 5000)[:rows]):
+            x[r, :V // 3] = x[r, V // 3 + n:] = -math.inf
+    elif kind == "turns":  # the same few threads' of every round
+        x[:, torch.arange(V) % 2048 >= 60] = -math.inf
+    elif kind == "negative ties":
+        x = (x.clamp(max=0.0) * 2).floor() / 2 - 1.0
+        x[0, ::7], x[0, 1::7] = -0.375, -0.25
+        x[0, 40:] = torch.where(x[0, 40:] == -0.25, -0.375, x[0, 40:])  # fewer than are asked for stand above them
+    elif kind == "wide":  # over all of the type's range, its lowest value too
+        x = torch.randn(rows, V, generator=g).sign() * torch.exp(torch.rand(rows, V, generator=g) * math.log(torch.finfo(dtype).max / 4))
+        x[:, ::3] = torch.finfo(dtype).min
+        x[0] = torch.where(torch.arange(V) % 1000 == 3, -x[0].abs(), torch.finfo(dtype).min)
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["random", "falling", "rising", "rank", "neighbours", "turns", "negative ties", "wide"])
+@pytest.mark.parametrize("V", [2000, 4000, 32000, 49155, 151936])
+def test_alternatives_that_lie_together(dtype, kind, V):
+    """The threshold of the wavefronts' maxima lets much of the row pass: short rows (one wavefront),
+    whole and split ones, of few and of all possible alternatives."""
+    logits, tokens = gathered(kind, 3, V, dtype), torch.arange(3)
+    for top in (5, 20, 64):
+        if kind == "wide":
+            # log p = (x - m) - log s rounds twice, each time to half a step of its value. The
+            # restatement's bound has the first one, 2^-24 |x - m|, and multiples of log p where p is
+            # not 0 in 64 bits; where it is (x - m below -745), the second, 2^-24 |log p|, comes to it
+            # (its value is off by the first: 1 + 2^-23).
+            want, bounds = ref.token_logprobs(logits, tokens, top, False)
+            got = bg.token_logprobs(logits.cuda(), tokens.cuda(), top=top)
+            assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+            for name in ("logprobs", "top_logprobs"):
+                near(getattr(got, name), want[name], bounds[name] + want[name].abs() * 2.0**-24 * (1 + 2.0**-23), name)
+            continue
+        check(logits, tokens, top, False, [None, None, grads_of((3,), top, 1)[2]] if top == 20 and V <= 4000 else None)
+
+
+def test_alternatives_of_many_rows_that_lie_together():
+    """A workgroup of 256 threads a row; a split row's parts of several rounds."""
+    for kind in ("falling", "rank", "turns", "negative ties"):
+        logits = gathered(kind, 420, 20000, torch.bfloat16)
+        tokens = torch.full((420,), -1)
+        tokens[::150] = 1
+        check(logits, tokens, 20)
+        check(gathered(kind, 1, 1200001, torch.float32), torch.tensor([7]), 64)
+
+
+@pytest.mark.parametrize("dtype, rows, V", [(torch.float32, 4, 32000), (torch.bfloat16, 32, 151936), (torch.float16, 200, 50257), (torch.float32, 600, 2000)])
+def test_the_time_of_alternatives_goes_by_the_row_and_not_by_its_order(dtype, rows, V):
+    """A few more passes over the row, and not two for each alternative (a hundred times as long)."""
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+
+    def time(x, top):
+        x, best = x.cuda(), math.inf
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for _ in range(10):
+                bg.token_logprobs(x, tokens, top=top)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    base = max(time(gathered("random", rows, V, dtype), 20), 0.08)  # (8 us a call: what the host takes)
+    for kind in ("random", "falling", "rising", "rank", "neighbours", "turns", "negative ties"):
+        took = time(gathered(kind, rows, V, dtype), 64)
+        assert took <= 10 * base, (kind, took, base)
+
+
 @pytest.mark.parametrize("top", [1, 6, 64])
 @pytest.mark.parametrize("V, rows", [(100, 9), (20000, 9), (50257, 9), (20000, 1030)])
 def test_alternatives_of_few_possible_tokens(V, rows, top):
