@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <iterator>
 #include <new>
 #include <type_traits>
 
@@ -185,20 +186,39 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Turn p) {
 
 int element_size(int data_type) { return data_type == DBS_CUDA_DTYPE_F32 ? 4 : 2; }
 
-// Tensors in place: the heads of all tokens as rows that lie apart, the heads of a token
-// in one run or the tokens of all sequences in equal steps. False: neither.
+// The heads that are written of tensor i. Sequences, tokens and heads lie in whatever order: a step that
+// continues the one within it is one with it. Where all three are left, what lies between
+// the rows of the innermost counts as written. False: these rows meet, or reach further than addresses do.
 bool region_of(const BeamgradRotary& a, int i, Region& r) {
-    const int64_t size = element_size(a.data_type), row = a.head_dim[i] * size;
-    const int64_t *st = a.to_strides + 3 * i, ss = st[0] * size, sn = st[1] * size, sh = st[2] * size;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(a.to[i]);
-    if (a.heads[i] == 1 || sh == row)
-        r = {base, {a.sequences, a.tokens}, {ss, sn}, a.heads[i] * row};
-    else if (a.tokens == 1)
-        r = {base, {a.sequences, a.heads[i]}, {ss, sh}, row};
-    else if (a.sequences == 1 || (ss % a.tokens == 0 && ss / a.tokens == sn))
-        r = {base, {static_cast<int64_t>(a.sequences) * a.tokens, a.heads[i]}, {sn, sh}, row};
-    else
-        return false;
+    struct Dim {
+        int64_t n, stride;
+        bool operator<(const Dim& other) const { return stride < other.stride; }
+    };
+    const int64_t size = element_size(a.data_type), *st = a.to_strides + 3 * i;
+    Dim all[] = {{a.sequences, st[0] * size}, {a.tokens, st[1] * size}, {a.heads[i], st[2] * size}}, left[3];
+    std::sort(std::begin(all), std::end(all));
+    int64_t run = a.head_dim[i] * size, next = run;  // next: where what lies innermost would go on
+    int levels = 0;
+    for (const Dim& d : all) {
+        if (d.n == 1) continue;
+        if (d.stride != next) {
+            left[levels++] = d;
+        } else if (levels > 0) {
+            left[levels - 1].n *= d.n;
+        }
+        if (__builtin_mul_overflow(d.n, d.stride, &next)) return false;
+        if (levels == 0) run = next;
+    }
+    if (levels == 3) {
+        if (left[0].stride < run) return false;
+        run += (left[0].n - 1) * left[0].stride;
+        left[0] = left[1], left[1] = left[2], levels = 2;
+    }
+    r = {reinterpret_cast<uintptr_t>(a.to[i]), {1, 1}, {0, 0}, run};
+    for (int d = 0; d < levels; ++d) {
+        r.n[1 - d] = left[d].n;
+        r.stride[1 - d] = left[d].stride;
+    }
     return true;
 }
 

@@ -122,7 +122,8 @@ void rotary_inplace_hip(Tensors heads, const Tensor& positions, const Tensor& fr
     const at::OptionalDeviceGuard guard(positions.device());
     const int status = run_rotary(heads, heads, positions, frequencies, counts, {interleaved, scale, inverse});
     TORCH_CHECK_VALUE(status != DBS_CUDA_STATUS_INVALID_ARGUMENT,
-                      "tensors that are turned in place must share no memory, and lie with a token's heads in one run or their tokens in equal steps");
+                      "tensors that are turned in place must share no memory (of one whose sequences, tokens and heads lie in three unrelated steps, "
+                      "what lies between the rows of the smallest step counts as its own)");
     check_status(status, "rotary");
     written(heads);
 }

@@ -181,9 +181,9 @@ DBS_CUDA_EXPORT int beamgrad_reorder_states_backward(const void* const* from, vo
  * from, to, heads, head_dim and the strides are host arrays, read before the call
  * returns; strides are of sequences, tokens and heads (three for each tensor), in
  * elements, and a head is contiguous. from[i] == to[i] for every i (with equal strides)
- * turns in place; otherwise no memory that is written may meet what is read. What
- * is written lies apart: a token's heads in one run, or the tokens of all sequences
- * in equal steps. head_dim is at most 1024, sequences * tokens fewer than 2^26, strides at
+ * turns in place; otherwise no memory that is written may meet what is read. No two rows
+ * that are written may meet; where sequences, tokens and heads lie in three steps of which
+ * none continues another, what lies between the rows of the smallest counts as written too. head_dim is at most 1024, sequences * tokens fewer than 2^26, strides at
  * most 2^40. */
 typedef struct BeamgradRotary {
     const void* const* from;

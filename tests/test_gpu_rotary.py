@@ -162,6 +162,65 @@ def test_strides_and_views():
     near(bg.rotary([one_token.transpose(1, 2).contiguous().transpose(1, 2)], at[:, :1].cuda(), f.cuda())[0], ref.rotary(one_token.cpu(), at[:, :1], f, False, 1.0))
 
 
+def placed(name, S, N, H, D):
+    """A buffer, and the tensors of it that are turned in place: layouts that programs have."""
+    if name == "heads first":
+        b = draw(1, S, H, N, D)
+        return b, lambda t: [t.transpose(1, 2)]
+    if name == "queries and keys, heads first":
+        b = draw(1, S, 2 * H + 1, N, D)
+        return b, lambda t: [t[:, :H].transpose(1, 2), t[:, H:H + 1].transpose(1, 2)]
+    if name == "in turns, heads first":
+        b = draw(1, S, H, N, 3, D)
+        return b, lambda t: [t[:, :, :, 0].transpose(1, 2), t[:, :, :, 2].transpose(1, 2)]
+    if name == "ends of heads, heads first":
+        b = draw(1, S, H, N, D + 8)
+        return b, lambda t: [t[..., 8:].transpose(1, 2)]
+    if name == "tokens first":
+        b = draw(1, N, S, H, D)
+        return b, lambda t: [t.transpose(0, 1)]
+    if name == "a cache with room, heads first":
+        b = draw(1, S, H, N + 3, D)
+        return b, lambda t: [t[:, :, 2:N + 2].transpose(1, 2)]
+    if name == "three steps":  # the ends of heads of some tokens of some heads
+        b = draw(1, S, H + 1, N + 3, D + 8)
+        return b, lambda t: [t[:, 1:, 2:N + 2, 8:].transpose(1, 2)]
+    if name == "a buffer of a model's layers":
+        b = draw(1, 2, S, H, N, D)
+        return b, lambda t: [x.transpose(1, 2) for x in t]
+    raise AssertionError(name)
+
+
+@pytest.mark.parametrize("S, N, H", [(1, 5, 3), (3, 5, 2), (2, 1, 3), (4, 7, 1), (3, 600, 2)])
+@pytest.mark.parametrize("name", ["heads first", "queries and keys, heads first", "in turns, heads first", "ends of heads, heads first", "tokens first",
+                                  "a cache with room, heads first", "three steps", "a buffer of a model's layers"])
+def test_layouts_in_place(name, S, N, H):
+    """What lies around the tensors stays as it is."""
+    buffer, views = placed(name, S, N, H, 16)
+    at, f = positions_of(S, N, 3), frequencies(12)
+    out, bound = buffer.double(), torch.zeros(buffer.shape, dtype=torch.float64)
+    for y, off, x in zip(views(out), views(bound), views(buffer), strict=True):
+        want, by = ref.rotary(x, at, f, False, 1.0)
+        y.copy_(want)
+        off.copy_(by)
+    got = buffer.cuda()
+    tensors = views(got)
+    assert all(a is b for a, b in zip(bg.rotary(tensors, at.cuda(), f.cuda(), inplace=True), tensors, strict=True))
+    near(got, (out, bound))
+
+
+def test_layouts_that_meet_are_refused():
+    at, f = positions_of(2, 3, 0).cuda(), frequencies(8).cuda()
+    buffer = torch.zeros(4000, device="cuda")
+    tensors = [[buffer.as_strided((2, 3, 4, 8), s)] for s in (
+        (0, 8, 24, 1), (96, 8, 23, 1), (95, 8, 24, 1), (96, 7, 24, 1), (8, 16, 40, 1), (40, 8, 16, 1), (24, 8, 0, 1))]
+    x = torch.zeros(2, 5, 3, 8, device="cuda")
+    tensors += [[x[:, :4].transpose(1, 2), x[:, 1:].transpose(1, 2)], [x[:, :4].transpose(1, 2), x[:, 3:4].transpose(1, 2)]]
+    for some in tensors:
+        with pytest.raises(ValueError, match="share no memory"):
+            bg.rotary(some, at, f, inplace=True)
+
+
 def test_many_tensors_of_one_call():
     """More than one launch holds."""
     at, f = positions_of(2, 3, 0), frequencies(8)
