@@ -17,7 +17,7 @@ struct Form {
 };
 
 void check_rotary(const Tensors& heads, const Tensor& positions, const Tensor& frequencies, const OptTensor& counts, double scale) {
-    TORCH_CHECK_VALUE(positions.dim() == 2 && index_type(positions) && positions.numel() > 0,
+    TORCH_CHECK_VALUE(positions.dim() == 2 && index_type(positions),
                       "positions must be an int32 or int64 [S, N] tensor, got ", positions.scalar_type(), " ", positions.sizes());
     const int64_t S = positions.size(0), N = positions.size(1);
     TORCH_CHECK_VALUE(positions.numel() < int64_t{1} << 26, "positions must have fewer than 2**26 tokens, got ", positions.sizes());
@@ -27,7 +27,7 @@ void check_rotary(const Tensors& heads, const Tensor& positions, const Tensor& f
                       frequencies.sizes(), " on ", frequencies.device());
     for (size_t i = 0; i < heads.size(); ++i) {
         const Tensor& t = heads[i];
-        TORCH_CHECK_VALUE(t.dim() == 4 && t.numel() > 0 && t.size(0) == S && t.size(1) == N, "tensors[", i, "] must be [S, N, H, D] = [", S, ", ", N,
+        TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == S && t.size(1) == N && t.size(2) > 0 && t.size(3) > 0, "tensors[", i, "] must be [S, N, H, D] = [", S, ", ", N,
                           ", H, D], got ", t.sizes());
         data_type(t, "tensors");
         TORCH_CHECK_VALUE(t.scalar_type() == heads[0].scalar_type(), "tensors must have one type, got ", heads[0].scalar_type(), " and ",
@@ -104,6 +104,7 @@ Tensors rotary_hip(Tensors heads, const Tensor& positions, const Tensor& frequen
         if (t.size(3) != 1 && t.stride(3) != 1) t = t.contiguous();
         out.push_back(fresh(t.sizes(), t.scalar_type(), t));
     }
+    if (positions.numel() == 0) return out;
     check_status(run_rotary(heads, out, positions, frequencies, counts, {interleaved, scale, inverse}), "rotary");
     return out;
 }
@@ -118,7 +119,7 @@ void rotary_inplace_hip(Tensors heads, const Tensor& positions, const Tensor& fr
                         bool inverse) {
     check_rotary(heads, positions, frequencies, counts, scale);
     check_inplace(heads);
-    if (heads.empty()) return;
+    if (heads.empty() || positions.numel() == 0) return;
     const at::OptionalDeviceGuard guard(positions.device());
     const int status = run_rotary(heads, heads, positions, frequencies, counts, {interleaved, scale, inverse});
     TORCH_CHECK_VALUE(status != DBS_CUDA_STATUS_INVALID_ARGUMENT,

@@ -230,6 +230,19 @@ def test_many_tensors_of_one_call():
     assert bg.rotary([], at.cuda(), f.cuda()) == []
 
 
+@pytest.mark.parametrize("S, N", [(0, 3), (2, 0), (0, 0)])
+def test_a_batch_without_tokens(S, N):
+    at, f = torch.zeros(S, N, dtype=torch.int64, device="cuda"), frequencies(8).cuda()
+    q, k = (torch.zeros(S, N, h, 10, device="cuda", dtype=torch.bfloat16).requires_grad_(True) for h in (4, 1))
+    out = bg.rotary([q, k], at, f, counts=torch.zeros(S, dtype=torch.int32, device="cuda"), scale=2.0)
+    assert [t.shape for t in out] == [(S, N, 4, 10), (S, N, 1, 10)] and out[0].dtype == torch.bfloat16
+    assert [t.shape for t in torch.autograd.grad(out, [q, k], out)] == [(S, N, 4, 10), (S, N, 1, 10)]
+    own = [q.detach(), k.detach()[..., 2:]]
+    assert bg.rotary(own, at, f, inplace=True)[0] is own[0]
+    many = torch.zeros(5, S, N, 2, 10, device="cuda")
+    assert torch.vmap(lambda a: bg.rotary([a], at, f)[0])(many).shape == many.shape
+
+
 def test_more_tokens_than_a_launch_has():
     """Every stretch of them alike: tokens at launches' edges, and the last."""
     n = (1 << 25) + 777

@@ -104,6 +104,20 @@ def test_rotary_refusals(change, error, message):
         turn(**change)
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("S, N", [(0, 3), (2, 0)])
+def test_rotary_of_a_batch_without_tokens_is_checked(S, N, inplace):
+    """As any other: it needs the GPU, and heads that fit."""
+    at = torch.zeros(S, N, dtype=I64)
+    with pytest.raises(RuntimeError, match="runs on the GPU"):
+        turn([torch.zeros(S, N, 4, 8)], at, inplace=inplace)
+    for bad in ((S, N, 0, 8), (S, N, 4, 7), (S, N, 4, 0), (S, N + 1, 4, 8), (S + 1, N, 4, 8)):
+        with pytest.raises(ValueError):
+            turn([torch.zeros(bad)], at, inplace=inplace)
+    with pytest.raises(ValueError, match="counts must be"):
+        turn([torch.zeros(S, N, 4, 8)], at, counts=torch.zeros(S + 1, dtype=I32), inplace=inplace)
+
+
 def test_frequencies():
     f = bg.rotary_frequencies(8, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
