@@ -136,6 +136,25 @@ def test_strides_and_many_pools():
     check(p, 22, 2)
 
 
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("pools_each", [1, 2])
+def test_more_sets_of_weights_than_a_launch_holds(pools_each, joint):
+    """A model of many layers: two launches choose, and lists of the second are moved by; what stays
+    and the pages given back are counted once. Pools of two widths take turns."""
+    for sets in (64, 65, 71, 130):
+        p = problem(torch.float32, [50, 9, 61, 40, 70], 8, 2, 3, sets, joint, seed=sets)
+        pools = p[0][:pools_each * sets]
+        pools[1::3] = [t.half() for t in pools[1::3]]
+        p = (pools, *p[1:])
+        pages, refs = p[2], p[4]
+        refs[pages[2, 1].long()] = 2  # written to: sequence 2 stays
+        refs[pages[4, 7].long()] = 3  # only given back
+        table = check(p, 20, 3, 2)
+        assert table.lengths.tolist() == [20, 9, 61, 20, 20]
+        # (5 tokens fit a page, so that the second one is not written to)
+        assert check(p, None, 3, 2, budgets=torch.tensor([0, 9, 5, 39, 33], dtype=torch.int32)).lengths.tolist() == [0, 9, 5, 39, 33]
+
+
 def test_evicted_caches_go_on():
     """Evict, extend, write, evict again; the pool's pages come back."""
     p = problem(torch.float32, [120, 90], 8, 2, 4, 1, False)
