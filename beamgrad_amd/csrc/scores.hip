@@ -44,7 +44,8 @@ constexpr int kManyThreads = 512;  // where rows are few
 constexpr int kAtOnce = 4;     // 16-byte reads of a thread in flight
 constexpr int kMaxTop = 64;
 constexpr int kKept = 512;     // values beside the alternatives that a workgroup ranks
-constexpr int kCounts = 1024;  // equal steps of values that are counted at once
+constexpr int kCounts = 1024;  // equal steps of values that are counted at once: 10 bits of
+constexpr int kPasses = 4;     // 32, at most
 constexpr int kMaxParts = 64;  // of a row
 constexpr int64_t kCacheBytes = int64_t{200} << 20;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -382,8 +383,8 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
         };
         uint32_t low = uniform(order_of(floor) >> kUnused), high = uniform(order_of(most) >> kUnused);
         int above = 0;
-        for (;;) {
-            tied = low == high;
+        for (int pass = 0;; ++pass) {
+            tied = low == high || pass == kPasses;  // (the last pass leaves one value, unless the row is being written)
             if (tied) break;
             const int shift = max(0, 22 - __builtin_clz(high - low));
             __syncthreads();  // what is read of LDS before is read
@@ -438,7 +439,7 @@ __device__ __forceinline__ void alternatives(const char* row, int from, int to, 
                 if (!tied || order_of(x) >> kUnused > low) keep(x, place);
             });
         __syncthreads();
-        n = uniform(lds.kept);
+        n = min(uniform(lds.kept), kKept);
     }
     if (tid < 8) lds.keys[n + tid] = 0;
     __syncthreads();
@@ -644,6 +645,7 @@ __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int p
     take_all();
     int m = uniform(found);
     if (m > kKept) {
+        __syncthreads();  // every wavefront has read how many there are
         const int lane = tid & 63, wave = tid >> 6;
         for (int i = wave; 1 << i < 2 * p.top; i += kThreads / 64) {
             const int each = min(1 << i, p.top), of = (p.top + each - 1) / each;
