@@ -237,9 +237,10 @@ __device__ __forceinline__ void choose(const float* from, int first, int end, in
 }
 
 // x: a sequence; y: a row of weights, the last: counts of pages, copied; z: a set.
-// 1024 rows of 4500 to 8000 weights, of which 4096 stay, in 38 us (26 MB read and 33 written;
-// the vector unit is busy for 42 % of it, the rest waits for the digits' counts); ten rows of
-// 900 in 9 us, most of it dependent reads: lengths, pages, their counts.
+// 1024 rows of 4500 to 8000 weights, of which 4096 stay, in 38 us (25 MB read and 49 written, 32 of
+// weights and 17 of lists, 1.9 TB/s; the vector unit is busy for 42 % of it, the rest waits for the digits' counts); ten rows of
+// 900 in 9 us, most of it dependent reads: lengths, pages, their counts. Equal weights, which one
+// counter takes, cost up to 1.7 times as much: 64 rows of 30000 in a call of 70 us 117.
 __global__ __launch_bounds__(kCutThreads) void evict_select(const Evict p, const WeightSet set) {
     __shared__ Choice lds;
     const int s = blockIdx.x, tid = threadIdx.x, head = blockIdx.y;
@@ -307,7 +308,8 @@ struct MoveSet {
 
 // x: a sequence; y: some columns of a head, the last (with `table`): the table; z: a pool.
 // 32 pools of 8 sequences of 4500 to 8000 tokens, each of 8 heads of 128 in bfloat16 keeping
-// 4096: 894 us, 4.3 GB, 4.8 TB/s.
+// 4096: 894 us, 4.3 GB, 4.8 TB/s. Every token behind the first that goes is moved: one of 4097 that goes
+// costs as much where it is the oldest, and next to nothing (the whole call 130 us) where it is the newest.
 __global__ __launch_bounds__(kMoveThreads) void evict_move(const Evict p, const MoveSet set, const bool table) {
     const int s = blockIdx.x, tid = threadIdx.x;
     const int keep = p.live[s];

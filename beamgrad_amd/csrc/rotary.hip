@@ -104,7 +104,9 @@ __device__ __forceinline__ void store_run(char* to, const Run<T, N>& r) {
 // behind what turns. The table of a token's angles costs some 60 operations for each pair, of
 // 64 bits most of them, and is made once for all heads of a tensor; beside it the
 // kernel is bound by HBM: queries and keys of 16384 tokens, 40 heads of 128 in bfloat16,
-// in 62 us, 5.4 TB/s. 32 tokens: 3.7 us, a launch and two dependent reads.
+// in 62 us, 5.4 TB/s. 32 tokens: 3.7 us, a launch and two dependent reads. PAIRS divides the pairs of a head,
+// so an odd number of them goes pair by pair: 63 of 64 pairs turned of those queries and keys, the last two
+// values copied, 201 us (in place 91); 62 of 64, two at once, 127 (61).
 template <class T, int PAIRS, bool INTERLEAVED, int TOKENS>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const Turn p) {
     extern __shared__ float2 units[];  // [TOKENS][pairs]

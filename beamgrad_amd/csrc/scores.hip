@@ -525,9 +525,11 @@ __device__ __forceinline__ void write_none(const Rows& p, uint32_t r, bool bad) 
 }
 
 // A workgroup for a row; a wavefront for a row of two rounds of its reads. Bound by HBM
-// where the rows fill the card: some 3080 of 4096 of 128256 in bfloat16 (the others have
-// no token) in 129 us, 6.1 TB/s; 490 of 660 of 50257 in float16, with the entropy and 4
-// alternatives, in 21 us. Few rows: latency, 4 of 32000 in float32 with 5 alternatives 7.1 us.
+// where the rows fill the card several times: some 3080 of 4096 of 128256 in bfloat16 (the others have
+// no token) in 129 us, 6.1 TB/s. Some hundred rows are two workgroups a CU, none of which has
+// a round on its way while it computes another: 490 of 50257 in float16 13.9 us, 3.5 TB/s, with 4 alternatives 17.2, with
+// the entropy too 17.9 (21 under a trace, among 170 rows without a token). Few rows: latency, 4 of 32000 in float32 with 5
+// alternatives 7 us.
 template <class T, bool ENTROPY, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
     __shared__ Shared<THREADS> lds;
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(THREADS) void score_rows(const Rows p) {
 
 // x: a part of `part` values of row y. Sums and alternatives go to the workspace.
 // Bound by latency: the read, the wavefronts' maxima, the ranking. 32 rows of 151936 in
-// bfloat16 with 20 alternatives 9.4 us (the bytes alone 1.9; a launch that does nothing 2 to 3).
+// bfloat16 with 20 alternatives 9.0 to 9.9 us (the bytes alone 1.9; a launch that does nothing 2 to 3).
 // With ONE a part is one round of the workgroup's reads, which stay in registers: they
 // begin while the token is still read, and are looked through for the alternatives.
 template <class T, bool ENTROPY, bool ONE>
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(kThreads) void score_parts(const Rows p, const int 
 // them, so what lies below it is none. (The last part may be short, and its j-th low.) Where
 // the largest lie in a few parts, much reaches it; then the same is asked of the j-th of the
 // ceil(top / j) parts in which it is largest, for j = 1, 2, 4 .. top, and the highest answer
-// counts: of no j more than 1 / j of the keys pass. 32 rows of 19 parts: 5.2 us, of two dependent reads and the ranking.
+// counts: of no j more than 1 / j of the keys pass. 32 rows of 19 parts: 5.0 us, of two dependent reads and the ranking.
 template <class T>
 __global__ __launch_bounds__(kThreads) void score_join(const Rows p, const int parts, const Sums* sums, const uint64_t* keys) {
     constexpr int kFirst = 4;  // keys of a thread that are read ahead

@@ -5,7 +5,9 @@
 //
 // Mathematics. With the log-sums that the attention left, a weight is
 // e^(scale q . k - lse) at once, without a pass for the softmax, and a key's sum needs
-// no other key. Q K^T is made of 16 x 16 blocks; a lane gets four rows of one key, adds
+// no other key. The exponent is one product and sum in units of log 2, fma(q . k, scale log2 e, -lse log2 e): its
+// second term is rounded by itself, so a weight is off by up to 2^-24 (|scale q . k| + |lse|) of its own beside the
+// score's rounding. Q K^T is made of 16 x 16 blocks; a lane gets four rows of one key, adds
 // their weights up, and a key's four lanes join at the end. Rows and their sums are in
 // a fixed order.
 //
@@ -37,7 +39,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSequences = kThreads;  // of a launch: a thread of each workgroup reads one's length
 constexpr int kNone = INT32_MIN;      // below every token
-constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 
 // of a lambda: its captures and arrays stay in registers
@@ -337,11 +338,14 @@ __global__ __launch_bounds__(kThreads, (ROWS > Dims<DTYPE, DP>::kRows ? 2 : Dims
 // it, and are not in the line. 64 keys stay with a wavefront, so that a block of queries
 // that is read from LDS serves 16 matrix instructions of width 128; a score costs the vector
 // unit a product, an exponential and a sum. Two prompts' ends of 512 tokens over 7700 and
-// 15100 of 32 heads of 128 in bfloat16: 143 us, 99 GFLOP, 650 to 690 TFLOP/s; with 2048
-// over 16000 in eight 820. The vector unit is busy for 64 % of the time and the matrix unit for
-// 36 %: they take turns, and with constant operands, which take less power, the 820
-// are 990. Queries read a block ahead, blocks without a loop and raised priority around
-// the products changed nothing.
+// 15100 of 32 heads of 128 in bfloat16: 145 us under a trace, 99 GFLOP, 680 TFLOP/s (a call, its join with it, 141 us
+// repeated without a pause, 129 among calls with other inputs); with 2048
+// over 16000 in eight 820; in float32 835 us, 119 TFLOP/s. The vector unit is busy for 64 % of the time and the matrix unit for
+// 36 %: neither is the limit by itself, but a wavefront's products of a block and what is computed
+// from them stand one after the other, and only two more wavefronts share its SIMD. With constant operands, which
+// take less power, the 820 are 990. Queries read a block ahead, blocks without a loop and raised priority around
+// the products changed nothing; products of 32 x 32 and a block's products among the exponentials
+// of the one before were not tried.
 template <int DTYPE, int DP>
 __global__ __launch_bounds__(kThreads, 3) void weigh_many(const Weigh p) {
     using E = Elem<DTYPE>;
@@ -692,7 +696,7 @@ bool lies_apart(const BeamgradWeights& a) {
 // Workgroups of a launch, a multiple of eight. The card holds three of many rows on a CU
 // (two with a large tree's table), but of three that share a CU the oldest runs fastest:
 // twice as many, in equal stretches, are done sooner (two prompts' ends of 512 tokens over
-// 7700 and 15100, 32 heads of 128, bfloat16: 143 us, 151 with one round; more rounds
+// 7700 and 15100, 32 heads of 128, bfloat16: 143 us a call, 151 with one round; more rounds
 // cost more beginnings than they gain). Few rows have shorter beginnings: four rounds (32
 // tokens over 2000 to 16000: 125 us, 140 with one). More rows that keys pass fill LDS of
 // a CU twice, and begin longer: one round (68 rows of 128 in bfloat16 over 32 x 2700 to 8000
